@@ -416,6 +416,97 @@ int spv_prefill_attn(void* out, const void* q, const void* k, const void* v,
                      int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim,
                      float scale, void* stream);
 
+/* --------------------------------------------------- shared-prefix attention */
+
+/* Attention of a batch whose sequences share long prefixes (no reference
+ * counterpart; the reference would hold the prefix in every sequence): entry b's
+ * row j attends the first prefix_lens[b] positions of sequence prefix_ids[b],
+ * then positions 0 .. start_b + j of its own sequence seq_ids[b], with one
+ * softmax(scale * q.k) over both. A prefix is a sequence of the same pool; the
+ * own sequence holds only what follows it. Entries with one prefix and one
+ * length walk it together, once.
+ *
+ * The plan lists that work. It depends on the prefixes, their lengths, the chunk
+ * and the heads, not on the sequences' own lengths, so it is made when requests
+ * are admitted and serves every layer and round until the next admission.
+ * prefix_ids and prefix_lens (B entries each) and plan are HOST pointers:
+ * prefix_ids[b] = -1 or prefix_lens[b] = 0 is no prefix. With plan NULL the call
+ * returns the plan's length in int32 words; otherwise it writes the plan
+ * (plan_ints words are there) and returns its length; a negative SPV_ERR_* on
+ * bad arguments. The caller copies the plan to the device and keeps both. */
+int64_t spv_shared_attn_plan(const int32_t* prefix_ids, const int32_t* prefix_lens,
+                             int32_t B, int32_t C, int32_t num_q_heads,
+                             int32_t num_kv_heads, int32_t block_size, int32_t* plan,
+                             int64_t plan_ints);
+
+/* Workspace of spv_shared_attn (partial results; needs no particular contents
+ * and may be another one in every call) for own contexts up to max_ctx;
+ * plan_host: the plan on the host. 0 for bad arguments. */
+size_t spv_shared_attn_workspace_bytes(const int32_t* plan_host, int32_t head_dim,
+                                       int32_t max_ctx);
+
+/* The attention, of any layer, by a plan made for the same B, C, heads and block
+ * size. Arguments as spv_verify_attn's; max_ctx bounds start_b + C (own
+ * positions). q_dtype f32, bf16 or f16, kv_dtype any, head_dim <= 256. Reads the
+ * contract forbids -- a prefix longer than its sequence, start_b + C beyond the
+ * written length or max_ctx, a block id outside the pool -- set ctr[7] = 1 + b
+ * (sticky) and read block 0, never outside the pool. A key beyond a row's last
+ * position does not reach the row, whatever it holds. Two launches. */
+int spv_shared_attn(void* out, const void* q, int q_dtype, const void* k_pool,
+                    const void* v_pool, int kv_dtype, const float* kv_scales,
+                    const int32_t* block_tables, int32_t max_blocks_per_seq,
+                    const int32_t* seq_ids, const int32_t* start_pos,
+                    const int32_t* seq_lens, int32_t* ctr, int32_t B, int32_t C,
+                    int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim,
+                    int32_t block_size, int32_t layer, int32_t capacity, int32_t max_ctx,
+                    float scale, const int32_t* plan_host, const int32_t* plan,
+                    void* workspace, size_t workspace_bytes, void* stream);
+
+/* ------------------------------------------------------------------ rotary */
+
+/* Rotary position embedding of a chunk (the reference's model code rotates
+ * queries and keys before it writes and attends, engine/model.py:174-181). Row x
+ * of head_dim elements: the pair of frequency i < rotary_dim / 2 -- elements
+ * (i, i + rotary_dim / 2), or (2i, 2i + 1) with interleaved != 0 -- turns by
+ * position * inv_freq[i] and is scaled by factor; elements from rotary_dim on
+ * are copied. inv_freq: rotary_dim / 2 float64 on the device. positions:
+ * (axes, B, C) int32; frequency i takes the positions of axis axis_of[i]
+ * (rotary_dim / 2 int32; may be NULL when axes = 1).
+ * q (B, C, num_q_heads, head_dim) and k (B, C, num_kv_heads, head_dim) in dtype
+ * (f32, bf16, f16); either may be NULL with its output. strides (HOST, 12
+ * values): the element strides (batch, token, head) of q_out, q, k_out, k; the
+ * last dim is contiguous. An output is its input (same strides) or overlaps no
+ * input. k_out is in k_out_dtype: dtype or f32. B * C <= 2^23. */
+int spv_rotary(void* q_out, const void* q, void* k_out, const void* k, int dtype,
+               int k_out_dtype, const int64_t* strides, const int32_t* positions,
+               const double* inv_freq, const int32_t* axis_of, int32_t axes, float factor,
+               int32_t B, int32_t C, int32_t num_q_heads, int32_t num_kv_heads,
+               int32_t head_dim, int32_t rotary_dim, int32_t interleaved, void* stream);
+
+/* spv_kv_append of a chunk whose keys are rotated on the way, and whose queries
+ * are rotated into q_out (q may be NULL): k_new / v_new in the pool's type dtype
+ * (not fp8), strides (HOST, 12 values) of q_out, q, k_new, v_new as above.
+ * positions NULL: token j of entry b is at start_b + j (axes = 1); positions are
+ * not the pool positions where a sequence continues a shared prefix, or has
+ * image tokens. may_alloc: the missing blocks are allocated first (one more
+ * launch), with spv_kv_append's exhaustion and table-width rules; without, the
+ * verdict of the last allocation stands. write_plan (B x C int32, or NULL)
+ * receives the chunk's pool rows as in spv_kv_append_plan, or, with follow_plan
+ * != 0, names them (a later layer's call: no table, length or counter is read or
+ * written). Both pools' rows outside the chunk stay as they are. */
+int spv_kv_rotary_append(void* q_out, const void* q, const void* k_new, const void* v_new,
+                         int dtype, const int64_t* strides, void* k_pool, void* v_pool,
+                         int32_t* block_tables, int32_t max_blocks_per_seq,
+                         int32_t* num_blocks, int32_t* seq_lens, int32_t* free_stack,
+                         int32_t* free_flag, int32_t* ctr, const int32_t* seq_ids,
+                         const int32_t* start_pos, const int32_t* positions,
+                         const double* inv_freq, const int32_t* axis_of, int32_t axes,
+                         float factor, int32_t B, int32_t C, int32_t num_q_heads,
+                         int32_t num_kv_heads, int32_t head_dim, int32_t rotary_dim,
+                         int32_t interleaved, int32_t layer, int32_t capacity,
+                         int32_t block_size, int32_t may_alloc, int32_t follow_plan,
+                         int32_t* write_plan, void* stream);
+
 /* -------------------------------------------------------------- sampling */
 
 /* Workspace needed by spv_verify_sample. Its first SPV_SAMPLE_COUNTER_BYTES

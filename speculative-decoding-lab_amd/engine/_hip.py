@@ -44,6 +44,7 @@ P = ctypes.c_void_p
 I = ctypes.c_int32
 F = ctypes.c_float
 S = ctypes.c_size_t
+L = ctypes.c_int64
 
 # name -> (restype, argtypes); mirrors include/specverify.h
 SIGNATURES = {
@@ -73,6 +74,12 @@ SIGNATURES = {
     "spv_time_next_attention": (I, [P, P]),
     "spv_verify_attn_static_max_bytes": (S, []),
     "spv_verify_attn_static": (I, [P, P, I, P, P, I, P, P, I, P, P, P, P, I, I, I, I, I, I, I, I, I, F, P]),
+    "spv_shared_attn_plan": (L, [P, P, I, I, I, I, I, P, L]),
+    "spv_shared_attn_workspace_bytes": (S, [P, I, I]),
+    "spv_shared_attn": (I, [P, P, I, P, P, I, P, P, I, P, P, P, P, I, I, I, I, I, I, I, I, I, F, P, P, P, S, P]),
+    "spv_rotary": (I, [P, P, P, P, I, I, P, P, P, P, I, F, I, I, I, I, I, I, I, P]),
+    "spv_kv_rotary_append": (I, [P, P, P, P, I, P, P, P, P, I, P, P, P, P, P, P, P, P, P, P, I, F, I, I, I, I, I, I,
+                                 I, I, I, I, I, I, P, P]),
     "spv_verify_sample_workspace_bytes": (S, [I, I, I]),
     "spv_verify_sample": (I, [P, P, I, F, P, P, P, P, P, P, I, I, I, I, P, P, P, P, P, P, P, I, P, S, P]),
     "spv_verify_sample_filtered_workspace_bytes": (S, [I, I, I, F, I]),

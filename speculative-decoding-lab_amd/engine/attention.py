@@ -10,6 +10,9 @@ Drop-in for the reference's engine/attention.py on the verify path:
 * ``paged_attention_prefill_chunk`` -- attention.py:121-167, one causal prefill
                                 launch over the dense chunk (``prefill_attention``
                                 takes the lengths as a device tensor)
+* ``shared_prefix_attention`` -- no counterpart: attention of a batch whose
+                                sequences continue shared prefixes, each prefix
+                                walked once (``SharedPrefix`` holds the groups)
 * ``_expand_to_q_heads``     -- attention.py:32-38 (kept for API parity; the
                                 kernels never materialise the expansion: kv head
                                 ``h // (Hq/Hkv)`` is indexed directly)
@@ -26,6 +29,7 @@ the plan start their page walk one round trip after launch.
 
 from __future__ import annotations
 
+import ctypes
 import math
 from typing import Optional, Sequence, Union
 
@@ -239,6 +243,104 @@ def paged_attention_decode(query_2d: torch.Tensor, kv: PagedKVCache, layer: int,
     q3 = query_2d.unsqueeze(1)
     out = paged_attention_extend(q3, kv, layer, seq_ids, [x - 1 for x in lengths], num_q_heads)
     return out.squeeze(1)
+
+
+class SharedPrefix:
+    """Which prefix each entry of a batch continues, for ``shared_prefix_attention``.
+
+    Entry ``b`` attends the first ``prefix_lens[b]`` positions of sequence
+    ``prefix_ids[b]`` of the cache (-1, or length 0: no prefix) before its own
+    sequence, which holds only what follows the prefix. Entries with the same
+    prefix and length read it together. Host lists: they change when requests
+    are admitted or leave, while every layer and round between uses the same
+    object. A prefix is a sequence like any other; the caller keeps it until
+    the last of its entries has left.
+    """
+
+    def __init__(self, kv: PagedKVCache, prefix_ids: Sequence[int], prefix_lens: Sequence[int], chunk: int,
+                 num_q_heads: int) -> None:
+        ids, lens = [int(s) for s in prefix_ids], [int(n) for n in prefix_lens]
+        if len(ids) != len(lens):
+            raise ValueError("one prefix length per prefix id")
+        if any(n < 0 for n in lens) or any(s < -1 for s in ids):
+            raise ValueError("prefix lengths must be >= 0, prefix ids >= -1 (none)")
+        self.chunk, self.num_q_heads = int(chunk), int(num_q_heads)
+        if self.chunk < 1 or self.num_q_heads < 1 or self.num_q_heads % kv.num_kv_heads:
+            raise ValueError("chunk must be >= 1 and query heads a multiple of the cache's {}".format(kv.num_kv_heads))
+        kv._refresh()
+        for s, n in zip(ids, lens):
+            if s >= 0 and n > 0 and n > kv._lens[kv._check_sid(s)]:
+                raise IndexError("prefix sequence {} holds {} positions, not {}".format(s, kv._lens[s], n))
+        self.kv, self.B = kv, len(ids)
+        self.longest = max([n for s, n in zip(ids, lens) if s >= 0], default=0)
+        self._host = self._dev = None
+        if not self.B:
+            return
+        c_ids, c_lens = ((ctypes.c_int32 * self.B)(*x) for x in (ids, lens))
+        args = (c_ids, c_lens, self.B, self.chunk, self.num_q_heads, kv.num_kv_heads, kv.block_size)
+        n = int(_hip.lib().spv_shared_attn_plan(*args, None, 0))
+        if n < 0:
+            raise _hip.HipLibraryError("spv_shared_attn_plan failed: {} ({})".format(_hip._ERRORS.get(n, "error"), n))
+        self._host = (ctypes.c_int32 * n)()
+        _hip.lib().spv_shared_attn_plan(*args, self._host, n)
+        self._dev = torch.frombuffer(self._host, dtype=torch.int32).to(kv.device)
+        self._bytes = (0, 0)  # the last max_ctx and its calls' workspace
+
+
+def shared_prefix_attention(query_3d: torch.Tensor, kv: PagedKVCache, layer: int,
+                            seq_ids: Union[Sequence[int], torch.Tensor],
+                            start_positions: Union[Sequence[int], torch.Tensor], max_ctx: int,
+                            prefix: SharedPrefix, scale: Optional[float] = None,
+                            out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """``verify_attention`` behind shared prefixes.
+
+    Row ``j`` of entry ``b`` attends its prefix (``prefix``) and then positions
+    ``0 .. start_positions[b] + j`` of sequence ``seq_ids[b]``, in one softmax.
+    ``start_positions`` and ``max_ctx`` (a bound on ``start + chunk``) count the
+    own sequence's positions, which begin behind the prefix; the chunk's keys
+    are already written. int32 device tensors cause no host sync. Reads of
+    positions that were never written raise ``IndexError`` at the next metadata
+    query, as in ``verify_attention``.
+    """
+    B, chunk, hq, d = query_3d.shape
+    if d != kv.head_dim or kv is not prefix.kv or (B, chunk, hq) != (prefix.B, prefix.chunk, prefix.num_q_heads):
+        raise ValueError("the query does not match the cache and its shared prefixes")
+    if query_3d.device != kv.device:
+        raise ValueError("query must live on {}".format(kv.device))
+    if not 0 <= int(layer) < kv.num_layers:
+        raise IndexError("layer {} out of range".format(layer))
+    max_ctx = int(max_ctx)
+    if max_ctx < chunk:
+        raise ValueError("max_ctx must be at least the chunk")
+    q = query_3d.contiguous()
+    if out is None:
+        out = torch.empty_like(q)
+    elif out.shape != q.shape or out.dtype != q.dtype or out.device != q.device or not out.is_contiguous() \
+            or _overlap(out, q):
+        raise ValueError("out must be a contiguous tensor like the query, apart from it")
+    if B == 0:
+        return out
+    if not isinstance(seq_ids, torch.Tensor):
+        seq_ids = [kv._check_sid(s) for s in seq_ids]
+    sid_t, start_t = _hip.i32s(kv.device, seq_ids, start_positions)
+    if sid_t.numel() != B or start_t.numel() != B:
+        raise ValueError("one seq_id and start position per batch row")
+    longest = max(max_ctx, prefix.longest)
+    if longest > kv.max_blocks_per_seq * kv.block_size:
+        kv._grow_width(-(-longest // kv.block_size))
+    if prefix._bytes[0] != max_ctx:
+        prefix._bytes = (max_ctx, int(_hip.lib().spv_shared_attn_workspace_bytes(prefix._host, d, max_ctx)))
+    nbytes = prefix._bytes[1]
+    # from the allocator in every call: ordered with its stream's work, and a
+    # captured graph's own
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=kv.device)
+    scale = 1.0 / math.sqrt(d) if scale is None else float(scale)
+    call("spv_shared_attn", ptr(out), ptr(q), _hip.dtype_code(q.dtype), ptr(kv.k_pool), ptr(kv.v_pool), kv._dt,
+         ptr(kv.scales), ptr(kv.tables_dev), kv.max_blocks_per_seq, ptr(sid_t), ptr(start_t), ptr(kv.lens_dev),
+         ptr(kv.allocator.ctr), B, chunk, hq, kv.num_kv_heads, d, kv.block_size, int(layer), kv.allocator.capacity,
+         max_ctx, scale, prefix._host, ptr(prefix._dev), ptr(ws), nbytes, _hip.stream_of(kv.device))
+    kv._stale = True
+    return out
 
 
 def prefill_attention(query_3d: torch.Tensor, key_3d: torch.Tensor, value_3d: torch.Tensor,
