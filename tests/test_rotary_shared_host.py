@@ -36,12 +36,14 @@ def _plan(lib, ids, lens, C=3, Hq=4, Hkv=2, bs=16):
 
 
 def _sections(plan):
-    """(groups, members, entries, items) of a plan as lists of records."""
-    ng, items = plan[8], plan[9]
-    at = plan[12:16]
+    """(groups, members, entries, shares, segments, tiles) of a plan as lists of records."""
+    ng, nsh, nseg, nt = plan[7:11]
+    at = plan[12:18]
     cut = lambda o, n, w: [plan[o + i * w:o + (i + 1) * w] for i in range(n)]  # noqa: E731
-    nm = sum(g[3] for g in cut(at[0], ng, 8))
-    return cut(at[0], ng, 8), plan[at[1]:at[1] + nm], cut(at[2], plan[2], 2), cut(at[3], items, 4)
+    groups = cut(at[0], ng, 6)
+    nm = sum(g[3] for g in groups)
+    shares = plan[at[3]:at[3] + (nsh + 1 if nsh else 1)]
+    return groups, plan[at[1]:at[1] + nm], cut(at[2], plan[2], 2), shares, cut(at[4], nseg, 5), cut(at[5], nt, 2)
 
 
 @pytest.mark.parametrize("ids,lens", [
@@ -56,26 +58,35 @@ def test_plan_covers_every_row_and_key_once(lib, ids, lens):
     C, Hq, Hkv, bs = 3, 4, 2, 16
     G = C * Hq // Hkv
     plan = _plan(lib, ids, lens, C, Hq, Hkv, bs)
-    groups, members, entries, items = _sections(plan)
+    assert plan[1] == len(plan)
+    groups, members, entries, shares, segs, tiles = _sections(plan)
     want = {}
     for b, (s, n) in enumerate(zip(ids, lens)):
         if s >= 0 and n > 0:
             want.setdefault((s, n), []).append(b)
     assert [(g[0], g[1]) for g in groups] == list(want)
-    part = 0
-    for gi, g in enumerate(groups):
-        sid, n, first, count, splits, keys, base = g[:7]
+    seen = 0
+    for gi, (sid, n, first, count, nt, tile0) in enumerate(groups):
         assert members[first:first + count] == want[(sid, n)]
         for rank, b in enumerate(members[first:first + count]):
             assert entries[b] == [gi, rank]
-        assert base == part and keys % bs == 0 and (splits - 1) * keys < n <= splits * keys
-        rows = count * G
-        tile = plan[7]
-        got = sorted((h, t, s) for q, h, t, s in items if q == gi)
-        assert got == [(h, t, s) for h in range(Hkv) for t in range(-(-rows // tile)) for s in range(splits)]
-        part += rows * Hkv * splits
-    assert plan[10] == part
+        assert nt == -(-count * G // 128)
+        for h in range(Hkv):
+            for t in range(nt):
+                at, k = tiles[tile0 + h * nt + t]
+                part = segs[at:at + k]
+                seen += k
+                assert all(x[:3] == [gi, h, t] for x in part)
+                assert part[0][3] == 0 and part[-1][4] == n
+                assert all(x[4] == y[3] for x, y in zip(part, part[1:]))
+                assert all(x[3] < x[4] and x[3] % 64 == 0 for x in part)
+    assert seen == len(segs)
     assert all(entries[b][0] == -1 for b, (s, n) in enumerate(zip(ids, lens)) if s < 0 or n == 0)
+    # the shares cover the segments in order, with equal numbers of 64-key units
+    assert shares[0] == 0 and shares[-1] == len(segs) and len(shares) % 8 == 1
+    units = [sum(-(-(x[4] - x[3]) // 64) for x in segs[a:b]) for a, b in zip(shares, shares[1:])]
+    assert all(a <= b for a, b in zip(shares, shares[1:]))
+    assert not units or max(units) - min(units) <= 1
 
 
 def test_plan_refusals(lib):
