@@ -12,6 +12,8 @@
 // off by up to 0.03 rad, and the fp64 one, in turns, by 2^-53 of some 10^5
 // turns. What is left of a turn goes to fp32 sin and cos (an error of 2^-24
 // turns at most), the products are fp32, and each result is rounded once.
+#include <type_traits>
+
 #include "spv_common.h"
 
 using namespace spv;
@@ -134,6 +136,269 @@ __global__ __launch_bounds__(256) void rotary_elem_kernel(RotaryParams p) {
   }
 }
 
+// Rows of whole 16-byte pieces. A workgroup takes TT tokens of one entry and a
+// slice of the heads. A thread keeps one token and one piece pair (the pieces
+// that rotate with each other; past the rotary width one piece) and goes over
+// the slice's heads with it, kAhead loads in flight. The turns of the
+// workgroup's tokens are computed once, into LDS, while the first rows travel.
+// The slices behind the query and key heads copy the values, one (16 positions,
+// head) each, transposed through LDS so that whole pages are stored as 16-byte
+// pieces.
+// What bounds it: the rows' bytes, each read and written once, for prompts; a
+// few dependent round trips (start, table, length, position) for decode chunks.
+constexpr int kVecThreads = 256;
+constexpr int kAhead = 4;
+constexpr int kMaxTT = 16;
+constexpr int kVT = 16;  // positions of a value tile
+
+typedef float f32x2_t __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x2_t __attribute__((ext_vector_type(2)));
+
+template <int DT>
+struct Piece {  // 16 bytes as fp32
+  static constexpr int E = DT == SPV_F32 ? 4 : 8;
+  float x[E];
+  __device__ __forceinline__ void unpack(u32x4_t w) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (DT == SPV_F32) {
+        x[i] = __uint_as_float(w[i]);
+      } else if constexpr (DT == SPV_BF16) {
+        x[2 * i] = __uint_as_float(w[i] << 16);
+        x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+      } else {
+        const uint32_t word = w[i];  // a bit cast of the vector's element itself takes element 0
+        const f16x2_t h = __builtin_bit_cast(f16x2_t, word);
+        x[2 * i] = (float)h[0];
+        x[2 * i + 1] = (float)h[1];
+      }
+    }
+  }
+  __device__ __forceinline__ u32x4_t pack() const {
+    u32x4_t w;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (DT == SPV_F32) w[i] = __float_as_uint(x[i]);
+      else if constexpr (DT == SPV_BF16)
+        w[i] = __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2_t{x[2 * i], x[2 * i + 1]}, bf16x2_t));
+      else w[i] = __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2_t{x[2 * i], x[2 * i + 1]}, f16x2_t));
+    }
+    return w;
+  }
+};
+
+// Host-chosen shape of the launch.
+struct VecShape {
+  int TT, items, hs, hpw, slices, tiles;  // tokens, pieces per row, heads at once, heads per slice, slices, tiles of C
+};
+
+template <int DT, bool APPEND>
+__device__ __forceinline__ void copy_values(const RotaryParams& p, int b, int tile, int h, uint8_t* lds) {
+  using T = typename std::conditional<DT == SPV_F32, uint32_t, uint16_t>::type;
+  constexpr int ES = sizeof(T), E = 16 / ES;
+  __shared__ int s_row[kVT];
+  const int s0 = p.start[b], first = (s0 >= 0 ? s0 / kVT * kVT : s0) + tile * kVT;  // the tile's positions
+  const int j0 = max(first - s0, 0), nt = min(p.C, first + kVT - s0) - j0;           // its chunk tokens
+  if (nt <= 0) return;
+  const int vec = p.d / E;
+  T* const sv = reinterpret_cast<T*>(lds);  // [token][d]
+  const uint8_t* src = p.v + ((long long)b * p.vs[0] + (long long)j0 * p.vs[1] + (long long)h * p.vs[2]) * ES;
+  for (int i = threadIdx.x; i < nt * vec; i += kVecThreads) {
+    const int t = i / vec, c = i - t * vec;
+    reinterpret_cast<u32x4_t*>(sv)[i] = *reinterpret_cast<const u32x4_t*>(src + (long long)t * p.vs[1] * ES + 16 * c);
+  }
+  if ((int)threadIdx.x < nt) {
+    int n;
+    s_row[threadIdx.x] = p.plan_in ? p.plan_in[(size_t)b * p.C + j0 + threadIdx.x] : pool_row(p, b, j0 + threadIdx.x, &n);
+  }
+  __syncthreads();
+  T* const pool = reinterpret_cast<T*>(p.vpool) + ((size_t)p.layer * p.cap * p.Hkv + h) * (size_t)p.d * p.bs;
+  const size_t step = (size_t)p.Hkv * p.d * p.bs;  // elements from a block's page to the next block's
+  if (nt == kVT && p.bs % kVT == 0 && s_row[0] >= 0 && s_row[kVT - 1] == s_row[0] + kVT - 1) {
+    // 16 tokens side by side in one page: 16-byte pieces of each dim's row
+    const int blk = s_row[0] / p.bs, off = s_row[0] - blk * p.bs;  // a multiple of 16, as the first position is
+    T* const dst = pool + blk * step + off;
+    constexpr int kPer = kVT / E;
+    for (int i = threadIdx.x; i < p.d * kPer; i += kVecThreads) {
+      const int e = i / kPer, q = i - e * kPer;
+      u32x4_t w;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        if constexpr (ES == 4) w[k] = sv[(q * E + k) * p.d + e];
+        else w[k] = sv[(q * E + 2 * k) * p.d + e] | (uint32_t)sv[(q * E + 2 * k + 1) * p.d + e] << 16;
+      }
+      *reinterpret_cast<u32x4_t*>(dst + (size_t)e * p.bs + q * E) = w;
+    }
+    return;
+  }
+  for (int i = threadIdx.x; i < nt * p.d; i += kVecThreads) {
+    const int e = i / nt, t = i - e * nt, row = s_row[t];  // tokens fastest: neighbours of a dim's row
+    if (row < 0) continue;
+    const int blk = row / p.bs, off = row - blk * p.bs;
+    pool[blk * step + (size_t)e * p.bs + off] = sv[t * p.d + e];
+  }
+}
+
+template <int DT, bool APPEND>
+__global__ __launch_bounds__(kVecThreads) void rotary_vec_kernel(RotaryParams p, VecShape v) {
+  constexpr int ES = DT == SPV_F32 ? 4 : 2, E = 16 / ES;
+  extern __shared__ __align__(16) uint8_t lds[];
+  __shared__ int s_row[kMaxTT];
+  const int x = blockIdx.x, slice = blockIdx.y;
+  const int b = x / v.tiles, tile = x - b * v.tiles;
+  if (APPEND && slice >= v.slices) {
+    copy_values<DT, APPEND>(p, b, tile, slice - v.slices, lds);
+    return;
+  }
+  const int j0 = tile * v.TT, nt = min(v.TT, p.C - j0);
+  if (nt <= 0) return;
+  const int c = threadIdx.x % v.items, rest = threadIdx.x / v.items, t = rest % v.TT, hs = rest / v.TT;
+  const int half = p.R / 2, n2 = half / E;  // frequencies, piece pairs of a row
+  const bool pair = c < n2;
+  const int c0 = !pair ? 2 * n2 + (c - n2) : p.interleaved ? 2 * c : c;  // the thread's pieces of a row
+  const int c1 = !pair ? c0 : p.interleaved ? 2 * c + 1 : c + n2;
+  const int H = p.Hq + p.Hkv, end = min((slice + 1) * v.hpw, H);
+  const bool mine = t < nt && hs < v.hs;
+  const int j = j0 + min(t, nt - 1);
+  const uint8_t* const qrow = p.q + ((long long)b * p.qs[0] + (long long)j * p.qs[1]) * ES;
+  const uint8_t* const krow = p.k + ((long long)b * p.ks[0] + (long long)j * p.ks[1]) * ES;
+  u32x4_t in[kAhead][2];
+  auto load = [&](int h, u32x4_t* w) {
+    const uint8_t* row = h < p.Hq ? qrow + (long long)h * p.qs[2] * ES : krow + (long long)(h - p.Hq) * p.ks[2] * ES;
+    w[0] = *reinterpret_cast<const u32x4_t*>(row + 16 * c0);
+    w[1] = *reinterpret_cast<const u32x4_t*>(row + 16 * c1);
+  };
+  const int h0 = slice * v.hpw + hs;
+  if (mine)
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u)
+      if (h0 + u * v.hs < end) load(h0 + u * v.hs, in[u]);
+  if constexpr (APPEND) {
+    if ((int)threadIdx.x < nt && (slice == 0 || end > p.Hq)) {
+      const int jj = j0 + threadIdx.x;
+      int row;
+      if (p.plan_in) {
+        row = p.plan_in[(size_t)b * p.C + jj];
+      } else {
+        int n;
+        row = pool_row(p, b, jj, &n);
+        if (slice == 0) {
+          if (p.plan_out) p.plan_out[(size_t)b * p.C + jj] = row;
+          if (jj == 0 && n > 0) {
+            const int sid = p.seq_ids[b], upto = p.start[b] + n;
+            if (p.seq_lens[sid] < upto) p.seq_lens[sid] = upto;
+          }
+        }
+      }
+      s_row[threadIdx.x] = row;
+    }
+  }
+  float2* const turns = reinterpret_cast<float2*>(lds);  // [token][frequency]
+  for (int i = threadIdx.x; i < nt * half; i += kVecThreads) {
+    const int tt = i / half, f = i - tt * half;
+    turns[i] = turn_of(p, b, j0 + tt, f);
+  }
+  __syncthreads();
+  if (!mine) return;
+  int blk = 0, off = 0, row = -1;
+  if constexpr (APPEND) {
+    if (end > p.Hq) {
+      row = s_row[t];
+      if (row >= 0) {
+        blk = row / p.bs;
+        off = row - blk * p.bs;
+      }
+    }
+  }
+  auto put = [&](int h, const u32x4_t* w) {
+    uint8_t* out;
+    if (h < p.Hq) {
+      out = p.q_out + ((long long)b * p.qos[0] + (long long)j * p.qos[1] + (long long)h * p.qos[2]) * ES;
+    } else if constexpr (APPEND) {
+      if (row < 0) return;
+      out = p.kpool + ((((size_t)p.layer * p.cap + blk) * p.Hkv + (h - p.Hq)) * p.bs + off) * (size_t)(p.d * ES);
+    } else {
+      out = p.k_out + ((long long)b * p.kos[0] + (long long)j * p.kos[1] + (long long)(h - p.Hq) * p.kos[2]) * ES;
+    }
+    if (!pair) {
+      *reinterpret_cast<u32x4_t*>(out + 16 * c0) = w[0];
+      return;
+    }
+    Piece<DT> a, d;
+    a.unpack(w[0]);
+    d.unpack(w[1]);
+    const float2* const tc = turns + t * half + c * E;
+    if (p.interleaved) {
+#pragma unroll
+      for (int i = 0; i < E / 2; ++i) {
+        const float2 r = tc[i], s = tc[E / 2 + i];
+        const float a0 = a.x[2 * i], a1 = a.x[2 * i + 1], d0 = d.x[2 * i], d1 = d.x[2 * i + 1];
+        a.x[2 * i] = a0 * r.x - a1 * r.y;
+        a.x[2 * i + 1] = a1 * r.x + a0 * r.y;
+        d.x[2 * i] = d0 * s.x - d1 * s.y;
+        d.x[2 * i + 1] = d1 * s.x + d0 * s.y;
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < E; ++i) {
+        const float2 r = tc[i];
+        const float a0 = a.x[i], d0 = d.x[i];
+        a.x[i] = a0 * r.x - d0 * r.y;
+        d.x[i] = d0 * r.x + a0 * r.y;
+      }
+    }
+    *reinterpret_cast<u32x4_t*>(out + 16 * c0) = a.pack();
+    *reinterpret_cast<u32x4_t*>(out + 16 * c1) = d.pack();
+  };
+  for (int h = h0; h < end; h += kAhead * v.hs) {
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u)
+      if (h + u * v.hs < end) put(h + u * v.hs, in[u]);
+    const int next = h + kAhead * v.hs;
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u)
+      if (next + u * v.hs < end) load(next + u * v.hs, in[u]);
+  }
+}
+
+size_t vec_lds(const RotaryParams& p, const VecShape& v, int es, bool append) {
+  const size_t turns = (size_t)v.TT * (p.R / 2) * sizeof(float2), values = append ? (size_t)kVT * p.d * es : 0;
+  return turns > values ? turns : values;
+}
+
+// Whether the vector kernel takes the call: whole 16-byte pieces that begin on
+// 16-byte addresses, and rows short enough for one workgroup's threads.
+bool vec_shape(const RotaryParams& p, int es, bool append, VecShape& v) {
+  const int E = 16 / es;
+  if (p.d % E || p.R % (2 * E)) return false;
+  auto aligned = [&](const void* ptr, const long long* st) {
+    if (!ptr) return true;
+    return (uintptr_t)ptr % 16 == 0 && st[0] * es % 16 == 0 && st[1] * es % 16 == 0 && st[2] * es % 16 == 0;
+  };
+  if (!aligned(p.q, p.qs) || !aligned(p.q_out, p.qos) || !aligned(p.k, p.ks)) return false;
+  if (append ? !aligned(p.v, p.vs) || (uintptr_t)p.kpool % 16 || (uintptr_t)p.vpool % 16 : !aligned(p.k_out, p.kos))
+    return false;
+  v.items = p.R / (2 * E) + (p.d - p.R) / E;
+  if (v.items > kVecThreads) return false;
+  v.TT = 1;
+  while (v.TT < kMaxTT && v.TT < p.C && 2 * v.TT * v.items <= kVecThreads) v.TT *= 2;
+  v.hs = kVecThreads / (v.items * v.TT);
+  const int H = p.Hq + p.Hkv;
+  v.tiles = (p.C + v.TT - 1) / v.TT;
+  // Slices of the heads until there are about 1,024 workgroups, each thread with one head at least.
+  const long long wgs = (long long)p.B * v.tiles, want = (1024 + wgs - 1) / wgs;
+  const int most = (H + v.hs - 1) / v.hs;
+  const int ns = (int)(want < most ? want : most);
+  v.hpw = ((H + ns - 1) / ns + v.hs - 1) / v.hs * v.hs;
+  v.slices = (H + v.hpw - 1) / v.hpw;
+  if (append) {  // value tiles: the chunk's positions by sixteens from a multiple of sixteen
+    const int vt = (p.C + kVT - 1) / kVT + 1;
+    if (vt > v.tiles) v.tiles = vt;
+  }
+  return (long long)p.B * v.tiles <= (1LL << 23) && v.slices + p.Hkv <= 65535 && vec_lds(p, v, es, append) <= 65536;
+}
+
 // Shapes and frequencies common to both entry points.
 bool rotary_args_ok(int dtype, int32_t B, int32_t C, int32_t hq, int32_t hkv, int32_t d, int32_t rotary_dim,
                     int32_t axes, int32_t interleaved, const double* inv_freq, const int32_t* axis_of) {
@@ -143,6 +408,17 @@ bool rotary_args_ok(int dtype, int32_t B, int32_t C, int32_t hq, int32_t hkv, in
     return false;
   if (rotary_dim > 0 && (!inv_freq || (axes > 1 && !axis_of))) return false;
   return (long long)B * C <= (1LL << 23);  // one workgroup of 256 threads per token at most
+}
+
+template <bool APPEND>
+void launch_vec(const RotaryParams& p, const VecShape& v, int dtype, hipStream_t s) {
+  const size_t smem = vec_lds(p, v, dtype_size(dtype), APPEND);
+  const dim3 grid((unsigned)(p.B * v.tiles), (unsigned)(v.slices + (APPEND ? p.Hkv : 0))), blk(kVecThreads);
+#define SPV_VEC(DT) hipLaunchKernelGGL((rotary_vec_kernel<DT, APPEND>), grid, blk, smem, s, p, v)
+  if (dtype == SPV_F32) SPV_VEC(SPV_F32);
+  else if (dtype == SPV_BF16) SPV_VEC(SPV_BF16);
+  else SPV_VEC(SPV_F16);
+#undef SPV_VEC
 }
 
 void set_strides(long long* dst, const int64_t* src) {
@@ -186,6 +462,12 @@ int spv_rotary(void* q_out, const void* q, void* k_out, const void* k, int dtype
   p.interleaved = interleaved;
   p.axes = axes;
   hipStream_t s = (hipStream_t)stream;
+  VecShape v;
+  if (k_out_dtype == dtype && vec_shape(p, dtype_size(dtype), false, v)) {
+    launch_vec<false>(p, v, dtype, s);
+    SPV_CHECK_LAUNCH();
+    return SPV_OK;
+  }
   const dim3 grid((unsigned)(B * C)), blk(256);
 #define SPV_ROT(DT, KO) hipLaunchKernelGGL((rotary_elem_kernel<DT, KO, false>), grid, blk, 0, s, p)
   if (dtype == SPV_F32) SPV_ROT(SPV_F32, SPV_F32);
@@ -262,6 +544,12 @@ int spv_kv_rotary_append(void* q_out, const void* q, const void* k_new, const vo
   p.cap = capacity;
   p.bs = block_size;
   hipStream_t s = (hipStream_t)stream;
+  VecShape v;
+  if (vec_shape(p, dtype_size(dtype), true, v)) {
+    launch_vec<true>(p, v, dtype, s);
+    SPV_CHECK_LAUNCH();
+    return SPV_OK;
+  }
   const dim3 grid((unsigned)(B * C)), blk(256);
 #define SPV_ROT(DT) hipLaunchKernelGGL((rotary_elem_kernel<DT, DT, true>), grid, blk, 0, s, p)
   if (dtype == SPV_F32) SPV_ROT(SPV_F32);

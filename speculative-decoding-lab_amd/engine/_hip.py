@@ -190,6 +190,12 @@ def i32(values, device: torch.device) -> torch.Tensor:
     return i32s(device, values)[0]
 
 
+def ids_ready(t, n: int, device: torch.device) -> bool:
+    """Whether ``t`` is already what ``i32`` would make of it: ``n`` int32 entries on ``device``."""
+    return (isinstance(t, torch.Tensor) and t.dtype is torch.int32 and t.numel() == n and t.device == device
+            and t.is_contiguous())
+
+
 PUT_INTS_MAX = 960  # SPV_PUT_INTS_MAX
 
 

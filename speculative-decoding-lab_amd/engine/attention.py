@@ -272,6 +272,8 @@ class SharedPrefix:
             if s >= 0 and n > 0 and n > kv._lens[kv._check_sid(s)]:
                 raise IndexError("prefix sequence {} holds {} positions, not {}".format(s, kv._lens[s], n))
         self.kv, self.B = kv, len(ids)
+        self.shape = (self.B, self.chunk, self.num_q_heads, kv.head_dim)
+        self.scale = 1.0 / math.sqrt(kv.head_dim)
         self.longest = max([n for s, n in zip(ids, lens) if s >= 0], default=0)
         self._host = self._dev = None
         if not self.B:
@@ -302,14 +304,14 @@ def shared_prefix_attention(query_3d: torch.Tensor, kv: PagedKVCache, layer: int
     positions that were never written raise ``IndexError`` at the next metadata
     query, as in ``verify_attention``.
     """
-    B, chunk, hq, d = query_3d.shape
-    if d != kv.head_dim or kv is not prefix.kv or (B, chunk, hq) != (prefix.B, prefix.chunk, prefix.num_q_heads):
+    if kv is not prefix.kv or query_3d.shape != prefix.shape:
         raise ValueError("the query does not match the cache and its shared prefixes")
     if query_3d.device != kv.device:
         raise ValueError("query must live on {}".format(kv.device))
-    if not 0 <= int(layer) < kv.num_layers:
+    if not 0 <= layer < kv.num_layers:
         raise IndexError("layer {} out of range".format(layer))
-    max_ctx = int(max_ctx)
+    layer, max_ctx = int(layer), int(max_ctx)
+    B, chunk, hq, d = prefix.shape
     if max_ctx < chunk:
         raise ValueError("max_ctx must be at least the chunk")
     q = query_3d.contiguous()
@@ -320,25 +322,27 @@ def shared_prefix_attention(query_3d: torch.Tensor, kv: PagedKVCache, layer: int
         raise ValueError("out must be a contiguous tensor like the query, apart from it")
     if B == 0:
         return out
-    if not isinstance(seq_ids, torch.Tensor):
-        seq_ids = [kv._check_sid(s) for s in seq_ids]
-    sid_t, start_t = _hip.i32s(kv.device, seq_ids, start_positions)
-    if sid_t.numel() != B or start_t.numel() != B:
-        raise ValueError("one seq_id and start position per batch row")
+    if _hip.ids_ready(seq_ids, B, kv.device) and _hip.ids_ready(start_positions, B, kv.device):
+        sid_t, start_t = seq_ids, start_positions
+    else:
+        if not isinstance(seq_ids, torch.Tensor):
+            seq_ids = [kv._check_sid(s) for s in seq_ids]
+        sid_t, start_t = _hip.i32s(kv.device, seq_ids, start_positions)
+        if sid_t.numel() != B or start_t.numel() != B:
+            raise ValueError("one seq_id and start position per batch row")
     longest = max(max_ctx, prefix.longest)
-    if longest > kv.max_blocks_per_seq * kv.block_size:
+    if longest > kv._maxb * kv.block_size:
         kv._grow_width(-(-longest // kv.block_size))
     if prefix._bytes[0] != max_ctx:
         prefix._bytes = (max_ctx, int(_hip.lib().spv_shared_attn_workspace_bytes(prefix._host, d, max_ctx)))
-    nbytes = prefix._bytes[1]
     # from the allocator in every call: ordered with its stream's work, and a
     # captured graph's own
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=kv.device)
-    scale = 1.0 / math.sqrt(d) if scale is None else float(scale)
-    call("spv_shared_attn", ptr(out), ptr(q), _hip.dtype_code(q.dtype), ptr(kv.k_pool), ptr(kv.v_pool), kv._dt,
-         ptr(kv.scales), ptr(kv.tables_dev), kv.max_blocks_per_seq, ptr(sid_t), ptr(start_t), ptr(kv.lens_dev),
-         ptr(kv.allocator.ctr), B, chunk, hq, kv.num_kv_heads, d, kv.block_size, int(layer), kv.allocator.capacity,
-         max_ctx, scale, prefix._host, ptr(prefix._dev), ptr(ws), nbytes, _hip.stream_of(kv.device))
+    ws = torch.empty(prefix._bytes[1], dtype=torch.uint8, device=kv.device)
+    call("spv_shared_attn", out.data_ptr(), q.data_ptr(), _hip.dtype_code(q.dtype), kv.k_pool.data_ptr(),
+         kv.v_pool.data_ptr(), kv._dt, ptr(kv.scales), kv.tables_dev.data_ptr(), kv._maxb, sid_t.data_ptr(),
+         start_t.data_ptr(), kv.lens_dev.data_ptr(), kv.allocator.ctr.data_ptr(), B, chunk, hq, kv.num_kv_heads, d,
+         kv.block_size, layer, kv.allocator.capacity, max_ctx, prefix.scale if scale is None else float(scale),
+         prefix._host, prefix._dev.data_ptr(), ws.data_ptr(), prefix._bytes[1], _hip.stream_of(kv.device))
     kv._stale = True
     return out
 

@@ -72,11 +72,15 @@ class Rotary:
         if len(axis_of) != n or any(a < 0 for a in axis_of):
             raise ValueError("every one of the rotary_dim / 2 = {} frequencies needs its axis".format(n))
         self.device = _hip.require_gpu(device)
-        self.interleaved = bool(interleaved)
+        self.interleaved = int(bool(interleaved))
         self.factor = float(factor)
         self.inv_freq = torch.tensor(inv_freq, dtype=torch.float64, device=self.device)
         self.axis_of = torch.tensor(axis_of, dtype=torch.int32, device=self.device)
         self._args = (ptr(self.inv_freq) if n else None, ptr(self.axis_of) if n else None, self.axes, self.factor)
+        # argument shapes, strides and types that passed the checks, with the launch's
+        # share of them: a serving loop repeats a few, and the checks cost as much
+        # host time as the launch
+        self._passed: dict = {}
 
     def _positions(self, positions: torch.Tensor, B: int, C: int) -> torch.Tensor:
         """int32 ``(axes, B, C)``; ``(B, C)`` stands for every axis."""
@@ -84,6 +88,8 @@ class Rotary:
             raise ValueError("positions must be an integer tensor")
         if positions.device != self.device:
             raise ValueError("positions must live on {}".format(self.device))
+        if positions.dtype is torch.int32 and positions.shape == (self.axes, B, C) and positions.is_contiguous():
+            return positions
         if positions.dim() == 2 and self.axes > 1:
             positions = positions.expand(self.axes, -1, -1)
         want = (B, C) if positions.dim() == 2 else (self.axes, B, C)
@@ -144,6 +150,17 @@ def _strides(*tensors: Optional[torch.Tensor]) -> ctypes.Array:
     return _Strides(*out)
 
 
+def _remember(rotary: Rotary, key, value):
+    if len(rotary._passed) >= 256:
+        rotary._passed.clear()
+    rotary._passed[key] = value
+    return value
+
+
+def _like(t: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
+    return torch.empty_like(t, dtype=dtype, memory_format=torch.contiguous_format)
+
+
 def rotary_embed(query: torch.Tensor, key: Optional[torch.Tensor], rotary: Rotary, positions: torch.Tensor,
                  query_out: Optional[torch.Tensor] = None, key_out: Optional[torch.Tensor] = None,
                  key_dtype: Optional[torch.dtype] = None) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
@@ -155,9 +172,40 @@ def rotary_embed(query: torch.Tensor, key: Optional[torch.Tensor], rotary: Rotar
     is the input itself (in place) or overlaps no input. ``key_dtype``
     float32 keeps the rotated keys unrounded.
     """
+    plain = query_out is None and key_out is None and key is not None
+    sig = (query.shape, query.stride(), query.dtype, query.device, key.shape, key.stride(), key.dtype, key.device,
+           key_dtype) if plain else None
+    done = rotary._passed.get(sig) if plain else None
+    if done is None:
+        done = _check_embed(query, key, rotary, query_out, key_out, key_dtype)
+        if plain and done[0]:
+            _remember(rotary, sig, done)
+    rows, B, C, hq, hkv, d, code, key_code, key_dtype, strides = done
+    pos = rotary._positions(positions, B, C)
+    if not rows:  # a copy where head rows are not contiguous
+        query, key = _rows(query), None if key is None else _rows(key)
+    if query_out is None:
+        query_out = _like(query, query.dtype)
+    if key is not None and key_out is None:
+        key_out = _like(key, key_dtype)
+    if B == 0 or C == 0:
+        return query_out, key_out
+    if strides is None:
+        strides = _strides(query_out, query, key_out, key)
+    call("spv_rotary", query_out.data_ptr(), query.data_ptr(), ptr(key_out), ptr(key), code, key_code, strides,
+         pos.data_ptr(), *rotary._args, B, C, hq, hkv, d, rotary.rotary_dim, rotary.interleaved,
+         _hip.stream_of(rotary.device))
+    return query_out, key_out
+
+
+def _dense(shape) -> Tuple[int, int, int]:
+    return shape[1] * shape[2] * shape[3], shape[2] * shape[3], shape[3]
+
+
+def _check_embed(query, key, rotary, query_out, key_out, key_dtype):
     if query.dim() != 4 or query.dtype not in _FLOATS:
         raise ValueError("query must be (B, C, heads, d) in float32, bfloat16 or float16")
-    B, C, hq, d = query.shape
+    B, C, hq, d = (int(n) for n in query.shape)
     if d != rotary.head_dim:
         raise ValueError("the rows have {} elements, the rotary frequencies are for {}".format(d, rotary.head_dim))
     if key is not None and (key.dim() != 4 or tuple(key.shape[:2]) != (B, C) or key.shape[3] != d
@@ -170,7 +218,6 @@ def rotary_embed(query: torch.Tensor, key: Optional[torch.Tensor], rotary: Rotar
         key_dtype = query.dtype
     if key_dtype not in (query.dtype, torch.float32):
         raise ValueError("key_dtype must be the query's dtype or float32")
-    pos = rotary._positions(positions, B, C)
     if query_out is not None:
         _check_out(query_out, query, () if key is None else (key,), query.dtype)
     if key_out is not None:
@@ -179,18 +226,12 @@ def rotary_embed(query: torch.Tensor, key: Optional[torch.Tensor], rotary: Rotar
         _check_out(key_out, key, (query,), key_dtype)
         if query_out is not None and not _apart(query_out, key_out):
             raise ValueError("the outputs overlap")
-    q, k = _rows(query), None if key is None else _rows(key)
-    if query_out is None:
-        query_out = torch.empty((B, C, hq, d), dtype=q.dtype, device=q.device)
-    if key is not None and key_out is None:
-        key_out = torch.empty(key.shape, dtype=key_dtype, device=q.device)
-    if B == 0 or C == 0:
-        return query_out, key_out
-    call("spv_rotary", ptr(query_out), ptr(q), ptr(key_out), ptr(k), _hip.dtype_code(q.dtype),
-         _hip.dtype_code(key_dtype), _strides(query_out, q, key_out, k), ptr(pos), *rotary._args, B, C, hq,
-         0 if k is None else int(k.shape[2]), d, rotary.rotary_dim, int(rotary.interleaved),
-         _hip.stream_of(rotary.device))
-    return query_out, key_out
+    rows = _rows(query) is query and (key is None or _rows(key) is key)
+    strides = None
+    if rows and query_out is None and key_out is None and key is not None:
+        strides = _Strides(*_dense(query.shape), *query.stride()[:3], *_dense(key.shape), *key.stride()[:3])
+    return (rows, B, C, hq, 0 if key is None else int(key.shape[2]), d, _hip.dtype_code(query.dtype),
+            _hip.dtype_code(key_dtype), key_dtype, strides)
 
 
 def rotary_append(query: Optional[torch.Tensor], k_new: torch.Tensor, v_new: torch.Tensor, kv: PagedKVCache,
@@ -210,6 +251,65 @@ def rotary_append(query: Optional[torch.Tensor], k_new: torch.Tensor, v_new: tor
     device tensors of distinct, added ``seq_ids``. A later layer's call of a
     round passes ``alloc=False`` and the first one's ``plan``.
     """
+    plain = query is not None and query_out is None
+    sig = (kv._dt, kv.num_kv_heads, kv.head_dim, kv.device, query.shape, query.stride(), query.dtype, query.device, k_new.shape,
+           k_new.stride(), k_new.dtype, k_new.device, v_new.shape, v_new.stride(), v_new.dtype,
+           v_new.device) if plain else None
+    done = rotary._passed.get(sig) if plain else None
+    if done is None:
+        done = _check_append(query, k_new, v_new, kv, rotary, query_out)
+        if plain and done[0]:
+            _remember(rotary, sig, done)
+    rows_ok, B, C, hq, strides = done
+    layer = int(layer)
+    if not 0 <= layer < kv.num_layers:
+        raise IndexError("layer {} out of range".format(layer))
+    if positions is not None:
+        pos = rotary._positions(positions, B, C)
+    elif rotary.axes > 1:
+        raise ValueError("a Rotary of several axes needs positions")
+    else:
+        pos = None
+    if _hip.ids_ready(seq_ids, B, kv.device) and _hip.ids_ready(start_positions, B, kv.device):
+        sid_t, start_t = seq_ids, start_positions
+    else:
+        sid_t, start_t = _append_ids(kv, seq_ids, start_positions, B, C)
+    q, k, v = query, k_new, v_new
+    if not rows_ok:
+        q, k, v = None if q is None else _rows(q), _rows(k), _rows(v)
+    if q is not None and query_out is None:
+        query_out = _like(q, q.dtype)
+    if B == 0 or C == 0:
+        return query_out
+    if kv.fp8:
+        if pos is None:
+            pos = start_t[:, None] + torch.arange(C, dtype=torch.int32, device=kv.device)
+        _append_fp8(q, k, v, kv, layer, sid_t, start_t, rotary, pos, alloc, query_out)
+        return query_out
+    a = kv.allocator
+    rows, follow = None, 0
+    if plan is not None and a.capacity * kv.block_size < 2 ** 31:
+        if alloc:
+            plan._reserve(B, C, kv.device)
+            rows = plan.rows
+        elif plan.ready:
+            plan._check(a.epoch, B, C, sid_t, start_t)
+            rows, follow = plan.rows, 1
+    call("spv_kv_rotary_append", ptr(query_out), ptr(q), k.data_ptr(), v.data_ptr(), kv._dt,
+         _strides(query_out, q, k, v) if strides is None else strides, kv.k_pool.data_ptr(), kv.v_pool.data_ptr(),
+         kv.tables_dev.data_ptr(), kv._maxb, kv.nblocks_dev.data_ptr(), kv.lens_dev.data_ptr(),
+         a.free_stack.data_ptr(), a.free_flag.data_ptr(), a.ctr.data_ptr(), sid_t.data_ptr(), start_t.data_ptr(),
+         ptr(pos), *rotary._args, B, C, hq, kv.num_kv_heads, kv.head_dim, rotary.rotary_dim, rotary.interleaved, layer,
+         a.capacity, kv.block_size, bool(alloc), follow, ptr(rows), _hip.stream_of(kv.device))
+    if not follow:
+        if rows is not None:
+            plan._record(a.epoch, sid_t, start_t)
+        kv._stale = True
+        a._stale = True
+    return query_out
+
+
+def _check_append(query, k_new, v_new, kv, rotary, query_out):
     if k_new.dim() != 4:
         raise ValueError("k/v must have shape (B, chunk, {}, {})".format(kv.num_kv_heads, kv.head_dim))
     B, C = int(k_new.shape[0]), int(k_new.shape[1])
@@ -230,16 +330,21 @@ def rotary_append(query: Optional[torch.Tensor], k_new: torch.Tensor, v_new: tor
             raise ValueError("query, keys and values must live on {}".format(kv.device))
     if query is not None and (query.dim() != 4 or tuple(query.shape[:2]) != (B, C) or query.shape[3] != d):
         raise ValueError("query must be ({}, {}, heads, {})".format(B, C, d))
-    if not 0 <= int(layer) < kv.num_layers:
-        raise IndexError("layer {} out of range".format(layer))
-    if positions is None and rotary.axes > 1:
-        raise ValueError("a Rotary of several axes needs positions")
     if query_out is not None:
         if query is None:
             raise ValueError("query_out without a query")
         _check_out(query_out, query, (k_new, v_new), dtype)
+    rows = all(_rows(t) is t for t in tensors)
+    strides = None
+    if rows and query is not None and query_out is None:
+        strides = _Strides(*_dense(query.shape), *query.stride()[:3], *k_new.stride()[:3], *v_new.stride()[:3])
+    return rows, B, C, 0 if query is None else int(query.shape[2]), strides
+
+
+def _append_ids(kv, seq_ids, start_positions, B, C):
+    """Sequence ids and start positions on the device; lists are checked as in ``write_block``."""
     given = [not isinstance(t, torch.Tensor) for t in (seq_ids, start_positions)]
-    if any(given):  # lists: checked here, as in write_block
+    if any(given):
         kv._refresh()
         if given[0]:
             seq_ids = [kv._check_sid(s) for s in seq_ids]
@@ -254,38 +359,7 @@ def rotary_append(query: Optional[torch.Tensor], k_new: torch.Tensor, v_new: tor
     sid_t, start_t = _hip.i32s(kv.device, seq_ids, start_positions)
     if sid_t.numel() != B or start_t.numel() != B:
         raise ValueError("one seq_id and start position per batch row")
-    pos = None if positions is None else rotary._positions(positions, B, C)
-    q, k, v = None if query is None else _rows(query), _rows(k_new), _rows(v_new)
-    if q is not None and query_out is None:
-        query_out = torch.empty(q.shape, dtype=dtype, device=q.device)
-    if B == 0 or C == 0:
-        return query_out
-    if kv.fp8:
-        if pos is None:
-            pos = start_t[:, None] + torch.arange(C, dtype=torch.int32, device=kv.device)
-        _append_fp8(q, k, v, kv, int(layer), sid_t, start_t, rotary, pos, alloc, query_out)
-        return query_out
-    a = kv.allocator
-    rows, follow = None, 0
-    if plan is not None and a.capacity * kv.block_size < 2 ** 31:
-        if alloc:
-            plan._reserve(B, C, kv.device)
-            rows = plan.rows
-        elif plan.ready:
-            plan._check(a.epoch, B, C, sid_t, start_t)
-            rows, follow = plan.rows, 1
-    call("spv_kv_rotary_append", ptr(query_out), ptr(q), ptr(k), ptr(v), kv._dt, _strides(query_out, q, k, v),
-         ptr(kv.k_pool), ptr(kv.v_pool), ptr(kv.tables_dev), kv.max_blocks_per_seq, ptr(kv.nblocks_dev),
-         ptr(kv.lens_dev), ptr(a.free_stack), ptr(a.free_flag), ptr(a.ctr), ptr(sid_t), ptr(start_t), ptr(pos),
-         *rotary._args, B, C, 0 if q is None else int(q.shape[2]), kv.num_kv_heads, d, rotary.rotary_dim,
-         int(rotary.interleaved), int(layer), a.capacity, kv.block_size, int(bool(alloc)), follow, ptr(rows),
-         _hip.stream_of(kv.device))
-    if rows is not None and not follow:
-        plan._record(a.epoch, sid_t, start_t)
-    if not follow:
-        kv._stale = True
-        a._stale = True
-    return query_out
+    return sid_t, start_t
 
 
 def _append_fp8(q, k, v, kv, layer, sid_t, start_t, rotary, pos, alloc, query_out) -> None:
@@ -294,5 +368,5 @@ def _append_fp8(q, k, v, kv, layer, sid_t, start_t, rotary, pos, alloc, query_ou
     call("spv_rotary", ptr(query_out), ptr(q), ptr(k32), ptr(k), _hip.dtype_code(k.dtype), _hip.SPV_F32,
          _strides(query_out, q, k32, k), ptr(pos), *rotary._args, k.shape[0], k.shape[1],
          0 if q is None else int(q.shape[2]), kv.num_kv_heads, kv.head_dim, rotary.rotary_dim,
-         int(rotary.interleaved), _hip.stream_of(kv.device))
+         rotary.interleaved, _hip.stream_of(kv.device))
     kv.write_block_device(layer, sid_t, start_t, k32, v.float(), alloc=alloc)

@@ -163,7 +163,7 @@ def test_rotary_arguments(kw):
 
 def test_embed_refuses_what_it_cannot_take():
     r = object.__new__(Rotary)
-    r.head_dim, r.device, r.axes, r.rotary_dim = 64, torch.device("cpu"), 1, 64
+    r.head_dim, r.device, r.axes, r.rotary_dim, r._passed = 64, torch.device("cpu"), 1, 64, {}
     q, k, pos = torch.zeros(2, 3, 4, 64), torch.zeros(2, 3, 2, 64), torch.zeros(2, 3, dtype=torch.int32)
     for args in ((q[0], k, r, pos), (q.double(), k.double(), r, pos), (q, k[:1], r, pos), (q, k.half(), r, pos),
                  (q[..., :32], None, r, pos), (q, k, r, pos.float()), (q, k, r, pos[:1]), (q, k, r, pos[None, :1])):
