@@ -50,9 +50,10 @@ namespace {
 
 constexpr float kLog2e = 1.4426950408889634f;
 
-// The plan: a header, then the groups, their members (batch entries), each
-// entry's place, the shares (first segment of each, and the end), the segments,
-// and per (group, kv head, tile) its segments.
+// The plan: a header, then the shares, the segments, the members of the groups
+// (batch entries), each entry's place, and per (group, kv head, tile) its segments.
+// A share repeats its first segment, so that a workgroup's first keys are two
+// loads away from its launch.
 enum : int {
   PH_MAGIC = 0,
   PH_INTS,  // length of the plan
@@ -61,26 +62,26 @@ enum : int {
   PH_HQ,
   PH_HKV,
   PH_BS,
-  PH_NG,    // groups
   PH_NSH,   // shares (a multiple of 8, or 0)
   PH_NSEG,  // segments
-  PH_NT,    // (group, kv head, tile) triples
   PH_MAXP,  // longest prefix
-  PH_GROUPS,
-  PH_MEMBERS,
-  PH_ENTRIES,
   PH_SHARES,
   PH_SEGS,
+  PH_MEMBERS,
+  PH_ENTRIES,
   PH_TILES,
   PH_WORDS
 };
-constexpr int kPlanMagic = 0x53505232;
-enum : int { G_SID = 0, G_LEN, G_FIRST, G_COUNT, G_NT, G_TILE0, G_WORDS };  // G_NT: tiles of a kv head
-enum : int { E_GROUP = 0, E_RANK, E_WORDS };
-enum : int { S_GROUP = 0, S_HEAD, S_TILE, S_KEY0, S_KEY1, S_WORDS };
+constexpr int kPlanMagic = 0x53505233;
+// A segment: sequence and length of the prefix, kv head, first member and first row
+// of the tile, its rows, the keys.
+enum : int { S_SID = 0, S_LEN, S_HEAD, S_FIRST, S_ROW0, S_ROWS, S_KEY0, S_KEY1, S_WORDS };
+enum : int { H_SEG = 0, H_END, H_COPY, H_WORDS = 16 };           // a share's segments; the first one's record
+enum : int { E_TILE0 = 0, E_NT, E_RANK, E_WORDS = 4 };            // first tile of kv head 0 (-1: no prefix), tiles per kv head
 enum : int { T_SEG = 0, T_COUNT, T_WORDS };
-constexpr int kTile = 128;  // rows
-constexpr int kUnit = 64;   // keys
+constexpr int kTile = 256;    // rows of a prefix tile
+constexpr int kUnit = 64;     // keys
+constexpr int kOwnRows = 64;  // rows of an entry that a workgroup takes over its own keys
 
 struct SharedParams {
   void* out;
@@ -93,12 +94,17 @@ struct SharedParams {
   const int32_t* start;
   const int32_t* lens;
   int32_t* ctr;
-  const int32_t* plan;
+  const int32_t* share_list;  // the plan's sections
+  const int32_t* segs;
+  const int32_t* members;
+  const int32_t* entries;
+  const int32_t* tiles;
   float* part_o;   // partial rows x d
   float* part_ml;  // partial rows x 2
   int maxb, B, C, Hq, Hkv, ratio, G, d, bs, layer, cap;
   int shares;              // workgroups that walk prefixes
-  int own_range, own_max;  // keys per own range (a multiple of the block size), ranges per entry at most
+  int own;                 // workgroups that walk entries' own keys
+  int own_range, own_max;  // keys per own range (whole blocks), ranges per entry at most
   int own_tiles;           // tiles of an entry's rows
   int max_ctx;
   long long own_part;      // first partial row of the own ranges
@@ -108,64 +114,62 @@ struct SharedParams {
 // One piece of work: rows [row0, row0 + rows) of a group's (or one entry's) row
 // order over keys [key0, key1) of one sequence.
 struct Item {
-  int group, sid, b, h, row0, rows, key0, key1, first, limit;  // limit: row j sees keys <= limit + j (an entry's own)
-  long long part;                                                // its first partial row
+  int first;  // the group's first member, or -1: an entry's own keys
+  int sid, b, h, row0, rows, key0, key1;
+  int start;       // own keys: row j sees keys <= start + j
+  long long part;  // its first partial row
 };
 
 __device__ __forceinline__ void flag_bad_read(const SharedParams& p, int b) {
   if (p.ctr) p.ctr[CTR_BAD_READ] = b + 1;
 }
 
-__device__ __forceinline__ void segment_item(const SharedParams& p, int seg, Item& it) {
-  const int32_t* s = p.plan + p.plan[PH_SEGS] + (size_t)seg * S_WORDS;
-  const int32_t* g = p.plan + p.plan[PH_GROUPS] + (size_t)s[S_GROUP] * G_WORDS;
-  it.group = s[S_GROUP];
-  it.sid = g[G_SID];
+__device__ __forceinline__ void segment_item(const SharedParams& p, const int32_t* s, int seg, Item& it) {
+  it.first = s[S_FIRST];
+  it.sid = s[S_SID];
   it.h = s[S_HEAD];
-  it.first = p.plan[PH_MEMBERS] + g[G_FIRST];
-  it.b = p.plan[it.first];
-  it.row0 = s[S_TILE] * kTile;
-  it.rows = min(kTile, g[G_COUNT] * p.G - it.row0);
+  it.row0 = s[S_ROW0];
+  it.rows = s[S_ROWS];
   it.key0 = s[S_KEY0];
   it.key1 = s[S_KEY1];
-  it.limit = 0x3fffffff;
+  it.start = 0x3fffffff;
+  it.b = 0;
   it.part = (long long)seg * kTile;
-  if (threadIdx.x == 0 && p.lens && p.lens[it.sid] < g[G_LEN]) flag_bad_read(p, it.b);
+  if (threadIdx.x == 0 && p.lens && p.lens[it.sid] < s[S_LEN]) flag_bad_read(p, p.members[it.first]);
 }
 
 // Own work `o`: false where the range has no keys.
 __device__ __forceinline__ bool own_item(const SharedParams& p, int o, Item& it) {
   const int s = o % p.own_max, bht = o / p.own_max, t = bht % p.own_tiles, bh = bht / p.own_tiles;
-  it.group = -1;
+  it.first = -1;
   it.b = bh / p.Hkv;
   it.h = bh - it.b * p.Hkv;
   it.sid = p.seq_ids[it.b];
-  it.limit = p.start[it.b];
-  const int L = it.limit + p.C, seen = min(max(L, 0), p.max_ctx);
-  if (threadIdx.x == 0 && s == 0 && it.h == 0 && (it.limit < 0 || L > p.max_ctx || (p.lens && p.lens[it.sid] < L)))
+  it.start = p.start[it.b];
+  const int L = it.start + p.C, seen = min(max(L, 0), p.max_ctx);
+  if (threadIdx.x == 0 && s == 0 && it.h == 0 && (it.start < 0 || L > p.max_ctx || (p.lens && p.lens[it.sid] < L)))
     flag_bad_read(p, it.b);
-  it.row0 = t * kTile;
-  it.rows = min(kTile, p.G - it.row0);
-  it.first = 0;
+  it.row0 = t * kOwnRows;
+  it.rows = min(kOwnRows, p.G - it.row0);
   it.key0 = s * p.own_range;
   it.key1 = min(it.key0 + p.own_range, seen);
   it.part = p.own_part + ((long long)bh * p.own_max + s) * p.G + it.row0;
   return it.key0 < it.key1;
 }
 
-// The share of workgroup `id`: workgroups go round-robin over the 8 XCDs, each of
-// which takes an eighth of the shares in a row -- of one kv head, if there are few --
-// so that its L2 serves one stretch of keys to all of its workgroups.
+// The share of the prefix workgroup `id`: workgroups go round-robin over the 8
+// XCDs, each of which takes an eighth of the shares in a row -- of one kv head, if
+// there are few -- so that its L2 serves one stretch of keys to all of them.
 __device__ __forceinline__ int share_of(const SharedParams& p, int id) { return (id & 7) * (p.shares >> 3) + (id >> 3); }
 
 // Row R of an item's row order: its entry, chunk token and q head.
 __device__ __forceinline__ void row_at(const SharedParams& p, const Item& it, int R, int& b, int& j, int& hq) {
   int r = R;
   b = it.b;
-  if (it.group >= 0) {
+  if (it.first >= 0) {
     const int m = R / p.G;
     r = R - m * p.G;
-    b = p.plan[it.first + m];
+    b = p.members[it.first + m];
   }
   j = r / p.ratio;
   hq = it.h * p.ratio + (r - j * p.ratio);
@@ -174,7 +178,7 @@ __device__ __forceinline__ void row_at(const SharedParams& p, const Item& it, in
 __device__ __forceinline__ int block_of(const SharedParams& p, const Item& it, int pos) {
   const int phys = p.tables[(size_t)it.sid * p.maxb + pos / p.bs];
   if ((unsigned)phys < (unsigned)p.cap) return phys;
-  flag_bad_read(p, it.b);
+  flag_bad_read(p, it.first >= 0 ? p.members[it.first] : it.b);
   return 0;
 }
 
@@ -191,8 +195,8 @@ __host__ __device__ constexpr size_t valu_lds(int d) {
   return (size_t)((kRows + 2 * kKeys) * (d + 1) + kRows * (kKeys + 1) + 2 * kRows) * sizeof(float);
 }
 
-// MD: a bound on head_dim.
-template <int QT, int KT, int MD>
+// MD: a bound on head_dim; TH: threads of the workgroup (at least 256).
+template <int QT, int KT, int MD, int TH>
 __device__ __forceinline__ void valu_item(const SharedParams& p, const Item& it, float* smem) {
   const int d = p.d, pitch = d + 1;
   float* Qs = smem;                    // [64][d], in log2 units
@@ -206,12 +210,12 @@ __device__ __forceinline__ void valu_item(const SharedParams& p, const Item& it,
   for (int r0 = 0; r0 < it.rows; r0 += kRows) {
     const int nr = min(kRows, it.rows - r0);
 #pragma unroll 1
-    for (int i = threadIdx.x; i < nr * d; i += kThreads) {
+    for (int i = threadIdx.x; i < nr * d; i += TH) {
       const int rr = i / d, e = i - rr * d;
       int b, j, hq;
       row_at(p, it, it.row0 + r0 + rr, b, j, hq);
       Qs[rr * pitch + e] = load_elem<QT>(p.q, (((size_t)b * p.C + j) * p.Hq + hq) * d + e) * p.scale_log2;
-      if (e == 0) Lim[rr] = it.group >= 0 ? it.limit : it.limit + j;
+      if (e == 0) Lim[rr] = it.first >= 0 ? it.start : it.start + j;
     }
     float m = -INFINITY, l = 0.f;  // of row threadIdx.x, kept by the first 64 threads
     float o[MD / 4];               // dims part, part + 4, ... of row `row`
@@ -222,7 +226,7 @@ __device__ __forceinline__ void valu_item(const SharedParams& p, const Item& it,
     for (int t0 = it.key0; t0 < it.key1; t0 += kKeys) {
       const int nt = min(kKeys, it.key1 - t0);
 #pragma unroll 1
-      for (int i = threadIdx.x; i < nt * d; i += kThreads) {
+      for (int i = threadIdx.x; i < nt * d; i += TH) {
         const int tt = i / d, e = i - tt * d;
         const int pos = t0 + tt, phys = block_of(p, it, pos), off = pos % p.bs;
         const size_t slot = ((size_t)p.layer * p.cap + phys) * p.Hkv + it.h;
@@ -238,7 +242,7 @@ __device__ __forceinline__ void valu_item(const SharedParams& p, const Item& it,
       }
       __syncthreads();
 #pragma unroll 1
-      for (int i = threadIdx.x; i < nr * kKeys; i += kThreads) {
+      for (int i = threadIdx.x; i < nr * kKeys; i += TH) {
         const int rr = i / kKeys, tt = i - rr * kKeys;
         float sc = -INFINITY;
         if (tt < nt && t0 + tt <= Lim[rr]) {
@@ -292,35 +296,37 @@ __device__ __forceinline__ void valu_item(const SharedParams& p, const Item& it,
   }
 }
 
-// Workgroups [0, shares) walk prefixes, the others entries' own keys.
+// Workgroups [0, own) walk entries' own keys, the others prefixes.
 template <typename F>
-__device__ __forceinline__ void for_items(const SharedParams& p, F&& run) {
-  const int id = blockIdx.x;
-  int s = 0, end = 1;
-  if (id < p.shares) {
-    const int32_t* sh = p.plan + p.plan[PH_SHARES] + share_of(p, id);
-    s = sh[0];
-    end = sh[1];
-  }
+__device__ __forceinline__ void for_segments(const SharedParams& p, F&& run) {
+  const int32_t* sh = p.share_list + (size_t)share_of(p, (int)blockIdx.x - p.own) * H_WORDS;
+  const int32_t* rec = sh + H_COPY;
+  const int end = sh[H_END];
 #pragma unroll 1
-  for (; s < end; ++s) {
+  for (int s = sh[H_SEG]; s < end; ++s) {
     Item it;
-    if (id < p.shares) segment_item(p, s, it);
-    else if (!own_item(p, id - p.shares, it)) return;
+    segment_item(p, rec, s, it);
     run(it);
+    rec = p.segs + (size_t)(s + 1) * S_WORDS;
   }
 }
 
 template <int QT, int KT>
 __global__ __launch_bounds__(kThreads) void shared_valu_kernel(SharedParams p) {
   extern __shared__ float smem[];
-  for_items(p, [&](const Item& it) { valu_item<QT, KT, kMaxD>(p, it, smem); });
+  if ((int)blockIdx.x < p.own) {
+    Item it;
+    if (own_item(p, blockIdx.x, it)) valu_item<QT, KT, kMaxD, kThreads>(p, it, smem);
+    return;
+  }
+  for_segments(p, [&](const Item& it) { valu_item<QT, KT, kMaxD, kThreads>(p, it, smem); });
 }
 
 // -------------------------------------------------------------- matrix kernels
 typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x4_t __attribute__((ext_vector_type(4)));
 typedef _Float16 f16x2_t __attribute__((ext_vector_type(2)));
 typedef unsigned short u16x2_t __attribute__((ext_vector_type(2)));
 typedef float f32x4_t __attribute__((ext_vector_type(4)));
@@ -352,115 +358,147 @@ __device__ __forceinline__ int stage_exponent(float mx) {
   return min(126, max(-126, 9 - e));
 }
 
-template <int D, int KT>
+constexpr int kWaves = 8;
+constexpr int kMfmaThreads = 64 * kWaves;
+
+template <int D>
 struct Lds {
   // 32 bytes of padding on a K row and a V^T row: their 16-byte reads meet no bank twice.
   static constexpr int KP = D + 16, VP = kUnit + 16;
-  static constexpr int kK = kUnit * KP, kV = D * VP;              // elements of a buffer
-  static constexpr size_t kBytes = 2 * (size_t)(kK + kV) * 2 + 64;  // two of each, and a word per wave
+  static constexpr int kK = kUnit * KP, kV = D * VP;  // elements of a slot
+  static constexpr size_t kWalk = 2 * (size_t)(2 * kK + 3 * kV);
+  static constexpr size_t kJoin = 4 * 64 * (size_t)(D / 16 * 2) * 16 + kWaves * 32 * 8;  // own keys: the waves' sums
+  static constexpr size_t kBytes = (kWalk > kJoin ? kWalk : kJoin) + 4 * kWaves;
 };
 
+// What both walks know of the call and the lane.
 template <int D, int KT>
-__global__ __launch_bounds__(kThreads, 2) void shared_mfma_kernel(SharedParams p) {
-  constexpr bool kF16 = KT == SPV_F16, kFp8 = KT == SPV_FP8E4M3;
-  constexpr int QT = kF16 ? SPV_F16 : SPV_BF16;
-  constexpr int ES = kFp8 ? 1 : 2;
-  constexpr int KS = D / 32, MT = D / 16, NT = 2;
-  using LD = Lds<D, KT>;
-  constexpr int KP = LD::KP, VP = LD::VP;
-  static_assert(valu_lds(D) <= LD::kBytes, "the any-shape walk reuses this memory");
-  __shared__ __align__(16) uint8_t smem[LD::kBytes];
-  uint16_t* const sK = reinterpret_cast<uint16_t*>(smem);
-  uint16_t* const sV = sK + 2 * LD::kK;
-  uint32_t* const sMax = reinterpret_cast<uint32_t*>(sV + 2 * LD::kV);
+struct Walk {
+  static constexpr bool kF16 = KT == SPV_F16, kFp8 = KT == SPV_FP8E4M3;
+  static constexpr int QT = kF16 ? SPV_F16 : SPV_BF16;
+  static constexpr int ES = kFp8 ? 1 : 2;
+  static constexpr int KS = D / 32, MT = D / 16, NT = 2;
+  const SharedParams& p;
+  uint8_t* const smem;
+  uint32_t* const sMax;
+  const int tid, lane, w, i16, g;
+  const float sl2, inv_sl2;
 
-  const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int i16 = lane & 15, g = lane >> 4;
-  const float sl2 = p.scale_log2, inv_sl2 = 1.f / p.scale_log2;
-  const f16x2_t ones = f16x2_t{(_Float16)1.f, (_Float16)1.f};
+  __device__ __forceinline__ Walk(const SharedParams& p_, uint8_t* smem_)
+      : p(p_), smem(smem_), sMax(reinterpret_cast<uint32_t*>(smem_ + Lds<D>::kBytes) - kWaves), tid(threadIdx.x),
+        lane(threadIdx.x & 63), w(__builtin_amdgcn_readfirstlane(threadIdx.x >> 6)), i16(threadIdx.x & 15),
+        g((threadIdx.x & 63) >> 4), sl2(p_.scale_log2), inv_sl2(1.f / p_.scale_log2) {}
 
-  auto wg_max = [&](uint32_t m) {  // the workgroup's largest m, in every thread
+  // The query fragments of the lane's rows r0 + 16 nt + i16 of an item: B operands, 8
+  // dims from 32 ks + 8 g on.
+  __device__ __forceinline__ void load_q(const Item& it, int r0, uint4 (&qf)[NT][KS], int (&lim)[NT], bool (&valid)[NT]) {
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      const int R = r0 + nt * 16 + i16;
+      valid[nt] = R < it.rows;
+      int b, j, hq;
+      row_at(p, it, it.row0 + min(R, it.rows - 1), b, j, hq);
+      lim[nt] = it.first >= 0 ? it.start : it.start + j;
+      const uint16_t* q = static_cast<const uint16_t*>(p.q) + (((size_t)b * p.C + j) * p.Hq + hq) * D + 8 * g;
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) qf[nt][ks] = *reinterpret_cast<const uint4*>(q + 32 * ks);
+    }
+  }
+  __device__ __forceinline__ f32x4_t mfma_qk(uint4 k, uint4 q, f32x4_t c) const {
+    if constexpr (kF16)
+      return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8_t, k), __builtin_bit_cast(f16x8_t, q), c, 0, 0, 0);
+    else
+      return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, k), __builtin_bit_cast(bf16x8_t, q), c, 0, 0, 0);
+  }
+  __device__ __forceinline__ int safe_id(const Item& it, int phys) const {
+    if ((unsigned)phys < (unsigned)p.cap) return phys;
+    flag_bad_read(p, it.first >= 0 ? p.members[it.first] : it.b);
+    return 0;
+  }
+  __device__ __forceinline__ float2 scales_of(int phys) const {
+    return *reinterpret_cast<const float2*>(p.scales + ((size_t)p.layer * p.cap + phys) * 2);
+  }
+  __device__ __forceinline__ const uint8_t* page(const void* pool, int phys, int h) const {
+    return static_cast<const uint8_t*>(pool) + (((size_t)p.layer * p.cap + phys) * p.Hkv + h) * (size_t)(16 * D * ES);
+  }
+  __device__ __forceinline__ uint32_t wg_max(uint32_t m) {  // the workgroup's largest m, in every thread
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) m = max(m, (uint32_t)__shfl_xor((int)m, o, 64));
     __syncthreads();
     if (lane == 0) sMax[w] = m;
     __syncthreads();
-    return max(max(sMax[0], sMax[1]), max(sMax[2], sMax[3]));
-  };
+    m = sMax[0];
+#pragma unroll
+    for (int k = 1; k < kWaves; ++k) m = max(m, sMax[k]);
+    return m;
+  }
 
-  for_items(p, [&](const Item& it) {
-    // This lane's rows (columns of S^T): 16 nt + i16 of the wave's 32.
-    int lim[NT];
-    bool valid[NT];
-    uint4 qf[NT][KS];
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-      const int R = w * 32 + nt * 16 + i16;
-      valid[nt] = R < it.rows;
-      int b, j, hq;
-      row_at(p, it, it.row0 + min(R, it.rows - 1), b, j, hq);
-      lim[nt] = it.group >= 0 ? it.limit : it.limit + j;
-      const uint16_t* q = static_cast<const uint16_t*>(p.q) + (((size_t)b * p.C + j) * p.Hq + hq) * D + 8 * g;
-#pragma unroll
-      for (int ks = 0; ks < KS; ++ks) qf[nt][ks] = *reinterpret_cast<const uint4*>(q + 32 * ks);
-    }
-    const bool active = w * 32 < it.rows;
+  // ---- a segment of a prefix: 256 rows, 32 per wave, 64 keys at a time in LDS.
+  __device__ __forceinline__ void prefix(const Item& it) {
+    using LD = Lds<D>;
+    constexpr int KP = LD::KP, VP = LD::VP;
+    uint16_t* const sK = reinterpret_cast<uint16_t*>(smem);
+    uint16_t* const sV = sK + 2 * LD::kK;
+    const f16x2_t ones = f16x2_t{(_Float16)1.f, (_Float16)1.f};
+    // Wave groups: waves 0-3 and 4-7, one of each per SIMD.
+    const int grp = w >> 2, gt = tid & 255, gw = w & 3;
     const int h = __builtin_amdgcn_readfirstlane(it.h), key0 = __builtin_amdgcn_readfirstlane(it.key0),
-              key1 = __builtin_amdgcn_readfirstlane(it.key1), own0 = __builtin_amdgcn_readfirstlane(it.limit);
-    const int pages = (key1 - key0 + 15) >> 4, ntiles = (key1 - key0 + kUnit - 1) / kUnit;
+              key1 = __builtin_amdgcn_readfirstlane(it.key1);
+    const int pages = (key1 - key0 + 15) >> 4, n = (key1 - key0 + kUnit - 1) / kUnit;
     const int32_t* table = p.tables + (size_t)__builtin_amdgcn_readfirstlane(it.sid) * p.maxb + (key0 >> 4);
 
-    // Block ids (and an fp8 page's scales) of 64 pages in the lanes of a register;
-    // pages past the range repeat its last one.
-    int ids = 0;
-    float ksc = 1.f, vsc = 1.f;
-    float vref = 1.f;  // fp8: the range's largest V scale
-    auto page_ids = [&](int first) {
-      const int phys = table[min(first + lane, pages - 1)];
-      if ((unsigned)phys >= (unsigned)p.cap) flag_bad_read(p, it.b);
-      return (unsigned)phys < (unsigned)p.cap ? phys : 0;
-    };
-    auto scales_of = [&](int phys) {
-      return *reinterpret_cast<const float2*>(p.scales + ((size_t)p.layer * p.cap + phys) * 2);
-    };
-    auto window = [&](int first) {
-      ids = page_ids(first);
+    // Block ids (and an fp8 page's scales) of 64 pages, 16 tiles, in the lanes of a
+    // register, the next 64 ids read half a window ahead; pages past the range
+    // repeat its last one.
+    int ids = 0, idn = 0;
+    float ksc = 1.f, vsc = 1.f, vref = 1.f;  // vref, fp8: the range's largest V scale
+    auto read_ids = [&](int first) { return table[min(first + lane, pages - 1)]; };
+    auto open_window = [&](int raw) {
+      ids = safe_id(it, raw);
       if constexpr (kFp8) {
         const float2 s = scales_of(ids);
         ksc = s.x;
         vsc = vref > 0.f ? s.y / vref : 0.f;
       }
     };
+    int raw = read_ids(0);
+    uint4 qf[NT][KS];
+    int lim[NT];
+    bool valid[NT];
+    load_q(it, w * 32, qf, lim, valid);
+    const bool active = w * 32 < it.rows;
 
-    // Staging. K: 16-byte pieces of a page in memory order. V: (dim, page pair,
-    // half) items: 8 keys of the even and 8 of the odd page. In a V^T row key 4 gg +
-    // j of page 2 q + hh sits at 32 q + 8 gg + 4 hh + j, so that lane group gg's
-    // 16-byte read holds its keys of both pages.
-    constexpr int kKN = kUnit * D * ES / 16 / kThreads;  // K pieces per thread
-    constexpr int kVN = 4 * D / kThreads;                // V items per thread
+    // Staging: each group stages half of a tile. K: 16-byte pieces of a page in
+    // memory order. V: (dim, page pair, half) items: 8 keys of the even and 8 of the
+    // odd page. In a V^T row key 4 gg + j of page 2 q + hh sits at 32 q + 8 gg +
+    // 4 hh + j, so that lane group gg's 16-byte read holds its keys of both pages.
+    constexpr int kKP = kUnit * D * ES / 16, kKN = kKP / 2 / 256;  // K pieces of a tile, per thread
+    constexpr int kVI = 4 * D, kVN = (kVI / 2 + 255) / 256;        // V items of a tile, per thread
+    static_assert(kKP / 2 % 256 == 0 || kKP / 2 < 256, "whole pieces per thread");
+    constexpr int kKN1 = kKN ? kKN : 1;
     struct Stage {
-      u32x4_t k[kKN];
+      u32x4_t k[kKN1];
       u32x4_t v[kVN][2];  // fp8: the first 8 bytes
     };
-    const size_t layer_base = (size_t)p.layer * p.cap;
-    auto page = [&](const void* pool, int phys) {
-      return static_cast<const uint8_t*>(pool) + ((layer_base + phys) * p.Hkv + h) * (size_t)(16 * D * ES);
-    };
     constexpr int kPer = D * ES;  // 16-byte pieces of a page
+    // Group threads beyond a half's pieces (the smallest tiles) repeat one of them.
+    auto k_piece = [&](int i) { return grp * (kKP / 2) + (gt + i * 256) % (kKP / 2); };
+    auto v_item = [&](int i) { return grp * (kVI / 2) + (gt + i * 256) % (kVI / 2); };
+    auto k_page = [&](int i) { return (grp * (kKP / 2) + (gw * 64 + i * 256) % (kKP / 2)) / kPer; };  // of the wave's pieces
+    auto v_pair = [&](int i) { return (grp * (kVI / 2) + (gw * 64 + i * 256) % (kVI / 2)) / (2 * D); };
     auto load = [&](Stage& S, int t) {
 #pragma unroll
-      for (int i = 0; i < kKN; ++i) {
-        const int pi = (w * 64 + i * kThreads) / kPer, c = (tid + i * kThreads) % kPer;
-        const int phys = __builtin_amdgcn_readlane(ids, (4 * t + pi) & 63);
-        S.k[i] = *reinterpret_cast<const u32x4_t*>(page(p.kpool, phys) + 16 * c);
+      for (int i = 0; i < kKN1; ++i) {
+        const int phys = __builtin_amdgcn_readlane(ids, (4 * t + k_page(i)) & 63);
+        S.k[i] = *reinterpret_cast<const u32x4_t*>(page(p.kpool, phys, h) + 16 * (k_piece(i) % kPer));
       }
 #pragma unroll
       for (int i = 0; i < kVN; ++i) {
-        const int q = (w * 64 + i * kThreads) / (2 * D), c = (tid + i * kThreads) % (2 * D);
+        const int q = v_pair(i), c = v_item(i) % (2 * D);
 #pragma unroll
         for (int hh = 0; hh < 2; ++hh) {
           const int phys = __builtin_amdgcn_readlane(ids, (4 * t + 2 * q + hh) & 63);
-          const uint8_t* v = page(p.vpool, phys) + 8 * ES * c;
+          const uint8_t* v = page(p.vpool, phys, h) + 8 * ES * c;
           if constexpr (kFp8) {
             const uint2 x = *reinterpret_cast<const uint2*>(v);
             S.v[i][hh] = u32x4_t{x.x, x.y, 0u, 0u};
@@ -470,19 +508,24 @@ __global__ __launch_bounds__(kThreads, 2) void shared_mfma_kernel(SharedParams p
         }
       }
     };
-    float vs = 1.f;          // bf16: the staging factor 2^vk
+    // Tile t's loads, by the window it lies in (tiles are loaded in order).
+    auto load_next = [&](Stage& S, int t) {
+      if (t < n) {
+        if ((t & 15) == 0) open_window(idn);
+        if ((t & 15) == 8) idn = read_ids(4 * (t + 8));
+      }
+      load(S, min(t, n - 1));
+    };
+    float vs = 1.f;     // bf16: the staging factor 2^vk
     int vk = 0;
-    uint32_t vmax = 0;       // bf16: largest |v| bits staged (both halves)
-    bool dirty = false;      // a value that some row of the tile may not see is not finite
-    // Zeroes the values of keys past the range's end, and looks for non-finite ones
-    // among the chunk's own keys, which earlier rows do not see: P = 0 would not
-    // keep them out of a product.
+    uint32_t vmax = 0;  // bf16: largest |v| bits staged (both halves)
+    // Zeroes the values of keys past the range's end.
     auto edge = [&](Stage& S, int t) {
       const int t0 = key0 + t * kUnit;
-      if (t0 + kUnit <= key1 && (it.group >= 0 || t0 + kUnit - 1 <= own0)) return;
+      if (t0 + kUnit <= key1) return;
 #pragma unroll
       for (int i = 0; i < kVN; ++i) {
-        const int idx = tid + i * kThreads, q = idx / (2 * D), half = idx & 1;
+        const int q = v_pair(i), half = gt & 1;
 #pragma unroll
         for (int hh = 0; hh < 2; ++hh) {
           u32x4_t x = S.v[i][hh];
@@ -490,24 +533,19 @@ __global__ __launch_bounds__(kThreads, 2) void shared_mfma_kernel(SharedParams p
 #pragma unroll
           for (int e = 0; e < 8; ++e) {
             constexpr uint32_t kMask = kFp8 ? 0xffu : 0xffffu;
-            const int word = e * ES / 4, shift = 8 * (e * ES % 4);
-            const uint32_t bits = (x[word] >> shift) & kMask;
-            const bool bad = kFp8 ? (bits & 0x7fu) == 0x7fu
-                                  : (kF16 ? (bits & 0x7c00u) == 0x7c00u : (bits & 0x7f80u) == 0x7f80u);
-            if (k0 + e >= key1) x[word] &= ~(kMask << shift);
-            else dirty |= bad && k0 + e > own0;
+            x[e * ES / 4] &= k0 + e >= key1 ? ~(kMask << (8 * (e * ES % 4))) : ~0u;
           }
           S.v[i][hh] = x;
         }
       }
     };
-    auto store = [&](Stage& S, int t, int buf) {
-      edge(S, t);
-      uint16_t* const K = sK + buf * LD::kK;
-      uint16_t* const V = sV + buf * LD::kV;
+    auto store = [&](Stage& S, int t, int kslot, int vslot) {
+      edge(S, min(t, n - 1));
+      uint16_t* const K = sK + kslot * LD::kK;
+      uint16_t* const V = sV + vslot * LD::kV;
 #pragma unroll
-      for (int i = 0; i < kKN; ++i) {
-        const int pi = (w * 64 + i * kThreads) / kPer, c = (tid + i * kThreads) % kPer;
+      for (int i = 0; i < kKN1; ++i) {
+        const int pi = k_page(i), c = k_piece(i) % kPer;
         if constexpr (kFp8) {  // 16 codes: bf16 values, exactly
           const int key = 16 * pi + c / (D / 16), col = c % (D / 16);
           const u32x4_t x = S.k[i];
@@ -526,33 +564,30 @@ __global__ __launch_bounds__(kThreads, 2) void shared_mfma_kernel(SharedParams p
       }
 #pragma unroll
       for (int i = 0; i < kVN; ++i) {
-        const int idx = tid + i * kThreads, q = idx / (2 * D), dim = (idx >> 1) % D, half = idx & 1;
+        const int q = v_pair(i), c = v_item(i) % (2 * D), dim = c >> 1, half = c & 1;
         uint2 y[2][2];  // [page][keys 0-3, 4-7 of the half]
 #pragma unroll
         for (int hh = 0; hh < 2; ++hh) {
           const u32x4_t x = S.v[i][hh];
+          uint32_t z[4];
           if constexpr (kF16) {
-            y[hh][0] = make_uint2(x[0], x[1]);
-            y[hh][1] = make_uint2(x[2], x[3]);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) z[e] = x[e];
           } else if constexpr (kFp8) {
-            uint32_t z[4];
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
               z[2 * e] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(x[e], 1.f, false));
               z[2 * e + 1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(x[e], 1.f, true));
             }
-            y[hh][0] = make_uint2(z[0], z[1]);
-            y[hh][1] = make_uint2(z[2], z[3]);
           } else {
-            uint32_t z[4];
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
               vmax = max_abs2(x[e], vmax);
               z[e] = pack2_f16(__uint_as_float(x[e] << 16) * vs, __uint_as_float(x[e] & 0xffff0000u) * vs);
             }
-            y[hh][0] = make_uint2(z[0], z[1]);
-            y[hh][1] = make_uint2(z[2], z[3]);
           }
+          y[hh][0] = make_uint2(z[0], z[1]);
+          y[hh][1] = make_uint2(z[2], z[3]);
         }
         uint16_t* const row = &V[dim * VP + 32 * q + 16 * half];
         *reinterpret_cast<uint4*>(row) = make_uint4(y[0][0].x, y[0][0].y, y[1][0].x, y[1][0].y);
@@ -562,15 +597,134 @@ __global__ __launch_bounds__(kThreads, 2) void shared_mfma_kernel(SharedParams p
 
     f32x4_t o[MT][NT];
     float m[NT], l[NT], thr[NT];  // thr: the score above which m must grow
-    bool again = false;
+    f32x4_t sc[4][NT];            // S^T of the tile in the walk
+    uint32_t ph[2][NT][4];        // its P, two pages an operand
+    float ks_t = 1.f, vs_t = 1.f;  // fp8: scales of the window of the tile in the walk
+    auto pv = [&](int vslot) {
+      const uint16_t* V = sV + vslot * LD::kV;
+#pragma unroll
+      for (int q = 0; q < 2; ++q)
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) {
+          const f16x8_t va =
+              __builtin_bit_cast(f16x8_t, *reinterpret_cast<const uint4*>(&V[(16 * mt + i16) * VP + 32 * q + 8 * g]));
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+            o[mt][nt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+                va, __builtin_bit_cast(f16x8_t, make_uint4(ph[q][nt][0], ph[q][nt][1], ph[q][nt][2], ph[q][nt][3])),
+                o[mt][nt], 0, 0, 0);
+        }
+    };
+    auto qk = [&](int kslot) {
+      const uint16_t* K = sK + kslot * LD::kK;
+#pragma unroll
+      for (int kt = 0; kt < 4; ++kt) {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) sc[kt][nt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+          const uint4 kf = *reinterpret_cast<const uint4*>(&K[(16 * kt + i16) * KP + 32 * ks + 8 * g]);
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) sc[kt][nt] = mfma_qk(kf, qf[nt][ks], sc[kt][nt]);
+        }
+      }
+    };
+    auto softmax = [&](int t) {
+      if constexpr (kFp8) {
+        if ((t & 15) == 0) ks_t = ksc, vs_t = vsc;
+#pragma unroll
+        for (int kt = 0; kt < 4; ++kt) {
+          const float f = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(ks_t), (4 * t + kt) & 63));
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) sc[kt][nt] *= f;
+        }
+      }
+      const int t0 = key0 + t * kUnit;
+      if (t0 + kUnit > key1) {
+#pragma unroll
+        for (int kt = 0; kt < 4; ++kt)
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int jj = 0; jj < 4; ++jj)
+              if (t0 + 16 * kt + 4 * g + jj >= key1) sc[kt][nt][jj] = -INFINITY;
+      }
+      float mx[NT];
+      bool grow = false;
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        float a0 = max3_raw(sc[0][nt][0], sc[0][nt][1], sc[0][nt][2]);
+        float a1 = max3_raw(sc[0][nt][3], sc[1][nt][0], sc[1][nt][1]);
+        float a2 = max3_raw(sc[1][nt][2], sc[1][nt][3], sc[2][nt][0]);
+        float a3 = max3_raw(sc[2][nt][1], sc[2][nt][2], sc[2][nt][3]);
+        float a4 = max3_raw(sc[3][nt][0], sc[3][nt][1], sc[3][nt][2]);
+        a0 = max3_raw(a0, a1, a2);
+        a3 = max3_raw(a3, a4, sc[3][nt][3]);
+        mx[nt] = fmaxf(a0, a3);
+        grow |= mx[nt] > thr[nt];
+      }
+      if (__any(grow)) {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          float a = fmaxf(mx[nt], __shfl_xor(mx[nt], 16, 64));
+          a = fmaxf(a, __shfl_xor(a, 32, 64));
+          const float m_new = fmaxf(m[nt], a * sl2);
+          const float alpha = m_new == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m[nt] - m_new);
+          l[nt] *= alpha;
+#pragma unroll
+          for (int mt = 0; mt < MT; ++mt) o[mt][nt] *= alpha;
+          m[nt] = m_new;
+          thr[nt] = (m_new + kSlack) * inv_sl2;
+        }
+      }
+#pragma unroll
+      for (int kt = 0; kt < 4; ++kt) {
+        float f = 1.f;
+        if constexpr (kFp8) f = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(vs_t), (4 * t + kt) & 63));
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          const float mu = m[nt] == -INFINITY ? 0.f : m[nt];
+          float e[4];
+#pragma unroll
+          for (int jj = 0; jj < 4; ++jj) e[jj] = __builtin_amdgcn_exp2f(fmaf(sc[kt][nt][jj], sl2, -mu));
+          if constexpr (kFp8) {
+            l[nt] += (e[0] + e[1]) + (e[2] + e[3]);
+#pragma unroll
+            for (int jj = 0; jj < 4; ++jj) e[jj] *= f;
+          }
+          const uint32_t p01 = pack2_f16(e[0], e[1]), p23 = pack2_f16(e[2], e[3]);
+          ph[kt >> 1][nt][2 * (kt & 1)] = p01;
+          ph[kt >> 1][nt][2 * (kt & 1) + 1] = p23;
+          if constexpr (!kFp8) {  // the sum takes P as it enters P V
+            l[nt] = __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2_t, p01), ones, l[nt], false);
+            l[nt] = __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2_t, p23), ones, l[nt], false);
+          }
+        }
+      }
+    };
+    // A phase ends at a workgroup barrier that no instruction is scheduled across.
+    auto phase_end = [] {
+      __builtin_amdgcn_sched_barrier(0);
+      __syncthreads();
+      __builtin_amdgcn_sched_barrier(0);
+    };
     if constexpr (kFp8) {
       float mx = 0.f;
-      for (int pg = tid; pg < pages; pg += kThreads) {
+      for (int pg = tid; pg < pages; pg += kMfmaThreads) {
         const int phys = table[pg];
         if ((unsigned)phys < (unsigned)p.cap) mx = fmaxf(mx, scales_of(phys).y);
       }
       vref = __uint_as_float(wg_max(__float_as_uint(mx)));
     }
+    // The walk. Group 0 runs phases M(0), V(0), M(1), V(1), ... and group 1 the same
+    // one phase later, a barrier after each, so that on every SIMD one wave's
+    // softmax runs beside the other's matrix instructions:
+    //   M(t): O^T += V^T P^T of tile t - 1, then S^T of tile t
+    //   V(t): softmax of tile t; stage the group's half of tile t + 1 + grp
+    // Tile x is whole in LDS after V(x - 2) of group 1 and V(x - 1) of group 0; its K
+    // is read in M(x), its V in M(x + 1) of either group: two K slots, three V slots.
+    bool again = false;
+    Stage st0, st1;
     for (int attempt = 0;; ++attempt) {
 #pragma unroll
       for (int mt = 0; mt < MT; ++mt)
@@ -582,164 +736,75 @@ __global__ __launch_bounds__(kThreads, 2) void shared_mfma_kernel(SharedParams p
         l[nt] = 0.f;
         thr[nt] = -INFINITY;
       }
-      Stage S;
-      window(0);
-      load(S, 0);
+      idn = raw;
+      load_next(st0, 0);
+      if (grp == 1) load_next(st1, 1);
       if constexpr (!kF16 && !kFp8) {
         // The largest finite |v| of the first tile, or (again) of the whole range.
         uint32_t mx = 0;
-        auto take = [&](const Stage& X) {
+        auto take = [&](u32x4_t x) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const uint32_t lo = x[e] & 0x7fffu, hi = (x[e] >> 16) & 0x7fffu;
+            mx = max(mx, lo < 0x7f80u ? lo : 0u);
+            mx = max(mx, hi < 0x7f80u ? hi : 0u);
+          }
+        };
+        if (!again) {
+          edge(st0, 0);
 #pragma unroll
           for (int i = 0; i < kVN; ++i)
 #pragma unroll
-            for (int hh = 0; hh < 2; ++hh) {
-              const u32x4_t x = X.v[i][hh];
+            for (int hh = 0; hh < 2; ++hh) take(st0.v[i][hh]);
+        } else {
+          for (int c = tid; c < pages * 2 * D; c += kMfmaThreads) {  // 8 keys of a dim
+            const int pg = c / (2 * D), k0 = key0 + 16 * pg + 8 * (c & 1);
+            u32x4_t x = *reinterpret_cast<const u32x4_t*>(page(p.vpool, safe_id(it, table[pg]), h) + 16 * (c % (2 * D)));
 #pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                const uint32_t lo = x[e] & 0x7fffu, hi = (x[e] >> 16) & 0x7fffu;
-                if (lo < 0x7f80u) mx = max(mx, lo);
-                if (hi < 0x7f80u) mx = max(mx, hi);
-              }
-            }
-        };
-        edge(S, 0);
-        take(S);
-        if (again) {
-          for (int t = 1; t < ntiles; ++t) {
-            if ((t & 15) == 0) window(4 * t);
-            load(S, t);
-            edge(S, t);
-            take(S);
+            for (int e = 0; e < 8; ++e) x[e / 2] &= k0 + e >= key1 ? ~(0xffffu << (16 * (e & 1))) : ~0u;
+            take(x);
           }
-          window(0);
-          load(S, 0);
         }
         vk = stage_exponent(__uint_as_float(wg_max(mx) << 16));
         vs = ldexpf(1.f, vk);
         vmax = 0;
       }
-      float ksn = ksc, vsn = vsc;  // the scales of the tile in the stage
-      store(S, 0, 0);
-      if (ntiles > 1) load(S, 1);
-      __syncthreads();
-      for (int t = 0; t < ntiles; ++t) {
-        const float ks_t = ksn, vs_t = vsn;
-        if (t + 1 < ntiles) {
-          store(S, t + 1, (t + 1) & 1);
-          if (((t + 2) & 15) == 0 && t + 2 < ntiles) window(4 * (t + 2));
-          if (t + 2 < ntiles) load(S, t + 2);
-        }
-        if ((t & 15) == 15) ksn = ksc, vsn = vsc;
+      store(st0, 0, 0, 0);
+      if (grp == 1) store(st1, 1, 1, 1);
+      load_next(st0, 1 + grp);
+      load_next(st1, 2 + grp);
+      phase_end();
+      if (grp == 1) phase_end();
+      if (active) qk(0);  // M(0)
+      phase_end();
+      int ksl = (1 + grp) & 1, vst = 1 + grp, vrd = 0;  // slots of the tile staged in V(t); V slot of tile t
+      auto step = [&](int t, Stage& X) {
+        if (active) softmax(t);
+        store(X, t + 1 + grp, ksl, vst);
+        load_next(X, t + 3 + grp);
+        phase_end();
         if (active) {
-          const uint16_t* K = sK + (t & 1) * LD::kK;
-          const uint16_t* V = sV + (t & 1) * LD::kV;
-          f32x4_t sc[4][NT];
-#pragma unroll
-          for (int kt = 0; kt < 4; ++kt) {
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt) sc[kt][nt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int ks = 0; ks < KS; ++ks) {
-              const uint4 kf = *reinterpret_cast<const uint4*>(&K[(16 * kt + i16) * KP + 32 * ks + 8 * g]);
-#pragma unroll
-              for (int nt = 0; nt < NT; ++nt)
-                sc[kt][nt] = kF16 ? __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8_t, kf),
-                                                                            __builtin_bit_cast(f16x8_t, qf[nt][ks]),
-                                                                            sc[kt][nt], 0, 0, 0)
-                                  : __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, kf),
-                                                                             __builtin_bit_cast(bf16x8_t, qf[nt][ks]),
-                                                                             sc[kt][nt], 0, 0, 0);
-            }
-          }
-          if constexpr (kFp8) {
-#pragma unroll
-            for (int kt = 0; kt < 4; ++kt) {
-              const float f = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(ks_t), (4 * t + kt) & 63));
-#pragma unroll
-              for (int nt = 0; nt < NT; ++nt) sc[kt][nt] *= f;
-            }
-          }
-          const int t0 = key0 + t * kUnit;
-          if (t0 + kUnit > key1 || (it.group < 0 && t0 + kUnit - 1 > own0)) {
-#pragma unroll
-            for (int kt = 0; kt < 4; ++kt)
-#pragma unroll
-              for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                for (int jj = 0; jj < 4; ++jj) {
-                  const int key = t0 + 16 * kt + 4 * g + jj;
-                  if (key >= key1 || key > lim[nt]) sc[kt][nt][jj] = -INFINITY;
-                }
-          }
-          float mx[NT];
-          bool grow = false;
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt) {
-            float a0 = max3_raw(sc[0][nt][0], sc[0][nt][1], sc[0][nt][2]);
-            float a1 = max3_raw(sc[0][nt][3], sc[1][nt][0], sc[1][nt][1]);
-            float a2 = max3_raw(sc[1][nt][2], sc[1][nt][3], sc[2][nt][0]);
-            float a3 = max3_raw(sc[2][nt][1], sc[2][nt][2], sc[2][nt][3]);
-            float a4 = max3_raw(sc[3][nt][0], sc[3][nt][1], sc[3][nt][2]);
-            a0 = max3_raw(a0, a1, a2);
-            a3 = max3_raw(a3, a4, sc[3][nt][3]);
-            mx[nt] = fmaxf(a0, a3);
-            grow |= mx[nt] > thr[nt];
-          }
-          if (__any(grow)) {
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-              float a = fmaxf(mx[nt], __shfl_xor(mx[nt], 16, 64));
-              a = fmaxf(a, __shfl_xor(a, 32, 64));
-              const float m_new = fmaxf(m[nt], a * sl2);
-              const float alpha = m_new == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m[nt] - m_new);
-              l[nt] *= alpha;
-#pragma unroll
-              for (int mt = 0; mt < MT; ++mt) o[mt][nt] *= alpha;
-              m[nt] = m_new;
-              thr[nt] = (m_new + kSlack) * inv_sl2;
-            }
-          }
-          uint32_t ph[2][NT][4];
-#pragma unroll
-          for (int kt = 0; kt < 4; ++kt) {
-            float f = 1.f;
-            if constexpr (kFp8)
-              f = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(vs_t), (4 * t + kt) & 63));
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-              const float mu = m[nt] == -INFINITY ? 0.f : m[nt];
-              float e[4];
-#pragma unroll
-              for (int jj = 0; jj < 4; ++jj) e[jj] = __builtin_amdgcn_exp2f(fmaf(sc[kt][nt][jj], sl2, -mu));
-              if constexpr (kFp8) {
-                l[nt] += (e[0] + e[1]) + (e[2] + e[3]);
-#pragma unroll
-                for (int jj = 0; jj < 4; ++jj) e[jj] *= f;
-              }
-              const uint32_t p01 = pack2_f16(e[0], e[1]), p23 = pack2_f16(e[2], e[3]);
-              ph[kt >> 1][nt][2 * (kt & 1)] = p01;
-              ph[kt >> 1][nt][2 * (kt & 1) + 1] = p23;
-              if constexpr (!kFp8) {  // the sum takes P as it enters P V
-                l[nt] = __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2_t, p01), ones, l[nt], false);
-                l[nt] = __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2_t, p23), ones, l[nt], false);
-              }
-            }
-          }
-#pragma unroll
-          for (int q = 0; q < 2; ++q)
-#pragma unroll
-            for (int mt = 0; mt < MT; ++mt) {
-              const f16x8_t va = __builtin_bit_cast(
-                  f16x8_t, *reinterpret_cast<const uint4*>(&V[(16 * mt + i16) * VP + 32 * q + 8 * g]));
-#pragma unroll
-              for (int nt = 0; nt < NT; ++nt)
-                o[mt][nt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
-                    va, __builtin_bit_cast(f16x8_t, make_uint4(ph[q][nt][0], ph[q][nt][1], ph[q][nt][2], ph[q][nt][3])),
-                    o[mt][nt], 0, 0, 0);
-            }
+          pv(vrd);
+          qk((t + 1) & 1);
         }
-        __syncthreads();
+        phase_end();
+        ksl ^= 1;
+        vst = vst == 2 ? 0 : vst + 1;
+        vrd = vrd == 2 ? 0 : vrd + 1;
+      };
+      int t = 0;
+      for (; t + 2 < n; t += 2) {
+        step(t, st0);
+        step(t + 1, st1);
       }
+      if (t + 1 < n) {
+        step(t, st0);
+        ++t;
+      }
+      if (active) softmax(t);
+      phase_end();
+      if (active) pv(vrd);
+      if (grp == 0) phase_end();
       if constexpr (kF16 || kFp8) break;
       if (attempt == 1) break;
       // bits of the largest |v| that stays within fp16 at this power
@@ -747,23 +812,281 @@ __global__ __launch_bounds__(kThreads, 2) void shared_mfma_kernel(SharedParams p
       again = __syncthreads_or((vmax & 0xffffu) > top || (vmax >> 16) > top);
       if (!again) break;
     }
-    if (it.group < 0 && __syncthreads_or(dirty)) {
-      valu_item<QT, KT, D>(p, it, reinterpret_cast<float*>(smem));
-      return;
-    }
-    const float post = kFp8 ? vref : ldexpf(1.f, -vk);
+    write(it, w * 32, o, m, l, valid, kFp8 ? vref : ldexpf(1.f, -vk));
+    __syncthreads();  // the slots are free for the next segment
+  }
+
+  // A wave's partial rows r0 + 16 nt + i16 of an item.
+  __device__ __forceinline__ void write(const Item& it, int r0, const f32x4_t (&o)[MT][NT], const float (&m)[NT],
+                                        float (&l)[NT], const bool (&valid)[NT], float post) {
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       l[nt] += __shfl_xor(l[nt], 16, 64);
       l[nt] += __shfl_xor(l[nt], 32, 64);
       if (!valid[nt]) continue;
-      const size_t row = (size_t)(it.part + w * 32 + nt * 16 + i16);
+      const size_t row = (size_t)(it.part + r0 + nt * 16 + i16);
       if (g == 0) *reinterpret_cast<float2*>(&p.part_ml[row * 2]) = make_float2(m[nt], l[nt]);
 #pragma unroll
       for (int mt = 0; mt < MT; ++mt)
         *reinterpret_cast<f32x4_t*>(&p.part_o[row * D + 16 * mt + 4 * g]) = o[mt][nt] * post;
     }
-  });
+  }
+
+  // ---- an entry's own keys: up to 64 rows, 32 per wave; a wave takes every fourth
+  // page (every eighth where there are at most 32 rows) straight into operand
+  // registers, one page in flight while one is computed, and the waves' sums join in LDS.
+  // P goes in two halves of bf16, beside each other in one operand over 16 keys
+  // twice (fp16 pages: one operand of 16 keys): 16 bits of P, and values of any size.
+  __device__ __forceinline__ void own(const Item& it) {
+    const bool wide = it.rows > 32;
+    const int nk = wide ? 4 : 8, kw = wide ? w & 3 : w, r0 = wide ? (w >> 2) * 32 : 0;
+    const int h = __builtin_amdgcn_readfirstlane(it.h), key0 = __builtin_amdgcn_readfirstlane(it.key0),
+              key1 = __builtin_amdgcn_readfirstlane(it.key1), start = __builtin_amdgcn_readfirstlane(it.start);
+    const int pages = (key1 - key0 + 15) >> 4;
+    const int32_t* table = p.tables + (size_t)__builtin_amdgcn_readfirstlane(it.sid) * p.maxb + (key0 >> 4);
+    const int mine = kw < pages ? (pages - 1 - kw) / nk + 1 : 0;  // pages kw, kw + nk, ...
+    uint4 qf[NT][KS];
+    int lim[NT];
+    bool valid[NT];
+    load_q(it, r0, qf, lim, valid);
+    f32x4_t o[MT][NT];
+    float m[NT], l[NT], thr[NT];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      m[nt] = -INFINITY;
+      l[nt] = 0.f;
+      thr[nt] = -INFINITY;
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt) o[mt][nt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    }
+    int ids = 0;
+    float ksc = 1.f, vsc = 1.f;
+    int dirty = 0;  // a value of the chunk that some of its rows do not see is not finite
+    struct Page {
+      uint4 k[KS];  // fp8: 8 bytes
+      uint2 v[MT];  // fp8: 4 bytes
+    };
+    auto load = [&](Page& P, int i) {
+      const int phys = __builtin_amdgcn_readlane(ids, i & 63);
+      const uint8_t* K = page(p.kpool, phys, h) + (i16 * D + 8 * g) * ES;
+      const uint8_t* V = page(p.vpool, phys, h) + (i16 * 16 + 4 * g) * ES;
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) {
+        if constexpr (kFp8) {
+          const uint2 x = *reinterpret_cast<const uint2*>(K + 32 * ks);
+          P.k[ks] = make_uint4(x.x, x.y, 0u, 0u);
+        } else {
+          P.k[ks] = *reinterpret_cast<const uint4*>(K + 64 * ks);
+        }
+      }
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt) {
+        if constexpr (kFp8) P.v[mt] = make_uint2(*reinterpret_cast<const uint32_t*>(V + 256 * mt), 0u);
+        else P.v[mt] = *reinterpret_cast<const uint2*>(V + 512 * mt);
+      }
+    };
+    auto compute = [&](Page& P, int i) {
+      const int k0 = key0 + 16 * (kw + nk * i);
+      f32x4_t sc[NT];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) sc[nt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) {
+        uint4 kf = P.k[ks];
+        if constexpr (kFp8) {
+          const uint32_t a = kf.x, b = kf.y;
+          kf = make_uint4(__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(a, 1.f, false)),
+                          __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(a, 1.f, true)),
+                          __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(b, 1.f, false)),
+                          __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(b, 1.f, true)));
+        }
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) sc[nt] = mfma_qk(kf, qf[nt][ks], sc[nt]);
+      }
+      float fv = 1.f;
+      if constexpr (kFp8) {
+        const float f = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(ksc), i & 63));
+        fv = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(vsc), i & 63));
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) sc[nt] *= f;
+      }
+      if (k0 + 16 > key1 || k0 + 15 > start) {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int jj = 0; jj < 4; ++jj) {
+            const int key = k0 + 4 * g + jj;
+            sc[nt][jj] = key >= key1 || key > lim[nt] ? -INFINITY : sc[nt][jj];
+          }
+        // Values past the range's end are zero; a chunk value that is not finite must
+        // not meet the P = 0 of the rows before it.
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) {
+          uint32_t x[2] = {P.v[mt].x, P.v[mt].y};
+#pragma unroll
+          for (int jj = 0; jj < 4; ++jj) {
+            constexpr uint32_t kMask = kFp8 ? 0xffu : 0xffffu;
+            const int word = jj * ES / 4, shift = 8 * (jj * ES % 4), key = k0 + 4 * g + jj;
+            const uint32_t bits = (x[word] >> shift) & kMask;
+            const bool bad = kFp8 ? (bits & 0x7fu) == 0x7fu
+                                  : (kF16 ? (bits & 0x7c00u) == 0x7c00u : (bits & 0x7f80u) == 0x7f80u);
+            x[word] &= key >= key1 ? ~(kMask << shift) : ~0u;
+            dirty |= (int)bad & (int)(key > start) & (int)(key < key1);
+          }
+          P.v[mt] = make_uint2(x[0], x[1]);
+        }
+      }
+      bool grow = false;
+      float mx[NT];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        mx[nt] = fmaxf(max3_raw(sc[nt][0], sc[nt][1], sc[nt][2]), sc[nt][3]);
+        grow |= mx[nt] > thr[nt];
+      }
+      if (__any(grow)) {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          float a = fmaxf(mx[nt], __shfl_xor(mx[nt], 16, 64));
+          a = fmaxf(a, __shfl_xor(a, 32, 64));
+          const float m_new = fmaxf(m[nt], a * sl2);
+          const float alpha = m_new == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m[nt] - m_new);
+          l[nt] *= alpha;
+#pragma unroll
+          for (int mt = 0; mt < MT; ++mt) o[mt][nt] *= alpha;
+          m[nt] = m_new;
+          thr[nt] = (m_new + kSlack) * inv_sl2;
+        }
+      }
+      uint4 pb[NT];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        const float mu = m[nt] == -INFINITY ? 0.f : m[nt];
+        float e[4];
+#pragma unroll
+        for (int jj = 0; jj < 4; ++jj) e[jj] = __builtin_amdgcn_exp2f(fmaf(sc[nt][jj], sl2, -mu));
+        l[nt] += (e[0] + e[1]) + (e[2] + e[3]);
+        if constexpr (kF16) {
+          pb[nt] = make_uint4(pack2_f16(e[0], e[1]), pack2_f16(e[2], e[3]), 0u, 0u);
+        } else {
+          uint32_t hi[2], lo[2];
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            const float a = e[2 * k] * fv, b = e[2 * k + 1] * fv;
+            hi[k] = __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2_t{a, b}, bf16x2_t));
+            const float ra = a - __uint_as_float(hi[k] << 16), rb = b - __uint_as_float(hi[k] & 0xffff0000u);
+            lo[k] = __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2_t{ra, rb}, bf16x2_t));
+          }
+          pb[nt] = make_uint4(hi[0], hi[1], lo[0], lo[1]);
+        }
+      }
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt) {
+        uint2 v = P.v[mt];
+        if constexpr (kFp8) {
+          const uint32_t c = v.x;
+          v = make_uint2(__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(c, 1.f, false)),
+                         __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(c, 1.f, true)));
+        }
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          if constexpr (kF16)
+            o[mt][nt] = __builtin_amdgcn_mfma_f32_16x16x16f16(__builtin_bit_cast(f16x4_t, v),
+                                                              __builtin_bit_cast(f16x4_t, make_uint2(pb[nt].x, pb[nt].y)),
+                                                              o[mt][nt], 0, 0, 0);
+          else
+            o[mt][nt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, make_uint4(v.x, v.y, v.x, v.y)),
+                                                                 __builtin_bit_cast(bf16x8_t, pb[nt]), o[mt][nt], 0, 0, 0);
+        }
+      }
+    };
+    for (int base = 0; base < mine; base += 64) {  // 64 of the wave's pages, their ids in the lanes
+      ids = safe_id(it, table[min(kw + nk * (base + lane), pages - 1)]);
+      if constexpr (kFp8) {
+        const float2 s = scales_of(ids);
+        ksc = s.x;
+        vsc = s.y;
+      }
+      const int last = min(mine, base + 64) - 1;
+      // Every load is unconditional (past the last page it repeats it), so that a page's
+      // use waits for its own loads alone.
+      Page A, B;
+      load(A, base);
+      for (int i = base;; i += 2) {
+        load(B, min(i + 1, last));
+        compute(A, i);
+        if (i + 1 > last) break;
+        load(A, min(i + 2, last));
+        compute(B, i + 1);
+        if (i + 2 > last) break;
+      }
+    }
+    if (__syncthreads_or(dirty)) {
+      valu_item<QT, KT, D, kMfmaThreads>(p, it, reinterpret_cast<float*>(smem));
+      return;
+    }
+    // Join the waves of the same rows: all take the largest m, then sums go down a
+    // tree through LDS, in one order.
+    float2* const sML = reinterpret_cast<float2*>(smem + 4 * 64 * (size_t)(MT * NT) * 16);
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      l[nt] += __shfl_xor(l[nt], 16, 64);
+      l[nt] += __shfl_xor(l[nt], 32, 64);
+      if (g == 0) sML[w * 32 + nt * 16 + i16] = make_float2(m[nt], l[nt]);
+    }
+    __syncthreads();
+    const int w0 = wide ? w & 4 : 0;  // the first wave of these rows
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      float M = -INFINITY, L = 0.f;
+      for (int k = 0; k < nk; ++k) M = fmaxf(M, sML[(w0 + k) * 32 + nt * 16 + i16].x);
+      const float ref = M == -INFINITY ? 0.f : M;
+      for (int k = 0; k < nk; ++k) {
+        const float2 x = sML[(w0 + k) * 32 + nt * 16 + i16];
+        L += x.y * __builtin_amdgcn_exp2f(x.x - ref);
+      }
+      const float f = __builtin_amdgcn_exp2f(m[nt] - ref);
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt) o[mt][nt] *= f;
+      m[nt] = M;
+      l[nt] = L;
+    }
+    f32x4_t* const sO = reinterpret_cast<f32x4_t*>(smem);
+    for (int half = nk / 2; half >= 1; half /= 2) {
+      const int slot = wide ? (w >> 2) * 2 : 0;  // wide: at most two senders per half of the rows
+      if (kw >= half && kw < 2 * half) {
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) sO[((slot + kw - half) * MT * NT + mt * NT + nt) * 64 + lane] = o[mt][nt];
+      }
+      __syncthreads();
+      if (kw < half) {
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) o[mt][nt] += sO[((slot + kw) * MT * NT + mt * NT + nt) * 64 + lane];
+      }
+      __syncthreads();
+    }
+    if (kw == 0) {
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) l[nt] *= 0.25f;  // `write` adds the four lane groups, which hold it each
+      write(it, r0, o, m, l, valid, 1.f);
+    }
+  }
+};
+
+template <int D, int KT>
+__global__ __launch_bounds__(kMfmaThreads, 2) void shared_mfma_kernel(SharedParams p) {
+  static_assert(valu_lds(D) <= Lds<D>::kBytes, "the any-shape walk reuses this memory");
+  __shared__ __align__(16) uint8_t smem[Lds<D>::kBytes];
+  Walk<D, KT> walk(p, smem);
+  if ((int)blockIdx.x < p.own) {
+    Item it;
+    if (own_item(p, blockIdx.x, it)) walk.own(it);
+    return;
+  }
+  for_segments(p, [&](const Item& it) { walk.prefix(it); });
 }
 
 // ----------------------------------------------------------------------- join
@@ -771,6 +1094,7 @@ __global__ __launch_bounds__(kThreads, 2) void shared_mfma_kernel(SharedParams p
 // head_dim = 4 LPR), or dims lane + 64 k of any head_dim up to 256. The row's
 // partials, the prefix's segments in key order and then its own ranges, are added
 // in that order whatever finished first.
+constexpr int kJoin = 4;
 template <int QT, int LPR, bool VEC>
 __global__ __launch_bounds__(kThreads) void shared_join_kernel(SharedParams p) {
   const int lane = threadIdx.x % LPR;
@@ -778,43 +1102,51 @@ __global__ __launch_bounds__(kThreads) void shared_join_kernel(SharedParams p) {
   if (row >= (long long)p.B * p.C * p.Hq) return;
   const int hq = (int)(row % p.Hq), bj = (int)(row / p.Hq), b = bj / p.C, j = bj - b * p.C;
   const int h = hq / p.ratio, r = j * p.ratio + (hq - h * p.ratio);
-  const int32_t* e = p.plan + p.plan[PH_ENTRIES] + (size_t)b * E_WORDS;
+  const int32_t* e = p.entries + (size_t)b * E_WORDS;
+  const int seen = min(max(p.start[b] + p.C, 0), p.max_ctx);
   int np = 0;
   long long pre = 0;  // the prefix's partial row of segment 0
-  if (e[E_GROUP] >= 0) {
-    const int32_t* g = p.plan + p.plan[PH_GROUPS] + (size_t)e[E_GROUP] * G_WORDS;
+  if (e[E_TILE0] >= 0) {
     const long long R = (long long)e[E_RANK] * p.G + r;
-    const int32_t* t = p.plan + p.plan[PH_TILES] + (size_t)(g[G_TILE0] + h * g[G_NT] + (int)(R / kTile)) * T_WORDS;
+    const int32_t* t = p.tiles + (size_t)(e[E_TILE0] + h * e[E_NT] + (int)(R / kTile)) * T_WORDS;
     np = t[T_COUNT];
     pre = (long long)t[T_SEG] * kTile + R % kTile;
   }
-  const int seen = min(max(p.start[b] + p.C, 0), p.max_ctx);
   const int n = np + (seen + p.own_range - 1) / p.own_range;
   const long long own = p.own_part + (long long)(b * p.Hkv + h) * p.own_max * p.G + r;
-  auto part = [&](int s) { return (size_t)(s < np ? pre + (long long)s * kTile : own + (long long)(s - np) * p.G); };
-  float M = -INFINITY;
-  for (int s = lane; s < n; s += LPR) M = fmaxf(M, p.part_ml[part(s) * 2]);
+  float M = -INFINITY, L = 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f};
+  for (int s0 = 0; s0 < n; s0 += kJoin) {  // kJoin partials a round trip
+    float2 ml[kJoin];
+    float x[kJoin][4];
 #pragma unroll
-  for (int o = LPR / 2; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor(M, o, LPR));
-  const float ref = M == -INFINITY ? 0.f : M;
-  float acc[4] = {0.f, 0.f, 0.f, 0.f}, L = 0.f;
-#pragma unroll 4
-  for (int s = 0; s < n; ++s) {
-    const size_t at = part(s);
-    const float2 ml = *reinterpret_cast<const float2*>(&p.part_ml[at * 2]);
-    const float w = exp2f(ml.x - ref);
-    L += w * ml.y;
-    const float* o = p.part_o + at * p.d;
-    if constexpr (VEC) {
-      const float4 x = *reinterpret_cast<const float4*>(o + 4 * lane);
-      acc[0] += w * x.x;
-      acc[1] += w * x.y;
-      acc[2] += w * x.z;
-      acc[3] += w * x.w;
-    } else {
+    for (int k = 0; k < kJoin; ++k) {
+      const int s = min(s0 + k, n - 1);
+      const size_t at = (size_t)(s < np ? pre + (long long)s * kTile : own + (long long)(s - np) * p.G);
+      ml[k] = *reinterpret_cast<const float2*>(&p.part_ml[at * 2]);
+      const float* o = p.part_o + at * p.d;
+      if constexpr (VEC) {
+        const float4 y = *reinterpret_cast<const float4*>(o + 4 * lane);
+        x[k][0] = y.x, x[k][1] = y.y, x[k][2] = y.z, x[k][3] = y.w;
+      } else {
 #pragma unroll
-      for (int k = 0; k < 4; ++k)
-        if (lane + 64 * k < p.d) acc[k] += w * o[lane + 64 * k];
+        for (int c = 0; c < 4; ++c) x[k][c] = lane + 64 * c < p.d ? o[lane + 64 * c] : 0.f;
+      }
+    }
+    float top = M;
+#pragma unroll
+    for (int k = 0; k < kJoin; ++k) top = fmaxf(top, ml[k].x);
+    const float ref = top == -INFINITY ? 0.f : top, keep = exp2f(M - ref);
+    M = top;
+    L *= keep;
+#pragma unroll
+    for (int c = 0; c < 4; ++c) acc[c] *= keep;
+#pragma unroll
+    for (int k = 0; k < kJoin; ++k) {
+      if (s0 + k >= n) break;
+      const float w = exp2f(ml[k].x - ref);
+      L += w * ml[k].y;
+#pragma unroll
+      for (int c = 0; c < 4; ++c) acc[c] += w * x[k][c];
     }
   }
   const float inv = 1.f / L;
@@ -848,62 +1180,78 @@ int make_plan(std::vector<int32_t>& plan, const int32_t* ids, const int32_t* len
   const long long G = (long long)C * (Hq / Hkv);
   std::vector<Group> groups;
   std::map<std::pair<int32_t, int32_t>, size_t> index;
-  std::vector<int32_t> entries(E_WORDS * (size_t)B);
+  std::vector<int32_t> entries(E_WORDS * (size_t)B, 0), of(B, -1);
   for (int b = 0; b < B; ++b) {
     if (ids[b] < -1 || lens[b] < 0) return SPV_ERR_ARG;
-    entries[E_WORDS * (size_t)b + E_GROUP] = -1;
-    entries[E_WORDS * (size_t)b + E_RANK] = 0;
+    entries[E_WORDS * (size_t)b + E_TILE0] = -1;
     if (ids[b] < 0 || lens[b] == 0) continue;
     const size_t g = index.emplace(std::make_pair(ids[b], lens[b]), groups.size()).first->second;
     if (g == groups.size()) groups.push_back({ids[b], lens[b], {}});
-    entries[E_WORDS * (size_t)b + E_GROUP] = (int)g;
     entries[E_WORDS * (size_t)b + E_RANK] = (int)groups[g].members.size();
+    of[b] = (int)g;
     groups[g].members.push_back(b);
   }
-  std::vector<int32_t> gw, mw, sh, sw, tw;
+  std::vector<int32_t> members, shares, segs, tiles;
+  std::vector<long long> tile0;
   long long units = 0, maxp = 0, triples = 0;
   for (const Group& x : groups) {
-    const long long tiles = ((long long)x.members.size() * G + kTile - 1) / kTile;
-    if (triples + tiles * Hkv > 0x7fffffffLL / kTile) return SPV_ERR_UNSUPPORTED;
-    const int32_t w[G_WORDS] = {x.sid, x.len, (int32_t)mw.size(), (int32_t)x.members.size(), (int32_t)tiles,
-                                (int32_t)triples};
-    gw.insert(gw.end(), w, w + G_WORDS);
-    mw.insert(mw.end(), x.members.begin(), x.members.end());
-    units += tiles * ((x.len + kUnit - 1) / kUnit);
-    triples += tiles * Hkv;
+    const long long nt = ((long long)x.members.size() * G + kTile - 1) / kTile;
+    tile0.push_back(triples);
+    triples += nt * Hkv;
+    if (triples > 0x7fffffffLL / kTile) return SPV_ERR_UNSUPPORTED;
+    units += nt * ((x.len + kUnit - 1) / kUnit);
     maxp = std::max<long long>(maxp, x.len);
   }
-  tw.resize(T_WORDS * (size_t)triples);
+  for (int b = 0; b < B; ++b)
+    if (of[b] >= 0) {
+      entries[E_WORDS * (size_t)b + E_TILE0] = (int32_t)tile0[of[b]];
+      entries[E_WORDS * (size_t)b + E_NT] = (int32_t)((groups[of[b]].members.size() * G + kTile - 1) / kTile);
+    }
+  tiles.resize(T_WORDS * (size_t)triples);
   // Shares: equal runs of the units of all kv heads, groups and tiles (in that
-  // order), two workgroups for each of the 256 CUs, or fewer where a share would be
+  // order), one workgroup for each of the 256 CUs, or fewer where a share would be
   // shorter than two units.
   const long long total = units * Hkv;
-  const long long nsh = total ? std::max(1LL, std::min(512LL, (total + 1) / 2) / 8) * 8 : 0;
-  long long at = 0, share = 0;  // the unit in hand, and the share it belongs to
+  const long long nsh = total ? std::max(1LL, std::min(256LL, (total + 1) / 2) / 8) * 8 : 0;
+  long long at = 0, share = 0;  // the unit in hand, and the share it opens next
   auto first_unit = [&](long long s) { return s * total / nsh; };
+  std::vector<int32_t> first_of(groups.size());
+  for (size_t g = 0; g < groups.size(); ++g) {
+    first_of[g] = (int32_t)members.size();
+    members.insert(members.end(), groups[g].members.begin(), groups[g].members.end());
+  }
+  std::vector<int32_t> begin;
   for (int h = 0; h < Hkv; ++h)
     for (size_t g = 0; g < groups.size(); ++g) {
-      const long long n = (groups[g].len + kUnit - 1) / kUnit, tiles = gw[G_WORDS * g + G_NT];
-      for (long long t = 0; t < tiles; ++t) {
-        int32_t* const tile = &tw[T_WORDS * (size_t)(gw[G_WORDS * g + G_TILE0] + h * tiles + t)];
-        tile[T_SEG] = (int32_t)(sw.size() / S_WORDS);
+      const long long n = (groups[g].len + kUnit - 1) / kUnit, rows = (long long)groups[g].members.size() * G;
+      const long long nt = (rows + kTile - 1) / kTile;
+      for (long long t = 0; t < nt; ++t) {
+        int32_t* const tile = &tiles[T_WORDS * (size_t)(tile0[g] + h * nt + t)];
+        tile[T_SEG] = (int32_t)(segs.size() / S_WORDS);
         for (long long u = 0; u < n;) {
-          while (first_unit(share) <= at) {  // this unit opens share `share` (empty ones before it too)
-            sh.push_back((int32_t)(sw.size() / S_WORDS));
-            if (++share == nsh) break;
+          while (share < nsh && first_unit(share) <= at) {  // (empty shares before it too)
+            begin.push_back((int32_t)(segs.size() / S_WORDS));
+            ++share;
           }
           const long long end = share == nsh ? total : first_unit(share);
           const long long take = std::min(n - u, end - at);
-          const int32_t w[S_WORDS] = {(int32_t)g, h, (int32_t)t, (int32_t)(u * kUnit),
+          const int32_t w[S_WORDS] = {groups[g].sid, groups[g].len, h, first_of[g], (int32_t)(t * kTile),
+                                      (int32_t)std::min<long long>(kTile, rows - t * kTile), (int32_t)(u * kUnit),
                                       (int32_t)std::min<long long>((u + take) * kUnit, groups[g].len)};
-          sw.insert(sw.end(), w, w + S_WORDS);
+          segs.insert(segs.end(), w, w + S_WORDS);
           u += take;
           at += take;
         }
-        tile[T_COUNT] = (int32_t)(sw.size() / S_WORDS) - tile[T_SEG];
+        tile[T_COUNT] = (int32_t)(segs.size() / S_WORDS) - tile[T_SEG];
       }
     }
-  while ((long long)sh.size() < nsh + 1) sh.push_back((int32_t)(sw.size() / S_WORDS));
+  begin.push_back((int32_t)(segs.size() / S_WORDS));
+  for (long long s = 0; s < nsh; ++s) {
+    int32_t w[H_WORDS] = {begin[s], begin[s + 1]};
+    if (begin[s] < begin[s + 1])
+      for (int i = 0; i < S_WORDS; ++i) w[H_COPY + i] = segs[S_WORDS * (size_t)begin[s] + i];
+    shares.insert(shares.end(), w, w + H_WORDS);
+  }
   plan.assign(PH_WORDS, 0);
   plan[PH_MAGIC] = kPlanMagic;
   plan[PH_B] = B;
@@ -911,32 +1259,35 @@ int make_plan(std::vector<int32_t>& plan, const int32_t* ids, const int32_t* len
   plan[PH_HQ] = Hq;
   plan[PH_HKV] = Hkv;
   plan[PH_BS] = bs;
-  plan[PH_NG] = (int32_t)groups.size();
   plan[PH_NSH] = (int32_t)nsh;
-  plan[PH_NSEG] = (int32_t)(sw.size() / S_WORDS);
-  plan[PH_NT] = (int32_t)triples;
+  plan[PH_NSEG] = (int32_t)(segs.size() / S_WORDS);
   plan[PH_MAXP] = (int32_t)maxp;
   auto add = [&](int word, const std::vector<int32_t>& v) {
+    while (plan.size() % 16) plan.push_back(0);
     plan[word] = (int32_t)plan.size();
     plan.insert(plan.end(), v.begin(), v.end());
   };
-  add(PH_GROUPS, gw);
-  add(PH_MEMBERS, mw);
+  add(PH_SHARES, shares);
+  // (a share past its last segment reads one record more than there are)
+  segs.resize(segs.size() + S_WORDS, 0);
+  add(PH_SEGS, segs);
+  add(PH_MEMBERS, members);
   add(PH_ENTRIES, entries);
-  add(PH_SHARES, sh);
-  add(PH_SEGS, sw);
-  add(PH_TILES, tw);
+  add(PH_TILES, tiles);
   plan[PH_INTS] = (int32_t)plan.size();
   return SPV_OK;
 }
 
-// The entries' own ranges for contexts up to max_ctx.
+// The entries' own ranges for contexts up to max_ctx: as many as make about 256
+// workgroups (one for each CU), none shorter than 256 keys (four waves with four pages each).
 void own_ranges(const int32_t* plan, int max_ctx, int* range, int* count) {
   const int bs = plan[PH_BS];
-  int keys = std::max(256, (max_ctx + 31) / 32);
-  keys = (keys + bs - 1) / bs * bs;
-  *range = keys;
-  *count = (max_ctx + keys - 1) / keys;
+  const long long G = (long long)plan[PH_C] * (plan[PH_HQ] / plan[PH_HKV]);
+  const long long wgs = (long long)plan[PH_B] * plan[PH_HKV] * ((G + kOwnRows - 1) / kOwnRows);
+  const long long want = std::max(1LL, std::min(256 / wgs, (long long)max_ctx / 256));
+  const long long keys = (max_ctx + want - 1) / want;
+  *range = (int)((keys + bs - 1) / bs * bs);
+  *count = (max_ctx + *range - 1) / *range;
 }
 
 long long part_rows(const int32_t* plan, int max_ctx) {
@@ -962,7 +1313,7 @@ int launch_valu(const SharedParams& p, long long grid, hipStream_t s) {
 
 template <int D, int KT>
 int launch_mfma(const SharedParams& p, long long grid, hipStream_t s) {
-  hipLaunchKernelGGL((shared_mfma_kernel<D, KT>), dim3((unsigned)grid), dim3(kThreads), 0, s, p);
+  hipLaunchKernelGGL((shared_mfma_kernel<D, KT>), dim3((unsigned)grid), dim3(kMfmaThreads), 0, s, p);
   SPV_CHECK_LAUNCH();
   return SPV_OK;
 }
@@ -978,7 +1329,7 @@ int launch_join(const SharedParams& p, hipStream_t s) {
 
 template <int QT>
 int launch(const SharedParams& p, int kv_dtype, hipStream_t s) {
-  const long long grid = p.shares + (long long)p.B * p.Hkv * p.own_tiles * p.own_max;
+  const long long grid = p.shares + p.own;
   int rc;
   // The matrix kernels apply the scale inside the exponent, to maxima of raw scores.
   const bool mfma = p.bs == 16 && (p.d == 64 || p.d == 128) && p.scale_log2 > 0.f && p.scale_log2 < INFINITY &&
@@ -1064,7 +1415,11 @@ int spv_shared_attn(void* out, const void* q, int q_dtype, const void* k_pool, c
   p.start = start_pos;
   p.lens = seq_lens;
   p.ctr = ctr;
-  p.plan = plan;
+  p.share_list = plan + h[PH_SHARES];
+  p.segs = plan + h[PH_SEGS];
+  p.members = plan + h[PH_MEMBERS];
+  p.entries = plan + h[PH_ENTRIES];
+  p.tiles = plan + h[PH_TILES];
   p.maxb = max_blocks_per_seq;
   p.B = B;
   p.C = C;
@@ -1079,13 +1434,13 @@ int spv_shared_attn(void* out, const void* q, int q_dtype, const void* k_pool, c
   p.shares = h[PH_NSH];
   p.max_ctx = max_ctx;
   own_ranges(h, max_ctx, &p.own_range, &p.own_max);
-  p.own_tiles = (p.G + kTile - 1) / kTile;
+  p.own_tiles = (p.G + kOwnRows - 1) / kOwnRows;
   p.own_part = (long long)h[PH_NSEG] * kTile;
   const long long rows = part_rows(h, max_ctx);
   // both grids: at most 2^32 threads
-  if (p.shares + (long long)B * num_kv_heads * p.own_tiles * p.own_max > (1LL << 23) ||
-      (long long)B * C * num_q_heads > (1LL << 23))
-    return SPV_ERR_UNSUPPORTED;
+  const long long own = (long long)B * num_kv_heads * p.own_tiles * p.own_max;
+  if (p.shares + own > (1LL << 22) || (long long)B * C * num_q_heads > (1LL << 23)) return SPV_ERR_UNSUPPORTED;
+  p.own = (int)own;
   p.part_ml = static_cast<float*>(workspace);
   p.part_o = p.part_ml + ml_floats((size_t)rows);
   p.scale_log2 = scale * kLog2e;
