@@ -11,18 +11,17 @@
 // So a prefix is walked once for all rows of all its entries: the rows of a
 // group (entries with one prefix and one length) that share a kv head are laid
 // end to end -- (member, chunk token, head of the group) -- and cut into tiles of
-// 128. All (tile, 64 keys) units, laid end to end, are cut into equal shares, one
-// per workgroup; a share's part of one tile is a segment and leaves a partial.
-// An entry's own keys are walked by further workgroups, one per (entry, kv head,
-// tile of its rows, range). A second launch joins each row's partials. Shares
-// and segments are listed on the host (the prefixes and their lengths change
-// when a request is admitted, not between rounds); the entries' own lengths are
-// read on the device.
+// 256, a prefix's keys into equal ranges; a segment is one tile over one range,
+// walked by one workgroup, and leaves a partial. Further workgroups walk the
+// entries' own keys, one per (entry, kv head, 64 of its rows, range). A second
+// launch joins each row's partials. The segments are listed on the host (the
+// prefixes and their lengths change when a request is admitted, not between
+// rounds); the entries' own lengths are read on the device.
 //
 // Matrix path (bf16 queries over bf16 or fp8 pages, fp16 over fp16, head_dim 64
-// or 128, 16-token blocks, a finite positive scale): a workgroup of four waves
-// takes 128 rows, 32 per wave, and stages 64 keys at a time in LDS (two buffers),
-// so a key read from the L2 once serves 128 rows. Per 16-key page and 16 rows
+// or 128, 16-token blocks, a finite positive scale): a workgroup of eight waves
+// takes a tile, 32 rows per wave, and stages 64 keys at a time in LDS, so that a
+// key read from the L2 once serves 256 rows. Per 16-key page and 16 rows
 //   S^T = K Q^T    v_mfma_f32_16x16x32, A = 16 keys x 32 dims, B = Q^T fragments
 //                  that stay in registers for the whole segment;
 //   O^T += V^T P^T v_mfma_f32_16x16x32_f16 over two pages, P in fp16.
@@ -50,10 +49,9 @@ namespace {
 
 constexpr float kLog2e = 1.4426950408889634f;
 
-// The plan: a header, then the shares, the segments, the members of the groups
-// (batch entries), each entry's place, and per (group, kv head, tile) its segments.
-// A share repeats its first segment, so that a workgroup's first keys are two
-// loads away from its launch.
+// The plan: a header, then the segments -- ordered by group, kv head, range, tile, so
+// that neighbours read the same keys --, the members of the groups (batch
+// entries), and each entry's place.
 enum : int {
   PH_MAGIC = 0,
   PH_INTS,  // length of the plan
@@ -62,23 +60,19 @@ enum : int {
   PH_HQ,
   PH_HKV,
   PH_BS,
-  PH_NSH,   // shares (a multiple of 8, or 0)
   PH_NSEG,  // segments
   PH_MAXP,  // longest prefix
-  PH_SHARES,
   PH_SEGS,
   PH_MEMBERS,
   PH_ENTRIES,
-  PH_TILES,
   PH_WORDS
 };
-constexpr int kPlanMagic = 0x53505233;
-// A segment: sequence and length of the prefix, kv head, first member and first row
-// of the tile, its rows, the keys.
+constexpr int kPlanMagic = 0x53505234;
+// A segment: sequence and length of the prefix, kv head, first member, first row of
+// the tile and its rows, the keys.
 enum : int { S_SID = 0, S_LEN, S_HEAD, S_FIRST, S_ROW0, S_ROWS, S_KEY0, S_KEY1, S_WORDS };
-enum : int { H_SEG = 0, H_END, H_COPY, H_WORDS = 16 };           // a share's segments; the first one's record
-enum : int { E_TILE0 = 0, E_NT, E_RANK, E_WORDS = 4 };            // first tile of kv head 0 (-1: no prefix), tiles per kv head
-enum : int { T_SEG = 0, T_COUNT, T_WORDS };
+// An entry: the group's first segment (-1: no prefix), its tiles, ranges, the entry's rank in it.
+enum : int { E_SEG = 0, E_TILES, E_RANGES, E_RANK, E_WORDS };
 constexpr int kTile = 256;    // rows of a prefix tile
 constexpr int kUnit = 64;     // keys
 constexpr int kOwnRows = 64;  // rows of an entry that a workgroup takes over its own keys
@@ -94,16 +88,13 @@ struct SharedParams {
   const int32_t* start;
   const int32_t* lens;
   int32_t* ctr;
-  const int32_t* share_list;  // the plan's sections
-  const int32_t* segs;
+  const int32_t* segs;  // the plan's sections
   const int32_t* members;
   const int32_t* entries;
-  const int32_t* tiles;
   float* part_o;   // partial rows x d
   float* part_ml;  // partial rows x 2
   int maxb, B, C, Hq, Hkv, ratio, G, d, bs, layer, cap;
-  int shares;              // workgroups that walk prefixes
-  int own;                 // workgroups that walk entries' own keys
+  int nseg, seg_wgs;       // segments, and their workgroups (a multiple of 8)
   int own_range, own_max;  // keys per own range (whole blocks), ranges per entry at most
   int own_tiles;           // tiles of an entry's rows
   int max_ctx;
@@ -124,7 +115,13 @@ __device__ __forceinline__ void flag_bad_read(const SharedParams& p, int b) {
   if (p.ctr) p.ctr[CTR_BAD_READ] = b + 1;
 }
 
-__device__ __forceinline__ void segment_item(const SharedParams& p, const int32_t* s, int seg, Item& it) {
+// The segment of workgroup `id`: workgroups go round-robin over the 8 XCDs, each of
+// which takes an eighth of the segments in a row, so that its L2 serves one range
+// of keys to workgroups that walk it side by side. False past the last one.
+__device__ __forceinline__ bool segment_item(const SharedParams& p, int id, Item& it) {
+  const int seg = (id & 7) * (p.seg_wgs >> 3) + (id >> 3);
+  if (seg >= p.nseg) return false;
+  const int32_t* s = p.segs + (size_t)seg * S_WORDS;
   it.first = s[S_FIRST];
   it.sid = s[S_SID];
   it.h = s[S_HEAD];
@@ -136,6 +133,7 @@ __device__ __forceinline__ void segment_item(const SharedParams& p, const int32_
   it.b = 0;
   it.part = (long long)seg * kTile;
   if (threadIdx.x == 0 && p.lens && p.lens[it.sid] < s[S_LEN]) flag_bad_read(p, p.members[it.first]);
+  return true;
 }
 
 // Own work `o`: false where the range has no keys.
@@ -156,11 +154,6 @@ __device__ __forceinline__ bool own_item(const SharedParams& p, int o, Item& it)
   it.part = p.own_part + ((long long)bh * p.own_max + s) * p.G + it.row0;
   return it.key0 < it.key1;
 }
-
-// The share of the prefix workgroup `id`: workgroups go round-robin over the 8
-// XCDs, each of which takes an eighth of the shares in a row -- of one kv head, if
-// there are few -- so that its L2 serves one stretch of keys to all of them.
-__device__ __forceinline__ int share_of(const SharedParams& p, int id) { return (id & 7) * (p.shares >> 3) + (id >> 3); }
 
 // Row R of an item's row order: its entry, chunk token and q head.
 __device__ __forceinline__ void row_at(const SharedParams& p, const Item& it, int R, int& b, int& j, int& hq) {
@@ -296,30 +289,15 @@ __device__ __forceinline__ void valu_item(const SharedParams& p, const Item& it,
   }
 }
 
-// Workgroups [0, own) walk entries' own keys, the others prefixes.
-template <typename F>
-__device__ __forceinline__ void for_segments(const SharedParams& p, F&& run) {
-  const int32_t* sh = p.share_list + (size_t)share_of(p, (int)blockIdx.x - p.own) * H_WORDS;
-  const int32_t* rec = sh + H_COPY;
-  const int end = sh[H_END];
-#pragma unroll 1
-  for (int s = sh[H_SEG]; s < end; ++s) {
-    Item it;
-    segment_item(p, rec, s, it);
-    run(it);
-    rec = p.segs + (size_t)(s + 1) * S_WORDS;
-  }
-}
-
+// Workgroups [0, seg_wgs) walk prefixes, the others entries' own keys: those are short
+// and fill the CUs that the prefixes leave.
 template <int QT, int KT>
 __global__ __launch_bounds__(kThreads) void shared_valu_kernel(SharedParams p) {
   extern __shared__ float smem[];
-  if ((int)blockIdx.x < p.own) {
-    Item it;
-    if (own_item(p, blockIdx.x, it)) valu_item<QT, KT, kMaxD, kThreads>(p, it, smem);
-    return;
-  }
-  for_segments(p, [&](const Item& it) { valu_item<QT, KT, kMaxD, kThreads>(p, it, smem); });
+  const int id = blockIdx.x;
+  Item it;
+  if (id < p.seg_wgs ? segment_item(p, id, it) : own_item(p, id - p.seg_wgs, it))
+    valu_item<QT, KT, kMaxD, kThreads>(p, it, smem);
 }
 
 // -------------------------------------------------------------- matrix kernels
@@ -813,7 +791,6 @@ struct Walk {
       if (!again) break;
     }
     write(it, w * 32, o, m, l, valid, kFp8 ? vref : ldexpf(1.f, -vk));
-    __syncthreads();  // the slots are free for the next segment
   }
 
   // A wave's partial rows r0 + 16 nt + i16 of an item.
@@ -1081,12 +1058,13 @@ __global__ __launch_bounds__(kMfmaThreads, 2) void shared_mfma_kernel(SharedPara
   static_assert(valu_lds(D) <= Lds<D>::kBytes, "the any-shape walk reuses this memory");
   __shared__ __align__(16) uint8_t smem[Lds<D>::kBytes];
   Walk<D, KT> walk(p, smem);
-  if ((int)blockIdx.x < p.own) {
-    Item it;
-    if (own_item(p, blockIdx.x, it)) walk.own(it);
-    return;
+  const int id = blockIdx.x;
+  Item it;
+  if (id < p.seg_wgs) {
+    if (segment_item(p, id, it)) walk.prefix(it);
+  } else if (own_item(p, id - p.seg_wgs, it)) {
+    walk.own(it);
   }
-  for_segments(p, [&](const Item& it) { walk.prefix(it); });
 }
 
 // ----------------------------------------------------------------------- join
@@ -1105,12 +1083,12 @@ __global__ __launch_bounds__(kThreads) void shared_join_kernel(SharedParams p) {
   const int32_t* e = p.entries + (size_t)b * E_WORDS;
   const int seen = min(max(p.start[b] + p.C, 0), p.max_ctx);
   int np = 0;
-  long long pre = 0;  // the prefix's partial row of segment 0
-  if (e[E_TILE0] >= 0) {
+  long long pre = 0, step = 0;  // the prefix's partial row of range s: pre + s * step
+  if (e[E_SEG] >= 0) {
     const long long R = (long long)e[E_RANK] * p.G + r;
-    const int32_t* t = p.tiles + (size_t)(e[E_TILE0] + h * e[E_NT] + (int)(R / kTile)) * T_WORDS;
-    np = t[T_COUNT];
-    pre = (long long)t[T_SEG] * kTile + R % kTile;
+    np = e[E_RANGES];
+    step = (long long)e[E_TILES] * kTile;
+    pre = (e[E_SEG] + (long long)h * np * e[E_TILES] + R / kTile) * kTile + R % kTile;
   }
   const int n = np + (seen + p.own_range - 1) / p.own_range;
   const long long own = p.own_part + (long long)(b * p.Hkv + h) * p.own_max * p.G + r;
@@ -1121,7 +1099,7 @@ __global__ __launch_bounds__(kThreads) void shared_join_kernel(SharedParams p) {
 #pragma unroll
     for (int k = 0; k < kJoin; ++k) {
       const int s = min(s0 + k, n - 1);
-      const size_t at = (size_t)(s < np ? pre + (long long)s * kTile : own + (long long)(s - np) * p.G);
+      const size_t at = (size_t)(s < np ? pre + s * step : own + (long long)(s - np) * p.G);
       ml[k] = *reinterpret_cast<const float2*>(&p.part_ml[at * 2]);
       const float* o = p.part_o + at * p.d;
       if constexpr (VEC) {
@@ -1175,15 +1153,37 @@ struct Group {
   std::vector<int> members;
 };
 
+// The range of keys per segment, in units: the one for which rounds of 256 workgroups
+// (one for each CU) end first, a workgroup taking its units and about as long as
+// kFixed more to start, to write its partial and to have it joined.
+constexpr int kCUs = 256, kFixed = 4;
+long long best_range(const std::vector<long long>& tiles, const std::vector<long long>& units) {
+  long long most = 1, best = 1, least = -1;
+  for (long long u : units) most = std::max(most, u);
+  // ceil(most / k) for every number of ranges k: no other length cuts the longest prefix evenly
+  for (long long k = 1; k <= most; ++k) {
+    const long long range = (most + k - 1) / k;
+    long long n = 0;
+    for (size_t g = 0; g < units.size(); ++g) n += tiles[g] * ((units[g] + range - 1) / range);
+    const long long time = (n + kCUs - 1) / kCUs * (range + kFixed);
+    if (least < 0 || time < least) {
+      least = time;
+      best = range;
+    }
+    if (n > 4 * kCUs && k > 1) break;  // more, shorter segments only add to the fixed part
+  }
+  return best;
+}
+
 int make_plan(std::vector<int32_t>& plan, const int32_t* ids, const int32_t* lens, int B, int C, int Hq, int Hkv,
               int bs) {
   const long long G = (long long)C * (Hq / Hkv);
   std::vector<Group> groups;
   std::map<std::pair<int32_t, int32_t>, size_t> index;
-  std::vector<int32_t> entries(E_WORDS * (size_t)B, 0), of(B, -1);
+  std::vector<int32_t> entries(E_WORDS * (size_t)B, 0), of(B, -1), members, segs;
   for (int b = 0; b < B; ++b) {
     if (ids[b] < -1 || lens[b] < 0) return SPV_ERR_ARG;
-    entries[E_WORDS * (size_t)b + E_TILE0] = -1;
+    entries[E_WORDS * (size_t)b + E_SEG] = -1;
     if (ids[b] < 0 || lens[b] == 0) continue;
     const size_t g = index.emplace(std::make_pair(ids[b], lens[b]), groups.size()).first->second;
     if (g == groups.size()) groups.push_back({ids[b], lens[b], {}});
@@ -1191,66 +1191,39 @@ int make_plan(std::vector<int32_t>& plan, const int32_t* ids, const int32_t* len
     of[b] = (int)g;
     groups[g].members.push_back(b);
   }
-  std::vector<int32_t> members, shares, segs, tiles;
-  std::vector<long long> tile0;
-  long long units = 0, maxp = 0, triples = 0;
+  std::vector<long long> tiles, units;
+  long long maxp = 0;
   for (const Group& x : groups) {
-    const long long nt = ((long long)x.members.size() * G + kTile - 1) / kTile;
-    tile0.push_back(triples);
-    triples += nt * Hkv;
-    if (triples > 0x7fffffffLL / kTile) return SPV_ERR_UNSUPPORTED;
-    units += nt * ((x.len + kUnit - 1) / kUnit);
+    tiles.push_back(((long long)x.members.size() * G + kTile - 1) / kTile);
+    units.push_back((x.len + kUnit - 1LL) / kUnit);
     maxp = std::max<long long>(maxp, x.len);
   }
-  for (int b = 0; b < B; ++b)
-    if (of[b] >= 0) {
-      entries[E_WORDS * (size_t)b + E_TILE0] = (int32_t)tile0[of[b]];
-      entries[E_WORDS * (size_t)b + E_NT] = (int32_t)((groups[of[b]].members.size() * G + kTile - 1) / kTile);
-    }
-  tiles.resize(T_WORDS * (size_t)triples);
-  // Shares: equal runs of the units of all kv heads, groups and tiles (in that
-  // order), one workgroup for each of the 256 CUs, or fewer where a share would be
-  // shorter than two units.
-  const long long total = units * Hkv;
-  const long long nsh = total ? std::max(1LL, std::min(256LL, (total + 1) / 2) / 8) * 8 : 0;
-  long long at = 0, share = 0;  // the unit in hand, and the share it opens next
-  auto first_unit = [&](long long s) { return s * total / nsh; };
-  std::vector<int32_t> first_of(groups.size());
+  std::vector<long long> all(tiles);
+  for (long long& t : all) t *= Hkv;
+  const long long range = best_range(all, units);
+  long long nseg = 0;
   for (size_t g = 0; g < groups.size(); ++g) {
-    first_of[g] = (int32_t)members.size();
-    members.insert(members.end(), groups[g].members.begin(), groups[g].members.end());
-  }
-  std::vector<int32_t> begin;
-  for (int h = 0; h < Hkv; ++h)
-    for (size_t g = 0; g < groups.size(); ++g) {
-      const long long n = (groups[g].len + kUnit - 1) / kUnit, rows = (long long)groups[g].members.size() * G;
-      const long long nt = (rows + kTile - 1) / kTile;
-      for (long long t = 0; t < nt; ++t) {
-        int32_t* const tile = &tiles[T_WORDS * (size_t)(tile0[g] + h * nt + t)];
-        tile[T_SEG] = (int32_t)(segs.size() / S_WORDS);
-        for (long long u = 0; u < n;) {
-          while (share < nsh && first_unit(share) <= at) {  // (empty shares before it too)
-            begin.push_back((int32_t)(segs.size() / S_WORDS));
-            ++share;
-          }
-          const long long end = share == nsh ? total : first_unit(share);
-          const long long take = std::min(n - u, end - at);
-          const int32_t w[S_WORDS] = {groups[g].sid, groups[g].len, h, first_of[g], (int32_t)(t * kTile),
-                                      (int32_t)std::min<long long>(kTile, rows - t * kTile), (int32_t)(u * kUnit),
-                                      (int32_t)std::min<long long>((u + take) * kUnit, groups[g].len)};
+    const Group& x = groups[g];
+    // equal ranges, of whole units
+    const long long ranges = (units[g] + range - 1) / range, per = (units[g] + ranges - 1) / ranges;
+    const long long used = (units[g] + per - 1) / per, rows = (long long)x.members.size() * G;
+    if ((nseg + tiles[g] * Hkv * used) > 0x7fffffffLL / kTile) return SPV_ERR_UNSUPPORTED;
+    for (int h = 0; h < Hkv; ++h)
+      for (long long s = 0; s < used; ++s)
+        for (long long t = 0; t < tiles[g]; ++t) {
+          const int32_t w[S_WORDS] = {x.sid, x.len, h, (int32_t)members.size(), (int32_t)(t * kTile),
+                                      (int32_t)std::min<long long>(kTile, rows - t * kTile), (int32_t)(s * per * kUnit),
+                                      (int32_t)std::min<long long>((s + 1) * per * kUnit, x.len)};
           segs.insert(segs.end(), w, w + S_WORDS);
-          u += take;
-          at += take;
         }
-        tile[T_COUNT] = (int32_t)(segs.size() / S_WORDS) - tile[T_SEG];
-      }
+    for (int b : x.members) {
+      int32_t* const e = &entries[E_WORDS * (size_t)b];
+      e[E_SEG] = (int32_t)nseg;
+      e[E_TILES] = (int32_t)tiles[g];
+      e[E_RANGES] = (int32_t)used;
     }
-  begin.push_back((int32_t)(segs.size() / S_WORDS));
-  for (long long s = 0; s < nsh; ++s) {
-    int32_t w[H_WORDS] = {begin[s], begin[s + 1]};
-    if (begin[s] < begin[s + 1])
-      for (int i = 0; i < S_WORDS; ++i) w[H_COPY + i] = segs[S_WORDS * (size_t)begin[s] + i];
-    shares.insert(shares.end(), w, w + H_WORDS);
+    nseg += tiles[g] * Hkv * used;
+    members.insert(members.end(), x.members.begin(), x.members.end());
   }
   plan.assign(PH_WORDS, 0);
   plan[PH_MAGIC] = kPlanMagic;
@@ -1259,21 +1232,16 @@ int make_plan(std::vector<int32_t>& plan, const int32_t* ids, const int32_t* len
   plan[PH_HQ] = Hq;
   plan[PH_HKV] = Hkv;
   plan[PH_BS] = bs;
-  plan[PH_NSH] = (int32_t)nsh;
-  plan[PH_NSEG] = (int32_t)(segs.size() / S_WORDS);
+  plan[PH_NSEG] = (int32_t)nseg;
   plan[PH_MAXP] = (int32_t)maxp;
   auto add = [&](int word, const std::vector<int32_t>& v) {
     while (plan.size() % 16) plan.push_back(0);
     plan[word] = (int32_t)plan.size();
     plan.insert(plan.end(), v.begin(), v.end());
   };
-  add(PH_SHARES, shares);
-  // (a share past its last segment reads one record more than there are)
-  segs.resize(segs.size() + S_WORDS, 0);
   add(PH_SEGS, segs);
   add(PH_MEMBERS, members);
   add(PH_ENTRIES, entries);
-  add(PH_TILES, tiles);
   plan[PH_INTS] = (int32_t)plan.size();
   return SPV_OK;
 }
@@ -1329,7 +1297,7 @@ int launch_join(const SharedParams& p, hipStream_t s) {
 
 template <int QT>
 int launch(const SharedParams& p, int kv_dtype, hipStream_t s) {
-  const long long grid = p.shares + p.own;
+  const long long grid = p.seg_wgs + (long long)p.B * p.Hkv * p.own_tiles * p.own_max;
   int rc;
   // The matrix kernels apply the scale inside the exponent, to maxima of raw scores.
   const bool mfma = p.bs == 16 && (p.d == 64 || p.d == 128) && p.scale_log2 > 0.f && p.scale_log2 < INFINITY &&
@@ -1415,11 +1383,9 @@ int spv_shared_attn(void* out, const void* q, int q_dtype, const void* k_pool, c
   p.start = start_pos;
   p.lens = seq_lens;
   p.ctr = ctr;
-  p.share_list = plan + h[PH_SHARES];
   p.segs = plan + h[PH_SEGS];
   p.members = plan + h[PH_MEMBERS];
   p.entries = plan + h[PH_ENTRIES];
-  p.tiles = plan + h[PH_TILES];
   p.maxb = max_blocks_per_seq;
   p.B = B;
   p.C = C;
@@ -1431,7 +1397,8 @@ int spv_shared_attn(void* out, const void* q, int q_dtype, const void* k_pool, c
   p.bs = block_size;
   p.layer = layer;
   p.cap = capacity;
-  p.shares = h[PH_NSH];
+  p.nseg = h[PH_NSEG];
+  p.seg_wgs = (p.nseg + 7) / 8 * 8;
   p.max_ctx = max_ctx;
   own_ranges(h, max_ctx, &p.own_range, &p.own_max);
   p.own_tiles = (p.G + kOwnRows - 1) / kOwnRows;
@@ -1439,8 +1406,7 @@ int spv_shared_attn(void* out, const void* q, int q_dtype, const void* k_pool, c
   const long long rows = part_rows(h, max_ctx);
   // both grids: at most 2^32 threads
   const long long own = (long long)B * num_kv_heads * p.own_tiles * p.own_max;
-  if (p.shares + own > (1LL << 22) || (long long)B * C * num_q_heads > (1LL << 23)) return SPV_ERR_UNSUPPORTED;
-  p.own = (int)own;
+  if (p.seg_wgs + own > (1LL << 22) || (long long)B * C * num_q_heads > (1LL << 23)) return SPV_ERR_UNSUPPORTED;
   p.part_ml = static_cast<float*>(workspace);
   p.part_o = p.part_ml + ml_floats((size_t)rows);
   p.scale_log2 = scale * kLog2e;

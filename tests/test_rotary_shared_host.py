@@ -36,11 +36,10 @@ def _plan(lib, ids, lens, C=3, Hq=4, Hkv=2, bs=16):
 
 
 def _sections(plan):
-    """(shares, segments, members, entries, tiles) of a plan as lists of records."""
-    B, nsh, nseg = plan[2], plan[7], plan[8]
-    at = plan[10:15]
+    """(segments, members, entries) of a plan as lists of records."""
+    at = plan[9:12]
     cut = lambda o, n, w: [plan[o + i * w:o + (i + 1) * w] for i in range(n)]  # noqa: E731
-    return cut(at[0], nsh, 16), cut(at[1], nseg, 8), plan[at[2]:at[3]], cut(at[3], B, 4), cut(at[4], (len(plan) - at[4]) // 2, 2)
+    return cut(at[0], plan[7], 8), plan[at[1]:at[2]], cut(at[2], plan[2], 4)
 
 
 @pytest.mark.parametrize("ids,lens", [
@@ -56,7 +55,7 @@ def test_plan_covers_every_row_and_key_once(lib, ids, lens):
     G = C * Hq // Hkv
     plan = _plan(lib, ids, lens, C, Hq, Hkv, bs)
     assert plan[1] == len(plan)
-    shares, segs, members, entries, tiles = _sections(plan)
+    segs, members, entries = _sections(plan)
     want = {}
     for b, (s, n) in enumerate(zip(ids, lens)):
         if s >= 0 and n > 0:
@@ -64,29 +63,21 @@ def test_plan_covers_every_row_and_key_once(lib, ids, lens):
     seen = 0
     for (sid, n), batch in want.items():
         rows = len(batch) * G
-        for rank, b in enumerate(batch):
-            assert entries[b][1:3] == [-(-rows // 256), rank] and entries[b][0] == entries[batch[0]][0]
+        first, nt, nr = entries[batch[0]][:3]
+        assert [entries[b] for b in batch] == [[first, nt, nr, rank] for rank in range(len(batch))]
+        assert first == seen and nt == -(-rows // 256)
         for h in range(Hkv):
-            for t in range(-(-rows // 256)):
-                at, k = tiles[entries[batch[0]][0] + h * -(-rows // 256) + t]
-                part = segs[at:at + k]
-                seen += k
+            for t in range(nt):
+                part = [segs[first + (h * nr + s) * nt + t] for s in range(nr)]
                 for x in part:
                     assert x[:3] == [sid, n, h] and members[x[3]:x[3] + len(batch)] == batch
                     assert x[4] == 256 * t and x[5] == min(256, rows - 256 * t)
                     assert x[6] < x[7] and x[6] % 64 == 0
                 assert part[0][6] == 0 and part[-1][7] == n
                 assert all(x[7] == y[6] for x, y in zip(part, part[1:]))
-    assert seen == len(segs) and len(tiles) == Hkv * sum(-(-len(x) * G // 256) for x in want.values())
+        seen += Hkv * nt * nr
+    assert seen == len(segs)
     assert all(entries[b][0] == -1 for b, (s, n) in enumerate(zip(ids, lens)) if s < 0 or n == 0)
-    # the shares cover the segments in order, with equal numbers of 64-key units
-    assert len(shares) % 8 == 0 and bool(shares) == bool(want)
-    units, at = [], 0
-    for s in shares:
-        assert s[0] == at and s[1] >= at and (s[0] == s[1] or s[2:10] == segs[s[0]])
-        units.append(sum(-(-(x[7] - x[6]) // 64) for x in segs[s[0]:s[1]]))
-        at = s[1]
-    assert at == len(segs) and (not units or max(units) - min(units) <= 1)
 
 
 def test_plan_refusals(lib):
