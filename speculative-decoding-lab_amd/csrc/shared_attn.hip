@@ -130,9 +130,9 @@ __device__ __forceinline__ bool segment_item(const SharedParams& p, int id, Item
   it.key0 = s[S_KEY0];
   it.key1 = s[S_KEY1];
   it.start = 0x3fffffff;
-  it.b = 0;
+  it.b = p.members[it.first];
   it.part = (long long)seg * kTile;
-  if (threadIdx.x == 0 && p.lens && p.lens[it.sid] < s[S_LEN]) flag_bad_read(p, p.members[it.first]);
+  if (threadIdx.x == 0 && p.lens && p.lens[it.sid] < s[S_LEN]) flag_bad_read(p, it.b);
   return true;
 }
 
@@ -171,7 +171,7 @@ __device__ __forceinline__ void row_at(const SharedParams& p, const Item& it, in
 __device__ __forceinline__ int block_of(const SharedParams& p, const Item& it, int pos) {
   const int phys = p.tables[(size_t)it.sid * p.maxb + pos / p.bs];
   if ((unsigned)phys < (unsigned)p.cap) return phys;
-  flag_bad_read(p, it.first >= 0 ? p.members[it.first] : it.b);
+  flag_bad_read(p, it.b);
   return 0;
 }
 
@@ -336,6 +336,7 @@ __device__ __forceinline__ int stage_exponent(float mx) {
   return min(126, max(-126, 9 - e));
 }
 
+#define SPV_INLINE __attribute__((always_inline))  // on the walks' lambdas: their operands stay in registers
 constexpr int kWaves = 8;
 constexpr int kMfmaThreads = 64 * kWaves;
 
@@ -390,14 +391,16 @@ struct Walk {
   }
   __device__ __forceinline__ int safe_id(const Item& it, int phys) const {
     if ((unsigned)phys < (unsigned)p.cap) return phys;
-    flag_bad_read(p, it.first >= 0 ? p.members[it.first] : it.b);
+    flag_bad_read(p, it.b);
     return 0;
   }
   __device__ __forceinline__ float2 scales_of(int phys) const {
     return *reinterpret_cast<const float2*>(p.scales + ((size_t)p.layer * p.cap + phys) * 2);
   }
-  __device__ __forceinline__ const uint8_t* page(const void* pool, int phys, int h) const {
-    return static_cast<const uint8_t*>(pool) + (((size_t)p.layer * p.cap + phys) * p.Hkv + h) * (size_t)(16 * D * ES);
+  // A block's page of kv head h, counted in pages (the host checks that they fit 31 bits), and its address.
+  __device__ __forceinline__ int page_of(int phys, int h) const { return (p.layer * p.cap + phys) * p.Hkv + h; }
+  __device__ __forceinline__ const uint8_t* page(const void* pool, int index) const {
+    return static_cast<const uint8_t*>(pool) + (size_t)(uint32_t)index * (16 * D * ES);
   }
   __device__ __forceinline__ uint32_t wg_max(uint32_t m) {  // the workgroup's largest m, in every thread
 #pragma unroll
@@ -411,8 +414,10 @@ struct Walk {
     return m;
   }
 
-  // ---- a segment of a prefix: 256 rows, 32 per wave, 64 keys at a time in LDS.
-  __device__ __forceinline__ void prefix(const Item& it) {
+  // ---- a segment of a prefix: 256 rows, 32 per wave, 64 keys at a time in LDS. False
+  // (bf16 values) where a value passed fp16's range: the caller then runs it again with
+  // `whole`, the staging power from the range's largest |v| instead of its first tile's.
+  __device__ __forceinline__ bool prefix(const Item& it, bool whole) {
     using LD = Lds<D>;
     constexpr int KP = LD::KP, VP = LD::VP;
     uint16_t* const sK = reinterpret_cast<uint16_t*>(smem);
@@ -425,16 +430,17 @@ struct Walk {
     const int pages = (key1 - key0 + 15) >> 4, n = (key1 - key0 + kUnit - 1) / kUnit;
     const int32_t* table = p.tables + (size_t)__builtin_amdgcn_readfirstlane(it.sid) * p.maxb + (key0 >> 4);
 
-    // Block ids (and an fp8 page's scales) of 64 pages, 16 tiles, in the lanes of a
-    // register, the next 64 ids read half a window ahead; pages past the range
-    // repeat its last one.
+    // Page numbers (and an fp8 page's scales) of 64 pages, 16 tiles, in the lanes of a
+    // register, the next 64 ids read with every tile (a branch around the read costs
+    // more than the read); pages past the range repeat its last one.
     int ids = 0, idn = 0;
     float ksc = 1.f, vsc = 1.f, vref = 1.f;  // vref, fp8: the range's largest V scale
-    auto read_ids = [&](int first) { return table[min(first + lane, pages - 1)]; };
-    auto open_window = [&](int raw) {
-      ids = safe_id(it, raw);
+    auto read_ids = [&](int first) SPV_INLINE { return table[min(first + lane, pages - 1)]; };
+    auto open_window = [&](int raw) SPV_INLINE {
+      const int phys = safe_id(it, raw);
+      ids = page_of(phys, h);
       if constexpr (kFp8) {
-        const float2 s = scales_of(ids);
+        const float2 s = scales_of(phys);
         ksc = s.x;
         vsc = vref > 0.f ? s.y / vref : 0.f;
       }
@@ -444,7 +450,6 @@ struct Walk {
     int lim[NT];
     bool valid[NT];
     load_q(it, w * 32, qf, lim, valid);
-    const bool active = w * 32 < it.rows;
 
     // Staging: each group stages half of a tile. K: 16-byte pieces of a page in
     // memory order. V: (dim, page pair, half) items: 8 keys of the even and 8 of the
@@ -460,23 +465,23 @@ struct Walk {
     };
     constexpr int kPer = D * ES;  // 16-byte pieces of a page
     // Group threads beyond a half's pieces (the smallest tiles) repeat one of them.
-    auto k_piece = [&](int i) { return grp * (kKP / 2) + (gt + i * 256) % (kKP / 2); };
-    auto v_item = [&](int i) { return grp * (kVI / 2) + (gt + i * 256) % (kVI / 2); };
-    auto k_page = [&](int i) { return (grp * (kKP / 2) + (gw * 64 + i * 256) % (kKP / 2)) / kPer; };  // of the wave's pieces
-    auto v_pair = [&](int i) { return (grp * (kVI / 2) + (gw * 64 + i * 256) % (kVI / 2)) / (2 * D); };
-    auto load = [&](Stage& S, int t) {
+    auto k_piece = [&](int i) SPV_INLINE { return grp * (kKP / 2) + (gt + i * 256) % (kKP / 2); };
+    auto v_item = [&](int i) SPV_INLINE { return grp * (kVI / 2) + (gt + i * 256) % (kVI / 2); };
+    auto k_page = [&](int i) SPV_INLINE { return (grp * (kKP / 2) + (gw * 64 + i * 256) % (kKP / 2)) / kPer; };  // of the wave's pieces
+    auto v_pair = [&](int i) SPV_INLINE { return (grp * (kVI / 2) + (gw * 64 + i * 256) % (kVI / 2)) / (2 * D); };
+    auto load = [&](Stage& S, int t) SPV_INLINE {
 #pragma unroll
       for (int i = 0; i < kKN1; ++i) {
-        const int phys = __builtin_amdgcn_readlane(ids, (4 * t + k_page(i)) & 63);
-        S.k[i] = *reinterpret_cast<const u32x4_t*>(page(p.kpool, phys, h) + 16 * (k_piece(i) % kPer));
+        const int pg = __builtin_amdgcn_readlane(ids, (4 * t + k_page(i)) & 63);
+        S.k[i] = *reinterpret_cast<const u32x4_t*>(page(p.kpool, pg) + 16 * (k_piece(i) % kPer));
       }
 #pragma unroll
       for (int i = 0; i < kVN; ++i) {
         const int q = v_pair(i), c = v_item(i) % (2 * D);
 #pragma unroll
         for (int hh = 0; hh < 2; ++hh) {
-          const int phys = __builtin_amdgcn_readlane(ids, (4 * t + 2 * q + hh) & 63);
-          const uint8_t* v = page(p.vpool, phys, h) + 8 * ES * c;
+          const int pg = __builtin_amdgcn_readlane(ids, (4 * t + 2 * q + hh) & 63);
+          const uint8_t* v = page(p.vpool, pg) + 8 * ES * c;
           if constexpr (kFp8) {
             const uint2 x = *reinterpret_cast<const uint2*>(v);
             S.v[i][hh] = u32x4_t{x.x, x.y, 0u, 0u};
@@ -486,19 +491,20 @@ struct Walk {
         }
       }
     };
-    // Tile t's loads, by the window it lies in (tiles are loaded in order).
-    auto load_next = [&](Stage& S, int t) {
-      if (t < n) {
-        if ((t & 15) == 0) open_window(idn);
-        if ((t & 15) == 8) idn = read_ids(4 * (t + 8));
-      }
+    // The window of tile t, before its loads (tiles are loaded in order).
+    auto window = [&](int t) SPV_INLINE {
+      if (t < n && (t & 15) == 0) open_window(idn);
+      idn = read_ids(4 * ((t & ~15) + 16));
+    };
+    auto load_next = [&](Stage& S, int t) SPV_INLINE {
+      window(t);
       load(S, min(t, n - 1));
     };
     float vs = 1.f;     // bf16: the staging factor 2^vk
     int vk = 0;
     uint32_t vmax = 0;  // bf16: largest |v| bits staged (both halves)
     // Zeroes the values of keys past the range's end.
-    auto edge = [&](Stage& S, int t) {
+    auto edge = [&](Stage& S, int t) SPV_INLINE {
       const int t0 = key0 + t * kUnit;
       if (t0 + kUnit <= key1) return;
 #pragma unroll
@@ -517,8 +523,7 @@ struct Walk {
         }
       }
     };
-    auto store = [&](Stage& S, int t, int kslot, int vslot) {
-      edge(S, min(t, n - 1));
+    auto store = [&](Stage& S, int kslot, int vslot) SPV_INLINE {
       uint16_t* const K = sK + kslot * LD::kK;
       uint16_t* const V = sV + vslot * LD::kV;
 #pragma unroll
@@ -578,7 +583,7 @@ struct Walk {
     f32x4_t sc[4][NT];            // S^T of the tile in the walk
     uint32_t ph[2][NT][4];        // its P, two pages an operand
     float ks_t = 1.f, vs_t = 1.f;  // fp8: scales of the window of the tile in the walk
-    auto pv = [&](int vslot) {
+    auto pv = [&](int vslot) SPV_INLINE {
       const uint16_t* V = sV + vslot * LD::kV;
 #pragma unroll
       for (int q = 0; q < 2; ++q)
@@ -593,21 +598,23 @@ struct Walk {
                 o[mt][nt], 0, 0, 0);
         }
     };
-    auto qk = [&](int kslot) {
+    auto qk = [&](int kslot) SPV_INLINE {
       const uint16_t* K = sK + kslot * LD::kK;
 #pragma unroll
-      for (int kt = 0; kt < 4; ++kt) {
+      for (int kt = 0; kt < 4; ++kt)
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) sc[kt][nt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int ks = 0; ks < KS; ++ks) {
+      for (int ks = 0; ks < KS; ++ks) {
+#pragma unroll
+        for (int kt = 0; kt < 4; ++kt) {
           const uint4 kf = *reinterpret_cast<const uint4*>(&K[(16 * kt + i16) * KP + 32 * ks + 8 * g]);
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) sc[kt][nt] = mfma_qk(kf, qf[nt][ks], sc[kt][nt]);
         }
       }
     };
-    auto softmax = [&](int t) {
+    auto softmax = [&](int t) SPV_INLINE {
       if constexpr (kFp8) {
         if ((t & 15) == 0) ks_t = ksc, vs_t = vsc;
 #pragma unroll
@@ -681,7 +688,7 @@ struct Walk {
       }
     };
     // A phase ends at a workgroup barrier that no instruction is scheduled across.
-    auto phase_end = [] {
+    auto phase_end = []() SPV_INLINE {
       __builtin_amdgcn_sched_barrier(0);
       __syncthreads();
       __builtin_amdgcn_sched_barrier(0);
@@ -697,13 +704,15 @@ struct Walk {
     // The walk. Group 0 runs phases M(0), V(0), M(1), V(1), ... and group 1 the same
     // one phase later, a barrier after each, so that on every SIMD one wave's
     // softmax runs beside the other's matrix instructions:
-    //   M(t): O^T += V^T P^T of tile t - 1, then S^T of tile t
-    //   V(t): softmax of tile t; stage the group's half of tile t + 1 + grp
-    // Tile x is whole in LDS after V(x - 2) of group 1 and V(x - 1) of group 0; its K
-    // is read in M(x), its V in M(x + 1) of either group: two K slots, three V slots.
-    bool again = false;
+    //   M(t): stage the group's half of tile t + 1, load that of tile t + 3;
+    //         O^T += V^T P^T of tile t - 1, then S^T of tile t
+    //   V(t): softmax of tile t
+    // The staging goes with the matrix instructions, which leave the other issue ports
+    // free (beside the softmax, the longer phase, it took a third more time). Tile x
+    // is staged in M(x - 1), its K read in M(x) and its V in M(x + 1) of either group:
+    // two K slots, three V slots.
     Stage st0, st1;
-    for (int attempt = 0;; ++attempt) {
+    {
 #pragma unroll
       for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
@@ -716,11 +725,11 @@ struct Walk {
       }
       idn = raw;
       load_next(st0, 0);
-      if (grp == 1) load_next(st1, 1);
+      load_next(st1, 1);
       if constexpr (!kF16 && !kFp8) {
-        // The largest finite |v| of the first tile, or (again) of the whole range.
+        // The largest finite |v| of the first tile, or of the whole range.
         uint32_t mx = 0;
-        auto take = [&](u32x4_t x) {
+        auto take = [&](u32x4_t x) SPV_INLINE {
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             const uint32_t lo = x[e] & 0x7fffu, hi = (x[e] >> 16) & 0x7fffu;
@@ -728,8 +737,8 @@ struct Walk {
             mx = max(mx, hi < 0x7f80u ? hi : 0u);
           }
         };
-        if (!again) {
-          edge(st0, 0);
+        edge(st0, 0);
+        if (!whole) {
 #pragma unroll
           for (int i = 0; i < kVN; ++i)
 #pragma unroll
@@ -737,7 +746,7 @@ struct Walk {
         } else {
           for (int c = tid; c < pages * 2 * D; c += kMfmaThreads) {  // 8 keys of a dim
             const int pg = c / (2 * D), k0 = key0 + 16 * pg + 8 * (c & 1);
-            u32x4_t x = *reinterpret_cast<const u32x4_t*>(page(p.vpool, safe_id(it, table[pg]), h) + 16 * (c % (2 * D)));
+            u32x4_t x = *reinterpret_cast<const u32x4_t*>(page(p.vpool, page_of(safe_id(it, table[pg]), h)) + 16 * (c % (2 * D)));
 #pragma unroll
             for (int e = 0; e < 8; ++e) x[e / 2] &= k0 + e >= key1 ? ~(0xffffu << (16 * (e & 1))) : ~0u;
             take(x);
@@ -747,27 +756,40 @@ struct Walk {
         vs = ldexpf(1.f, vk);
         vmax = 0;
       }
-      store(st0, 0, 0, 0);
-      if (grp == 1) store(st1, 1, 1, 1);
-      load_next(st0, 1 + grp);
-      load_next(st1, 2 + grp);
+      edge(st0, 0);
+      store(st0, 0, 0);
+      load_next(st0, 2);
+      edge(st1, min(1, n - 1));
+      store(st1, 1, 1);
+      load_next(st1, 3);
       phase_end();
       if (grp == 1) phase_end();
-      if (active) qk(0);  // M(0)
+      qk(0);  // M(0); tiles 0 and 1 are staged above
       phase_end();
-      int ksl = (1 + grp) & 1, vst = 1 + grp, vrd = 0;  // slots of the tile staged in V(t); V slot of tile t
-      auto step = [&](int t, Stage& X) {
-        if (active) softmax(t);
-        store(X, t + 1 + grp, ksl, vst);
-        load_next(X, t + 3 + grp);
+      int vrd = 0;  // V slot of tile t
+      auto step = [&](int t, Stage& X) SPV_INLINE {  // V(t), M(t + 1); X: tile t + 2
+        softmax(t);
+        edge(X, min(t + 2, n - 1));
+        window(t + 4);
         phase_end();
-        if (active) {
-          pv(vrd);
-          qk((t + 1) & 1);
+        __builtin_amdgcn_s_setprio(1);
+        store(X, t & 1, vrd == 0 ? 2 : vrd - 1);
+        load(X, min(t + 4, n - 1));
+        pv(vrd);
+        qk((t + 1) & 1);
+        // kAhead operand reads in flight ahead of the matrix instructions (left alone the
+        // scheduler keeps two, and each pair waits for its own: 0.83 PFLOP/s; three to
+        // eight ahead, 0.86 to 0.91)
+        constexpr int kAhead = 4;
+        __builtin_amdgcn_sched_group_barrier(0x100, kAhead, 0);
+#pragma unroll
+        for (int i = 0; i < 2 * MT + 4 * KS - kAhead; ++i) {
+          __builtin_amdgcn_sched_group_barrier(0x008, 2, 0);
+          __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
         }
+        __builtin_amdgcn_sched_group_barrier(0x008, 2 * kAhead, 0);
+        __builtin_amdgcn_s_setprio(0);
         phase_end();
-        ksl ^= 1;
-        vst = vst == 2 ? 0 : vst + 1;
         vrd = vrd == 2 ? 0 : vrd + 1;
       };
       int t = 0;
@@ -779,18 +801,18 @@ struct Walk {
         step(t, st0);
         ++t;
       }
-      if (active) softmax(t);
+      softmax(t);
       phase_end();
-      if (active) pv(vrd);
+      pv(vrd);
       if (grp == 0) phase_end();
-      if constexpr (kF16 || kFp8) break;
-      if (attempt == 1) break;
-      // bits of the largest |v| that stays within fp16 at this power
-      const uint32_t top = min(__float_as_uint(ldexpf(65504.f, -vk)) >> 16, 0x7f7fu);
-      again = __syncthreads_or((vmax & 0xffffu) > top || (vmax >> 16) > top);
-      if (!again) break;
+      if constexpr (!kF16 && !kFp8) {
+        // bits of the largest |v| that stays within fp16 at this power
+        const uint32_t top = min(__float_as_uint(ldexpf(65504.f, -vk)) >> 16, 0x7f7fu);
+        if (__syncthreads_or((vmax & 0xffffu) > top || (vmax >> 16) > top) && !whole) return false;
+      }
     }
     write(it, w * 32, o, m, l, valid, kFp8 ? vref : ldexpf(1.f, -vk));
+    return true;
   }
 
   // A wave's partial rows r0 + 16 nt + i16 of an item.
@@ -843,10 +865,10 @@ struct Walk {
       uint4 k[KS];  // fp8: 8 bytes
       uint2 v[MT];  // fp8: 4 bytes
     };
-    auto load = [&](Page& P, int i) {
-      const int phys = __builtin_amdgcn_readlane(ids, i & 63);
-      const uint8_t* K = page(p.kpool, phys, h) + (i16 * D + 8 * g) * ES;
-      const uint8_t* V = page(p.vpool, phys, h) + (i16 * 16 + 4 * g) * ES;
+    auto load = [&](Page& P, int i) SPV_INLINE {
+      const int pg = __builtin_amdgcn_readlane(ids, i & 63);
+      const uint8_t* K = page(p.kpool, pg) + (i16 * D + 8 * g) * ES;
+      const uint8_t* V = page(p.vpool, pg) + (i16 * 16 + 4 * g) * ES;
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) {
         if constexpr (kFp8) {
@@ -862,7 +884,7 @@ struct Walk {
         else P.v[mt] = *reinterpret_cast<const uint2*>(V + 512 * mt);
       }
     };
-    auto compute = [&](Page& P, int i) {
+    auto compute = [&](Page& P, int i) SPV_INLINE {
       const int k0 = key0 + 16 * (kw + nk * i);
       f32x4_t sc[NT];
 #pragma unroll
@@ -977,9 +999,10 @@ struct Walk {
       }
     };
     for (int base = 0; base < mine; base += 64) {  // 64 of the wave's pages, their ids in the lanes
-      ids = safe_id(it, table[min(kw + nk * (base + lane), pages - 1)]);
+      const int phys = safe_id(it, table[min(kw + nk * (base + lane), pages - 1)]);
+      ids = page_of(phys, h);
       if constexpr (kFp8) {
-        const float2 s = scales_of(ids);
+        const float2 s = scales_of(phys);
         ksc = s.x;
         vsc = s.y;
       }
@@ -1061,7 +1084,9 @@ __global__ __launch_bounds__(kMfmaThreads, 2) void shared_mfma_kernel(SharedPara
   const int id = blockIdx.x;
   Item it;
   if (id < p.seg_wgs) {
-    if (segment_item(p, id, it)) walk.prefix(it);
+    if (segment_item(p, id, it))
+      for (int whole = 0; !walk.prefix(it, whole); ++whole) {
+      }
   } else if (own_item(p, id - p.seg_wgs, it)) {
     walk.own(it);
   }
@@ -1300,7 +1325,8 @@ int launch(const SharedParams& p, int kv_dtype, hipStream_t s) {
   const long long grid = p.seg_wgs + (long long)p.B * p.Hkv * p.own_tiles * p.own_max;
   int rc;
   // The matrix kernels apply the scale inside the exponent, to maxima of raw scores.
-  const bool mfma = p.bs == 16 && (p.d == 64 || p.d == 128) && p.scale_log2 > 0.f && p.scale_log2 < INFINITY &&
+  // They count pages in 31 bits.
+  const bool mfma = (long long)(p.layer + 1) * p.cap * p.Hkv < (1LL << 31) && p.bs == 16 && (p.d == 64 || p.d == 128) && p.scale_log2 > 0.f && p.scale_log2 < INFINITY &&
                     ((QT == SPV_BF16 && (kv_dtype == SPV_BF16 || kv_dtype == SPV_FP8E4M3)) ||
                      (QT == SPV_F16 && kv_dtype == SPV_F16));
   if (mfma) {
