@@ -31,9 +31,10 @@
 // output alone takes 1.7e-3); fp16 has 11 bits. bf16 values are staged as fp16
 // times a power of two per segment, chosen from the first tile's largest |v|
 // (which lands in [2^8, 2^9): every value from 2^-25 of it up is exact, a smaller
-// one is off by at most 2^-33 of it); where a later value would pass fp16's range
-// the segment runs again with the power from its largest |v|. fp8 codes are fp16
-// values; a block's V scale, over the segment's largest, multiplies P.
+// one is off by at most 2^-33 of it); where a later value would pass fp16's range, or
+// the first tile was so small beside the rest that it says nothing, the segment is
+// walked again in fp32 (the any-shape walk, some thirty times as long). fp8 codes are
+// fp16 values; a block's V scale, over the segment's largest, multiplies P.
 #include <math.h>
 
 #include <algorithm>
@@ -363,10 +364,10 @@ struct Walk {
   const int tid, lane, w, i16, g;
   const float sl2, inv_sl2;
 
-  __device__ __forceinline__ Walk(const SharedParams& p_, uint8_t* smem_)
-      : p(p_), smem(smem_), sMax(reinterpret_cast<uint32_t*>(smem_ + Lds<D>::kBytes) - kWaves), tid(threadIdx.x),
-        lane(threadIdx.x & 63), w(__builtin_amdgcn_readfirstlane(threadIdx.x >> 6)), i16(threadIdx.x & 15),
-        g((threadIdx.x & 63) >> 4), sl2(p_.scale_log2), inv_sl2(1.f / p_.scale_log2) {}
+  __device__ __forceinline__ Walk(const SharedParams& p_, uint8_t* smem_, int tid_)
+      : p(p_), smem(smem_), sMax(reinterpret_cast<uint32_t*>(smem_ + Lds<D>::kBytes) - kWaves), tid(tid_),
+        lane(tid_ & 63), w(__builtin_amdgcn_readfirstlane(tid_ >> 6)), i16(tid_ & 15), g((tid_ & 63) >> 4),
+        sl2(p_.scale_log2), inv_sl2(1.f / p_.scale_log2) {}
 
   // The query fragments of the lane's rows r0 + 16 nt + i16 of an item: B operands, 8
   // dims from 32 ks + 8 g on.
@@ -415,9 +416,8 @@ struct Walk {
   }
 
   // ---- a segment of a prefix: 256 rows, 32 per wave, 64 keys at a time in LDS. False
-  // (bf16 values) where a value passed fp16's range: the caller then runs it again with
-  // `whole`, the staging power from the range's largest |v| instead of its first tile's.
-  __device__ __forceinline__ bool prefix(const Item& it, bool whole) {
+  // (bf16 values) where a value passed fp16's range: nothing is written then.
+  __device__ __forceinline__ bool prefix(const Item& it) {
     using LD = Lds<D>;
     constexpr int KP = LD::KP, VP = LD::VP;
     uint16_t* const sK = reinterpret_cast<uint16_t*>(smem);
@@ -502,6 +502,7 @@ struct Walk {
     };
     float vs = 1.f;     // bf16: the staging factor 2^vk
     int vk = 0;
+    bool seen = true;   // whether the first tile has a value to choose it from
     uint32_t vmax = 0;  // bf16: largest |v| bits staged (both halves)
     // Zeroes the values of keys past the range's end.
     auto edge = [&](Stage& S, int t) SPV_INLINE {
@@ -521,6 +522,25 @@ struct Walk {
           }
           S.v[i][hh] = x;
         }
+      }
+    };
+    // bf16 values to fp16, in place, in the softmax's phase: beside the matrix
+    // instructions they left no registers for the operands' read-ahead (0.69 PFLOP/s).
+    auto convert = [&](Stage& S) SPV_INLINE {
+      if constexpr (!kF16 && !kFp8) {
+#pragma unroll
+        for (int i = 0; i < kVN; ++i)
+#pragma unroll
+          for (int hh = 0; hh < 2; ++hh) {
+            u32x4_t x = S.v[i][hh];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const uint32_t y = x[e];
+              vmax = max_abs2(y, vmax);
+              x[e] = pack2_f16(__uint_as_float(y << 16) * vs, __uint_as_float(y & 0xffff0000u) * vs);
+            }
+            S.v[i][hh] = x;
+          }
       }
     };
     auto store = [&](Stage& S, int kslot, int vslot) SPV_INLINE {
@@ -564,10 +584,7 @@ struct Walk {
             }
           } else {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              vmax = max_abs2(x[e], vmax);
-              z[e] = pack2_f16(__uint_as_float(x[e] << 16) * vs, __uint_as_float(x[e] & 0xffff0000u) * vs);
-            }
+            for (int e = 0; e < 4; ++e) z[e] = x[e];
           }
           y[hh][0] = make_uint2(z[0], z[1]);
           y[hh][1] = make_uint2(z[2], z[3]);
@@ -727,39 +744,31 @@ struct Walk {
       load_next(st0, 0);
       load_next(st1, 1);
       if constexpr (!kF16 && !kFp8) {
-        // The largest finite |v| of the first tile, or of the whole range.
-        uint32_t mx = 0;
-        auto take = [&](u32x4_t x) SPV_INLINE {
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const uint32_t lo = x[e] & 0x7fffu, hi = (x[e] >> 16) & 0x7fffu;
-            mx = max(mx, lo < 0x7f80u ? lo : 0u);
-            mx = max(mx, hi < 0x7f80u ? hi : 0u);
-          }
-        };
+        uint32_t mx = 0;  // the largest finite |v| of the first tile
         edge(st0, 0);
-        if (!whole) {
 #pragma unroll
-          for (int i = 0; i < kVN; ++i)
+        for (int i = 0; i < kVN; ++i)
 #pragma unroll
-            for (int hh = 0; hh < 2; ++hh) take(st0.v[i][hh]);
-        } else {
-          for (int c = tid; c < pages * 2 * D; c += kMfmaThreads) {  // 8 keys of a dim
-            const int pg = c / (2 * D), k0 = key0 + 16 * pg + 8 * (c & 1);
-            u32x4_t x = *reinterpret_cast<const u32x4_t*>(page(p.vpool, page_of(safe_id(it, table[pg]), h)) + 16 * (c % (2 * D)));
+          for (int hh = 0; hh < 2; ++hh) {
+            const u32x4_t x = st0.v[i][hh];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) x[e / 2] &= k0 + e >= key1 ? ~(0xffffu << (16 * (e & 1))) : ~0u;
-            take(x);
+            for (int e = 0; e < 4; ++e) {
+              const uint32_t lo = x[e] & 0x7fffu, hi = (x[e] >> 16) & 0x7fffu;
+              mx = max(mx, lo < 0x7f80u ? lo : 0u);
+              mx = max(mx, hi < 0x7f80u ? hi : 0u);
+            }
           }
-        }
-        vk = stage_exponent(__uint_as_float(wg_max(mx) << 16));
+        mx = wg_max(mx);
+        seen = mx > 0;
+        vk = stage_exponent(__uint_as_float(mx << 16));
         vs = ldexpf(1.f, vk);
-        vmax = 0;
       }
       edge(st0, 0);
+      convert(st0);
       store(st0, 0, 0);
       load_next(st0, 2);
       edge(st1, min(1, n - 1));
+      convert(st1);
       store(st1, 1, 1);
       load_next(st1, 3);
       phase_end();
@@ -770,6 +779,7 @@ struct Walk {
       auto step = [&](int t, Stage& X) SPV_INLINE {  // V(t), M(t + 1); X: tile t + 2
         softmax(t);
         edge(X, min(t + 2, n - 1));
+        convert(X);
         window(t + 4);
         phase_end();
         __builtin_amdgcn_s_setprio(1);
@@ -802,13 +812,21 @@ struct Walk {
         ++t;
       }
       softmax(t);
+      if constexpr (!kF16 && !kFp8) {
+        // bits of the largest |v| that stays within fp16 at this power; with an all-zero
+        // first tile (power 0) anything but zeros is too much
+        const uint32_t top = seen ? min(__float_as_uint(ldexpf(65504.f, -vk)) >> 16, 0x7f7fu) : 0u;
+        const bool passed = __any((vmax & 0xffffu) > top || (vmax >> 16) > top);
+        if (lane == 0) sMax[w] = passed;
+      }
       phase_end();
       pv(vrd);
       if (grp == 0) phase_end();
       if constexpr (!kF16 && !kFp8) {
-        // bits of the largest |v| that stays within fp16 at this power
-        const uint32_t top = min(__float_as_uint(ldexpf(65504.f, -vk)) >> 16, 0x7f7fu);
-        if (__syncthreads_or((vmax & 0xffffu) > top || (vmax >> 16) > top) && !whole) return false;
+        uint32_t passed = 0;
+#pragma unroll
+        for (int k = 0; k < kWaves; ++k) passed |= sMax[k];
+        if (__builtin_amdgcn_readfirstlane(passed)) return false;
       }
     }
     write(it, w * 32, o, m, l, valid, kFp8 ? vref : ldexpf(1.f, -vk));
@@ -831,12 +849,13 @@ struct Walk {
     }
   }
 
-  // ---- an entry's own keys: up to 64 rows, 32 per wave; a wave takes every fourth
+  // ---- an entry's own keys: up to 64 rows, 32 per wave (false: the chunk holds a value
+  // that is not finite; nothing is written then); a wave takes every fourth
   // page (every eighth where there are at most 32 rows) straight into operand
   // registers, one page in flight while one is computed, and the waves' sums join in LDS.
   // P goes in two halves of bf16, beside each other in one operand over 16 keys
   // twice (fp16 pages: one operand of 16 keys): 16 bits of P, and values of any size.
-  __device__ __forceinline__ void own(const Item& it) {
+  __device__ __forceinline__ bool own(const Item& it) {
     const bool wide = it.rows > 32;
     const int nk = wide ? 4 : 8, kw = wide ? w & 3 : w, r0 = wide ? (w >> 2) * 32 : 0;
     const int h = __builtin_amdgcn_readfirstlane(it.h), key0 = __builtin_amdgcn_readfirstlane(it.key0),
@@ -1021,8 +1040,7 @@ struct Walk {
       }
     }
     if (__syncthreads_or(dirty)) {
-      valu_item<QT, KT, D, kMfmaThreads>(p, it, reinterpret_cast<float*>(smem));
-      return;
+      return false;
     }
     // Join the waves of the same rows: all take the largest m, then sums go down a
     // tree through LDS, in one order.
@@ -1073,6 +1091,7 @@ struct Walk {
       for (int nt = 0; nt < NT; ++nt) l[nt] *= 0.25f;  // `write` adds the four lane groups, which hold it each
       write(it, r0, o, m, l, valid, 1.f);
     }
+    return true;
   }
 };
 
@@ -1080,16 +1099,18 @@ template <int D, int KT>
 __global__ __launch_bounds__(kMfmaThreads, 2) void shared_mfma_kernel(SharedParams p) {
   static_assert(valu_lds(D) <= Lds<D>::kBytes, "the any-shape walk reuses this memory");
   __shared__ __align__(16) uint8_t smem[Lds<D>::kBytes];
-  Walk<D, KT> walk(p, smem);
   const int id = blockIdx.x;
+  Walk<D, KT> walk(p, smem, threadIdx.x);
   Item it;
+  bool done;
   if (id < p.seg_wgs) {
-    if (segment_item(p, id, it))
-      for (int whole = 0; !walk.prefix(it, whole); ++whole) {
-      }
-  } else if (own_item(p, id - p.seg_wgs, it)) {
-    walk.own(it);
+    if (!segment_item(p, id, it)) return;
+    done = walk.prefix(it);
+  } else {
+    if (!own_item(p, id - p.seg_wgs, it)) return;
+    done = walk.own(it);
   }
+  if (!done) valu_item<Walk<D, KT>::QT, KT, D, kMfmaThreads>(p, it, reinterpret_cast<float*>(smem));
 }
 
 // ----------------------------------------------------------------------- join
