@@ -347,7 +347,8 @@ struct Lds {
   static constexpr int KP = D + 16, VP = kUnit + 16;
   static constexpr int kK = kUnit * KP, kV = D * VP;  // elements of a slot
   static constexpr size_t kWalk = 2 * (size_t)(2 * kK + 3 * kV);
-  static constexpr size_t kJoin = 4 * 64 * (size_t)(D / 16 * 2) * 16 + kWaves * 32 * 8;  // own keys: the waves' sums
+  static constexpr int kJP = D / 2 + 4;  // own keys: half of a wave's row of sums, padded
+  static constexpr size_t kJoinRows = kWaves * 32 * (size_t)kJP * 4, kJoin = kJoinRows + kWaves * 32 * 8;
   static constexpr size_t kBytes = (kWalk > kJoin ? kWalk : kJoin) + 4 * kWaves;
 };
 
@@ -829,23 +830,37 @@ struct Walk {
         if (__builtin_amdgcn_readfirstlane(passed)) return false;
       }
     }
-    write(it, w * 32, o, m, l, valid, kFp8 ? vref : ldexpf(1.f, -vk));
+    write(it, o, m, l, valid, kFp8 ? vref : ldexpf(1.f, -vk));
     return true;
   }
 
-  // A wave's partial rows r0 + 16 nt + i16 of an item.
-  __device__ __forceinline__ void write(const Item& it, int r0, const f32x4_t (&o)[MT][NT], const float (&m)[NT],
+  // The partial rows of a wave of the prefix walk, 16 at a time through memory of its own in
+  // LDS: they leave as whole rows (1152 x 2 rows over 2048 keys 20.8 us, 21.9 where each
+  // lane stored its own 16 bytes).
+  __device__ __forceinline__ void write(const Item& it, const f32x4_t (&o)[MT][NT], const float (&m)[NT],
                                         float (&l)[NT], const bool (&valid)[NT], float post) {
+    constexpr int P = D + 4, kQ = D / 4;
+    float* const s = reinterpret_cast<float*>(smem) + w * 16 * P;
+    __syncthreads();  // the other waves have read their last pages
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       l[nt] += __shfl_xor(l[nt], 16, 64);
       l[nt] += __shfl_xor(l[nt], 32, 64);
-      if (!valid[nt]) continue;
-      const size_t row = (size_t)(it.part + r0 + nt * 16 + i16);
-      if (g == 0) *reinterpret_cast<float2*>(&p.part_ml[row * 2]) = make_float2(m[nt], l[nt]);
+      const int r0 = w * 32 + nt * 16;
+      if (g == 0 && valid[nt])
+        *reinterpret_cast<float2*>(&p.part_ml[(size_t)(it.part + r0 + i16) * 2]) = make_float2(m[nt], l[nt]);
 #pragma unroll
-      for (int mt = 0; mt < MT; ++mt)
-        *reinterpret_cast<f32x4_t*>(&p.part_o[row * D + 16 * mt + 4 * g]) = o[mt][nt] * post;
+      for (int mt = 0; mt < MT; ++mt) *reinterpret_cast<f32x4_t*>(&s[i16 * P + 16 * mt + 4 * g]) = o[mt][nt] * post;
+      __builtin_amdgcn_wave_barrier();
+      const int rows = it.rows - r0;
+#pragma unroll
+      for (int k = 0; k < 16 * kQ / 64; ++k) {
+        const int r = (k * 64 + lane) / kQ, q = lane % kQ;
+        if (r < rows)
+          *reinterpret_cast<f32x4_t*>(&p.part_o[(size_t)(it.part + r0 + r) * D + 4 * q]) =
+              *reinterpret_cast<const f32x4_t*>(&s[r * P + 4 * q]);
+      }
+      __builtin_amdgcn_wave_barrier();
     }
   }
 
@@ -856,6 +871,7 @@ struct Walk {
   // P goes in two halves of bf16, beside each other in one operand over 16 keys
   // twice (fp16 pages: one operand of 16 keys): 16 bits of P, and values of any size.
   __device__ __forceinline__ bool own(const Item& it) {
+    using LD = Lds<D>;
     const bool wide = it.rows > 32;
     const int nk = wide ? 4 : 8, kw = wide ? w & 3 : w, r0 = wide ? (w >> 2) * 32 : 0;
     const int h = __builtin_amdgcn_readfirstlane(it.h), key0 = __builtin_amdgcn_readfirstlane(it.key0),
@@ -1042,9 +1058,9 @@ struct Walk {
     if (__syncthreads_or(dirty)) {
       return false;
     }
-    // Join the waves of the same rows: all take the largest m, then sums go down a
-    // tree through LDS, in one order.
-    float2* const sML = reinterpret_cast<float2*>(smem + 4 * 64 * (size_t)(MT * NT) * 16);
+    // Join the waves of the same rows: all take the largest m; then every thread adds up
+    // four dims of a row over the waves, in their order, half of the dims at a time.
+    float2* const sML = reinterpret_cast<float2*>(smem + LD::kJoinRows);
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       l[nt] += __shfl_xor(l[nt], 16, 64);
@@ -1055,41 +1071,41 @@ struct Walk {
     const int w0 = wide ? w & 4 : 0;  // the first wave of these rows
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-      float M = -INFINITY, L = 0.f;
+      float M = -INFINITY;
       for (int k = 0; k < nk; ++k) M = fmaxf(M, sML[(w0 + k) * 32 + nt * 16 + i16].x);
-      const float ref = M == -INFINITY ? 0.f : M;
-      for (int k = 0; k < nk; ++k) {
-        const float2 x = sML[(w0 + k) * 32 + nt * 16 + i16];
-        L += x.y * __builtin_amdgcn_exp2f(x.x - ref);
-      }
-      const float f = __builtin_amdgcn_exp2f(m[nt] - ref);
+      const float f = __builtin_amdgcn_exp2f(m[nt] - (M == -INFINITY ? 0.f : M));
 #pragma unroll
       for (int mt = 0; mt < MT; ++mt) o[mt][nt] *= f;
-      m[nt] = M;
-      l[nt] = L;
     }
-    f32x4_t* const sO = reinterpret_cast<f32x4_t*>(smem);
-    for (int half = nk / 2; half >= 1; half /= 2) {
-      const int slot = wide ? (w >> 2) * 2 : 0;  // wide: at most two senders per half of the rows
-      if (kw >= half && kw < 2 * half) {
-#pragma unroll
-        for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt) sO[((slot + kw - half) * MT * NT + mt * NT + nt) * 64 + lane] = o[mt][nt];
+    if (tid < it.rows) {
+      const int first = wide ? (tid >> 5) * 4 : 0, r = tid & 31;
+      float M = -INFINITY, L = 0.f;
+      for (int k = 0; k < nk; ++k) M = fmaxf(M, sML[(first + k) * 32 + r].x);
+      const float ref = M == -INFINITY ? 0.f : M;
+      for (int k = 0; k < nk; ++k) {
+        const float2 x = sML[(first + k) * 32 + r];
+        L += x.y * __builtin_amdgcn_exp2f(x.x - ref);
       }
-      __syncthreads();
-      if (kw < half) {
-#pragma unroll
-        for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt) o[mt][nt] += sO[((slot + kw) * MT * NT + mt * NT + nt) * 64 + lane];
-      }
-      __syncthreads();
+      *reinterpret_cast<float2*>(&p.part_ml[(size_t)(it.part + tid) * 2]) = make_float2(M, L);
     }
-    if (kw == 0) {
+    float* const sO = reinterpret_cast<float*>(smem);  // [wave][row][half of the dims], padded
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) l[nt] *= 0.25f;  // `write` adds the four lane groups, which hold it each
-      write(it, r0, o, m, l, valid, 1.f);
+    for (int half = 0; half < 2; ++half) {
+      if (half) __syncthreads();
+#pragma unroll
+      for (int mt = 0; mt < MT / 2; ++mt)
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+          *reinterpret_cast<f32x4_t*>(&sO[(w * 32 + nt * 16 + i16) * LD::kJP + 16 * mt + 4 * g]) =
+              o[half * (MT / 2) + mt][nt];
+      __syncthreads();
+      constexpr int kQ = D / 8;  // pieces of four dims in half a row
+      for (int i = tid; i < it.rows * kQ; i += kMfmaThreads) {
+        const int r = i / kQ, q = i - r * kQ, first = wide ? (r >> 5) * 4 : 0;
+        f32x4_t x = *reinterpret_cast<const f32x4_t*>(&sO[(first * 32 + (r & 31)) * LD::kJP + 4 * q]);
+        for (int k = 1; k < nk; ++k) x += *reinterpret_cast<const f32x4_t*>(&sO[((first + k) * 32 + (r & 31)) * LD::kJP + 4 * q]);
+        *reinterpret_cast<f32x4_t*>(&p.part_o[(size_t)(it.part + r) * D + half * (D / 2) + 4 * q]) = x;
+      }
     }
     return true;
   }
@@ -1199,11 +1215,17 @@ struct Group {
   std::vector<int> members;
 };
 
-// The range of keys per segment, in units: the one for which rounds of 256 workgroups
-// (one for each CU) end first, a workgroup taking its units and about as long as
-// kFixed more to start, to write its partial and to have it joined.
-constexpr int kCUs = 256, kFixed = 4;
-long long best_range(const std::vector<long long>& tiles, const std::vector<long long>& units) {
+// The range of keys per segment, in units of 64 keys for a tile of 256 rows (2.3 us of a
+// CU for head_dim 128): the one for which the workgroups, one for each of 256 CUs at a time,
+// end first. A workgroup takes its units and about as long as kFixed more to start and to
+// end; each partial adds a kPartials-th of a unit to the whole, for it is written and read
+// again at the rate of memory; and own keys' workgroups (one per entry and kv head, that
+// many at least) which find no CU free beside the segments wait for the first to end.
+// 1152 rows x 2 kv heads over 2048 keys, bf16: 16 ranges take 28.3 us and 8.4 in the join, 8
+// ranges 20.8 and 5.7; 1008 rows x 2 over 32768 keys of fp8 with 32 such workgroups: 31
+// ranges take 49.1 and 11.7, 27 ranges 43.4 and 10.1.
+constexpr int kCUs = 256, kFixed = 4, kPartials = 20;
+long long best_range(const std::vector<long long>& tiles, const std::vector<long long>& units, long long own) {
   long long most = 1, best = 1, least = -1;
   for (long long u : units) most = std::max(most, u);
   // ceil(most / k) for every number of ranges k: no other length cuts the longest prefix evenly
@@ -1211,7 +1233,9 @@ long long best_range(const std::vector<long long>& tiles, const std::vector<long
     const long long range = (most + k - 1) / k;
     long long n = 0;
     for (size_t g = 0; g < units.size(); ++g) n += tiles[g] * ((units[g] + range - 1) / range);
-    const long long time = (n + kCUs - 1) / kCUs * (range + kFixed);
+    const long long rounds = (n + kCUs - 1) / kCUs;
+    const long long late = n + own > rounds * kCUs ? kFixed : 0;
+    const long long time = (rounds * (range + kFixed) + late) * kPartials + n;
     if (least < 0 || time < least) {
       least = time;
       best = range;
@@ -1246,7 +1270,7 @@ int make_plan(std::vector<int32_t>& plan, const int32_t* ids, const int32_t* len
   }
   std::vector<long long> all(tiles);
   for (long long& t : all) t *= Hkv;
-  const long long range = best_range(all, units);
+  const long long range = best_range(all, units, (long long)B * Hkv);
   long long nseg = 0;
   for (size_t g = 0; g < groups.size(); ++g) {
     const Group& x = groups[g];
