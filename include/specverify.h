@@ -428,7 +428,8 @@ int spv_prefill_attn(void* out, const void* q, const void* k, const void* v,
  *
  * The plan lists that work. It depends on the prefixes, their lengths, the chunk
  * and the heads, not on the sequences' own lengths, so it is made when requests
- * are admitted and serves every layer and round until the next admission.
+ * are admitted and serves every layer and round until the next admission. (head_dim and
+ * kv_dtype only weigh how the prefixes are cut.)
  * prefix_ids and prefix_lens (B entries each) and plan are HOST pointers:
  * prefix_ids[b] = -1 or prefix_lens[b] = 0 is no prefix. With plan NULL the call
  * returns the plan's length in int32 words; otherwise it writes the plan
@@ -436,8 +437,8 @@ int spv_prefill_attn(void* out, const void* q, const void* k, const void* v,
  * bad arguments. The caller copies the plan to the device and keeps both. */
 int64_t spv_shared_attn_plan(const int32_t* prefix_ids, const int32_t* prefix_lens,
                              int32_t B, int32_t C, int32_t num_q_heads,
-                             int32_t num_kv_heads, int32_t block_size, int32_t* plan,
-                             int64_t plan_ints);
+                             int32_t num_kv_heads, int32_t head_dim, int32_t block_size,
+                             int kv_dtype, int32_t* plan, int64_t plan_ints);
 
 /* Workspace of spv_shared_attn (partial results; needs no particular contents
  * and may be another one in every call) for own contexts up to max_ctx;

@@ -355,10 +355,10 @@ struct Lds {
 // What both walks know of the call and the lane.
 template <int D, int KT>
 struct Walk {
-  static constexpr bool kF16 = KT == SPV_F16, kFp8 = KT == SPV_FP8E4M3;
-  static constexpr int QT = kF16 ? SPV_F16 : SPV_BF16;
-  static constexpr int ES = kFp8 ? 1 : 2;
-  static constexpr int KS = D / 32, MT = D / 16, NT = 2;
+  static constexpr bool kF16 = KT == SPV_F16, kFp8 = KT == SPV_FP8E4M3, kF32 = KT == SPV_F32;
+  static constexpr int QT = kF16 ? SPV_F16 : kF32 ? SPV_F32 : SPV_BF16;
+  static constexpr int ES = kFp8 ? 1 : kF32 ? 4 : 2;
+  static constexpr int KS = kF32 ? D / 16 : D / 32, MT = D / 16, NT = 2;  // KS: 16-byte pieces of a row per lane
   const SharedParams& p;
   uint8_t* const smem;
   uint32_t* const sMax;
@@ -371,7 +371,7 @@ struct Walk {
         sl2(p_.scale_log2), inv_sl2(1.f / p_.scale_log2) {}
 
   // The query fragments of the lane's rows r0 + 16 nt + i16 of an item: B operands, 8
-  // dims from 32 ks + 8 g on.
+  // dims from 32 ks + 8 g on (fp32: 4 dims from 16 ks + 4 g on).
   __device__ __forceinline__ void load_q(const Item& it, int r0, uint4 (&qf)[NT][KS], int (&lim)[NT], bool (&valid)[NT]) {
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
@@ -380,9 +380,9 @@ struct Walk {
       int b, j, hq;
       row_at(p, it, it.row0 + min(R, it.rows - 1), b, j, hq);
       lim[nt] = it.first >= 0 ? it.start : it.start + j;
-      const uint16_t* q = static_cast<const uint16_t*>(p.q) + (((size_t)b * p.C + j) * p.Hq + hq) * D + 8 * g;
+      const uint8_t* q = static_cast<const uint8_t*>(p.q) + (((size_t)b * p.C + j) * p.Hq + hq) * (D * (kF32 ? 4 : 2)) + 16 * g;
 #pragma unroll
-      for (int ks = 0; ks < KS; ++ks) qf[nt][ks] = *reinterpret_cast<const uint4*>(q + 32 * ks);
+      for (int ks = 0; ks < KS; ++ks) qf[nt][ks] = *reinterpret_cast<const uint4*>(q + 64 * ks);
     }
   }
   __device__ __forceinline__ f32x4_t mfma_qk(uint4 k, uint4 q, f32x4_t c) const {
@@ -864,21 +864,27 @@ struct Walk {
     }
   }
 
-  // ---- an entry's own keys: up to 64 rows, 32 per wave (false: the chunk holds a value
-  // that is not finite; nothing is written then); a wave takes every fourth
-  // page (every eighth where there are at most 32 rows) straight into operand
-  // registers, one page in flight while one is computed, and the waves' sums join in LDS.
+  // ---- an entry's own keys, and in fp32 a segment too: 32 rows per wave (false: the chunk
+  // holds a value that is not finite; nothing is written then). nk waves share the
+  // rows (8 up to 32 rows, 4 up to 64, 2 up to 128, 1 up to 256) and take every nk-th
+  // page straight into operand registers, one page in flight while one is computed;
+  // their sums join in LDS.
   // P goes in two halves of bf16, beside each other in one operand over 16 keys
   // twice (fp16 pages: one operand of 16 keys): 16 bits of P, and values of any size.
-  __device__ __forceinline__ bool own(const Item& it) {
+  // fp32: v_mfma_f32_16x16x4_f32, four to a 16-byte piece of K or V, whose four elements
+  // take turns as the contracted index (the query's and P's, in the same lanes, do the
+  // same). At 256 operations a clock and CU the matrix cores take 32 times as long over a
+  // page as its 8 KB (head_dim 128) take from the L1, so every wave reads it for itself;
+  // K's registers are loaded again while V's are used, and the other way round.
+  __device__ __forceinline__ bool pages(const Item& it) {
     using LD = Lds<D>;
-    const bool wide = it.rows > 32;
-    const int nk = wide ? 4 : 8, kw = wide ? w & 3 : w, r0 = wide ? (w >> 2) * 32 : 0;
+    const int nk_log2 = it.rows <= 32 ? 3 : it.rows <= 64 ? 2 : it.rows <= 128 ? 1 : 0, nk = 1 << nk_log2;
+    const int kw = w & (nk - 1), r0 = (w >> nk_log2) * 32;
     const int h = __builtin_amdgcn_readfirstlane(it.h), key0 = __builtin_amdgcn_readfirstlane(it.key0),
               key1 = __builtin_amdgcn_readfirstlane(it.key1), start = __builtin_amdgcn_readfirstlane(it.start);
-    const int pages = (key1 - key0 + 15) >> 4;
+    const int count = (key1 - key0 + 15) >> 4;
     const int32_t* table = p.tables + (size_t)__builtin_amdgcn_readfirstlane(it.sid) * p.maxb + (key0 >> 4);
-    const int mine = kw < pages ? (pages - 1 - kw) / nk + 1 : 0;  // pages kw, kw + nk, ...
+    const int mine = kw < count ? ((count - 1 - kw) >> nk_log2) + 1 : 0;  // pages kw, kw + nk, ...
     uint4 qf[NT][KS];
     int lim[NT];
     bool valid[NT];
@@ -897,13 +903,12 @@ struct Walk {
     float ksc = 1.f, vsc = 1.f;
     int dirty = 0;  // a value of the chunk that some of its rows do not see is not finite
     struct Page {
-      uint4 k[KS];  // fp8: 8 bytes
-      uint2 v[MT];  // fp8: 4 bytes
+      uint4 k[KS];           // fp8: 8 bytes
+      uint32_t v[MT][ES == 4 ? 4 : 2];  // fp8: 4 bytes
     };
-    auto load = [&](Page& P, int i) SPV_INLINE {
+    auto load_k = [&](Page& P, int i) SPV_INLINE {
       const int pg = __builtin_amdgcn_readlane(ids, i & 63);
-      const uint8_t* K = page(p.kpool, pg) + (i16 * D + 8 * g) * ES;
-      const uint8_t* V = page(p.vpool, pg) + (i16 * 16 + 4 * g) * ES;
+      const uint8_t* K = page(p.kpool, pg) + i16 * D * ES + (kFp8 ? 8 : 16) * g;
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) {
         if constexpr (kFp8) {
@@ -913,13 +918,25 @@ struct Walk {
           P.k[ks] = *reinterpret_cast<const uint4*>(K + 64 * ks);
         }
       }
+    };
+    auto load_v = [&](Page& P, int i) SPV_INLINE {
+      const int pg = __builtin_amdgcn_readlane(ids, i & 63);
+      const uint8_t* V = page(p.vpool, pg) + (i16 * 16 + 4 * g) * ES;
 #pragma unroll
       for (int mt = 0; mt < MT; ++mt) {
-        if constexpr (kFp8) P.v[mt] = make_uint2(*reinterpret_cast<const uint32_t*>(V + 256 * mt), 0u);
-        else P.v[mt] = *reinterpret_cast<const uint2*>(V + 512 * mt);
+        if constexpr (kFp8) {
+          P.v[mt][0] = *reinterpret_cast<const uint32_t*>(V + 256 * mt);
+          P.v[mt][1] = 0u;
+        } else if constexpr (kF32) {
+          const uint4 x = *reinterpret_cast<const uint4*>(V + 1024 * mt);
+          P.v[mt][0] = x.x, P.v[mt][1] = x.y, P.v[mt][2] = x.z, P.v[mt][3] = x.w;
+        } else {
+          const uint2 x = *reinterpret_cast<const uint2*>(V + 512 * mt);
+          P.v[mt][0] = x.x, P.v[mt][1] = x.y;
+        }
       }
     };
-    auto compute = [&](Page& P, int i) SPV_INLINE {
+    auto compute = [&](Page& P, int i, int next) SPV_INLINE {  // fp32: `next` is loaded into P
       const int k0 = key0 + 16 * (kw + nk * i);
       f32x4_t sc[NT];
 #pragma unroll
@@ -934,9 +951,21 @@ struct Walk {
                           __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(b, 1.f, false)),
                           __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(b, 1.f, true)));
         }
+        if constexpr (kF32) {
+          const uint32_t k[4] = {kf.x, kf.y, kf.z, kf.w};
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) sc[nt] = mfma_qk(kf, qf[nt][ks], sc[nt]);
+          for (int c = 0; c < 4; ++c)
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+              const uint32_t x[4] = {qf[nt][ks].x, qf[nt][ks].y, qf[nt][ks].z, qf[nt][ks].w};
+              sc[nt] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(k[c]), __uint_as_float(x[c]), sc[nt], 0, 0, 0);
+            }
+        } else {
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) sc[nt] = mfma_qk(kf, qf[nt][ks], sc[nt]);
+        }
       }
+      if constexpr (kF32) load_k(P, next);
       float fv = 1.f;
       if constexpr (kFp8) {
         const float f = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(ksc), i & 63));
@@ -956,18 +985,15 @@ struct Walk {
         // not meet the P = 0 of the rows before it.
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt) {
-          uint32_t x[2] = {P.v[mt].x, P.v[mt].y};
 #pragma unroll
           for (int jj = 0; jj < 4; ++jj) {
-            constexpr uint32_t kMask = kFp8 ? 0xffu : 0xffffu;
+            constexpr uint32_t kMask = kFp8 ? 0xffu : kF32 ? ~0u : 0xffffu;
+            constexpr uint32_t kInf = kFp8 ? 0x7fu : kF16 ? 0x7c00u : kF32 ? 0x7f800000u : 0x7f80u;
             const int word = jj * ES / 4, shift = 8 * (jj * ES % 4), key = k0 + 4 * g + jj;
-            const uint32_t bits = (x[word] >> shift) & kMask;
-            const bool bad = kFp8 ? (bits & 0x7fu) == 0x7fu
-                                  : (kF16 ? (bits & 0x7c00u) == 0x7c00u : (bits & 0x7f80u) == 0x7f80u);
-            x[word] &= key >= key1 ? ~(kMask << shift) : ~0u;
+            const bool bad = ((P.v[mt][word] >> shift) & kInf) == kInf;
+            P.v[mt][word] &= key >= key1 ? ~(kMask << shift) : ~0u;
             dirty |= (int)bad & (int)(key > start) & (int)(key < key1);
           }
-          P.v[mt] = make_uint2(x[0], x[1]);
         }
       }
       bool grow = false;
@@ -999,7 +1025,9 @@ struct Walk {
 #pragma unroll
         for (int jj = 0; jj < 4; ++jj) e[jj] = __builtin_amdgcn_exp2f(fmaf(sc[nt][jj], sl2, -mu));
         l[nt] += (e[0] + e[1]) + (e[2] + e[3]);
-        if constexpr (kF16) {
+        if constexpr (kF32) {
+          pb[nt] = make_uint4(__float_as_uint(e[0]), __float_as_uint(e[1]), __float_as_uint(e[2]), __float_as_uint(e[3]));
+        } else if constexpr (kF16) {
           pb[nt] = make_uint4(pack2_f16(e[0], e[1]), pack2_f16(e[2], e[3]), 0u, 0u);
         } else {
           uint32_t hi[2], lo[2];
@@ -1015,7 +1043,17 @@ struct Walk {
       }
 #pragma unroll
       for (int mt = 0; mt < MT; ++mt) {
-        uint2 v = P.v[mt];
+        if constexpr (kF32) {
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+              const uint32_t x[4] = {pb[nt].x, pb[nt].y, pb[nt].z, pb[nt].w};
+              o[mt][nt] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(P.v[mt][c]), __uint_as_float(x[c]), o[mt][nt], 0, 0, 0);
+            }
+          continue;
+        }
+        uint2 v = make_uint2(P.v[mt][0], P.v[mt][1]);
         if constexpr (kFp8) {
           const uint32_t c = v.x;
           v = make_uint2(__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(c, 1.f, false)),
@@ -1032,9 +1070,14 @@ struct Walk {
                                                                  __builtin_bit_cast(bf16x8_t, pb[nt]), o[mt][nt], 0, 0, 0);
         }
       }
+      if constexpr (kF32) {
+        __builtin_amdgcn_sched_barrier(0);  // V's registers are free only now
+        load_v(P, next);
+        __builtin_amdgcn_sched_barrier(0);
+      }
     };
     for (int base = 0; base < mine; base += 64) {  // 64 of the wave's pages, their ids in the lanes
-      const int phys = safe_id(it, table[min(kw + nk * (base + lane), pages - 1)]);
+      const int phys = safe_id(it, table[min(kw + nk * (base + lane), count - 1)]);
       ids = page_of(phys, h);
       if constexpr (kFp8) {
         const float2 s = scales_of(phys);
@@ -1044,15 +1087,23 @@ struct Walk {
       const int last = min(mine, base + 64) - 1;
       // Every load is unconditional (past the last page it repeats it), so that a page's
       // use waits for its own loads alone.
-      Page A, B;
-      load(A, base);
-      for (int i = base;; i += 2) {
-        load(B, min(i + 1, last));
-        compute(A, i);
-        if (i + 1 > last) break;
-        load(A, min(i + 2, last));
-        compute(B, i + 1);
-        if (i + 2 > last) break;
+      Page A;
+      load_k(A, base);
+      load_v(A, base);
+      if constexpr (kF32) {
+        for (int i = base; i <= last; ++i) compute(A, i, min(i + 1, last));
+      } else {
+        Page B;
+        for (int i = base;; i += 2) {
+          load_k(B, min(i + 1, last));
+          load_v(B, min(i + 1, last));
+          compute(A, i, 0);
+          if (i + 1 > last) break;
+          load_k(A, min(i + 2, last));
+          load_v(A, min(i + 2, last));
+          compute(B, i + 1, 0);
+          if (i + 2 > last) break;
+        }
       }
     }
     if (__syncthreads_or(dirty)) {
@@ -1068,7 +1119,7 @@ struct Walk {
       if (g == 0) sML[w * 32 + nt * 16 + i16] = make_float2(m[nt], l[nt]);
     }
     __syncthreads();
-    const int w0 = wide ? w & 4 : 0;  // the first wave of these rows
+    const int w0 = w & -nk;  // the first wave of these rows
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       float M = -INFINITY;
@@ -1078,7 +1129,7 @@ struct Walk {
       for (int mt = 0; mt < MT; ++mt) o[mt][nt] *= f;
     }
     if (tid < it.rows) {
-      const int first = wide ? (tid >> 5) * 4 : 0, r = tid & 31;
+      const int first = (tid >> 5) << nk_log2, r = tid & 31;
       float M = -INFINITY, L = 0.f;
       for (int k = 0; k < nk; ++k) M = fmaxf(M, sML[(first + k) * 32 + r].x);
       const float ref = M == -INFINITY ? 0.f : M;
@@ -1101,7 +1152,7 @@ struct Walk {
       __syncthreads();
       constexpr int kQ = D / 8;  // pieces of four dims in half a row
       for (int i = tid; i < it.rows * kQ; i += kMfmaThreads) {
-        const int r = i / kQ, q = i - r * kQ, first = wide ? (r >> 5) * 4 : 0;
+        const int r = i / kQ, q = i - r * kQ, first = (r >> 5) << nk_log2;
         f32x4_t x = *reinterpret_cast<const f32x4_t*>(&sO[(first * 32 + (r & 31)) * LD::kJP + 4 * q]);
         for (int k = 1; k < nk; ++k) x += *reinterpret_cast<const f32x4_t*>(&sO[((first + k) * 32 + (r & 31)) * LD::kJP + 4 * q]);
         *reinterpret_cast<f32x4_t*>(&p.part_o[(size_t)(it.part + r) * D + half * (D / 2) + 4 * q]) = x;
@@ -1121,10 +1172,11 @@ __global__ __launch_bounds__(kMfmaThreads, 2) void shared_mfma_kernel(SharedPara
   bool done;
   if (id < p.seg_wgs) {
     if (!segment_item(p, id, it)) return;
-    done = walk.prefix(it);
+    if constexpr (KT == SPV_F32) done = walk.pages(it);
+    else done = walk.prefix(it);
   } else {
     if (!own_item(p, id - p.seg_wgs, it)) return;
-    done = walk.own(it);
+    done = walk.pages(it);
   }
   if (!done) valu_item<Walk<D, KT>::QT, KT, D, kMfmaThreads>(p, it, reinterpret_cast<float*>(smem));
 }
@@ -1215,17 +1267,22 @@ struct Group {
   std::vector<int> members;
 };
 
-// The range of keys per segment, in units of 64 keys for a tile of 256 rows (2.3 us of a
-// CU for head_dim 128): the one for which the workgroups, one for each of 256 CUs at a time,
-// end first. A workgroup takes its units and about as long as kFixed more to start and to
-// end; each partial adds a kPartials-th of a unit to the whole, for it is written and read
-// again at the rate of memory; and own keys' workgroups (one per entry and kv head, that
-// many at least) which find no CU free beside the segments wait for the first to end.
-// 1152 rows x 2 kv heads over 2048 keys, bf16: 16 ranges take 28.3 us and 8.4 in the join, 8
-// ranges 20.8 and 5.7; 1008 rows x 2 over 32768 keys of fp8 with 32 such workgroups: 31
-// ranges take 49.1 and 11.7, 27 ranges 43.4 and 10.1.
-constexpr int kCUs = 256, kFixed = 4, kPartials = 20;
-long long best_range(const std::vector<long long>& tiles, const std::vector<long long>& units, long long own) {
+// ns that a CU takes for a unit of 64 keys with a tile of 256 rows: 8.4 MFLOP at head_dim 128.
+long long unit_ns(int kv_dtype, int d, int bs) {
+  const bool mfma = bs == 16 && (d == 64 || d == 128);
+  return (mfma ? kv_dtype == SPV_F32 ? 14000LL : 2300LL : 70000LL) * d / 128 + 1;
+}
+// The range of keys per segment, in units: the one for which the workgroups, one for each
+// of 256 CUs at a time, end first. A workgroup takes its units and about kFixed ns more to
+// start and to end; a partial of 256 rows adds kPartial ns to the whole at head_dim 128, for
+// it is written and read again at the rate of memory; and own keys' workgroups (one per
+// entry and kv head, that many at least) which find no CU free beside the segments wait for the
+// first to end. bf16, 1152 rows x 2 kv heads over 2048 keys: 16 ranges take 28.3 us and
+// 8.4 in the join, 8 ranges 20.8 and 5.7; 1008 rows x 2 over 32768 keys of fp8 with 32 such
+// workgroups: 31 ranges take 49.1 and 11.7, 27 ranges 43.4 and 10.1.
+constexpr int kCUs = 256, kFixed = 9000, kPartial = 110;
+long long best_range(const std::vector<long long>& tiles, const std::vector<long long>& units, long long own,
+                     long long unit, int d) {
   long long most = 1, best = 1, least = -1;
   for (long long u : units) most = std::max(most, u);
   // ceil(most / k) for every number of ranges k: no other length cuts the longest prefix evenly
@@ -1235,7 +1292,7 @@ long long best_range(const std::vector<long long>& tiles, const std::vector<long
     for (size_t g = 0; g < units.size(); ++g) n += tiles[g] * ((units[g] + range - 1) / range);
     const long long rounds = (n + kCUs - 1) / kCUs;
     const long long late = n + own > rounds * kCUs ? kFixed : 0;
-    const long long time = (rounds * (range + kFixed) + late) * kPartials + n;
+    const long long time = rounds * (range * unit + kFixed) + late + n * kPartial * d / 128;
     if (least < 0 || time < least) {
       least = time;
       best = range;
@@ -1245,8 +1302,8 @@ long long best_range(const std::vector<long long>& tiles, const std::vector<long
   return best;
 }
 
-int make_plan(std::vector<int32_t>& plan, const int32_t* ids, const int32_t* lens, int B, int C, int Hq, int Hkv,
-              int bs) {
+int make_plan(std::vector<int32_t>& plan, const int32_t* ids, const int32_t* lens, int B, int C, int Hq, int Hkv, int d,
+              int bs, int kv_dtype) {
   const long long G = (long long)C * (Hq / Hkv);
   std::vector<Group> groups;
   std::map<std::pair<int32_t, int32_t>, size_t> index;
@@ -1270,7 +1327,7 @@ int make_plan(std::vector<int32_t>& plan, const int32_t* ids, const int32_t* len
   }
   std::vector<long long> all(tiles);
   for (long long& t : all) t *= Hkv;
-  const long long range = best_range(all, units, (long long)B * Hkv);
+  const long long range = best_range(all, units, (long long)B * Hkv, unit_ns(kv_dtype, d, bs), d);
   long long nseg = 0;
   for (size_t g = 0; g < groups.size(); ++g) {
     const Group& x = groups[g];
@@ -1371,15 +1428,15 @@ int launch(const SharedParams& p, int kv_dtype, hipStream_t s) {
   int rc;
   // The matrix kernels apply the scale inside the exponent, to maxima of raw scores.
   // They count pages in 31 bits.
-  const bool mfma = (long long)(p.layer + 1) * p.cap * p.Hkv < (1LL << 31) && p.bs == 16 && (p.d == 64 || p.d == 128) && p.scale_log2 > 0.f && p.scale_log2 < INFINITY &&
-                    ((QT == SPV_BF16 && (kv_dtype == SPV_BF16 || kv_dtype == SPV_FP8E4M3)) ||
-                     (QT == SPV_F16 && kv_dtype == SPV_F16));
+  const bool mfma = (long long)(p.layer + 1) * p.cap * p.Hkv < (1LL << 31) && p.bs == 16 &&
+                    (p.d == 64 || p.d == 128) && p.scale_log2 > 0.f && p.scale_log2 < INFINITY &&
+                    ((QT == SPV_BF16 && kv_dtype == SPV_FP8E4M3) || QT == kv_dtype);
   if (mfma) {
     if constexpr (QT == SPV_BF16) {
       if (kv_dtype == SPV_BF16) rc = p.d == 64 ? launch_mfma<64, SPV_BF16>(p, grid, s) : launch_mfma<128, SPV_BF16>(p, grid, s);
       else rc = p.d == 64 ? launch_mfma<64, SPV_FP8E4M3>(p, grid, s) : launch_mfma<128, SPV_FP8E4M3>(p, grid, s);
-    } else if constexpr (QT == SPV_F16) {
-      rc = p.d == 64 ? launch_mfma<64, SPV_F16>(p, grid, s) : launch_mfma<128, SPV_F16>(p, grid, s);
+    } else {
+      rc = p.d == 64 ? launch_mfma<64, QT>(p, grid, s) : launch_mfma<128, QT>(p, grid, s);
     }
   } else switch (kv_dtype) {
     case SPV_F32: rc = launch_valu<QT, SPV_F32>(p, grid, s); break;
@@ -1398,15 +1455,16 @@ int launch(const SharedParams& p, int kv_dtype, hipStream_t s) {
 extern "C" {
 
 int64_t spv_shared_attn_plan(const int32_t* prefix_ids, const int32_t* prefix_lens, int32_t B, int32_t C,
-                             int32_t num_q_heads, int32_t num_kv_heads, int32_t block_size, int32_t* plan,
-                             int64_t plan_ints) {
+                             int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim, int32_t block_size,
+                             int kv_dtype, int32_t* plan, int64_t plan_ints) {
   if (!prefix_ids || !prefix_lens || B < 1 || B > 65535 || C < 1 || num_kv_heads < 1 ||
-      num_q_heads < num_kv_heads || num_q_heads % num_kv_heads || block_size < 1 ||
+      num_q_heads < num_kv_heads || num_q_heads % num_kv_heads || block_size < 1 || head_dim < 1 ||
+      head_dim > kMaxD || dtype_size(kv_dtype) == 0 ||
       (long long)C * num_q_heads > (1 << 20) || (long long)B * C * num_q_heads > (1LL << 30))
     return SPV_ERR_ARG;
   try {
     std::vector<int32_t> p;
-    const int rc = make_plan(p, prefix_ids, prefix_lens, B, C, num_q_heads, num_kv_heads, block_size);
+    const int rc = make_plan(p, prefix_ids, prefix_lens, B, C, num_q_heads, num_kv_heads, head_dim, block_size, kv_dtype);
     if (rc != SPV_OK) return rc;
     if (!plan) return (int64_t)p.size();
     if (plan_ints < (int64_t)p.size()) return SPV_ERR_WORKSPACE;

@@ -74,7 +74,7 @@ SIGNATURES = {
     "spv_time_next_attention": (I, [P, P]),
     "spv_verify_attn_static_max_bytes": (S, []),
     "spv_verify_attn_static": (I, [P, P, I, P, P, I, P, P, I, P, P, P, P, I, I, I, I, I, I, I, I, I, F, P]),
-    "spv_shared_attn_plan": (L, [P, P, I, I, I, I, I, P, L]),
+    "spv_shared_attn_plan": (L, [P, P, I, I, I, I, I, I, I, P, L]),
     "spv_shared_attn_workspace_bytes": (S, [P, I, I]),
     "spv_shared_attn": (I, [P, P, I, P, P, I, P, P, I, P, P, P, P, I, I, I, I, I, I, I, I, I, F, P, P, P, S, P]),
     "spv_rotary": (I, [P, P, P, P, I, I, P, P, P, P, I, F, I, I, I, I, I, I, I, P]),

@@ -279,7 +279,8 @@ class SharedPrefix:
         if not self.B:
             return
         c_ids, c_lens = ((ctypes.c_int32 * self.B)(*x) for x in (ids, lens))
-        args = (c_ids, c_lens, self.B, self.chunk, self.num_q_heads, kv.num_kv_heads, kv.block_size)
+        args = (c_ids, c_lens, self.B, self.chunk, self.num_q_heads, kv.num_kv_heads, kv.head_dim, kv.block_size,
+                kv._dt)
         n = int(_hip.lib().spv_shared_attn_plan(*args, None, 0))
         if n < 0:
             raise _hip.HipLibraryError("spv_shared_attn_plan failed: {} ({})".format(_hip._ERRORS.get(n, "error"), n))

@@ -23,15 +23,15 @@ def lib():
     return _hip.lib()
 
 
-def _plan(lib, ids, lens, C=3, Hq=4, Hkv=2, bs=16):
+def _plan(lib, ids, lens, C=3, Hq=4, Hkv=2, bs=16, d=128, dtype=_hip.SPV_BF16):
     n = len(ids)
     a, b = (I32 * n)(*ids), (I32 * n)(*lens)
-    need = lib.spv_shared_attn_plan(a, b, n, C, Hq, Hkv, bs, None, 0)
+    need = lib.spv_shared_attn_plan(a, b, n, C, Hq, Hkv, d, bs, dtype, None, 0)
     if need < 0:
         return need
     buf = (I32 * need)()
-    assert lib.spv_shared_attn_plan(a, b, n, C, Hq, Hkv, bs, buf, need - 1) == _hip.SPV_ERR_WORKSPACE
-    assert lib.spv_shared_attn_plan(a, b, n, C, Hq, Hkv, bs, buf, need) == need
+    assert lib.spv_shared_attn_plan(a, b, n, C, Hq, Hkv, d, bs, dtype, buf, need - 1) == _hip.SPV_ERR_WORKSPACE
+    assert lib.spv_shared_attn_plan(a, b, n, C, Hq, Hkv, d, bs, dtype, buf, need) == need
     return list(buf)
 
 
@@ -42,6 +42,7 @@ def _sections(plan):
     return cut(at[0], plan[7], 8), plan[at[1]:at[2]], cut(at[2], plan[2], 4)
 
 
+@pytest.mark.parametrize("dtype,d,bs", [(_hip.SPV_BF16, 128, 16), (_hip.SPV_F32, 64, 16), (_hip.SPV_F16, 96, 7)])
 @pytest.mark.parametrize("ids,lens", [
     ([7, 7, 7], [100, 100, 100]),
     ([7, -1, 3, 7, 3, 5], [100, 50, 17, 100, 17, 0]),
@@ -49,11 +50,11 @@ def _sections(plan):
     ([-1, -1], [0, 9]),                      # nobody has one
     ([0] * 200 + [1] * 57, [5000] * 200 + [33] * 57),
 ])
-def test_plan_covers_every_row_and_key_once(lib, ids, lens):
+def test_plan_covers_every_row_and_key_once(lib, ids, lens, dtype, d, bs):
     """Items tile (rows of a group) x (keys of its prefix) without gap or overlap, for every kv head."""
-    C, Hq, Hkv, bs = 3, 4, 2, 16
+    C, Hq, Hkv = 3, 4, 2
     G = C * Hq // Hkv
-    plan = _plan(lib, ids, lens, C, Hq, Hkv, bs)
+    plan = _plan(lib, ids, lens, C, Hq, Hkv, bs, d, dtype)
     assert plan[1] == len(plan)
     segs, members, entries = _sections(plan)
     want = {}
@@ -87,7 +88,9 @@ def test_plan_refusals(lib):
     assert _plan(lib, [1], [1], Hq=5, Hkv=2) == ARG
     assert _plan(lib, [1], [1], C=0) == ARG
     assert _plan(lib, [1], [1], bs=0) == ARG
-    assert lib.spv_shared_attn_plan(None, None, 1, 1, 2, 2, 16, None, 0) == ARG
+    assert _plan(lib, [1], [1], d=0) == ARG and _plan(lib, [1], [1], d=257) == ARG
+    assert _plan(lib, [1], [1], dtype=17) == ARG
+    assert lib.spv_shared_attn_plan(None, None, 1, 1, 2, 2, 64, 16, _hip.SPV_BF16, None, 0) == ARG
     assert lib.spv_shared_attn_workspace_bytes(None, 64, 16) == 0
     plan = (I32 * 4096)(*_plan(lib, [1, 1], [40, 40]))
     assert lib.spv_shared_attn_workspace_bytes(plan, 64, 2) == 0       # max_ctx below the chunk
