@@ -1182,15 +1182,18 @@ __global__ __launch_bounds__(kMfmaThreads, 2) void shared_mfma_kernel(SharedPara
 }
 
 // ----------------------------------------------------------------------- join
-// LPR lanes per (entry, chunk token, q head): four consecutive dims per lane (VEC,
-// head_dim = 4 LPR), or dims lane + 64 k of any head_dim up to 256. The row's
-// partials, the prefix's segments in key order and then its own ranges, are added
-// in that order whatever finished first.
-constexpr int kJoin = 4;
-template <int QT, int LPR, bool VEC>
+// LPR lanes per (entry, chunk token, q head), four consecutive dims each (VEC, head_dim =
+// 4 LPR), or dims lane + 64 k of any head_dim up to 256; GROUPS such sets of lanes share a
+// row's partials. The partials, the prefix's segments in key order and then the entry's own
+// ranges, are added in an order that is the row's alone, whatever finished first. With few
+// rows latency bounds it: a wave then serves one row, each group reading kJoin partials at
+// a time (28 partials of 2016 rows of 64: 5.9 us, one group 10.1; 10 of 1440 rows of 128: 4.9
+// and 8.7); with many, the rate of memory (about 5 of 14336 rows: 11.5 us, one group 9.6).
+constexpr int kJoin = 4, kFewRows = 8192;
+template <int QT, int LPR, int GROUPS, bool VEC>
 __global__ __launch_bounds__(kThreads) void shared_join_kernel(SharedParams p) {
-  const int lane = threadIdx.x % LPR;
-  const long long row = (long long)blockIdx.x * (kThreads / LPR) + threadIdx.x / LPR;
+  const int lane = threadIdx.x % LPR, group = threadIdx.x / LPR % GROUPS;
+  const long long row = (long long)blockIdx.x * (kThreads / (LPR * GROUPS)) + threadIdx.x / (LPR * GROUPS);
   if (row >= (long long)p.B * p.C * p.Hq) return;
   const int hq = (int)(row % p.Hq), bj = (int)(row / p.Hq), b = bj / p.C, j = bj - b * p.C;
   const int h = hq / p.ratio, r = j * p.ratio + (hq - h * p.ratio);
@@ -1207,12 +1210,18 @@ __global__ __launch_bounds__(kThreads) void shared_join_kernel(SharedParams p) {
   const int n = np + (seen + p.own_range - 1) / p.own_range;
   const long long own = p.own_part + (long long)(b * p.Hkv + h) * p.own_max * p.G + r;
   float M = -INFINITY, L = 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f};
-  for (int s0 = 0; s0 < n; s0 += kJoin) {  // kJoin partials a round trip
+  for (int s0 = group; s0 < n; s0 += GROUPS * kJoin) {  // kJoin partials a round trip
     float2 ml[kJoin];
     float x[kJoin][4];
 #pragma unroll
     for (int k = 0; k < kJoin; ++k) {
-      const int s = min(s0 + k, n - 1);
+      const int s = s0 + k * GROUPS;
+      if (s0 + k * GROUPS >= n) {
+        ml[k] = make_float2(-INFINITY, 0.f);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) x[k][c] = 0.f;
+        continue;
+      }
       const size_t at = (size_t)(s < np ? pre + s * step : own + (long long)(s - np) * p.G);
       ml[k] = *reinterpret_cast<const float2*>(&p.part_ml[at * 2]);
       const float* o = p.part_o + at * p.d;
@@ -1234,13 +1243,23 @@ __global__ __launch_bounds__(kThreads) void shared_join_kernel(SharedParams p) {
     for (int c = 0; c < 4; ++c) acc[c] *= keep;
 #pragma unroll
     for (int k = 0; k < kJoin; ++k) {
-      if (s0 + k >= n) break;
+      if (s0 + k * GROUPS >= n) break;
       const float w = exp2f(ml[k].x - ref);
       L += w * ml[k].y;
 #pragma unroll
       for (int c = 0; c < 4; ++c) acc[c] += w * x[k][c];
     }
   }
+#pragma unroll
+  for (int step = LPR; step < LPR * GROUPS; step *= 2) {  // join the groups
+    const float other = __shfl_xor(M, step, 64), top = fmaxf(M, other), ref = top == -INFINITY ? 0.f : top;
+    const float mine = exp2f(M - ref), theirs = exp2f(other - ref);
+    L = L * mine + __shfl_xor(L, step, 64) * theirs;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) acc[k] = acc[k] * mine + __shfl_xor(acc[k], step, 64) * theirs;
+    M = top;
+  }
+  if (group) return;
   const float inv = 1.f / L;
 #pragma unroll
   for (int k = 0; k < 4; ++k) acc[k] *= inv;
@@ -1413,11 +1432,11 @@ int launch_mfma(const SharedParams& p, long long grid, hipStream_t s) {
   return SPV_OK;
 }
 
-template <int QT, int LPR, bool VEC>
+template <int QT, int LPR, int GROUPS, bool VEC>
 int launch_join(const SharedParams& p, hipStream_t s) {
-  const long long rows = (long long)p.B * p.C * p.Hq, per = kThreads / LPR;
-  hipLaunchKernelGGL((shared_join_kernel<QT, LPR, VEC>), dim3((unsigned)((rows + per - 1) / per)), dim3(kThreads), 0, s,
-                     p);
+  const long long rows = (long long)p.B * p.C * p.Hq, per = kThreads / (LPR * GROUPS);
+  hipLaunchKernelGGL((shared_join_kernel<QT, LPR, GROUPS, VEC>), dim3((unsigned)((rows + per - 1) / per)), dim3(kThreads),
+                     0, s, p);
   SPV_CHECK_LAUNCH();
   return SPV_OK;
 }
@@ -1445,9 +1464,10 @@ int launch(const SharedParams& p, int kv_dtype, hipStream_t s) {
     default: rc = launch_valu<QT, SPV_FP8E4M3>(p, grid, s); break;
   }
   if (rc != SPV_OK) return rc;
-  if (p.d == 128) return launch_join<QT, 32, true>(p, s);
-  if (p.d == 64) return launch_join<QT, 16, true>(p, s);
-  return launch_join<QT, 64, false>(p, s);
+  const bool few = (long long)p.B * p.C * p.Hq < kFewRows;
+  if (p.d == 128) return few ? launch_join<QT, 32, 2, true>(p, s) : launch_join<QT, 32, 1, true>(p, s);
+  if (p.d == 64) return few ? launch_join<QT, 16, 4, true>(p, s) : launch_join<QT, 16, 1, true>(p, s);
+  return launch_join<QT, 64, 1, false>(p, s);
 }
 
 }  // namespace

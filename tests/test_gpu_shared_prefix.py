@@ -97,6 +97,8 @@ SHAPES = [
     (2, 3, 2, 1, 256, 24, [90], [0, 0], [25, 0]),
     (2, 3, 2, 1, 9, 16, [20], [0, 0], [25, 0]),
     (2, 40, 8, 2, 64, 16, [90], [0, 0], [25, 0]),                         # long chunks
+    (80, 7, 16, 2, 128, 16, [150, 33], [0, 1] * 40, list(range(80))),      # many rows
+    (150, 4, 14, 2, 64, 16, [70], [0, 0, -1] * 50, list(range(150))),
 ]
 
 
