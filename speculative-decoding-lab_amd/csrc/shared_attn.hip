@@ -77,6 +77,7 @@ enum : int { E_SEG = 0, E_TILES, E_RANGES, E_RANK, E_WORDS };
 constexpr int kTile = 256;    // rows of a prefix tile
 constexpr int kUnit = 64;     // keys
 constexpr int kOwnRows = 64;  // rows of an entry that a workgroup takes over its own keys
+constexpr int kPagesRows = 64;  // segments of at most so many rows are walked like own keys
 
 struct SharedParams {
   void* out;
@@ -158,13 +159,9 @@ __device__ __forceinline__ bool own_item(const SharedParams& p, int o, Item& it)
 
 // Row R of an item's row order: its entry, chunk token and q head.
 __device__ __forceinline__ void row_at(const SharedParams& p, const Item& it, int R, int& b, int& j, int& hq) {
-  int r = R;
-  b = it.b;
-  if (it.first >= 0) {
-    const int m = R / p.G;
-    r = R - m * p.G;
-    b = p.members[it.first + m];
-  }
+  const int m = it.first >= 0 ? R / p.G : 0, r = R - m * p.G;
+  const int member = p.members[max(it.first, 0) + m];  // (the entries' section follows the members')
+  b = it.first >= 0 ? member : it.b;
   j = r / p.ratio;
   hq = it.h * p.ratio + (r - j * p.ratio);
 }
@@ -864,7 +861,7 @@ struct Walk {
     }
   }
 
-  // ---- an entry's own keys, and in fp32 a segment too: 32 rows per wave (false: the chunk
+  // ---- an entry's own keys, and a segment of few rows or in fp32: 32 rows per wave (false: the chunk
   // holds a value that is not finite; nothing is written then). nk waves share the
   // rows (8 up to 32 rows, 4 up to 64, 2 up to 128, 1 up to 256) and take every nk-th
   // page straight into operand registers, one page in flight while one is computed;
@@ -1172,12 +1169,14 @@ __global__ __launch_bounds__(kMfmaThreads, 2) void shared_mfma_kernel(SharedPara
   bool done;
   if (id < p.seg_wgs) {
     if (!segment_item(p, id, it)) return;
-    if constexpr (KT == SPV_F32) done = walk.pages(it);
-    else done = walk.prefix(it);
-  } else {
-    if (!own_item(p, id - p.seg_wgs, it)) return;
-    done = walk.pages(it);
+  } else if (!own_item(p, id - p.seg_wgs, it)) {
+    return;
   }
+  // A segment of few rows is walked as own keys are, its pages shared out over the waves: 28
+  // rows x 2 kv heads of 64 behind 32768 fp16 keys take 10.2 us, 15.3 in a tile of 256 rows
+  // (63 x 2 of fp8 13.5 and 18.5; 72 x 2 of 128, bf16, 29.5 and 22.0).
+  if (KT != SPV_F32 && it.first >= 0 && it.rows > kPagesRows) done = walk.prefix(it);
+  else done = walk.pages(it);
   if (!done) valu_item<Walk<D, KT>::QT, KT, D, kMfmaThreads>(p, it, reinterpret_cast<float*>(smem));
 }
 
