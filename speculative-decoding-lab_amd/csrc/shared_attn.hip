@@ -440,7 +440,7 @@ struct Walk {
       if constexpr (kFp8) {
         const float2 s = scales_of(phys);
         ksc = s.x;
-        vsc = vref > 0.f ? s.y / vref : 0.f;
+        vsc = s.y;
       }
     };
     int raw = read_ids(0);
@@ -597,7 +597,10 @@ struct Walk {
     float m[NT], l[NT], thr[NT];  // thr: the score above which m must grow
     f32x4_t sc[4][NT];            // S^T of the tile in the walk
     uint32_t ph[2][NT][4];        // its P, two pages an operand
-    float ks_t = 1.f, vs_t = 1.f;  // fp8: scales of the window of the tile in the walk
+    // fp8, of the window of the tile in the walk: a page's K scale times the softmax's, log2 of
+    // its V scale over vref, and the inverse of that ratio. Pages whose ratio is below 2^-100
+    // count as 2^-100: their P vanishes in fp16 either way.
+    float ks_t = 1.f, vl_t = 0.f, vi_t = 1.f;
     auto pv = [&](int vslot) SPV_INLINE {
       const uint16_t* V = sV + vslot * LD::kV;
 #pragma unroll
@@ -630,13 +633,23 @@ struct Walk {
       }
     };
     auto softmax = [&](int t) SPV_INLINE {
+      // fp8: scores stay raw codes' products; a page's K scale goes into the exponent's
+      // multiplier and its V scale, as a logarithm, into the addend.
+      float slf[4], lv[4], vi[4];
       if constexpr (kFp8) {
-        if ((t & 15) == 0) ks_t = ksc, vs_t = vsc;
+        if ((t & 15) == 0) {
+          ks_t = ksc * sl2;
+          if (ks_t == 0.f) ks_t = 1e-38f;  // (a masked -inf times 0 would be NaN)
+          const float ratio = vref > 0.f ? vsc / vref : 0.f;
+          vl_t = ratio < 0x1p-100f ? -100.f : __builtin_amdgcn_logf(ratio);
+          vi_t = __builtin_amdgcn_exp2f(-vl_t);
+        }
 #pragma unroll
         for (int kt = 0; kt < 4; ++kt) {
-          const float f = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(ks_t), (4 * t + kt) & 63));
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt) sc[kt][nt] *= f;
+          const int at = (4 * t + kt) & 63;
+          slf[kt] = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(ks_t), at));
+          lv[kt] = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(vl_t), at));
+          vi[kt] = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(vi_t), at));
         }
       }
       const int t0 = key0 + t * kUnit;
@@ -653,14 +666,22 @@ struct Walk {
       bool grow = false;
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
-        float a0 = max3_raw(sc[0][nt][0], sc[0][nt][1], sc[0][nt][2]);
-        float a1 = max3_raw(sc[0][nt][3], sc[1][nt][0], sc[1][nt][1]);
-        float a2 = max3_raw(sc[1][nt][2], sc[1][nt][3], sc[2][nt][0]);
-        float a3 = max3_raw(sc[2][nt][1], sc[2][nt][2], sc[2][nt][3]);
-        float a4 = max3_raw(sc[3][nt][0], sc[3][nt][1], sc[3][nt][2]);
-        a0 = max3_raw(a0, a1, a2);
-        a3 = max3_raw(a3, a4, sc[3][nt][3]);
-        mx[nt] = fmaxf(a0, a3);
+        if constexpr (kFp8) {  // in log2 units
+          float a[4];
+#pragma unroll
+          for (int kt = 0; kt < 4; ++kt)
+            a[kt] = max3_raw(max3_raw(sc[kt][nt][0], sc[kt][nt][1], sc[kt][nt][2]), sc[kt][nt][3], sc[kt][nt][3]) * slf[kt];
+          mx[nt] = max3_raw(max3_raw(a[0], a[1], a[2]), a[3], a[3]);
+        } else {
+          float a0 = max3_raw(sc[0][nt][0], sc[0][nt][1], sc[0][nt][2]);
+          float a1 = max3_raw(sc[0][nt][3], sc[1][nt][0], sc[1][nt][1]);
+          float a2 = max3_raw(sc[1][nt][2], sc[1][nt][3], sc[2][nt][0]);
+          float a3 = max3_raw(sc[2][nt][1], sc[2][nt][2], sc[2][nt][3]);
+          float a4 = max3_raw(sc[3][nt][0], sc[3][nt][1], sc[3][nt][2]);
+          a0 = max3_raw(a0, a1, a2);
+          a3 = max3_raw(a3, a4, sc[3][nt][3]);
+          mx[nt] = fmaxf(a0, a3);
+        }
         grow |= mx[nt] > thr[nt];
       }
       if (__any(grow)) {
@@ -668,30 +689,25 @@ struct Walk {
         for (int nt = 0; nt < NT; ++nt) {
           float a = fmaxf(mx[nt], __shfl_xor(mx[nt], 16, 64));
           a = fmaxf(a, __shfl_xor(a, 32, 64));
-          const float m_new = fmaxf(m[nt], a * sl2);
+          const float m_new = fmaxf(m[nt], kFp8 ? a : a * sl2);
           const float alpha = m_new == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m[nt] - m_new);
           l[nt] *= alpha;
 #pragma unroll
           for (int mt = 0; mt < MT; ++mt) o[mt][nt] *= alpha;
           m[nt] = m_new;
-          thr[nt] = (m_new + kSlack) * inv_sl2;
+          thr[nt] = kFp8 ? m_new + kSlack : (m_new + kSlack) * inv_sl2;
         }
       }
 #pragma unroll
       for (int kt = 0; kt < 4; ++kt) {
-        float f = 1.f;
-        if constexpr (kFp8) f = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(vs_t), (4 * t + kt) & 63));
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
           const float mu = m[nt] == -INFINITY ? 0.f : m[nt];
+          const float mul = kFp8 ? slf[kt] : sl2, add = kFp8 ? lv[kt] - mu : -mu;
           float e[4];
 #pragma unroll
-          for (int jj = 0; jj < 4; ++jj) e[jj] = __builtin_amdgcn_exp2f(fmaf(sc[kt][nt][jj], sl2, -mu));
-          if constexpr (kFp8) {
-            l[nt] += (e[0] + e[1]) + (e[2] + e[3]);
-#pragma unroll
-            for (int jj = 0; jj < 4; ++jj) e[jj] *= f;
-          }
+          for (int jj = 0; jj < 4; ++jj) e[jj] = __builtin_amdgcn_exp2f(fmaf(sc[kt][nt][jj], mul, add));
+          if constexpr (kFp8) l[nt] = fmaf((e[0] + e[1]) + (e[2] + e[3]), vi[kt], l[nt]);
           const uint32_t p01 = pack2_f16(e[0], e[1]), p23 = pack2_f16(e[2], e[3]);
           ph[kt >> 1][nt][2 * (kt & 1)] = p01;
           ph[kt >> 1][nt][2 * (kt & 1) + 1] = p23;
@@ -708,14 +724,6 @@ struct Walk {
       __syncthreads();
       __builtin_amdgcn_sched_barrier(0);
     };
-    if constexpr (kFp8) {
-      float mx = 0.f;
-      for (int pg = tid; pg < pages; pg += kMfmaThreads) {
-        const int phys = table[pg];
-        if ((unsigned)phys < (unsigned)p.cap) mx = fmaxf(mx, scales_of(phys).y);
-      }
-      vref = __uint_as_float(wg_max(__float_as_uint(mx)));
-    }
     // The walk. Group 0 runs phases M(0), V(0), M(1), V(1), ... and group 1 the same
     // one phase later, a barrier after each, so that on every SIMD one wave's
     // softmax runs beside the other's matrix instructions:
@@ -741,6 +749,14 @@ struct Walk {
       idn = raw;
       load_next(st0, 0);
       load_next(st1, 1);
+      if constexpr (kFp8) {
+        float mx = 0.f;
+        for (int pg = tid; pg < pages; pg += kMfmaThreads) {
+          const int phys = table[pg];
+          if ((unsigned)phys < (unsigned)p.cap) mx = fmaxf(mx, scales_of(phys).y);
+        }
+        vref = __uint_as_float(wg_max(__float_as_uint(mx)));
+      }
       if constexpr (!kF16 && !kFp8) {
         uint32_t mx = 0;  // the largest finite |v| of the first tile
         edge(st0, 0);
