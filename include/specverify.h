@@ -441,8 +441,8 @@ int64_t spv_shared_attn_plan(const int32_t* prefix_ids, const int32_t* prefix_le
                              int kv_dtype, int32_t* plan, int64_t plan_ints);
 
 /* Workspace of spv_shared_attn (partial results; needs no particular contents
- * and may be another one in every call) for own contexts up to max_ctx;
- * plan_host: the plan on the host. 0 for bad arguments. */
+ * and may be another one in every call, on a 16-byte address) for own contexts up
+ * to max_ctx; plan_host: the plan on the host. 0 for bad arguments. */
 size_t spv_shared_attn_workspace_bytes(const int32_t* plan_host, int32_t head_dim,
                                        int32_t max_ctx);
 

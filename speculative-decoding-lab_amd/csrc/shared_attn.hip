@@ -1461,8 +1461,9 @@ int launch(const SharedParams& p, int kv_dtype, hipStream_t s) {
   const long long grid = p.seg_wgs + (long long)p.B * p.Hkv * p.own_tiles * p.own_max;
   int rc;
   // The matrix kernels apply the scale inside the exponent, to maxima of raw scores.
-  // They count pages in 31 bits.
-  const bool mfma = (long long)(p.layer + 1) * p.cap * p.Hkv < (1LL << 31) && p.bs == 16 &&
+  // They count pages in 31 bits and load 16 bytes at a time.
+  const auto aligned = [](const void* x) { return (uintptr_t)x % 16 == 0; };
+  const bool mfma = aligned(p.q) && aligned(p.kpool) && aligned(p.vpool) && (long long)(p.layer + 1) * p.cap * p.Hkv < (1LL << 31) && p.bs == 16 &&
                     (p.d == 64 || p.d == 128) && p.scale_log2 > 0.f && p.scale_log2 < INFINITY &&
                     ((QT == SPV_BF16 && kv_dtype == SPV_FP8E4M3) || QT == kv_dtype);
   if (mfma) {
@@ -1480,6 +1481,7 @@ int launch(const SharedParams& p, int kv_dtype, hipStream_t s) {
   }
   if (rc != SPV_OK) return rc;
   const bool few = (long long)p.B * p.C * p.Hq < kFewRows;
+  if (!aligned(p.out)) return launch_join<QT, 64, 1, false>(p, s);
   if (p.d == 128) return few ? launch_join<QT, 32, 2, true>(p, s) : launch_join<QT, 32, 1, true>(p, s);
   if (p.d == 64) return few ? launch_join<QT, 16, 4, true>(p, s) : launch_join<QT, 16, 1, true>(p, s);
   return launch_join<QT, 64, 1, false>(p, s);
@@ -1535,7 +1537,8 @@ int spv_shared_attn(void* out, const void* q, int q_dtype, const void* k_pool, c
   if (head_dim < 1 || head_dim > 256 || layer < 0 || capacity < 1 || max_ctx < C || max_ctx > (1 << 30)) return SPV_ERR_ARG;
   const int longest = std::max(max_ctx, h[PH_MAXP]);
   if (max_blocks_per_seq < (longest + block_size - 1) / block_size) return SPV_ERR_ARG;
-  if (workspace_bytes < spv_shared_attn_workspace_bytes(h, head_dim, max_ctx)) return SPV_ERR_WORKSPACE;
+  if (workspace_bytes < spv_shared_attn_workspace_bytes(h, head_dim, max_ctx) || (uintptr_t)workspace % 16)
+    return SPV_ERR_WORKSPACE;
   SharedParams p{};
   p.out = out;
   p.q = q;

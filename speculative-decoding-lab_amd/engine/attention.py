@@ -334,16 +334,18 @@ def shared_prefix_attention(query_3d: torch.Tensor, kv: PagedKVCache, layer: int
     longest = max(max_ctx, prefix.longest)
     if longest > kv._maxb * kv.block_size:
         kv._grow_width(-(-longest // kv.block_size))
-    if prefix._bytes[0] != max_ctx:
-        prefix._bytes = (max_ctx, int(_hip.lib().spv_shared_attn_workspace_bytes(prefix._host, d, max_ctx)))
+    known, ws_bytes = prefix._bytes
+    if known != max_ctx:
+        ws_bytes = int(_hip.lib().spv_shared_attn_workspace_bytes(prefix._host, d, max_ctx))
+        prefix._bytes = (max_ctx, ws_bytes)
     # from the allocator in every call: ordered with its stream's work, and a
     # captured graph's own
-    ws = torch.empty(prefix._bytes[1], dtype=torch.uint8, device=kv.device)
+    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=kv.device)
     call("spv_shared_attn", out.data_ptr(), q.data_ptr(), _hip.dtype_code(q.dtype), kv.k_pool.data_ptr(),
          kv.v_pool.data_ptr(), kv._dt, ptr(kv.scales), kv.tables_dev.data_ptr(), kv._maxb, sid_t.data_ptr(),
          start_t.data_ptr(), kv.lens_dev.data_ptr(), kv.allocator.ctr.data_ptr(), B, chunk, hq, kv.num_kv_heads, d,
          kv.block_size, layer, kv.allocator.capacity, max_ctx, prefix.scale if scale is None else float(scale),
-         prefix._host, prefix._dev.data_ptr(), ws.data_ptr(), prefix._bytes[1], _hip.stream_of(kv.device))
+         prefix._host, prefix._dev.data_ptr(), ws.data_ptr(), ws_bytes, _hip.stream_of(kv.device))
     kv._stale = True
     return out
 

@@ -194,6 +194,29 @@ def test_magnitudes_of_values(cuda, dtype, where):
         _check(out, want, dtype)
 
 
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("B", [1, 9])
+def test_fp8_pages_of_very_different_scales(cuda, d, B):
+    """Pages of zeros (keys, values, both) and of values 2^-40 and 2^-110 times the others' among
+    a prefix's pages; what they add to the sums is the keys' share alone."""
+    g = torch.Generator().manual_seed(37)
+    C, hq, hkv, plen = 5, 16, 2, 300
+    kv, _ = _pool(cuda, [C + 8] * B + [plen], hkv, d, 16, FP8, g)
+    k, v = (torch.randn(1, plen, hkv, d, generator=g) for _ in range(2))
+    k[:, 16:32] = 0
+    v[:, 48:64] = 0
+    k[:, 80:96] = v[:, 80:96] = 0
+    v[:, 112:128] *= 2.0 ** -40
+    v[:, 208:224] *= 2.0 ** -110
+    kv.truncate(B, 0)
+    kv.write_block(0, [B], [0], k.to(BF16).to(cuda), v.to(BF16).to(cuda))
+    ctx = [gather_ctx(kv, 0, s, n).cpu().double() for s, n in enumerate([C + 8] * B + [plen])]
+    prefix = SharedPrefix(kv, [B] * B, [plen] * B, C, hq)
+    q = _q(g, B, C, hq, d, kv, cuda)
+    out = shared_prefix_attention(q, kv, 0, list(range(B)), [8] * B, C + 8, prefix)
+    _check(out, _want(q, ctx, list(range(B)), [8] * B, [B] * B, [plen] * B), q.dtype)
+
+
 @pytest.mark.parametrize("dtype", [F32, BF16, F16])
 @pytest.mark.parametrize("d", [64, 128, 80])
 @pytest.mark.parametrize("bad", [float("inf"), float("-inf"), float("nan")])
@@ -290,6 +313,37 @@ def test_strided_queries_and_own_output(cuda):
     got = shared_prefix_attention(q, kv, 0, [1, 0], [28, 10], 30, p, out=out)
     assert got is out
     _check(out, _want(q, ctx, [1, 0], [28, 10], [2, 2], [100, 100]), BF16)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("d", [64, 128])
+def test_rows_on_any_address(cuda, dtype, d):
+    """Queries and outputs one element behind a 16-byte address."""
+    g = torch.Generator().manual_seed(43)
+    kv, (ctx,) = _pool(cuda, [12, 30, 100], 2, d, 16, dtype, g)
+    p = SharedPrefix(kv, [2, 2], [100, 100], 2, 4)
+    q = _q(g, 2, 2, 4, d, kv, cuda)
+    buf_q, buf_out = (torch.empty(q.numel() + 1, dtype=dtype, device=cuda) for _ in range(2))
+    odd = buf_q[1:].view(q.shape)
+    odd.copy_(q)
+    want = _want(q, ctx, [0, 1], [10, 28], [2, 2], [100, 100])
+    _check(shared_prefix_attention(odd, kv, 0, [0, 1], [10, 28], 30, p), want, dtype)
+    out = buf_out[1:].view(q.shape)
+    _check(shared_prefix_attention(q, kv, 0, [0, 1], [10, 28], 30, p, out=out), want, dtype)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16, FP8])
+def test_one_sequence_in_several_entries(cuda, dtype):
+    """Entries that read the same own sequence, as of different positions, and one whose
+    prefix is its own sequence."""
+    g = torch.Generator().manual_seed(47)
+    C, hq, hkv, d = 3, 8, 2, 64
+    kv, (ctx,) = _pool(cuda, [90, 150], hkv, d, 16, dtype, g)
+    sids, starts, ids, lens = [0, 0, 0, 1, 1], [5, 87, 40, 0, 147], [1, 1, -1, 1, 0], [150, 70, 0, 33, 90]
+    p = SharedPrefix(kv, ids, lens, C, hq)
+    q = _q(g, len(sids), C, hq, d, kv, cuda)
+    out = shared_prefix_attention(q, kv, 0, sids, starts, 150, p)
+    _check(out, _want(q, ctx, sids, starts, ids, lens), q.dtype)
 
 
 def test_captured_graphs_and_streams(cuda):
