@@ -76,9 +76,10 @@ enum : int {
   PH_SEGS,
   PH_MEMBERS,
   PH_ENTRIES,
+  PH_OWN,  // keys of an own range at least
   PH_WORDS
 };
-constexpr int kPlanMagic = 0x53505234;
+constexpr int kPlanMagic = 0x53505235;
 // A segment: sequence and length of the prefix, kv head, first member, first row of
 // the tile and its rows, the keys.
 enum : int { S_SID = 0, S_LEN, S_HEAD, S_FIRST, S_ROW0, S_ROWS, S_KEY0, S_KEY1, S_WORDS };
@@ -1405,6 +1406,7 @@ int make_plan(std::vector<int32_t>& plan, const int32_t* ids, const int32_t* len
   plan[PH_BS] = bs;
   plan[PH_NSEG] = (int32_t)nseg;
   plan[PH_MAXP] = (int32_t)maxp;
+  plan[PH_OWN] = kv_dtype == SPV_F32 ? 64 : 256;
   auto add = [&](int word, const std::vector<int32_t>& v) {
     while (plan.size() % 16) plan.push_back(0);
     plan[word] = (int32_t)plan.size();
@@ -1418,12 +1420,17 @@ int make_plan(std::vector<int32_t>& plan, const int32_t* ids, const int32_t* len
 }
 
 // The entries' own ranges for contexts up to max_ctx: as many as make about 256
-// workgroups (one for each CU), none shorter than 256 keys (four waves with four pages each).
+// workgroups (one for each CU), none shorter than PH_OWN keys: 256 (four waves with four
+// pages each), 64 in fp32, where a page takes a wave sixteen times as long. Where the
+// prefixes' segments leave CUs free, half of that (24 x 2 rows of own and prefix, bf16: 13.0
+// us, 15.4 with 256 keys; with the segments of 192 x 2 rows 24.8 and 21.2).
 void own_ranges(const int32_t* plan, int max_ctx, int* range, int* count) {
   const int bs = plan[PH_BS];
-  const long long G = (long long)plan[PH_C] * (plan[PH_HQ] / plan[PH_HKV]);
+  const long long G = (long long)plan[PH_C] * (plan[PH_HQ] / plan[PH_HKV]), least = plan[PH_OWN];
   const long long wgs = (long long)plan[PH_B] * plan[PH_HKV] * ((G + kOwnRows - 1) / kOwnRows);
-  const long long want = std::max(1LL, std::min(256 / wgs, (long long)max_ctx / 256));
+  const long long all = std::min(kCUs / wgs, max_ctx / least);
+  const long long beside = std::min((kCUs - std::min(kCUs, plan[PH_NSEG])) / wgs, max_ctx / (least / 2));
+  const long long want = std::max({1LL, all, beside});
   const long long keys = (max_ctx + want - 1) / want;
   *range = (int)((keys + bs - 1) / bs * bs);
   *count = (max_ctx + *range - 1) / *range;

@@ -296,10 +296,8 @@ def rotary_append(query: Optional[torch.Tensor], k_new: torch.Tensor, v_new: tor
             plan._check(a.epoch, B, C, sid_t, start_t)
             rows, follow = plan.rows, 1
     call("spv_kv_rotary_append", ptr(query_out), ptr(q), k.data_ptr(), v.data_ptr(), kv._dt,
-         _strides(query_out, q, k, v) if strides is None else strides, kv.k_pool.data_ptr(), kv.v_pool.data_ptr(),
-         kv.tables_dev.data_ptr(), kv._maxb, kv.nblocks_dev.data_ptr(), kv.lens_dev.data_ptr(),
-         a.free_stack.data_ptr(), a.free_flag.data_ptr(), a.ctr.data_ptr(), sid_t.data_ptr(), start_t.data_ptr(),
-         ptr(pos), *rotary._args, B, C, hq, kv.num_kv_heads, kv.head_dim, rotary.rotary_dim, rotary.interleaved, layer,
+         _strides(query_out, q, k, v) if strides is None else strides, *kv._addresses(), sid_t.data_ptr(),
+         start_t.data_ptr(), ptr(pos), *rotary._args, B, C, hq, kv.num_kv_heads, kv.head_dim, rotary.rotary_dim, rotary.interleaved, layer,
          a.capacity, kv.block_size, bool(alloc), follow, ptr(rows), _hip.stream_of(kv.device))
     if not follow:
         if rows is not None:
