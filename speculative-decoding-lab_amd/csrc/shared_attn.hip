@@ -76,7 +76,8 @@ enum : int {
   PH_SEGS,
   PH_MEMBERS,
   PH_ENTRIES,
-  PH_OWN,  // keys of an own range at least
+  PH_OWN,   // keys of an own range at least
+  PH_TILE,  // rows of a tile
   PH_WORDS
 };
 constexpr int kPlanMagic = 0x53505235;
@@ -85,7 +86,7 @@ constexpr int kPlanMagic = 0x53505235;
 enum : int { S_SID = 0, S_LEN, S_HEAD, S_FIRST, S_ROW0, S_ROWS, S_KEY0, S_KEY1, S_WORDS };
 // An entry: the group's first segment (-1: no prefix), its tiles, ranges, the entry's rank in it.
 enum : int { E_SEG = 0, E_TILES, E_RANGES, E_RANK, E_WORDS };
-constexpr int kTile = 256;    // rows of a prefix tile
+constexpr int kTile = 256;    // rows of a prefix tile (fp32: 64, 128 or 256)
 constexpr int kUnit = 64;     // keys
 constexpr int kOwnRows = 64;  // rows of an entry that a workgroup takes over its own keys
 constexpr int kPagesRows = 64;  // segments of at most so many rows are walked like own keys
@@ -107,6 +108,7 @@ struct SharedParams {
   float* part_o;   // partial rows x d
   float* part_ml;  // partial rows x 2
   int maxb, B, C, Hq, Hkv, ratio, G, d, bs, layer, cap;
+  int tile;                // rows of a segment
   int nseg, seg_wgs;       // segments, and their workgroups (a multiple of 8)
   int own_range, own_max;  // keys per own range (whole blocks), ranges per entry at most
   int own_tiles;           // tiles of an entry's rows
@@ -144,7 +146,7 @@ __device__ __forceinline__ bool segment_item(const SharedParams& p, int id, Item
   it.key1 = s[S_KEY1];
   it.start = 0x3fffffff;
   it.b = p.members[it.first];
-  it.part = (long long)seg * kTile;
+  it.part = (long long)seg * p.tile;
   if (threadIdx.x == 0 && p.lens && p.lens[it.sid] < s[S_LEN]) flag_bad_read(p, it.b);
   return true;
 }
@@ -1230,8 +1232,8 @@ __global__ __launch_bounds__(kThreads) void shared_join_kernel(SharedParams p) {
   if (e[E_SEG] >= 0) {
     const long long R = (long long)e[E_RANK] * p.G + r;
     np = e[E_RANGES];
-    step = (long long)e[E_TILES] * kTile;
-    pre = (e[E_SEG] + (long long)h * np * e[E_TILES] + R / kTile) * kTile + R % kTile;
+    step = (long long)e[E_TILES] * p.tile;
+    pre = (e[E_SEG] + (long long)h * np * e[E_TILES] + R / p.tile) * p.tile + R % p.tile;
   }
   const int n = np + (seen + p.own_range - 1) / p.own_range;
   const long long own = p.own_part + (long long)(b * p.Hkv + h) * p.own_max * p.G + r;
@@ -1325,9 +1327,12 @@ long long unit_ns(int kv_dtype, int d, int bs) {
 // first to end. bf16, 1152 rows x 2 kv heads over 2048 keys: 16 ranges take 28.3 us and
 // 8.4 in the join, 8 ranges 20.8 and 5.7; 1008 rows x 2 over 32768 keys of fp8 with 32 such
 // workgroups: 31 ranges take 49.1 and 11.7, 27 ranges 43.4 and 10.1.
+// fp32 tiles may have fewer rows, where the matrix cores of more CUs are worth reading the
+// keys again: ten entries of 30 rows x 2 behind three prefixes of up to 1501 keys take 19.1 us in
+// tiles of 64 rows, 23.3 in tiles of 256 (32 such entries behind 4096 keys 59.9 and 68.9).
 constexpr int kCUs = 256, kFixed = 9000, kPartial = 110;
 long long best_range(const std::vector<long long>& tiles, const std::vector<long long>& units, long long own,
-                     long long unit, int d) {
+                     long long unit, int d, int rows, long long* range_out) {
   long long most = 1, best = 1, least = -1;
   for (long long u : units) most = std::max(most, u);
   // ceil(most / k) for every number of ranges k: no other length cuts the longest prefix evenly
@@ -1337,14 +1342,15 @@ long long best_range(const std::vector<long long>& tiles, const std::vector<long
     for (size_t g = 0; g < units.size(); ++g) n += tiles[g] * ((units[g] + range - 1) / range);
     const long long rounds = (n + kCUs - 1) / kCUs;
     const long long late = n + own > rounds * kCUs ? kFixed : 0;
-    const long long time = rounds * (range * unit + kFixed) + late + n * kPartial * d / 128;
+    const long long time = rounds * (range * unit * rows / kTile + kFixed) + late + n * kPartial * d / 128 * rows / kTile;
     if (least < 0 || time < least) {
       least = time;
       best = range;
     }
     if (n > 4 * kCUs && k > 1) break;  // more, shorter segments only add to the fixed part
   }
-  return best;
+  *range_out = best;
+  return least;
 }
 
 int make_plan(std::vector<int32_t>& plan, const int32_t* ids, const int32_t* lens, int B, int C, int Hq, int Hkv, int d,
@@ -1364,27 +1370,39 @@ int make_plan(std::vector<int32_t>& plan, const int32_t* ids, const int32_t* len
     groups[g].members.push_back(b);
   }
   std::vector<long long> tiles, units;
-  long long maxp = 0;
+  long long maxp = 0, range = 1, least = -1;
+  int tile = kTile;
   for (const Group& x : groups) {
-    tiles.push_back(((long long)x.members.size() * G + kTile - 1) / kTile);
     units.push_back((x.len + kUnit - 1LL) / kUnit);
     maxp = std::max<long long>(maxp, x.len);
   }
-  std::vector<long long> all(tiles);
-  for (long long& t : all) t *= Hkv;
-  const long long range = best_range(all, units, (long long)B * Hkv, unit_ns(kv_dtype, d, bs), d);
+  for (int rows = kTile; rows >= (kv_dtype == SPV_F32 ? kPagesRows : kTile); rows /= 2) {
+    std::vector<long long> cut, all;
+    for (const Group& x : groups) {
+      cut.push_back(((long long)x.members.size() * G + rows - 1) / rows);
+      all.push_back(cut.back() * Hkv);
+    }
+    long long best = 1;
+    const long long time = best_range(all, units, (long long)B * Hkv, unit_ns(kv_dtype, d, bs), d, rows, &best);
+    if (least < 0 || time < least) {
+      least = time;
+      range = best;
+      tile = rows;
+      tiles = cut;
+    }
+  }
   long long nseg = 0;
   for (size_t g = 0; g < groups.size(); ++g) {
     const Group& x = groups[g];
     // equal ranges, of whole units
     const long long ranges = (units[g] + range - 1) / range, per = (units[g] + ranges - 1) / ranges;
     const long long used = (units[g] + per - 1) / per, rows = (long long)x.members.size() * G;
-    if ((nseg + tiles[g] * Hkv * used) > 0x7fffffffLL / kTile) return SPV_ERR_UNSUPPORTED;
+    if ((nseg + tiles[g] * Hkv * used) > 0x7fffffffLL / tile) return SPV_ERR_UNSUPPORTED;
     for (int h = 0; h < Hkv; ++h)
       for (long long s = 0; s < used; ++s)
         for (long long t = 0; t < tiles[g]; ++t) {
-          const int32_t w[S_WORDS] = {x.sid, x.len, h, (int32_t)members.size(), (int32_t)(t * kTile),
-                                      (int32_t)std::min<long long>(kTile, rows - t * kTile), (int32_t)(s * per * kUnit),
+          const int32_t w[S_WORDS] = {x.sid, x.len, h, (int32_t)members.size(), (int32_t)(t * tile),
+                                      (int32_t)std::min<long long>(tile, rows - t * tile), (int32_t)(s * per * kUnit),
                                       (int32_t)std::min<long long>((s + 1) * per * kUnit, x.len)};
           segs.insert(segs.end(), w, w + S_WORDS);
         }
@@ -1406,6 +1424,7 @@ int make_plan(std::vector<int32_t>& plan, const int32_t* ids, const int32_t* len
   plan[PH_BS] = bs;
   plan[PH_NSEG] = (int32_t)nseg;
   plan[PH_MAXP] = (int32_t)maxp;
+  plan[PH_TILE] = tile;
   plan[PH_OWN] = kv_dtype == SPV_F32 ? 64 : 256;
   auto add = [&](int word, const std::vector<int32_t>& v) {
     while (plan.size() % 16) plan.push_back(0);
@@ -1423,14 +1442,15 @@ int make_plan(std::vector<int32_t>& plan, const int32_t* ids, const int32_t* len
 // workgroups (one for each CU), none shorter than PH_OWN keys: 256 (four waves with four
 // pages each), 64 in fp32, where a page takes a wave sixteen times as long. Where the
 // prefixes' segments leave CUs free, half of that (24 x 2 rows of own and prefix, bf16: 13.0
-// us, 15.4 with 256 keys; with the segments of 192 x 2 rows 24.8 and 21.2).
+// us, 15.4 with 256 keys); and up to twice as long where the CUs beside them then do (192 x 2
+// rows 21.2 us, 24.8 where some wait; 12 entries of 30 x 2 rows in fp32 19.1 and 26.9).
 void own_ranges(const int32_t* plan, int max_ctx, int* range, int* count) {
   const int bs = plan[PH_BS];
   const long long G = (long long)plan[PH_C] * (plan[PH_HQ] / plan[PH_HKV]), least = plan[PH_OWN];
   const long long wgs = (long long)plan[PH_B] * plan[PH_HKV] * ((G + kOwnRows - 1) / kOwnRows);
   const long long all = std::min(kCUs / wgs, max_ctx / least);
   const long long beside = std::min((kCUs - std::min(kCUs, plan[PH_NSEG])) / wgs, max_ctx / (least / 2));
-  const long long want = std::max({1LL, all, beside});
+  const long long want = std::max(1LL, 2 * beside >= all ? beside : all);
   const long long keys = (max_ctx + want - 1) / want;
   *range = (int)((keys + bs - 1) / bs * bs);
   *count = (max_ctx + *range - 1) / *range;
@@ -1440,7 +1460,7 @@ long long part_rows(const int32_t* plan, int max_ctx) {
   int range, count;
   own_ranges(plan, max_ctx, &range, &count);
   const long long G = (long long)plan[PH_C] * (plan[PH_HQ] / plan[PH_HKV]);
-  return (long long)plan[PH_NSEG] * kTile + (long long)plan[PH_B] * plan[PH_HKV] * count * G;
+  return (long long)plan[PH_NSEG] * plan[PH_TILE] + (long long)plan[PH_B] * plan[PH_HKV] * count * G;
 }
 
 // Floats of the (m, l) pairs at the workspace's head: whole 16-byte pieces, so that the rows behind them are aligned.
@@ -1581,12 +1601,13 @@ int spv_shared_attn(void* out, const void* q, int q_dtype, const void* k_pool, c
   p.bs = block_size;
   p.layer = layer;
   p.cap = capacity;
+  p.tile = h[PH_TILE];
   p.nseg = h[PH_NSEG];
   p.seg_wgs = (p.nseg + 7) / 8 * 8;
   p.max_ctx = max_ctx;
   own_ranges(h, max_ctx, &p.own_range, &p.own_max);
   p.own_tiles = (p.G + kOwnRows - 1) / kOwnRows;
-  p.own_part = (long long)h[PH_NSEG] * kTile;
+  p.own_part = (long long)h[PH_NSEG] * h[PH_TILE];
   const long long rows = part_rows(h, max_ctx);
   // both grids: at most 2^32 threads
   const long long own = (long long)B * num_kv_heads * p.own_tiles * p.own_max;

@@ -252,8 +252,8 @@ def rotary_append(query: Optional[torch.Tensor], k_new: torch.Tensor, v_new: tor
     round passes ``alloc=False`` and the first one's ``plan``.
     """
     plain = query is not None and query_out is None
-    sig = (kv._dt, kv.num_kv_heads, kv.head_dim, kv.device, query.shape, query.stride(), query.dtype, query.device, k_new.shape,
-           k_new.stride(), k_new.dtype, k_new.device, v_new.shape, v_new.stride(), v_new.dtype,
+    sig = (kv._dt, kv.num_kv_heads, kv.head_dim, kv.device, query.shape, query.stride(), query.dtype, query.device,
+           k_new.shape, k_new.stride(), k_new.dtype, k_new.device, v_new.shape, v_new.stride(), v_new.dtype,
            v_new.device) if plain else None
     done = rotary._passed.get(sig) if plain else None
     if done is None:
@@ -297,8 +297,9 @@ def rotary_append(query: Optional[torch.Tensor], k_new: torch.Tensor, v_new: tor
             rows, follow = plan.rows, 1
     call("spv_kv_rotary_append", ptr(query_out), ptr(q), k.data_ptr(), v.data_ptr(), kv._dt,
          _strides(query_out, q, k, v) if strides is None else strides, *kv._addresses(), sid_t.data_ptr(),
-         start_t.data_ptr(), ptr(pos), *rotary._args, B, C, hq, kv.num_kv_heads, kv.head_dim, rotary.rotary_dim, rotary.interleaved, layer,
-         a.capacity, kv.block_size, bool(alloc), follow, ptr(rows), _hip.stream_of(kv.device))
+         start_t.data_ptr(), ptr(pos), *rotary._args, B, C, hq, kv.num_kv_heads, kv.head_dim, rotary.rotary_dim,
+         rotary.interleaved, layer, a.capacity, kv.block_size, bool(alloc), follow, ptr(rows),
+         _hip.stream_of(kv.device))
     if not follow:
         if rows is not None:
             plan._record(a.epoch, sid_t, start_t)

@@ -57,6 +57,8 @@ def test_plan_covers_every_row_and_key_once(lib, ids, lens, dtype, d, bs):
     plan = _plan(lib, ids, lens, C, Hq, Hkv, bs, d, dtype)
     assert plan[1] == len(plan)
     segs, members, entries = _sections(plan)
+    tile = plan[13]
+    assert tile == 256 or (dtype == _hip.SPV_F32 and tile in (64, 128))
     want = {}
     for b, (s, n) in enumerate(zip(ids, lens)):
         if s >= 0 and n > 0:
@@ -66,13 +68,13 @@ def test_plan_covers_every_row_and_key_once(lib, ids, lens, dtype, d, bs):
         rows = len(batch) * G
         first, nt, nr = entries[batch[0]][:3]
         assert [entries[b] for b in batch] == [[first, nt, nr, rank] for rank in range(len(batch))]
-        assert first == seen and nt == -(-rows // 256)
+        assert first == seen and nt == -(-rows // tile)
         for h in range(Hkv):
             for t in range(nt):
                 part = [segs[first + (h * nr + s) * nt + t] for s in range(nr)]
                 for x in part:
                     assert x[:3] == [sid, n, h] and members[x[3]:x[3] + len(batch)] == batch
-                    assert x[4] == 256 * t and x[5] == min(256, rows - 256 * t)
+                    assert x[4] == tile * t and x[5] == min(tile, rows - tile * t)
                     assert x[6] < x[7] and x[6] % 64 == 0
                 assert part[0][6] == 0 and part[-1][7] == n
                 assert all(x[7] == y[6] for x, y in zip(part, part[1:]))
