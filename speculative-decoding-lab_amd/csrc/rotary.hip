@@ -46,12 +46,17 @@ struct RotaryParams {
   int B, C, Hq, Hkv, d, R, interleaved, axes, maxb, layer, cap, bs;
 };
 
+// A pair turned by t = (c, s), with the same roundings in every kernel.
+__device__ __forceinline__ float2 turned(float a, float b, float2 t) {
+  return make_float2(fmaf(a, t.x, -(b * t.y)), fmaf(b, t.x, a * t.y));
+}
+
 // cos and sin of position * inv_freq_i, times the factor.
 __device__ __forceinline__ float2 turn_of(const RotaryParams& p, int b, int j, int i) {
   const int axis = p.axis_of ? min(max(p.axis_of[i], 0), p.axes - 1) : 0;
   const int pos = p.positions ? p.positions[((size_t)axis * p.B + b) * p.C + j] : p.start[b] + j;
-  const double t = (double)pos * (p.inv_freq[i] * kInvTwoPi);
-  const float f = (float)(t - __builtin_rint(t));  // turns, in [-1/2, 1/2]
+  const double turns = p.inv_freq[i] * kInvTwoPi;
+  const float f = (float)fma((double)pos, turns, -__builtin_rint((double)pos * turns));  // in [-1/2, 1/2]
   float s, c;
   sincospif(2.f * f, &s, &c);
   return make_float2(c * p.factor, s * p.factor);
@@ -117,8 +122,9 @@ __global__ __launch_bounds__(256) void rotary_elem_kernel(RotaryParams p) {
       const int e0 = p.interleaved ? 2 * i : i, e1 = p.interleaved ? 2 * i + 1 : i + half;
       const float a = load_elem<DT>(src, in + e0), c = load_elem<DT>(src, in + e1);
       const float2 t = turn_of(p, b, j, i);
-      put(e0, a * t.x - c * t.y);
-      put(e1, c * t.x + a * t.y);
+      const float2 y = turned(a, c, t);
+      put(e0, y.x);
+      put(e1, y.y);
     } else {
       const int e = p.R + (i - half);
       put(e, load_elem<DT>(src, in + e));
@@ -139,18 +145,19 @@ __global__ __launch_bounds__(256) void rotary_elem_kernel(RotaryParams p) {
 // Rows of whole 16-byte pieces. A workgroup takes TT tokens of one entry and a
 // slice of the heads. A thread keeps one token and one piece pair (the pieces
 // that rotate with each other; past the rotary width one piece) and goes over
-// the slice's heads with it, kAhead loads in flight. The turns of the
+// the slice's heads with it; the waves of a CU keep enough loads in flight (four
+// heads ahead per thread and 16 tokens a workgroup took 18.4 us over the 75.5 MB
+// below). The turns of the
 // workgroup's tokens are computed once, into LDS, while the first rows travel.
 // The slices behind the query and key heads copy the values, one (16 positions,
 // head) each, transposed through LDS so that whole pages are stored as 16-byte
 // pieces.
 // What bounds it: the rows' bytes, each read and written once, for prompts (75.5 MB of
-// bf16 queries and keys in 17.5 us, 4.3 TB/s; with the values and the cache's writes 30.7 MB
-// a layer in 10.6); a few dependent round trips (start, table, length, position) for decode
+// bf16 queries and keys in 15.2 us, 5.0 TB/s; with the values and the cache's writes 30.7 MB
+// a layer in 9.3); a few dependent round trips (start, table, length, position) for decode
 // chunks (8 tokens 3.9 us, 32 chunks of 6 tokens 4.5).
 constexpr int kVecThreads = 256;
-constexpr int kAhead = 4;
-constexpr int kMaxTT = 16;
+constexpr int kMaxTT = 8;
 constexpr int kVT = 16;  // positions of a value tile
 
 typedef float f32x2_t __attribute__((ext_vector_type(2)));
@@ -265,17 +272,14 @@ __global__ __launch_bounds__(kVecThreads) void rotary_vec_kernel(RotaryParams p,
   const int j = j0 + min(t, nt - 1);
   const uint8_t* const qrow = p.q + ((long long)b * p.qs[0] + (long long)j * p.qs[1]) * ES;
   const uint8_t* const krow = p.k + ((long long)b * p.ks[0] + (long long)j * p.ks[1]) * ES;
-  u32x4_t in[kAhead][2];
-  auto load = [&](int h, u32x4_t* w) {
+  u32x4_t in0{}, in1{};
+  auto load = [&](int h) {
     const uint8_t* row = h < p.Hq ? qrow + (long long)h * p.qs[2] * ES : krow + (long long)(h - p.Hq) * p.ks[2] * ES;
-    w[0] = *reinterpret_cast<const u32x4_t*>(row + 16 * c0);
-    w[1] = *reinterpret_cast<const u32x4_t*>(row + 16 * c1);
+    in0 = *reinterpret_cast<const u32x4_t*>(row + 16 * c0);
+    in1 = *reinterpret_cast<const u32x4_t*>(row + 16 * c1);
   };
   const int h0 = slice * v.hpw + hs;
-  if (mine)
-#pragma unroll
-    for (int u = 0; u < kAhead; ++u)
-      if (h0 + u * v.hs < end) load(h0 + u * v.hs, in[u]);
+  if (mine && h0 < end) load(h0);
   if constexpr (APPEND) {
     if ((int)threadIdx.x < nt && (slice == 0 || end > p.Hq)) {
       const int jj = j0 + threadIdx.x;
@@ -313,54 +317,45 @@ __global__ __launch_bounds__(kVecThreads) void rotary_vec_kernel(RotaryParams p,
       }
     }
   }
-  auto put = [&](int h, const u32x4_t* w) {
-    uint8_t* out;
-    if (h < p.Hq) {
-      out = p.q_out + ((long long)b * p.qos[0] + (long long)j * p.qos[1] + (long long)h * p.qos[2]) * ES;
-    } else if constexpr (APPEND) {
-      if (row < 0) return;
-      out = p.kpool + ((((size_t)p.layer * p.cap + blk) * p.Hkv + (h - p.Hq)) * p.bs + off) * (size_t)(p.d * ES);
-    } else {
-      out = p.k_out + ((long long)b * p.kos[0] + (long long)j * p.kos[1] + (long long)(h - p.Hq) * p.kos[2]) * ES;
-    }
-    if (!pair) {
-      *reinterpret_cast<u32x4_t*>(out + 16 * c0) = w[0];
-      return;
-    }
-    Piece<DT> a, d;
-    a.unpack(w[0]);
-    d.unpack(w[1]);
-    const float2* const tc = turns + t * half + c * E;
-    if (p.interleaved) {
-#pragma unroll
-      for (int i = 0; i < E / 2; ++i) {
-        const float2 r = tc[i], s = tc[E / 2 + i];
-        const float a0 = a.x[2 * i], a1 = a.x[2 * i + 1], d0 = d.x[2 * i], d1 = d.x[2 * i + 1];
-        a.x[2 * i] = a0 * r.x - a1 * r.y;
-        a.x[2 * i + 1] = a1 * r.x + a0 * r.y;
-        d.x[2 * i] = d0 * s.x - d1 * s.y;
-        d.x[2 * i + 1] = d1 * s.x + d0 * s.y;
-      }
-    } else {
+  // Where the rows go: chosen by values, for a choice between the arguments' addresses becomes a
+  // load from one of them for every head.
+  const long long qstep = p.qos[2] * ES, kstep = APPEND ? (long long)p.bs * p.d * ES : p.kos[2] * ES;
+  uint8_t* const qdst = p.q_out + ((long long)b * p.qos[0] + (long long)j * p.qos[1]) * ES;
+  uint8_t* const kdst =
+      APPEND ? p.kpool + ((((size_t)p.layer * p.cap + blk) * p.Hkv) * p.bs + off) * (size_t)(p.d * ES)
+             : p.k_out + ((long long)b * p.kos[0] + (long long)j * p.kos[1]) * ES;
+  auto put = [&](int h) {
+    if (APPEND && h >= p.Hq && row < 0) return;
+    uint8_t* const out = h < p.Hq ? qdst + h * qstep : kdst + (h - p.Hq) * kstep;
+    u32x4_t y0 = in0, y1 = in1;  // past the rotary width both are the one piece
+    if (pair) {
+      Piece<DT> a, d;
+      a.unpack(y0);
+      d.unpack(y1);
+      const float2* const tc = turns + t * half + c * E;
 #pragma unroll
       for (int i = 0; i < E; ++i) {
-        const float2 r = tc[i];
-        const float a0 = a.x[i], d0 = d.x[i];
-        a.x[i] = a0 * r.x - d0 * r.y;
-        d.x[i] = d0 * r.x + a0 * r.y;
+        // neighbours: pairs within a piece, the first half of them in the first
+        if (p.interleaved) {
+          float* const z = i < E / 2 ? &a.x[2 * i] : &d.x[2 * i - E];
+          const float2 y = turned(z[0], z[1], tc[i]);
+          z[0] = y.x;
+          z[1] = y.y;
+        } else {
+          const float2 y = turned(a.x[i], d.x[i], tc[i]);
+          a.x[i] = y.x;
+          d.x[i] = y.y;
+        }
       }
+      y0 = a.pack();
+      y1 = d.pack();
     }
-    *reinterpret_cast<u32x4_t*>(out + 16 * c0) = a.pack();
-    *reinterpret_cast<u32x4_t*>(out + 16 * c1) = d.pack();
+    *reinterpret_cast<u32x4_t*>(out + 16 * c0) = y0;
+    *reinterpret_cast<u32x4_t*>(out + 16 * c1) = y1;
   };
-  for (int h = h0; h < end; h += kAhead * v.hs) {
-#pragma unroll
-    for (int u = 0; u < kAhead; ++u)
-      if (h + u * v.hs < end) put(h + u * v.hs, in[u]);
-    const int next = h + kAhead * v.hs;
-#pragma unroll
-    for (int u = 0; u < kAhead; ++u)
-      if (next + u * v.hs < end) load(next + u * v.hs, in[u]);
+  for (int h = h0; h < end; h += v.hs) {
+    put(h);
+    if (h + v.hs < end) load(h + v.hs);
   }
 }
 
