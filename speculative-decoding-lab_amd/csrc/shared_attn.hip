@@ -390,7 +390,8 @@ struct Walk {
       int b, j, hq;
       row_at(p, it, it.row0 + min(R, it.rows - 1), b, j, hq);
       lim[nt] = it.first >= 0 ? it.start : it.start + j;
-      const uint8_t* q = static_cast<const uint8_t*>(p.q) + (((size_t)b * p.C + j) * p.Hq + hq) * (D * (kF32 ? 4 : 2)) + 16 * g;
+      const uint8_t* q =
+          static_cast<const uint8_t*>(p.q) + (((size_t)b * p.C + j) * p.Hq + hq) * (D * (kF32 ? 4 : 2)) + 16 * g;
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) qf[nt][ks] = *reinterpret_cast<const uint4*>(q + 64 * ks);
     }
@@ -683,7 +684,8 @@ struct Walk {
           float a[4];
 #pragma unroll
           for (int kt = 0; kt < 4; ++kt)
-            a[kt] = max3_raw(max3_raw(sc[kt][nt][0], sc[kt][nt][1], sc[kt][nt][2]), sc[kt][nt][3], sc[kt][nt][3]) * slf[kt];
+            a[kt] = slf[kt] * max3_raw(max3_raw(sc[kt][nt][0], sc[kt][nt][1], sc[kt][nt][2]), sc[kt][nt][3],
+                                       sc[kt][nt][3]);
           mx[nt] = max3_raw(max3_raw(a[0], a[1], a[2]), a[3], a[3]);
         } else {
           float a0 = max3_raw(sc[0][nt][0], sc[0][nt][1], sc[0][nt][2]);
@@ -1180,7 +1182,8 @@ struct Walk {
       for (int i = tid; i < it.rows * kQ; i += kMfmaThreads) {
         const int r = i / kQ, q = i - r * kQ, first = (r >> 5) << nk_log2;
         f32x4_t x = *reinterpret_cast<const f32x4_t*>(&sO[(first * 32 + (r & 31)) * LD::kJP + 4 * q]);
-        for (int k = 1; k < nk; ++k) x += *reinterpret_cast<const f32x4_t*>(&sO[((first + k) * 32 + (r & 31)) * LD::kJP + 4 * q]);
+        for (int k = 1; k < nk; ++k)
+          x += *reinterpret_cast<const f32x4_t*>(&sO[((first + k) * 32 + (r & 31)) * LD::kJP + 4 * q]);
         *reinterpret_cast<f32x4_t*>(&p.part_o[(size_t)(it.part + r) * D + half * (D / 2) + 4 * q]) = x;
       }
     }
@@ -1342,7 +1345,8 @@ long long best_range(const std::vector<long long>& tiles, const std::vector<long
     for (size_t g = 0; g < units.size(); ++g) n += tiles[g] * ((units[g] + range - 1) / range);
     const long long rounds = (n + kCUs - 1) / kCUs;
     const long long late = n + own > rounds * kCUs ? kFixed : 0;
-    const long long time = rounds * (range * unit * rows / kTile + kFixed) + late + n * kPartial * d / 128 * rows / kTile;
+    const long long time =
+        rounds * (range * unit * rows / kTile + kFixed) + late + n * kPartial * d / 128 * rows / kTile;
     if (least < 0 || time < least) {
       least = time;
       best = range;
@@ -1500,7 +1504,8 @@ int launch(const SharedParams& p, int kv_dtype, hipStream_t s) {
   // The matrix kernels apply the scale inside the exponent, to maxima of raw scores.
   // They count pages in 31 bits and load 16 bytes at a time.
   const auto aligned = [](const void* x) { return (uintptr_t)x % 16 == 0; };
-  const bool mfma = aligned(p.q) && aligned(p.kpool) && aligned(p.vpool) && (long long)(p.layer + 1) * p.cap * p.Hkv < (1LL << 31) && p.bs == 16 &&
+  const bool mfma = aligned(p.q) && aligned(p.kpool) && aligned(p.vpool) &&
+                    (long long)(p.layer + 1) * p.cap * p.Hkv < (1LL << 31) && p.bs == 16 &&
                     (p.d == 64 || p.d == 128) && p.scale_log2 > 0.f && p.scale_log2 < INFINITY &&
                     ((QT == SPV_BF16 && kv_dtype == SPV_FP8E4M3) || QT == kv_dtype);
   if (mfma) {

@@ -254,7 +254,8 @@ class SharedPrefix:
     prefix and length read it together. Host lists: they change when requests
     are admitted or leave, while every layer and round between uses the same
     object. A prefix is a sequence like any other; the caller keeps it until
-    the last of its entries has left.
+    the last of its entries has left, and this object as long as a captured
+    graph that used it may replay.
     """
 
     def __init__(self, kv: PagedKVCache, prefix_ids: Sequence[int], prefix_lens: Sequence[int], chunk: int,

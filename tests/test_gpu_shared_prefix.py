@@ -346,6 +346,34 @@ def test_one_sequence_in_several_entries(cuda, dtype):
     _check(out, _want(q, ctx, sids, starts, ids, lens), q.dtype)
 
 
+@pytest.mark.parametrize("dtype,q_dtype", [(BF16, BF16), (F32, F32), (BF16, F16)])
+def test_blocks_past_32_bit_offsets(cuda, dtype, q_dtype):
+    """The last blocks of pools of more than 2^31 elements, written and attended: bit for bit what
+    a small pool gives (its blocks 0, 1, ... in the same order)."""
+    g = torch.Generator().manual_seed(53)
+    B, C, hq, hkv, d, P, cap = 3, 4, 8, 2, 128, 200, 540_000
+    rot = Rotary(d, cuda)
+    data = [[torch.randn(b, n, h, d, generator=g).to(dtype).to(cuda) for h in (hkv, hkv)]
+            for b, n in ((1, P), (B, C))]
+    q = torch.randn(B, C, hq, d, generator=g).to(q_dtype).to(cuda)
+    outs = []
+    for blocks in (40, cap):
+        kv = PagedKVCache(1, hkv, d, blocks, 16, cuda, dtype, max_seqs=B + 1)
+        kv.allocator.load_free_list(torch.arange(blocks, dtype=torch.int32))  # the last ones first
+        kv.add_sequence(B)
+        rotary_append(None, *data[0], kv, 0, [B], [0], rot)
+        rotary_append(None, *data[1], kv, 0, list(range(B)), [0] * B, rot)
+        prefix = SharedPrefix(kv, [B] * B, [P] * B, C, hq)
+        outs.append(shared_prefix_attention(q, kv, 0, list(range(B)), [0] * B, C, prefix))
+        used = [b for s in range(B + 1) for b in kv.block_tables[s]]
+        assert min(used) >= blocks - 20
+        outs.append(gather_ctx(kv, 0, B, P))
+        del kv, prefix
+    assert cap * hkv * 16 * d > 2 ** 31
+    assert torch.equal(outs[0], outs[2]) and torch.equal(outs[1], outs[3])
+    assert bool(torch.isfinite(outs[0]).all())
+
+
 def test_captured_graphs_and_streams(cuda):
     """Two graphs of one plan, captured at the same time and replayed on two streams with
     new start positions, equal eager calls."""
