@@ -1448,11 +1448,15 @@ int make_plan(std::vector<int32_t>& plan, const int32_t* ids, const int32_t* len
 // prefixes' segments leave CUs free, half of that (24 x 2 rows of own and prefix, bf16: 13.0
 // us, 15.4 with 256 keys); and up to twice as long where the CUs beside them then do (192 x 2
 // rows 21.2 us, 24.8 where some wait; 12 entries of 30 x 2 rows in fp32 19.1 and 26.9).
+// Long contexts of fewer entries and heads than CUs are cut into up to 1024, of 4 PH_OWN keys at
+// least, so that the longest do not end alone: 64 entries x 2 kv heads of 16 to 4000 keys behind
+// 2000 take 73.5 us, 95.5 with 256 (200 entries of up to 3000 behind 500 149.7 and 137.3).
 void own_ranges(const int32_t* plan, int max_ctx, int* range, int* count) {
   const int bs = plan[PH_BS];
   const long long G = (long long)plan[PH_C] * (plan[PH_HQ] / plan[PH_HKV]), least = plan[PH_OWN];
   const long long wgs = (long long)plan[PH_B] * plan[PH_HKV] * ((G + kOwnRows - 1) / kOwnRows);
-  const long long all = std::min(kCUs / wgs, max_ctx / least);
+  long long all = std::min(kCUs / wgs, max_ctx / least);
+  if (wgs < kCUs) all = std::max(all, std::min(4 * kCUs / wgs, max_ctx / (4 * least)));
   const long long beside = std::min((kCUs - std::min(kCUs, plan[PH_NSEG])) / wgs, max_ctx / (least / 2));
   const long long want = std::max(1LL, 2 * beside >= all ? beside : all);
   const long long keys = (max_ctx + want - 1) / want;
