@@ -76,11 +76,15 @@ class Rotary:
         self.factor = float(factor)
         self.inv_freq = torch.tensor(inv_freq, dtype=torch.float64, device=self.device)
         self.axis_of = torch.tensor(axis_of, dtype=torch.int32, device=self.device)
-        self._args = (ptr(self.inv_freq) if n else None, ptr(self.axis_of) if n else None, self.axes, self.factor)
         # argument shapes, strides and types that passed the checks, with the launch's
         # share of them: a serving loop repeats a few, and the checks cost as much
         # host time as the launch
         self._passed: dict = {}
+
+    def _args(self) -> tuple:
+        """The launch arguments of the frequencies, asked anew in every call: a copy of this
+        object has tensors of its own, and a caller may replace them."""
+        return self.inv_freq.data_ptr(), self.axis_of.data_ptr(), self.axes, self.factor
 
     def _positions(self, positions: torch.Tensor, B: int, C: int) -> torch.Tensor:
         """int32 ``(axes, B, C)``; ``(B, C)`` stands for every axis."""
@@ -193,7 +197,7 @@ def rotary_embed(query: torch.Tensor, key: Optional[torch.Tensor], rotary: Rotar
     if strides is None:
         strides = _strides(query_out, query, key_out, key)
     call("spv_rotary", query_out.data_ptr(), query.data_ptr(), ptr(key_out), ptr(key), code, key_code, strides,
-         pos.data_ptr(), *rotary._args, B, C, hq, hkv, d, rotary.rotary_dim, rotary.interleaved,
+         pos.data_ptr(), *rotary._args(), B, C, hq, hkv, d, rotary.rotary_dim, rotary.interleaved,
          _hip.stream_of(rotary.device))
     return query_out, key_out
 
@@ -297,7 +301,7 @@ def rotary_append(query: Optional[torch.Tensor], k_new: torch.Tensor, v_new: tor
             rows, follow = plan.rows, 1
     call("spv_kv_rotary_append", ptr(query_out), ptr(q), k.data_ptr(), v.data_ptr(), kv._dt,
          _strides(query_out, q, k, v) if strides is None else strides, *kv._addresses(), sid_t.data_ptr(),
-         start_t.data_ptr(), ptr(pos), *rotary._args, B, C, hq, kv.num_kv_heads, kv.head_dim, rotary.rotary_dim,
+         start_t.data_ptr(), ptr(pos), *rotary._args(), B, C, hq, kv.num_kv_heads, kv.head_dim, rotary.rotary_dim,
          rotary.interleaved, layer, a.capacity, kv.block_size, bool(alloc), follow, ptr(rows),
          _hip.stream_of(kv.device))
     if not follow:
@@ -365,7 +369,7 @@ def _append_fp8(q, k, v, kv, layer, sid_t, start_t, rotary, pos, alloc, query_ou
     """The rotated keys in float32, then the quantising append of both."""
     k32 = torch.empty(k.shape, dtype=torch.float32, device=k.device)
     call("spv_rotary", ptr(query_out), ptr(q), ptr(k32), ptr(k), _hip.dtype_code(k.dtype), _hip.SPV_F32,
-         _strides(query_out, q, k32, k), ptr(pos), *rotary._args, k.shape[0], k.shape[1],
+         _strides(query_out, q, k32, k), ptr(pos), *rotary._args(), k.shape[0], k.shape[1],
          0 if q is None else int(q.shape[2]), kv.num_kv_heads, kv.head_dim, rotary.rotary_dim,
          rotary.interleaved, _hip.stream_of(kv.device))
     kv.write_block_device(layer, sid_t, start_t, k32, v.float(), alloc=alloc)
