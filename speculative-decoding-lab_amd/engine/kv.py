@@ -180,7 +180,6 @@ class PagedKVCache:
         self.tables_dev = torch.full((self._max_seqs, self._maxb), -1, dtype=torch.int32, device=device)
         self.nblocks_dev = torch.zeros(self._max_seqs, dtype=torch.int32, device=device)
         self.lens_dev = torch.zeros(self._max_seqs, dtype=torch.int32, device=device)
-        self._known: Optional[tuple] = None
         self._nb: List[int] = []     # host mirror of table lengths
         self._lens: List[int] = []   # host mirror of sequence lengths
         self._stale = False
@@ -247,16 +246,12 @@ class PagedKVCache:
         self._maxb = new
 
     def _addresses(self) -> tuple:
-        """What a write takes of the cache: the addresses of its pools, tables and free list,
-        asked once for the tables in place (every answer costs host time, and a layer's call is short)."""
-        known = self._known
-        if known is None or known[0] is not self.tables_dev:
-            a = self.allocator
-            known = self._known = (self.tables_dev, (
-                self.k_pool.data_ptr(), self.v_pool.data_ptr(), self.tables_dev.data_ptr(), self._maxb,
+        """What a write takes of the cache: the addresses of its pools, tables and free list, asked
+        anew in every call (a memo of them cannot tell a copied or replaced tensor from its origin)."""
+        a = self.allocator
+        return (self.k_pool.data_ptr(), self.v_pool.data_ptr(), self.tables_dev.data_ptr(), self._maxb,
                 self.nblocks_dev.data_ptr(), self.lens_dev.data_ptr(), a.free_stack.data_ptr(),
-                a.free_flag.data_ptr(), a.ctr.data_ptr()))
-        return known[1]
+                a.free_flag.data_ptr(), a.ctr.data_ptr())
 
     def _check_sid(self, seq_id: int) -> int:
         seq_id = int(seq_id)

@@ -12,7 +12,8 @@ import torch
 from engine import _hip
 from engine import kv as kv_module
 from engine import rotary as rotary_module
-from engine.rotary import Rotary, rotary_embed
+from engine.kv import PagedKVCache
+from engine.rotary import Rotary, rotary_append, rotary_embed
 
 
 @pytest.fixture
@@ -50,3 +51,36 @@ def test_replaced_frequencies_are_used(launches):
     rot.factor = 0.5
     _embed(launches, rot)
     assert launches[-1][1][11] == 0.5
+
+
+def _append(launches, kv, rot):
+    x = torch.zeros(1, 2, kv.num_kv_heads, kv.head_dim)
+    ids = torch.zeros(1, dtype=torch.int32)
+    rotary_append(x, x, x, kv, 0, ids, ids, rot)
+    name, args = launches[-1]
+    assert name == "spv_kv_rotary_append"
+    return args[6:15]
+
+
+def _of(kv):
+    a = kv.allocator
+    return (kv.k_pool.data_ptr(), kv.v_pool.data_ptr(), kv.tables_dev.data_ptr(), kv._maxb, kv.nblocks_dev.data_ptr(),
+            kv.lens_dev.data_ptr(), a.free_stack.data_ptr(), a.free_flag.data_ptr(), a.ctr.data_ptr())
+
+
+def test_a_copied_cache_is_appended_to_in_its_own_memory(launches):
+    kv, rot = PagedKVCache(1, 1, 8, 4, 16, "cpu", torch.float32), Rotary(8, "cpu")
+    assert _append(launches, kv, rot) == _of(kv)
+    other = copy.deepcopy(kv)
+    assert not set(_of(other)) & set(_of(kv)) - {kv._maxb}
+    assert _append(launches, other, rot) == _of(other)
+
+
+@pytest.mark.parametrize("name", ["k_pool", "v_pool", "tables_dev", "nblocks_dev", "lens_dev"])
+def test_a_replaced_tensor_of_the_cache_is_used(launches, name):
+    kv, rot = PagedKVCache(1, 1, 8, 4, 16, "cpu", torch.float32), Rotary(8, "cpu")
+    _append(launches, kv, rot)
+    setattr(kv, name, getattr(kv, name).clone())
+    assert _append(launches, kv, rot) == _of(kv)
+    kv.allocator.free_stack = kv.allocator.free_stack.clone()
+    assert _append(launches, kv, rot) == _of(kv)
