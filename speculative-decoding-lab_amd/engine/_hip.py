@@ -151,6 +151,16 @@ def stream_of(device: torch.device) -> int:
     return torch._C._cuda_getCurrentRawStream(idx)
 
 
+def kept_for(stream: int, made_on: int, *tensors: torch.Tensor) -> int:
+    """``stream``, the current one, after keeping the memory of a handle's ``tensors`` from reuse
+    until its work so far is done, where they were made on another one. What a captured graph
+    uses its owner keeps."""
+    if stream != made_on and not torch.cuda.is_current_stream_capturing():
+        for t in tensors:
+            t.record_stream(torch.cuda.current_stream(t.device))
+    return stream
+
+
 def dtype_code(dtype: torch.dtype) -> int:
     if dtype not in _DTYPE_CODE:
         raise HipLibraryError("unsupported dtype {}".format(dtype))

@@ -255,7 +255,8 @@ class SharedPrefix:
     are admitted or leave, while every layer and round between uses the same
     object. A prefix is a sequence like any other; the caller keeps it until
     the last of its entries has left, and this object as long as a captured
-    graph that used it may replay.
+    graph that used it may replay (calls outside a graph, on any stream, keep
+    what they need of it themselves).
     """
 
     def __init__(self, kv: PagedKVCache, prefix_ids: Sequence[int], prefix_lens: Sequence[int], chunk: int,
@@ -288,6 +289,7 @@ class SharedPrefix:
         self._host = (ctypes.c_int32 * n)()
         _hip.lib().spv_shared_attn_plan(*args, self._host, n)
         self._dev = torch.frombuffer(self._host, dtype=torch.int32).to(kv.device)
+        self._made_on = _hip.stream_of(kv.device)
         self._bytes = (0, 0)  # the last max_ctx and its calls' workspace
 
 
@@ -346,7 +348,8 @@ def shared_prefix_attention(query_3d: torch.Tensor, kv: PagedKVCache, layer: int
          kv.v_pool.data_ptr(), kv._dt, ptr(kv.scales), kv.tables_dev.data_ptr(), kv._maxb, sid_t.data_ptr(),
          start_t.data_ptr(), kv.lens_dev.data_ptr(), kv.allocator.ctr.data_ptr(), B, chunk, hq, kv.num_kv_heads, d,
          kv.block_size, layer, kv.allocator.capacity, max_ctx, prefix.scale if scale is None else float(scale),
-         prefix._host, prefix._dev.data_ptr(), ws.data_ptr(), ws_bytes, _hip.stream_of(kv.device))
+         prefix._host, prefix._dev.data_ptr(), ws.data_ptr(), ws_bytes,
+         _hip.kept_for(_hip.stream_of(kv.device), prefix._made_on, prefix._dev))
     kv._stale = True
     return out
 

@@ -42,7 +42,8 @@ class Rotary:
     ``interleaved``; ``rotary_dim`` (default: the whole row) leaves the rest of
     the row as it is. ``factor`` scales the rotated elements. With several
     position axes, ``sections`` gives the number of consecutive frequencies of
-    each, or ``axis_of`` the axis of every frequency.
+    each, or ``axis_of`` the axis of every frequency. The caller keeps this object as
+    long as a captured graph that used it may replay.
     """
 
     def __init__(self, head_dim: int, device: torch.device, base: float = 10000.0,
@@ -80,6 +81,11 @@ class Rotary:
         # share of them: a serving loop repeats a few, and the checks cost as much
         # host time as the launch
         self._passed: dict = {}
+        self._made_on = _hip.stream_of(self.device)
+
+    def _stream(self) -> int:
+        """The current stream, for a launch that reads the frequencies."""
+        return _hip.kept_for(_hip.stream_of(self.device), self._made_on, self.inv_freq, self.axis_of)
 
     def _args(self) -> tuple:
         """The launch arguments of the frequencies, asked anew in every call: a copy of this
@@ -198,7 +204,7 @@ def rotary_embed(query: torch.Tensor, key: Optional[torch.Tensor], rotary: Rotar
         strides = _strides(query_out, query, key_out, key)
     call("spv_rotary", query_out.data_ptr(), query.data_ptr(), ptr(key_out), ptr(key), code, key_code, strides,
          pos.data_ptr(), *rotary._args(), B, C, hq, hkv, d, rotary.rotary_dim, rotary.interleaved,
-         _hip.stream_of(rotary.device))
+         rotary._stream())
     return query_out, key_out
 
 
@@ -303,7 +309,7 @@ def rotary_append(query: Optional[torch.Tensor], k_new: torch.Tensor, v_new: tor
          _strides(query_out, q, k, v) if strides is None else strides, *kv._addresses(), sid_t.data_ptr(),
          start_t.data_ptr(), ptr(pos), *rotary._args(), B, C, hq, kv.num_kv_heads, kv.head_dim, rotary.rotary_dim,
          rotary.interleaved, layer, a.capacity, kv.block_size, bool(alloc), follow, ptr(rows),
-         _hip.stream_of(kv.device))
+         rotary._stream())
     if not follow:
         if rows is not None:
             plan._record(a.epoch, sid_t, start_t)
@@ -371,5 +377,5 @@ def _append_fp8(q, k, v, kv, layer, sid_t, start_t, rotary, pos, alloc, query_ou
     call("spv_rotary", ptr(query_out), ptr(q), ptr(k32), ptr(k), _hip.dtype_code(k.dtype), _hip.SPV_F32,
          _strides(query_out, q, k32, k), ptr(pos), *rotary._args(), k.shape[0], k.shape[1],
          0 if q is None else int(q.shape[2]), kv.num_kv_heads, kv.head_dim, rotary.rotary_dim,
-         rotary.interleaved, _hip.stream_of(kv.device))
+         rotary.interleaved, rotary._stream())
     kv.write_block_device(layer, sid_t, start_t, k32, v.float(), alloc=alloc)
