@@ -256,7 +256,8 @@ def rotary_append(query: Optional[torch.Tensor], k_new: torch.Tensor, v_new: tor
     write plans, and ``query`` (B, C, Hq, d, or None) rotated in the same launch.
     ``k_new`` / ``v_new`` (B, C, Hkv, d) and ``query`` share the pool's dtype
     (an fp8 pool: one of float32, bfloat16, float16; the rotated keys are
-    quantised unrounded). ``positions``: as in ``rotary_embed``; None takes the
+    quantised unrounded). fp8 pools, and pools of 2^31 token rows or more, are
+    written in a launch behind the rotation's and ignore ``plan``. ``positions``: as in ``rotary_embed``; None takes the
     pool positions ``start_positions[b] + j``. No host synchronisation with
     device tensors of distinct, added ``seq_ids``. A later layer's call of a
     round passes ``alloc=False`` and the first one's ``plan``.
@@ -291,14 +292,14 @@ def rotary_append(query: Optional[torch.Tensor], k_new: torch.Tensor, v_new: tor
         query_out = _like(q, q.dtype)
     if B == 0 or C == 0:
         return query_out
-    if kv.fp8:
+    a = kv.allocator
+    if kv.fp8 or a.capacity * kv.block_size >= 2 ** 31:
         if pos is None:
             pos = start_t[:, None] + torch.arange(C, dtype=torch.int32, device=kv.device)
-        _append_fp8(q, k, v, kv, layer, sid_t, start_t, rotary, pos, alloc, query_out)
+        _append_apart(q, k, v, kv, layer, sid_t, start_t, rotary, pos, alloc, query_out)
         return query_out
-    a = kv.allocator
     rows, follow = None, 0
-    if plan is not None and a.capacity * kv.block_size < 2 ** 31:
+    if plan is not None:
         if alloc:
             plan._reserve(B, C, kv.device)
             rows = plan.rows
@@ -371,11 +372,14 @@ def _append_ids(kv, seq_ids, start_positions, B, C):
     return sid_t, start_t
 
 
-def _append_fp8(q, k, v, kv, layer, sid_t, start_t, rotary, pos, alloc, query_out) -> None:
-    """The rotated keys in float32, then the quantising append of both."""
-    k32 = torch.empty(k.shape, dtype=torch.float32, device=k.device)
-    call("spv_rotary", ptr(query_out), ptr(q), ptr(k32), ptr(k), _hip.dtype_code(k.dtype), _hip.SPV_F32,
-         _strides(query_out, q, k32, k), ptr(pos), *rotary._args(), k.shape[0], k.shape[1],
+def _append_apart(q, k, v, kv, layer, sid_t, start_t, rotary, pos, alloc, query_out) -> None:
+    """The rotated keys by themselves, then the append of both: an fp8 pool's, which quantises
+    (from float32, so that a key is rounded once), and that of a pool of 2^31 token rows or
+    more (the one launch counts rows in 32 bits)."""
+    dtype = torch.float32 if kv.fp8 else k.dtype
+    turned = torch.empty(k.shape, dtype=dtype, device=k.device)
+    call("spv_rotary", ptr(query_out), ptr(q), ptr(turned), ptr(k), _hip.dtype_code(k.dtype), _hip.dtype_code(dtype),
+         _strides(query_out, q, turned, k), ptr(pos), *rotary._args(), k.shape[0], k.shape[1],
          0 if q is None else int(q.shape[2]), kv.num_kv_heads, kv.head_dim, rotary.rotary_dim,
          rotary.interleaved, rotary._stream())
-    kv.write_block_device(layer, sid_t, start_t, k32, v.float(), alloc=alloc)
+    kv.write_block_device(layer, sid_t, start_t, turned, v.to(dtype), alloc=alloc)
