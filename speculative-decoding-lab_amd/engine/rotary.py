@@ -295,7 +295,7 @@ def rotary_append(query: Optional[torch.Tensor], k_new: torch.Tensor, v_new: tor
     a = kv.allocator
     if kv.fp8 or a.capacity * kv.block_size >= 2 ** 31:
         if pos is None:
-            pos = start_t[:, None] + torch.arange(C, dtype=torch.int32, device=kv.device)
+            pos = start_t.view(B, 1) + torch.arange(C, dtype=torch.int32, device=kv.device)
         _append_apart(q, k, v, kv, layer, sid_t, start_t, rotary, pos, alloc, query_out)
         return query_out
     rows, follow = None, 0

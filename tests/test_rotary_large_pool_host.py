@@ -34,3 +34,13 @@ def test_pools_of_2_31_rows_are_written_in_two_launches(launches, alloc, with_qu
     out = rotary_append(x if with_query else None, x, x, kv, 0, ids, ids, rot, alloc=alloc, plan=WritePlan())
     assert (out is not None) == with_query
     assert launches == (["spv_kv_rotary_append"] if one else ["spv_rotary", "spv_kv_append"])
+
+
+@pytest.mark.parametrize("shape", [(), (1,), (1, 1)])
+def test_one_entry_of_any_shape_over_fp8(launches, shape):
+    """Start positions of one entry, however they are shaped, as every other call takes them."""
+    kv, rot = PagedKVCache(1, 1, 8, 4, 16, "cpu", torch.float8_e4m3fn), Rotary(8, "cpu")
+    x, ids = torch.zeros(1, 2, 1, 8), torch.zeros(shape, dtype=torch.int32)
+    del launches[:]
+    rotary_append(x, x, x, kv, 0, ids, ids, rot)
+    assert launches == ["spv_rotary", "spv_kv_append_fp8"]
