@@ -892,8 +892,27 @@ struct Walk {
     }
   }
 
-  // ---- an entry's own keys, and a segment of few rows or in fp32: 32 rows per wave (false: the chunk
-  // holds a value that is not finite; nothing is written then). nk waves share the
+  // Whether one of an item's values is not finite: each wave looks through every eighth page.
+  __device__ __forceinline__ bool values_not_finite(const Item& it) const {
+    constexpr int kPer = 16 / ES;  // elements of a 16-byte piece, of one dim
+    constexpr uint32_t kMask = kFp8 ? 0x7fu : kF16 ? 0x7c00u : kF32 ? 0x7f800000u : 0x7f80u;
+    const int32_t* table = p.tables + (size_t)it.sid * p.maxb + (it.key0 >> 4);
+    bool found = false;
+    for (int i = w; it.key0 + 16 * i < it.key1; i += kWaves) {
+      const uint8_t* v = page(p.vpool, page_of(safe_id(it, table[i]), it.h));
+      const int left = it.key1 - it.key0 - 16 * i;
+      for (int c = lane; c < D * ES; c += 64) {
+        const u32x4_t x = *reinterpret_cast<const u32x4_t*>(v + 16 * c);
+#pragma unroll
+        for (int e = 0; e < kPer; ++e)
+          found |= ((x[e * ES / 4] >> (8 * (e * ES % 4))) & kMask) == kMask && (c * kPer + e) % 16 < left;
+      }
+    }
+    return found;
+  }
+
+  // ---- an entry's own keys, and a segment of few rows or in fp32: 32 rows per wave (false: a value
+  // is not finite; nothing is written then). nk waves share the
   // rows (8 up to 32 rows, 4 up to 64, 2 up to 128, 1 up to 256) and take every nk-th
   // page straight into operand registers, one page in flight while one is computed;
   // their sums join in LDS.
@@ -929,7 +948,6 @@ struct Walk {
     }
     int ids = 0;
     float ksc = 1.f, vsc = 1.f;
-    int dirty = 0;  // a value of the chunk that some of its rows do not see is not finite
     struct Page {
       uint4 k[KS];           // fp8: 8 bytes
       uint32_t v[MT][ES == 4 ? 4 : 2];  // fp8: 4 bytes
@@ -1009,18 +1027,14 @@ struct Walk {
             const int key = k0 + 4 * g + jj;
             sc[nt][jj] = key >= key1 || key > lim[nt] ? -INFINITY : sc[nt][jj];
           }
-        // Values past the range's end are zero; a chunk value that is not finite must
-        // not meet the P = 0 of the rows before it.
+        // Values past the range's end are zero.
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt) {
 #pragma unroll
           for (int jj = 0; jj < 4; ++jj) {
             constexpr uint32_t kMask = kFp8 ? 0xffu : kF32 ? ~0u : 0xffffu;
-            constexpr uint32_t kInf = kFp8 ? 0x7fu : kF16 ? 0x7c00u : kF32 ? 0x7f800000u : 0x7f80u;
             const int word = jj * ES / 4, shift = 8 * (jj * ES % 4), key = k0 + 4 * g + jj;
-            const bool bad = ((P.v[mt][word] >> shift) & kInf) == kInf;
             P.v[mt][word] &= key >= key1 ? ~(kMask << shift) : ~0u;
-            dirty |= (int)bad & (int)(key > start) & (int)(key < key1);
           }
         }
       }
@@ -1134,9 +1148,18 @@ struct Walk {
         }
       }
     }
-    if (__syncthreads_or(dirty)) {
-      return false;
-    }
+    // A value that is not finite must meet neither the P = 0 of rows that do not see it nor a lower
+    // half of P (which may be zero or of the other sign): the sums show it as NaN or an infinity,
+    // and the any-shape walk takes the item. Keys or queries that are not finite show so, too, but
+    // are as right here.
+    float z = 0.f;
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) z = fmaf(o[mt][nt][c], 0.f, z);
+    if (__syncthreads_or(z != z) && __syncthreads_or(values_not_finite(it))) return false;
     // Join the waves of the same rows: all take the largest m; then every thread adds up
     // four dims of a row over the waves, in their order, half of the dims at a time.
     float2* const sML = reinterpret_cast<float2*>(smem + LD::kJoinRows);
