@@ -33,9 +33,9 @@
 // output alone takes 1.7e-3); fp16 has 11 bits. bf16 values are staged as fp16
 // times a power of two per segment, chosen from the first tile's largest |v|
 // (which lands in [2^8, 2^9): every value from 2^-25 of it up is exact, a smaller
-// one is off by at most 2^-33 of it); where a later value would pass fp16's range, or
-// the first tile was so small beside the rest that it says nothing, the segment is
-// walked again in fp32 (the any-shape walk, some thirty times as long). fp8 codes are
+// one is off by at most 2^-33 of it); where a later value would pass fp16's range, or the
+// first tile is all zeros, the segment is walked again page by page as own keys are, in any
+// range (7168 x 2 rows over 8192 keys 275 us where every segment is, 115 where none). fp8 codes are
 // fp16 values; a block's K scale goes into the exponent's multiplier, its V scale, over
 // the segment's largest, as a logarithm into the addend.
 //
@@ -339,9 +339,8 @@ __device__ __forceinline__ uint32_t max_abs2(uint32_t w, uint32_t m) {
   return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2_t, w & 0x7fff7fffu),
                                                                 __builtin_bit_cast(u16x2_t, m)));
 }
-// The staging power for a largest finite |v| of mx: mx 2^k in [2^8, 2^9), 0 where all are zero.
+// The staging power for a largest finite |v| of mx > 0: mx 2^k in [2^8, 2^9).
 __device__ __forceinline__ int stage_exponent(float mx) {
-  if (!(mx > 0.f)) return 0;
   int e;
   frexpf(mx, &e);
   return min(126, max(-126, 9 - e));
@@ -428,7 +427,8 @@ struct Walk {
   }
 
   // ---- a segment of a prefix: 256 rows, 32 per wave, 64 keys at a time in LDS. False
-  // (bf16 values) where a value passed fp16's range: nothing is written then.
+  // (bf16 values) where a value passed fp16's range or the first tile is all zeros: nothing
+  // is written then.
   __device__ __forceinline__ bool prefix(const Item& it) {
     using LD = Lds<D>;
     constexpr int KP = LD::KP, VP = LD::VP;
@@ -514,7 +514,6 @@ struct Walk {
     };
     float vs = 1.f;     // bf16: the staging factor 2^vk
     int vk = 0;
-    bool seen = true;   // whether the first tile has a value to choose it from
     uint32_t vmax = 0;  // bf16: largest |v| bits staged (both halves)
     // Zeroes the values of keys past the range's end.
     auto edge = [&](Stage& S, int t) SPV_INLINE {
@@ -788,7 +787,7 @@ struct Walk {
             }
           }
         mx = wg_max(mx);
-        seen = mx > 0;
+        if (mx == 0) return false;  // all zero: nothing to choose the power from
         vk = stage_exponent(__uint_as_float(mx << 16));
         vs = ldexpf(1.f, vk);
       }
@@ -842,9 +841,8 @@ struct Walk {
       }
       softmax(t);
       if constexpr (!kF16 && !kFp8) {
-        // bits of the largest |v| that stays within fp16 at this power; with an all-zero
-        // first tile (power 0) anything but zeros is too much
-        const uint32_t top = seen ? min(__float_as_uint(ldexpf(65504.f, -vk)) >> 16, 0x7f7fu) : 0u;
+        // bits of the largest |v| that stays within fp16 at this power
+        const uint32_t top = min(__float_as_uint(ldexpf(65504.f, -vk)) >> 16, 0x7f7fu);
         const bool passed = __any((vmax & 0xffffu) > top || (vmax >> 16) > top);
         if (lane == 0) sMax[w] = passed;
       }
@@ -1221,7 +1219,6 @@ __global__ __launch_bounds__(kMfmaThreads, 2) void shared_mfma_kernel(SharedPara
   const int id = blockIdx.x;
   Walk<D, KT> walk(p, smem, threadIdx.x);
   Item it;
-  bool done;
   if (id < p.seg_wgs) {
     if (!segment_item(p, id, it)) return;
   } else if (!own_item(p, id - p.seg_wgs, it)) {
@@ -1230,8 +1227,17 @@ __global__ __launch_bounds__(kMfmaThreads, 2) void shared_mfma_kernel(SharedPara
   // A segment of few rows is walked as own keys are, its pages shared out over the waves: 28
   // rows x 2 kv heads of 64 behind 32768 fp16 keys take 10.2 us, 15.3 in a tile of 256 rows
   // (63 x 2 of fp8 13.5 and 18.5; 72 x 2 of 128, bf16, 29.5 and 22.0).
-  if (KT != SPV_F32 && it.first >= 0 && it.rows > kPagesRows) done = walk.prefix(it);
-  else done = walk.pages(it);
+  // Where the tile's staging does not hold its values, they go the same way.
+  bool done = false;
+  if (KT != SPV_F32 && it.first >= 0 && it.rows > kPagesRows) {
+    done = walk.prefix(it);
+    if (!done) {  // read again, so that nothing of it stays in registers across the walk
+      int again = id;
+      asm volatile("" : "+s"(again));
+      segment_item(p, again, it);
+    }
+  }
+  if (!done) done = walk.pages(it);
   if (!done) valu_item<Walk<D, KT>::QT, KT, D, kMfmaThreads>(p, it, reinterpret_cast<float*>(smem));
 }
 

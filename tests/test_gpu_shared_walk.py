@@ -4,7 +4,9 @@ against float64.
 A row's error is held to half a step of the output type, eps / 2 of the element, and to what
 the weights' rounding adds: at most 2^-11 of sum w |v| (fp16 weights, 2^-12 each, and the sum
 that divides them), 2^-10 with the fp32 exponents and sums beside it (scores of a few tens in
-log2 units at 2^-24, products of bf16 or fp16 values exact).
+log2 units at 2^-24, products of bf16 or fp16 values exact). In fp32 a score of 8 log2 units,
+the sum of some hundred products of 2^-24 each, is off by about 2^-19 at most: 2^-17 of sum w |v|.
+Plans are cut by hand where a test needs long segments.
 """
 
 from __future__ import annotations
@@ -14,6 +16,7 @@ import torch
 
 from engine.attention import SharedPrefix, gather_ctx, shared_prefix_attention
 from engine.kv import PagedKVCache
+from shared_plans import recut
 
 pytestmark = pytest.mark.gpu
 
@@ -32,19 +35,22 @@ def cache(cuda, contexts, dtype):
     return kv
 
 
-def exact(q, kv, starts, ids, lens):
-    """The attention of entry b over its prefix and its own sequence b in float64, and sum w |v|."""
+def exact(q, kv, starts, ids, lens, own=None):
+    """The attention of entry b over its prefix and its own sequence (b, or own[b]) in float64, and
+    sum w |v|."""
     B, C, hq, d = q.shape
     q, out = q.double(), []
     contexts = {}
+
+    def context(sid, n):
+        if (sid, n) not in contexts:
+            contexts[sid, n] = gather_ctx(kv, 0, sid, n).double()
+        return contexts[sid, n]
+
     for b in range(B):
-        n = starts[b] + C
-        parts = [gather_ctx(kv, 0, b, n).double()]
+        parts = [context(b if own is None else own[b], starts[b] + C)]
         if ids[b] >= 0 and lens[b]:
-            at = (ids[b], lens[b])
-            if at not in contexts:
-                contexts[at] = gather_ctx(kv, 0, *at).double()
-            parts.insert(0, contexts[at])
+            parts.insert(0, context(ids[b], lens[b]))
         k, v = torch.cat(parts, 1).permute(0, 2, 1, 3).contiguous()  # (kv heads, positions, d)
         hkv, total = k.shape[:2]
         each = []
@@ -56,20 +62,20 @@ def exact(q, kv, starts, ids, lens):
     return [torch.stack(x) for x in zip(*out)]
 
 
-def near(out, want, size, dtype):
+def near(out, want, size, dtype, fp32):
     err = (out - want).abs()
-    bound = torch.finfo(dtype).eps / 2 * want.abs() + (2.0 ** -10 if dtype != F32 else 2.0 ** -17) * size
+    bound = torch.finfo(dtype).eps / 2 * want.abs() + (2.0 ** -10 if dtype != F32 else fp32) * size
     worst = float((err / bound.clamp(min=1e-300)).max())
     assert worst <= 1, worst
 
 
-def close(out, want, size):
+def close(out, want, size, fp32=2.0 ** -17):
     """Every finite element, by the bound above; infinities and NaN where they belong."""
     dtype, out = out.dtype, out.double()
     fine = torch.isfinite(want)
     assert torch.equal(torch.isnan(out), torch.isnan(want))
     assert torch.equal(out[~fine].nan_to_num(), want[~fine].nan_to_num())
-    near(out[fine], want[fine], size[fine], dtype)
+    near(out[fine], want[fine], size[fine], dtype, fp32)
 
 
 @pytest.mark.parametrize("dtype", [BF16, F16, F32])
@@ -93,3 +99,109 @@ def test_infinite_values_that_are_seen(cuda, dtype, d, B, where):
     want, size = exact(q, kv, [30] * B, ids, lens)
     assert bool(torch.isposinf(want).any()) and bool(torch.isneginf(want).any()) and bool(torch.isnan(want).any())
     close(out, want, size)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32, FP8])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("first", [1.0, 0.0, 2.0 ** -14])
+@pytest.mark.parametrize("later", [1.0, 2.0 ** 5, 2.0 ** 10, 2.0 ** 40])
+def test_values_of_other_sizes_behind_the_first_tile(cuda, dtype, d, first, later):
+    """The first 64 keys' values scaled by ``first``, a page's behind them by ``later``, in one segment
+    of eight units: whether or not a tile's staging holds both."""
+    if dtype == F16 and later > 2.0 ** 10:
+        pytest.skip("past the type")
+    g = torch.Generator().manual_seed(79)
+    B, C, hq, hkv, P = 8, 5, 8, 2, 500
+    parts = [[torch.randn(1, n, hkv, d, generator=g) for _ in range(2)] for n in [9 + C] * B + [P]]
+    parts[B][1][:, :64] *= first
+    parts[B][1][:, 208:224] *= later
+    kv = cache(cuda, parts, dtype)
+    q = torch.randn(B, C, hq, d, generator=g).to(BF16 if dtype == FP8 else dtype).to(cuda)
+    ids, lens = [B] * B, [P] * B
+    prefix = SharedPrefix(kv, ids, lens, C, hq)
+    segs = recut(prefix, ids, lens, lambda units: units)
+    assert len(segs) == hkv and all(s[5] == B * C * hq // hkv > 64 and s[7] - s[6] == P for s in segs)
+    out = shared_prefix_attention(q, kv, 0, list(range(B)), [9] * B, 9 + C, prefix)
+    close(out, *exact(q, kv, [9] * B, ids, lens))
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32, FP8])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("slope", [-60.0, 60.0])
+def test_scores_that_rise_or_fall_along_a_segment(cuda, dtype, d, slope):
+    """The reference maximum grows in every tile of a segment, or in none behind the first. (fp32
+    scores of up to 90 log2 units are off by 2^-15.)"""
+    g = torch.Generator().manual_seed(83)
+    B, C, hq, hkv, P = 8, 5, 8, 2, 700
+    u = torch.randn(d, generator=g)
+    u = u / u.norm() * d ** 0.25
+    parts = [[torch.randn(1, n, hkv, d, generator=g) for _ in range(2)] for n in [9 + C] * B + [P]]
+    parts[B][0].add_((slope * torch.arange(P) / P)[None, :, None, None] * u)
+    kv = cache(cuda, parts, dtype)
+    q = (0.5 * torch.randn(B, C, hq, d, generator=g) + u).to(BF16 if dtype == FP8 else dtype).to(cuda)
+    ids, lens = [B] * B, [P] * B
+    prefix = SharedPrefix(kv, ids, lens, C, hq)
+    recut(prefix, ids, lens, lambda units: units)
+    out = shared_prefix_attention(q, kv, 0, list(range(B)), [9] * B, 9 + C, prefix)
+    close(out, *exact(q, kv, [9] * B, ids, lens), fp32=2.0 ** -14)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, FP8])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("P", [65, 129, 1024, 1088, 1090, 2049, 2100, 2500, 4200])
+def test_long_segments(cuda, dtype, d, P):
+    """Segments of 2 to 66 units of 64 keys, their last one whole or not, by tiles of more than 64
+    rows: page numbers and scales change hands every 16 units, values go round three slots."""
+    g = torch.Generator().manual_seed(P)
+    B, C, hq, hkv = 9, 4, 8, 1
+    parts = [[torch.randn(1, n, hkv, d, generator=g) for _ in range(2)] for n in [3 + C] * B + [P]]
+    if dtype == FP8:  # each page with scales of its own
+        for x in parts[B]:
+            x.mul_((2.0 ** torch.randint(-3, 1, (-(-P // 16),), generator=g)).repeat_interleave(16)[:P].view(1, P, 1, 1))
+    kv = cache(cuda, parts, dtype)
+    q = torch.randn(B, C, hq, d, generator=g).to(BF16 if dtype == FP8 else dtype).to(cuda)
+    ids, lens = [B] * B, [P] * B
+    want = exact(q, kv, [3] * B, ids, lens)
+    for units in (lambda n: n, lambda n: (n + 1) // 2):
+        prefix = SharedPrefix(kv, ids, lens, C, hq)
+        segs = recut(prefix, ids, lens, units)
+        assert max(s[7] - s[6] for s in segs) == min(P, units(-(-P // 64)) * 64) and max(s[5] for s in segs) == 256
+        out = shared_prefix_attention(q, kv, 0, list(range(B)), [3] * B, 3 + C, prefix)
+        close(out, *want)
+
+
+@pytest.mark.parametrize("tile", [64, 128, 256])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("P", [70, 1500, 2100])
+@pytest.mark.parametrize("dtype", [F32, BF16, F16, FP8])
+def test_tiles_of_every_size(cuda, dtype, tile, d, P):
+    """fp32 walks page by page in tiles of up to 256 rows (few waves then share them); the 16-bit
+    types may be given any of them by a plan, too."""
+    g = torch.Generator().manual_seed(P + tile)
+    B, C, hq, hkv = 10, 5, 12, 2  # 300 rows
+    parts = [[torch.randn(1, n, hkv, d, generator=g) for _ in range(2)] for n in [3 + C] * B + [P]]
+    kv = cache(cuda, parts, dtype)
+    q = torch.randn(B, C, hq, d, generator=g).to(BF16 if dtype == FP8 else dtype).to(cuda)
+    ids, lens = [B] * B, [P] * B
+    prefix = SharedPrefix(kv, ids, lens, C, hq)
+    segs = recut(prefix, ids, lens, lambda n: n, tile)
+    assert max(s[5] for s in segs) == tile
+    out = shared_prefix_attention(q, kv, 0, list(range(B)), [3] * B, 3 + C, prefix)
+    close(out, *exact(q, kv, [3] * B, ids, lens))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16, FP8])
+@pytest.mark.parametrize("C,n", [(2, 9000), (10, 4500)])
+def test_long_own_contexts_in_one_range(cuda, dtype, C, n):
+    """Own contexts of more pages than a wave's lanes hold the numbers of (64 pages for each of
+    8 waves up to 32 rows, of 4 up to 64): more entries than CUs leave one range each."""
+    g = torch.Generator().manual_seed(n)
+    B, hq, hkv, d, P = 150, 8, 2, 64, 40
+    parts = [[torch.randn(1, m, hkv, d, generator=g) for _ in range(2)] for m in (n, P)]
+    kv = cache(cuda, parts, dtype)
+    q = torch.randn(B, C, hq, d, generator=g).to(BF16 if dtype == FP8 else dtype).to(cuda)
+    starts = [n - C - 7 * b for b in range(B)]
+    out = shared_prefix_attention(q, kv, 0, [0] * B, starts, n, SharedPrefix(kv, [1] * B, [P] * B, C, hq))
+    some = [0, 1, 40, B - 1]
+    pick = lambda x: [x[i] for i in some]  # noqa: E731
+    close(out[some], *exact(q[some], kv, pick(starts), [1] * 4, [P] * 4, own=[0] * 4))
