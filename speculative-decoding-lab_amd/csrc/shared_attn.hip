@@ -37,7 +37,9 @@
 // first tile is all zeros, the segment is walked again page by page as own keys are, in any
 // range (7168 x 2 rows over 8192 keys 275 us where every segment is, 115 where none). fp8 codes are
 // fp16 values; a block's K scale goes into the exponent's multiplier, its V scale, over
-// the segment's largest, as a logarithm into the addend.
+// the segment's largest, as a logarithm into the addend, so that P carries it; segments whose V scales
+// (zeros aside) lie more than 2^12 apart are walked page by page, too (P in two halves of bf16, with
+// fp32's exponents).
 //
 // What bounds it: with long prefixes and many rows the walk, 0.90 to 0.97 PFLOP/s of its
 // steady state (head_dim 128, bf16; the matrix instructions and the softmax beside each
@@ -322,8 +324,16 @@ typedef float f32x4_t __attribute__((ext_vector_type(4)));
 typedef float f32x2_t __attribute__((ext_vector_type(2)));
 
 // A row's scores may exceed its reference maximum by this much (log2 units) before
-// its sums are rescaled: P stays below 2^8, far inside fp16.
+// its sums are rescaled: P stays below 2^8.
 constexpr float kSlack = 8.f;
+// The tiled walk's reference lies this much below the maximum that it was taken from: P in fp16
+// is at most 2^15 then, has fp16's whole 11 bits from 2^-21 of the maximum's up, and is off by at
+// most 2^-32 of that below.
+constexpr float kShift = 7.f;
+// The tiled walk over fp8 pages takes V scales down to this fraction of a segment's largest. It puts
+// the ratio into P: at 2^-12 a row whose weight is on such a page still has P of 2^-5, and what P
+// loses on other pages' small weights, 2^-32 times their values, is 2^-20 of its own.
+constexpr float kScaleRange = 0x1p-12f;
 
 __device__ __forceinline__ uint32_t pack2_f16(float a, float b) {
   return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2_t{a, b}, f16x2_t));
@@ -414,21 +424,26 @@ struct Walk {
   __device__ __forceinline__ const uint8_t* page(const void* pool, int index) const {
     return static_cast<const uint8_t*>(pool) + (size_t)(uint32_t)index * (16 * D * ES);
   }
-  __device__ __forceinline__ uint32_t wg_max(uint32_t m) {  // the workgroup's largest m, in every thread
+  // The workgroup's largest of either half of m (16 bits each), in every thread.
+  __device__ __forceinline__ uint32_t wg_max2(uint32_t m) {
+    const auto larger = [](uint32_t a, uint32_t b) {
+      return __builtin_bit_cast(uint32_t,
+                                __builtin_elementwise_max(__builtin_bit_cast(u16x2_t, a), __builtin_bit_cast(u16x2_t, b)));
+    };
 #pragma unroll
-    for (int o = 32; o > 0; o >>= 1) m = max(m, (uint32_t)__shfl_xor((int)m, o, 64));
+    for (int o = 32; o > 0; o >>= 1) m = larger(m, (uint32_t)__shfl_xor((int)m, o, 64));
     __syncthreads();
     if (lane == 0) sMax[w] = m;
     __syncthreads();
     m = sMax[0];
 #pragma unroll
-    for (int k = 1; k < kWaves; ++k) m = max(m, sMax[k]);
+    for (int k = 1; k < kWaves; ++k) m = larger(m, sMax[k]);
     return m;
   }
 
   // ---- a segment of a prefix: 256 rows, 32 per wave, 64 keys at a time in LDS. False
-  // (bf16 values) where a value passed fp16's range or the first tile is all zeros: nothing
-  // is written then.
+  // where a bf16 value passed fp16's range, the first bf16 tile is all zeros, or the V scales of
+  // fp8 pages lie too far apart: nothing is written then.
   __device__ __forceinline__ bool prefix(const Item& it) {
     using LD = Lds<D>;
     constexpr int KP = LD::KP, VP = LD::VP;
@@ -446,7 +461,7 @@ struct Walk {
     // register, the next 64 ids read with every tile (a branch around the read costs
     // more than the read); pages past the range repeat its last one.
     int ids = 0, idn = 0;
-    float ksc = 1.f, vsc = 1.f, vref = 1.f;  // vref, fp8: the range's largest V scale
+    float ksc = 1.f, vsc = 1.f, vref = 1.f;  // vref, fp8: a bound on the range's V scales
     auto read_ids = [&](int first) SPV_INLINE { return table[min(first + lane, pages - 1)]; };
     auto open_window = [&](int raw) SPV_INLINE {
       const int phys = safe_id(it, raw);
@@ -611,8 +626,8 @@ struct Walk {
     f32x4_t sc[4][NT];            // S^T of the tile in the walk
     uint32_t ph[2][NT][4];        // its P, two pages an operand
     // fp8, of the window of the tile in the walk: a page's K scale times the softmax's, log2 of
-    // its V scale over vref, and the inverse of that ratio. Pages whose ratio is below 2^-100
-    // count as 2^-100: their P vanishes in fp16 either way.
+    // its V scale over vref, and the inverse of that ratio. Pages of scale 0, of zeros, count as
+    // 2^-100.
     float ks_t = 1.f, vl_t = 0.f, vi_t = 1.f;
     auto pv = [&](int vslot) SPV_INLINE {
       const uint16_t* V = sV + vslot * LD::kV;
@@ -654,7 +669,7 @@ struct Walk {
           ks_t = ksc * sl2;
           if (ks_t == 0.f) ks_t = 1e-38f;  // (a masked -inf times 0 would be NaN)
           const float ratio = vref > 0.f ? vsc / vref : 0.f;
-          vl_t = ratio < 0x1p-100f ? -100.f : __builtin_amdgcn_logf(ratio);
+          vl_t = ratio == 0.f ? -100.f : __builtin_amdgcn_logf(ratio);
           vi_t = __builtin_amdgcn_exp2f(-vl_t);
         }
 #pragma unroll
@@ -703,13 +718,13 @@ struct Walk {
         for (int nt = 0; nt < NT; ++nt) {
           float a = fmaxf(mx[nt], __shfl_xor(mx[nt], 16, 64));
           a = fmaxf(a, __shfl_xor(a, 32, 64));
-          const float m_new = fmaxf(m[nt], kFp8 ? a : a * sl2);
+          const float m_new = fmaxf(m[nt], (kFp8 ? a : a * sl2) - kShift);
           const float alpha = m_new == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m[nt] - m_new);
           l[nt] *= alpha;
 #pragma unroll
           for (int mt = 0; mt < MT; ++mt) o[mt][nt] *= alpha;
           m[nt] = m_new;
-          thr[nt] = kFp8 ? m_new + kSlack : (m_new + kSlack) * inv_sl2;
+          thr[nt] = kFp8 ? m_new + (kShift + kSlack) : (m_new + (kShift + kSlack)) * inv_sl2;
         }
       }
 #pragma unroll
@@ -764,12 +779,19 @@ struct Walk {
       load_next(st0, 0);
       load_next(st1, 1);
       if constexpr (kFp8) {
-        float mx = 0.f;
+        float mx = 0.f, mn = INFINITY;  // of scales that are not 0 (pages of zeros)
         for (int pg = tid; pg < pages; pg += kMfmaThreads) {
           const int phys = table[pg];
-          if ((unsigned)phys < (unsigned)p.cap) mx = fmaxf(mx, scales_of(phys).y);
+          if ((unsigned)phys >= (unsigned)p.cap) continue;
+          const float s = scales_of(phys).y;
+          mx = fmaxf(mx, s);
+          if (s > 0.f) mn = fminf(mn, s);
         }
-        vref = __uint_as_float(wg_max(__float_as_uint(mx)));
+        // both over the workgroup at once, as bf16: the largest rounded up, the smallest down
+        const uint32_t both =
+            wg_max2((__float_as_uint(mx) + 0xffffu) >> 16 | (0xffffu - (__float_as_uint(mn) >> 16)) << 16);
+        vref = __uint_as_float(both << 16);
+        if (__uint_as_float((0xffffu - (both >> 16)) << 16) < vref * kScaleRange) return false;
       }
       if constexpr (!kF16 && !kFp8) {
         uint32_t mx = 0;  // the largest finite |v| of the first tile
@@ -786,7 +808,7 @@ struct Walk {
               mx = max(mx, hi < 0x7f80u ? hi : 0u);
             }
           }
-        mx = wg_max(mx);
+        mx = wg_max2(mx);
         if (mx == 0) return false;  // all zero: nothing to choose the power from
         vk = stage_exponent(__uint_as_float(mx << 16));
         vs = ldexpf(1.f, vk);

@@ -205,3 +205,25 @@ def test_long_own_contexts_in_one_range(cuda, dtype, C, n):
     some = [0, 1, 40, B - 1]
     pick = lambda x: [x[i] for i in some]  # noqa: E731
     close(out[some], *exact(q[some], kv, pick(starts), [1] * 4, [P] * 4, own=[0] * 4))
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("margin", [0.0, 8.0, 25.0])
+@pytest.mark.parametrize("power", [-3, -8, -11, -13, -16, -18, -22, -40])
+def test_fp8_rows_on_pages_of_small_v_scale(cuda, d, margin, power):
+    """Five pages of values 2^power times the others'; the queries' scores on their keys lie ``margin``
+    (natural units) above the rest, so that from 8 on those pages hold most of a row's weight."""
+    g = torch.Generator().manual_seed(71)
+    B, C, hq, hkv, P = 8, 5, 8, 2, 400
+    assert B * C * (hq // hkv) > 64
+    u = torch.randn(d, generator=g)
+    u = u / u.norm() * d ** 0.5
+    k, v = (torch.randn(1, P, hkv, d, generator=g) for _ in range(2))
+    k[:, 80:160] += 2 * u
+    v[:, 80:160] *= 2.0 ** power
+    own = [[torch.randn(1, 9 + C, hkv, d, generator=g) for _ in range(2)] for _ in range(B)]
+    kv = cache(cuda, [*own, (k, v)], FP8)
+    q = (torch.randn(B, C, hq, d, generator=g) + margin / 2 * d ** -0.5 * u).to(BF16).to(cuda)
+    ids, lens = [B] * B, [P] * B
+    out = shared_prefix_attention(q, kv, 0, list(range(B)), [9] * B, 9 + C, SharedPrefix(kv, ids, lens, C, hq))
+    close(out, *exact(q, kv, [9] * B, ids, lens))
