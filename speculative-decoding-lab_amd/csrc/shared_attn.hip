@@ -317,7 +317,6 @@ __global__ __launch_bounds__(kThreads) void shared_valu_kernel(SharedParams p) {
 typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
-typedef _Float16 f16x4_t __attribute__((ext_vector_type(4)));
 typedef _Float16 f16x2_t __attribute__((ext_vector_type(2)));
 typedef unsigned short u16x2_t __attribute__((ext_vector_type(2)));
 typedef float f32x4_t __attribute__((ext_vector_type(4)));
@@ -326,7 +325,7 @@ typedef float f32x2_t __attribute__((ext_vector_type(2)));
 // A row's scores may exceed its reference maximum by this much (log2 units) before
 // its sums are rescaled: P stays below 2^8.
 constexpr float kSlack = 8.f;
-// The tiled walk's reference lies this much below the maximum that it was taken from: P in fp16
+// Where P goes in fp16, the reference lies this much below the maximum that it was taken from: P
 // is at most 2^15 then, has fp16's whole 11 bits from 2^-21 of the maximum's up, and is off by at
 // most 2^-32 of that below.
 constexpr float kShift = 7.f;
@@ -936,8 +935,10 @@ struct Walk {
   // rows (8 up to 32 rows, 4 up to 64, 2 up to 128, 1 up to 256) and take every nk-th
   // page straight into operand registers, one page in flight while one is computed;
   // their sums join in LDS.
-  // P goes in two halves of bf16, beside each other in one operand over 16 keys
-  // twice (fp16 pages: one operand of 16 keys): 16 bits of P, and values of any size.
+  // P goes in two halves of bf16 (fp16 pages: of fp16), beside each other in one operand over
+  // 16 keys twice: 16 bits of P (22), and values of any size. (fp16 P in one half, over 16 keys
+  // once, gave errors of 2.5e-4 against float64 where the output's rounding alone gives 2.1e-4; 64
+  // entries of 7 x 16 rows over up to 4000 own keys then took 56.5 us, 58.9 with two.)
   // fp32: v_mfma_f32_16x16x4_f32, four to a 16-byte piece of K or V, whose four elements
   // take turns as the contracted index (the query's and P's, in the same lanes, do the
   // same). At 256 operations a clock and CU the matrix cores take 32 times as long over a
@@ -1070,13 +1071,14 @@ struct Walk {
         for (int nt = 0; nt < NT; ++nt) {
           float a = fmaxf(mx[nt], __shfl_xor(mx[nt], 16, 64));
           a = fmaxf(a, __shfl_xor(a, 32, 64));
-          const float m_new = fmaxf(m[nt], a * sl2);
+          constexpr float kBelow = kF16 ? kShift : 0.f;
+          const float m_new = fmaxf(m[nt], a * sl2 - kBelow);
           const float alpha = m_new == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m[nt] - m_new);
           l[nt] *= alpha;
 #pragma unroll
           for (int mt = 0; mt < MT; ++mt) o[mt][nt] *= alpha;
           m[nt] = m_new;
-          thr[nt] = (m_new + kSlack) * inv_sl2;
+          thr[nt] = (m_new + (kBelow + kSlack)) * inv_sl2;
         }
       }
       uint4 pb[NT];
@@ -1090,7 +1092,14 @@ struct Walk {
         if constexpr (kF32) {
           pb[nt] = make_uint4(__float_as_uint(e[0]), __float_as_uint(e[1]), __float_as_uint(e[2]), __float_as_uint(e[3]));
         } else if constexpr (kF16) {
-          pb[nt] = make_uint4(pack2_f16(e[0], e[1]), pack2_f16(e[2], e[3]), 0u, 0u);
+          uint32_t hi[2], lo[2];
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            hi[k] = pack2_f16(e[2 * k], e[2 * k + 1]);
+            const f16x2_t h = __builtin_bit_cast(f16x2_t, hi[k]);
+            lo[k] = pack2_f16(e[2 * k] - (float)h[0], e[2 * k + 1] - (float)h[1]);
+          }
+          pb[nt] = make_uint4(hi[0], hi[1], lo[0], lo[1]);
         } else {
           uint32_t hi[2], lo[2];
 #pragma unroll
@@ -1124,9 +1133,8 @@ struct Walk {
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
           if constexpr (kF16)
-            o[mt][nt] = __builtin_amdgcn_mfma_f32_16x16x16f16(__builtin_bit_cast(f16x4_t, v),
-                                                              __builtin_bit_cast(f16x4_t, make_uint2(pb[nt].x, pb[nt].y)),
-                                                              o[mt][nt], 0, 0, 0);
+            o[mt][nt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8_t, make_uint4(v.x, v.y, v.x, v.y)),
+                                                                __builtin_bit_cast(f16x8_t, pb[nt]), o[mt][nt], 0, 0, 0);
           else
             o[mt][nt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, make_uint4(v.x, v.y, v.x, v.y)),
                                                                  __builtin_bit_cast(bf16x8_t, pb[nt]), o[mt][nt], 0, 0, 0);

@@ -62,20 +62,20 @@ def exact(q, kv, starts, ids, lens, own=None):
     return [torch.stack(x) for x in zip(*out)]
 
 
-def near(out, want, size, dtype, fp32):
+def near(out, want, size, dtype, fp32, half):
     err = (out - want).abs()
-    bound = torch.finfo(dtype).eps / 2 * want.abs() + (2.0 ** -10 if dtype != F32 else fp32) * size
+    bound = torch.finfo(dtype).eps / 2 * want.abs() + (half if dtype != F32 else fp32) * size
     worst = float((err / bound.clamp(min=1e-300)).max())
     assert worst <= 1, worst
 
 
-def close(out, want, size, fp32=2.0 ** -17):
+def close(out, want, size, fp32=2.0 ** -17, half=2.0 ** -10):
     """Every finite element, by the bound above; infinities and NaN where they belong."""
     dtype, out = out.dtype, out.double()
     fine = torch.isfinite(want)
     assert torch.equal(torch.isnan(out), torch.isnan(want))
     assert torch.equal(out[~fine].nan_to_num(), want[~fine].nan_to_num())
-    near(out[fine], want[fine], size[fine], dtype, fp32)
+    near(out[fine], want[fine], size[fine], dtype, fp32, half)
 
 
 @pytest.mark.parametrize("dtype", [BF16, F16, F32])
@@ -99,6 +99,22 @@ def test_infinite_values_that_are_seen(cuda, dtype, d, B, where):
     want, size = exact(q, kv, [30] * B, ids, lens)
     assert bool(torch.isposinf(want).any()) and bool(torch.isneginf(want).any()) and bool(torch.isnan(want).any())
     close(out, want, size)
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("B,C,hq", [(4, 1, 14), (2, 7, 8), (30, 3, 16)])
+def test_fp16_weights_keep_their_bits(cuda, d, B, C, hq):
+    """Few rows behind a prefix, and own keys alone: the output's rounding and what fp32 arithmetic
+    adds, no more (P in one fp16 would add up to 2^-12 of every weight)."""
+    g = torch.Generator().manual_seed(97)
+    hkv, P = 2, 600
+    parts = [[torch.randn(1, n, hkv, d, generator=g) for _ in range(2)] for n in [200 + C] * B + [P]]
+    kv = cache(cuda, parts, F16)
+    q = torch.randn(B, C, hq, d, generator=g).half().to(cuda)
+    few = B * C * hq // hkv <= 64
+    ids, lens = [B if few else -1] * B, [P if few else 0] * B
+    out = shared_prefix_attention(q, kv, 0, list(range(B)), [200] * B, 200 + C, SharedPrefix(kv, ids, lens, C, hq))
+    close(out, *exact(q, kv, [200] * B, ids, lens), half=2.0 ** -17)
 
 
 @pytest.mark.parametrize("dtype", [BF16, F16, F32, FP8])
