@@ -33,9 +33,11 @@
 // output alone takes 1.7e-3); fp16 has 11 bits. bf16 values are staged as fp16
 // times a power of two per segment, chosen from the first tile's largest |v|
 // (which lands in [2^8, 2^9): every value from 2^-25 of it up is exact, a smaller
-// one is off by at most 2^-33 of it); where a later value would pass fp16's range, or the
+// one is off by at most 2^-33 of it). Where a later value would pass fp16's range, a page has 32
+// dims that all lie below 2^-12 of that largest (a row whose weight is there would lose bits), or the
 // first tile is all zeros, the segment is walked again page by page as own keys are, in any
-// range (7168 x 2 rows over 8192 keys 275 us where every segment is, 115 where none). fp8 codes are
+// range (7168 x 2 rows over 8192 keys 280 us where every segment is, 114 where none). fp16 values
+// are staged as they are: beside values of 2^15 P's 2^-32 is 2^-17, in either walk. fp8 codes are
 // fp16 values; a block's K scale goes into the exponent's multiplier, its V scale, over
 // the segment's largest, as a logarithm into the addend, so that P carries it; segments whose V scales
 // (zeros aside) lie more than 2^12 apart are walked page by page, too (P in two halves of bf16, with
@@ -441,8 +443,8 @@ struct Walk {
   }
 
   // ---- a segment of a prefix: 256 rows, 32 per wave, 64 keys at a time in LDS. False
-  // where a bf16 value passed fp16's range, the first bf16 tile is all zeros, or the V scales of
-  // fp8 pages lie too far apart: nothing is written then.
+  // where bf16 values do not fit the staging (above) or the V scales of fp8 pages lie too far apart:
+  // nothing is written then.
   __device__ __forceinline__ bool prefix(const Item& it) {
     using LD = Lds<D>;
     constexpr int KP = LD::KP, VP = LD::VP;
@@ -526,9 +528,12 @@ struct Walk {
       window(t);
       load(S, min(t, n - 1));
     };
-    float vs = 1.f;     // bf16: the staging factor 2^vk
+    float vs = 1.f;  // bf16: the staging factor 2^vk
     int vk = 0;
-    uint32_t vmax = 0;  // bf16: largest |v| bits staged (both halves)
+    // bf16, as bits of |v|: a little less than what a page's largest has to reach, what none may
+    // pass, the largest so far (of either half of a word), and whether one of the wave's pages (32
+    // dims of it) is too small.
+    uint32_t low2 = 0, top = 0, vmax = 0, small = 0;
     // Zeroes the values of keys past the range's end.
     auto edge = [&](Stage& S, int t) SPV_INLINE {
       const int t0 = key0 + t * kUnit;
@@ -551,6 +556,7 @@ struct Walk {
     };
     // bf16 values to fp16, in place, in the softmax's phase: beside the matrix
     // instructions they left no registers for the operands' read-ahead (0.69 PFLOP/s).
+    // A wave's 64 pieces are 32 dims of a page.
     auto convert = [&](Stage& S) SPV_INLINE {
       if constexpr (!kF16 && !kFp8) {
 #pragma unroll
@@ -558,13 +564,18 @@ struct Walk {
 #pragma unroll
           for (int hh = 0; hh < 2; ++hh) {
             u32x4_t x = S.v[i][hh];
+            uint32_t most = 0;
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
               const uint32_t y = x[e];
-              vmax = max_abs2(y, vmax);
+              most = max_abs2(y, most);
               x[e] = pack2_f16(__uint_as_float(y << 16) * vs, __uint_as_float(y & 0xffff0000u) * vs);
             }
             S.v[i][hh] = x;
+            vmax = max_abs2(most, vmax);
+            const u16x2_t over = __builtin_elementwise_sub_sat(__builtin_bit_cast(u16x2_t, most),
+                                                               __builtin_bit_cast(u16x2_t, low2));
+            small |= (uint32_t)(__ballot(most != 0) != 0) & (uint32_t)(__ballot(__builtin_bit_cast(uint32_t, over) != 0) == 0);
           }
       }
     };
@@ -807,10 +818,14 @@ struct Walk {
               mx = max(mx, hi < 0x7f80u ? hi : 0u);
             }
           }
-        mx = wg_max2(mx);
+        mx = __builtin_amdgcn_readfirstlane(wg_max2(mx));
         if (mx == 0) return false;  // all zero: nothing to choose the power from
         vk = stage_exponent(__uint_as_float(mx << 16));
         vs = ldexpf(1.f, vk);
+        // 2^-12 and 2^7 times the first tile's largest (a power of two is 2^7 in a bf16's bits)
+        const uint32_t low = mx > 12 << 7 ? mx - (12 << 7) - 1 : 0;
+        low2 = low | low << 16;
+        top = min(mx + (7 << 7), 0x7f7fu);
       }
       edge(st0, 0);
       convert(st0);
@@ -862,9 +877,7 @@ struct Walk {
       }
       softmax(t);
       if constexpr (!kF16 && !kFp8) {
-        // bits of the largest |v| that stays within fp16 at this power
-        const uint32_t top = min(__float_as_uint(ldexpf(65504.f, -vk)) >> 16, 0x7f7fu);
-        const bool passed = __any((vmax & 0xffffu) > top || (vmax >> 16) > top);
+        const bool passed = small || __any((vmax & 0xffffu) > top || (vmax >> 16) > top);
         if (lane == 0) sMax[w] = passed;
       }
       phase_end();

@@ -243,3 +243,29 @@ def test_fp8_rows_on_pages_of_small_v_scale(cuda, d, margin, power):
     ids, lens = [B] * B, [P] * B
     out = shared_prefix_attention(q, kv, 0, list(range(B)), [9] * B, 9 + C, SharedPrefix(kv, ids, lens, C, hq))
     close(out, *exact(q, kv, [9] * B, ids, lens))
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("margin", [0.0, 8.0, 14.0, 19.0, 25.0])
+@pytest.mark.parametrize("dtype,power", [(BF16, -8), (BF16, -12), (BF16, -16), (BF16, -20), (BF16, -24), (BF16, -27),
+                                         (BF16, -31), (BF16, -60), (F16, -8), (F16, -12), (F32, -8), (F32, -60)])
+def test_rows_on_pages_of_small_values(cuda, dtype, d, margin, power):
+    """As over fp8: pages whose values are 2^power times the others', with most of a row's weight from
+    a margin of 8 on, in one segment with the others."""
+    g = torch.Generator().manual_seed(89)
+    B, C, hq, hkv, P = 8, 5, 8, 2, 400
+    u = torch.randn(d, generator=g)
+    u = u / u.norm() * d ** 0.5
+    k, v = (torch.randn(1, P, hkv, d, generator=g) for _ in range(2))
+    k[:, 80:160] += 2 * u
+    v[:, 80:160] *= 2.0 ** power
+    own = [[torch.randn(1, 9 + C, hkv, d, generator=g) for _ in range(2)] for _ in range(B)]
+    kv = cache(cuda, [*own, (k, v)], dtype)
+    q = (torch.randn(B, C, hq, d, generator=g) + margin / 2 * d ** -0.5 * u).to(dtype).to(cuda)
+    ids, lens = [B] * B, [P] * B
+    prefix = SharedPrefix(kv, ids, lens, C, hq)
+    segs = recut(prefix, ids, lens, lambda n: n)
+    assert all(s[5] > 64 and s[7] - s[6] == P for s in segs)
+    out = shared_prefix_attention(q, kv, 0, list(range(B)), [9] * B, 9 + C, prefix)
+    # fp32: scores of up to 60 log2 units
+    close(out, *exact(q, kv, [9] * B, ids, lens), fp32=2.0 ** -15)
