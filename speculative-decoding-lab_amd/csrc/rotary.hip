@@ -10,8 +10,9 @@
 //
 // The angle is formed and reduced in fp64: at position 10^6 the fp32 product is
 // off by up to 0.03 rad, and the fp64 one, in turns, by 2^-53 of some 10^5
-// turns. What is left of a turn goes to fp32 sin and cos (an error of 2^-24
-// turns at most), the products are fp32, and each result is rounded once.
+// turns. What is left of a turn, in fp32, goes to fp32 sin and cos, and what that rounding
+// leaves (up to 2^-26 turns, as much as the rounding of sin and cos) to their first-order terms;
+// the products are fp32, and each result is rounded once.
 #include <type_traits>
 
 #include "spv_common.h"
@@ -56,10 +57,11 @@ __device__ __forceinline__ float2 turn_of(const RotaryParams& p, int b, int j, i
   const int axis = p.axis_of ? min(max(p.axis_of[i], 0), p.axes - 1) : 0;
   const int pos = p.positions ? p.positions[((size_t)axis * p.B + b) * p.C + j] : p.start[b] + j;
   const double turns = p.inv_freq[i] * kInvTwoPi;
-  const float f = (float)fma((double)pos, turns, -__builtin_rint((double)pos * turns));  // in [-1/2, 1/2]
+  const double r = fma((double)pos, turns, -__builtin_rint((double)pos * turns));  // in [-1/2, 1/2]
+  const float f = (float)r, rest = (float)(r - f) * 6.283185307f;  // what f leaves, in radians
   float s, c;
   sincospif(2.f * f, &s, &c);
-  return make_float2(c * p.factor, s * p.factor);
+  return make_float2(fmaf(-s, rest, c) * p.factor, fmaf(c, rest, s) * p.factor);
 }
 
 // The pool row (block * block_size + offset) of chunk token j of entry b, or -1

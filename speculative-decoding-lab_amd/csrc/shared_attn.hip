@@ -30,7 +30,9 @@
 // S^T's accumulator layout is P^T's operand layout (lane l: keys 4 (l / 16) .. + 3
 // of row l % 16), so the softmax moves no data between lanes. P in bf16 (8 bits)
 // would miss the library's bf16 bar (2e-3 per sequence, of which rounding the
-// output alone takes 1.7e-3); fp16 has 11 bits. bf16 values are staged as fp16
+// output alone takes 1.7e-3); fp16 has 11 bits. (fp16 outputs, whose rounding takes 2.1e-4, are
+// 2.85e-4 off float64 so; in two halves P would add nothing to 2.1e-4, and 7168 x 2 rows over 8192
+// keys would take 137 us for 114, 1008 x 2 of head_dim 64 over 32768 keys 49 for 41.) bf16 values are staged as fp16
 // times a power of two per segment, chosen from the first tile's largest |v|
 // (which lands in [2^8, 2^9): every value from 2^-25 of it up is exact, a smaller
 // one is off by at most 2^-33 of it). Where a later value would pass fp16's range, a page has 32
