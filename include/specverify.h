@@ -452,7 +452,11 @@ size_t spv_shared_attn_workspace_bytes(const int32_t* plan_host, int32_t head_di
  * contract forbids -- a prefix longer than its sequence, start_b + C beyond the
  * written length or max_ctx, a block id outside the pool -- set ctr[7] = 1 + b
  * (sticky) and read block 0, never outside the pool. A key beyond a row's last
- * position does not reach the row, whatever it holds. Two launches. */
+ * position does not reach the row, whatever it holds; a key that it does reach counts as in
+ * the definition, infinities included. Scores and sums are fp32. Over 16-bit and fp8 pages a
+ * weight meets its value with 11 bits or more, and what a key adds is off by at most 2^-32 of the
+ * largest |v| beside that (a weight below 2^-32 of the row's largest may count as 0).
+ * B * C * num_q_heads <= 2^23. Two launches. */
 int spv_shared_attn(void* out, const void* q, int q_dtype, const void* k_pool,
                     const void* v_pool, int kv_dtype, const float* kv_scales,
                     const int32_t* block_tables, int32_t max_blocks_per_seq,
@@ -494,7 +498,8 @@ int spv_rotary(void* q_out, const void* q, void* k_out, const void* k, int dtype
  * verdict of the last allocation stands. write_plan (B x C int32, or NULL)
  * receives the chunk's pool rows as in spv_kv_append_plan, or, with follow_plan
  * != 0, names them (a later layer's call: no table, length or counter is read or
- * written). Both pools' rows outside the chunk stay as they are. */
+ * written). Both pools' rows outside the chunk stay as they are. capacity * block_size <
+ * 2^31 (beyond: spv_rotary, then spv_kv_append). */
 int spv_kv_rotary_append(void* q_out, const void* q, const void* k_new, const void* v_new,
                          int dtype, const int64_t* strides, void* k_pool, void* v_pool,
                          int32_t* block_tables, int32_t max_blocks_per_seq,

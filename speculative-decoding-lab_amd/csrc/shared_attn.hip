@@ -45,10 +45,10 @@
 // (zeros aside) lie more than 2^12 apart are walked page by page, too (P in two halves of bf16, with
 // fp32's exponents).
 //
-// What bounds it: with long prefixes and many rows the walk, 0.90 to 0.97 PFLOP/s of its
-// steady state (head_dim 128, bf16; the matrix instructions and the softmax beside each
-// other, without staging or operand reads, reach 1.2); 7168 x 2 rows over 8192 keys and
-// up to 1024 own keys an entry (64 GFLOP) take 103 us, 9 of them in the join. With short ones the
+// What bounds it: with long prefixes and many rows the walk (7168 x 2 bf16 rows: each further
+// 8192 keys take 49 us, 1.2 PFLOP/s; 6272 x 2 of head_dim 64 0.73, over fp8 0.76 to 0.79) and
+// its segments' starts and ends: 7168 x 2 rows over 8192 keys and up to 1024 own keys an entry (64
+// GFLOP) take 103 us and 9 in the join. With short ones the
 // launches, the first pages' round trips and the partials, which are written and
 // read at the rate of memory: 1152 x 2 rows over 2048 keys 21 us and 5 in the join.
 #include <math.h>
@@ -1270,8 +1270,8 @@ __global__ __launch_bounds__(kMfmaThreads, 2) void shared_mfma_kernel(SharedPara
     return;
   }
   // A segment of few rows is walked as own keys are, its pages shared out over the waves: 28
-  // rows x 2 kv heads of 64 behind 32768 fp16 keys take 10.2 us, 15.3 in a tile of 256 rows
-  // (63 x 2 of fp8 13.5 and 18.5; 72 x 2 of 128, bf16, 29.5 and 22.0).
+  // rows x 2 kv heads of 64 behind 32768 fp16 keys take 10.6 us, 15.3 in a tile of 256 rows
+  // (63 x 2 of fp8 13.0 and 18.5; 72 x 2 of 128, bf16, 29.5 and 22.5).
   // Where the tile's staging does not hold its values, they go the same way.
   bool done = false;
   if (KT != SPV_F32 && it.first >= 0 && it.rows > kPagesRows) {
