@@ -445,8 +445,8 @@ struct Walk {
   }
 
   // ---- a segment of a prefix: 256 rows, 32 per wave, 64 keys at a time in LDS. False
-  // where bf16 values do not fit the staging (above) or the V scales of fp8 pages lie too far apart:
-  // nothing is written then.
+  // where bf16 values do not fit the staging (above), the V scales of fp8 pages lie too far apart, or
+  // an fp16 value that makes a sum so is not finite: nothing is written then.
   __device__ __forceinline__ bool prefix(const Item& it) {
     using LD = Lds<D>;
     constexpr int KP = LD::KP, VP = LD::VP;
@@ -891,6 +891,9 @@ struct Walk {
         for (int k = 0; k < kWaves; ++k) passed |= sMax[k];
         if (__builtin_amdgcn_readfirstlane(passed)) return false;
       }
+      // (an infinite value and a weight that is 0 in fp16)
+      if constexpr (kF16)
+        if (__syncthreads_or(sums_not_finite(o)) && __syncthreads_or(values_not_finite(it))) return false;
     }
     write(it, o, m, l, valid, kFp8 ? vref : ldexpf(1.f, -vk));
     return true;
@@ -926,6 +929,16 @@ struct Walk {
     }
   }
 
+  __device__ __forceinline__ bool sums_not_finite(const f32x4_t (&o)[MT][NT]) const {  // of the lane
+    float z = 0.f;
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) z = fmaf(o[mt][nt][c], 0.f, z);
+    return z != z;
+  }
   // Whether one of an item's values is not finite: each wave looks through every eighth page.
   __device__ __forceinline__ bool values_not_finite(const Item& it) const {
     constexpr int kPer = 16 / ES;  // elements of a 16-byte piece, of one dim
@@ -1195,14 +1208,7 @@ struct Walk {
     // half of P (which may be zero or of the other sign): the sums show it as NaN or an infinity,
     // and the any-shape walk takes the item. Keys or queries that are not finite show so, too, but
     // are as right here.
-    float z = 0.f;
-#pragma unroll
-    for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int c = 0; c < 4; ++c) z = fmaf(o[mt][nt][c], 0.f, z);
-    if (__syncthreads_or(z != z) && __syncthreads_or(values_not_finite(it))) return false;
+    if (__syncthreads_or(sums_not_finite(o)) && __syncthreads_or(values_not_finite(it))) return false;
     // Join the waves of the same rows: all take the largest m; then every thread adds up
     // four dims of a row over the waves, in their order, half of the dims at a time.
     float2* const sML = reinterpret_cast<float2*>(smem + LD::kJoinRows);

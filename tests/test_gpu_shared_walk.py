@@ -269,3 +269,44 @@ def test_rows_on_pages_of_small_values(cuda, dtype, d, margin, power):
     out = shared_prefix_attention(q, kv, 0, list(range(B)), [9] * B, 9 + C, prefix)
     # fp32: scores of up to 60 log2 units
     close(out, *exact(q, kv, [9] * B, ids, lens), fp32=2.0 ** -15)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("B", [1, 20])
+def test_an_infinite_value_of_little_weight(cuda, dtype, d, B):
+    """A weight of e^-50, nothing in fp16, still takes an infinite value to its dimension."""
+    g = torch.Generator().manual_seed(101)
+    C, hq, hkv, P = 4, 8, 2, 300
+    u = torch.randn(d, generator=g)
+    u = u / u.norm() * d ** 0.25
+    parts = [[torch.randn(1, n, hkv, d, generator=g) for _ in range(2)] for n in [9 + C] * B + [P]]
+    parts[B][0][:, 100:120] += 25 * u
+    parts[B][0][:, 200:220] -= 25 * u
+    parts[B][1][0, 210, 0, 7], parts[B][1][0, 211, 1, 9] = float("inf"), -float("inf")
+    kv = cache(cuda, parts, dtype)
+    q = (0.5 * torch.randn(B, C, hq, d, generator=g) + u).to(dtype).to(cuda)
+    ids, lens = [B] * B, [P] * B
+    prefix = SharedPrefix(kv, ids, lens, C, hq)
+    recut(prefix, ids, lens, lambda units: units)
+    out = shared_prefix_attention(q, kv, 0, list(range(B)), [9] * B, 9 + C, prefix)
+    want, size = exact(q, kv, [9] * B, ids, lens)
+    assert int(torch.isinf(want).sum()) == B * C * hq
+    close(out, want, size, fp32=2.0 ** -15)
+
+
+def test_rows_of_nan_queries(cuda):
+    """A NaN in an entry's queries is that row's alone, and sends nothing to a slower walk's result."""
+    g = torch.Generator().manual_seed(103)
+    B, C, hq, hkv, d, P = 20, 4, 8, 2, 64, 300
+    for dtype in (BF16, F16, F32, FP8):
+        parts = [[torch.randn(1, n, hkv, d, generator=g) for _ in range(2)] for n in [9 + C] * B + [P]]
+        kv = cache(cuda, parts, dtype)
+        q = torch.randn(B, C, hq, d, generator=g).to(BF16 if dtype == FP8 else dtype).to(cuda)
+        prefix = SharedPrefix(kv, [B] * B, [P] * B, C, hq)
+        want = shared_prefix_attention(q, kv, 0, list(range(B)), [9] * B, 9 + C, prefix)
+        q[3, 1, 2, 5] = float("nan")
+        out = shared_prefix_attention(q, kv, 0, list(range(B)), [9] * B, 9 + C, prefix)
+        assert bool(torch.isnan(out[3, 1, 2]).all())
+        out[3, 1, 2] = want[3, 1, 2]
+        assert torch.equal(out, want)
