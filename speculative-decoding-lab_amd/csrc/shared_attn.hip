@@ -32,8 +32,8 @@
 // would miss the library's bf16 bar (2e-3 per sequence, of which rounding the
 // output alone takes 1.7e-3); fp16 has 11 bits. (fp16 outputs, whose rounding takes 2.1e-4, are
 // 2.85e-4 off float64 so; in two halves P would add nothing to 2.1e-4, and 7168 x 2 rows over 8192
-// keys would take 137 us for 114, 1008 x 2 of head_dim 64 over 32768 keys 49 for 41.) bf16 values are staged as fp16
-// times a power of two per segment, chosen from the first tile's largest |v|
+// keys would take 137 us for 114, 1008 x 2 of head_dim 64 over 32768 keys 49 for 41.)
+// bf16 values are staged as fp16 times a power of two per segment, chosen from the first tile's largest |v|
 // (which lands in [2^8, 2^9): every value from 2^-25 of it up is exact, a smaller
 // one is off by at most 2^-33 of it). Where a later value would pass fp16's range, a page has 32
 // dims that all lie below 2^-12 of that largest (a row whose weight is there would lose bits), or the

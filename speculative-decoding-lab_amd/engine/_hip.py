@@ -151,10 +151,10 @@ def stream_of(device: torch.device) -> int:
     return torch._C._cuda_getCurrentRawStream(idx)
 
 
-def kept_for(stream: int, made_on: int, *tensors: torch.Tensor) -> int:
+def kept_for(stream: int, made_on: Optional[int], *tensors: torch.Tensor) -> int:
     """``stream``, the current one, after keeping the memory of a handle's ``tensors`` from reuse
-    until its work so far is done, where they were made on another one. What a captured graph
-    uses its owner keeps."""
+    until its work so far is done, where they were not made on it (None: unknown). What a captured
+    graph uses its owner keeps."""
     if stream != made_on and not torch.cuda.is_current_stream_capturing():
         for t in tensors:
             t.record_stream(torch.cuda.current_stream(t.device))

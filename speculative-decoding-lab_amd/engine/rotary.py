@@ -83,14 +83,40 @@ class Rotary:
         self._passed: dict = {}
         self._made_on = _hip.stream_of(self.device)
 
+    @property
+    def inv_freq(self) -> torch.Tensor:
+        """The frequencies, ``rotary_dim / 2`` float64 on the device; may be replaced by others."""
+        return self._inv_freq
+
+    @inv_freq.setter
+    def inv_freq(self, t: torch.Tensor) -> None:
+        self._inv_freq = self._readable(t, torch.float64)
+
+    @property
+    def axis_of(self) -> torch.Tensor:
+        """The position axis of every frequency, int32 on the device; may be replaced by others."""
+        return self._axis_of
+
+    @axis_of.setter
+    def axis_of(self, t: torch.Tensor) -> None:
+        self._axis_of = self._readable(t, torch.int32)
+
+    def _readable(self, t: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
+        n = self.rotary_dim // 2
+        if not isinstance(t, torch.Tensor) or t.dtype is not dtype or tuple(t.shape) != (n,) or \
+                t.device != self.device or not t.is_contiguous():
+            raise ValueError("the kernels read {} contiguous {} on {}".format(n, dtype, self.device))
+        self._made_on = None  # a caller's tensor may be of any stream
+        return t
+
     def _stream(self) -> int:
         """The current stream, for a launch that reads the frequencies."""
-        return _hip.kept_for(_hip.stream_of(self.device), self._made_on, self.inv_freq, self.axis_of)
+        return _hip.kept_for(_hip.stream_of(self.device), self._made_on, self._inv_freq, self._axis_of)
 
     def _args(self) -> tuple:
         """The launch arguments of the frequencies, asked anew in every call: a copy of this
         object has tensors of its own, and a caller may replace them."""
-        return self.inv_freq.data_ptr(), self.axis_of.data_ptr(), self.axes, self.factor
+        return self._inv_freq.data_ptr(), self._axis_of.data_ptr(), self.axes, self.factor
 
     def _positions(self, positions: torch.Tensor, B: int, C: int) -> torch.Tensor:
         """int32 ``(axes, B, C)``; ``(B, C)`` stands for every axis."""
@@ -257,10 +283,11 @@ def rotary_append(query: Optional[torch.Tensor], k_new: torch.Tensor, v_new: tor
     ``k_new`` / ``v_new`` (B, C, Hkv, d) and ``query`` share the pool's dtype
     (an fp8 pool: one of float32, bfloat16, float16; the rotated keys are
     quantised unrounded). fp8 pools, and pools of 2^31 token rows or more, are
-    written in a launch behind the rotation's and ignore ``plan``. ``positions``: as in ``rotary_embed``; None takes the
-    pool positions ``start_positions[b] + j``. No host synchronisation with
-    device tensors of distinct, added ``seq_ids``. A later layer's call of a
-    round passes ``alloc=False`` and the first one's ``plan``.
+    written in a launch behind the rotation's and ignore ``plan``.
+    ``positions``: as in ``rotary_embed``; None takes the pool positions
+    ``start_positions[b] + j``. No host synchronisation with device tensors of
+    distinct, added ``seq_ids``. A later layer's call of a round passes
+    ``alloc=False`` and the first one's ``plan``.
     """
     plain = query is not None and query_out is None
     sig = (kv._dt, kv.num_kv_heads, kv.head_dim, kv.device, query.shape, query.stride(), query.dtype, query.device,

@@ -84,3 +84,18 @@ def test_a_replaced_tensor_of_the_cache_is_used(launches, name):
     assert _append(launches, kv, rot) == _of(kv)
     kv.allocator.free_stack = kv.allocator.free_stack.clone()
     assert _append(launches, kv, rot) == _of(kv)
+
+
+@pytest.mark.parametrize("bad", [torch.ones(4), torch.ones(3, dtype=torch.float64), torch.ones(8, dtype=torch.float64)[::2],
+                                 torch.ones(4, dtype=torch.float64, device="meta"), [1.0] * 4, None])
+def test_frequencies_that_a_launch_cannot_read_are_refused(launches, bad):
+    """Another type, length, layout or device: the kernels read rotary_dim / 2 float64 in a row."""
+    rot = Rotary(8, "cpu")
+    with pytest.raises(ValueError):
+        rot.inv_freq = bad
+    with pytest.raises(ValueError):
+        rot.axis_of = bad
+    before = _embed(launches, rot)
+    assert before == (rot.inv_freq.data_ptr(), rot.axis_of.data_ptr())
+    rot.axis_of = torch.zeros(4, dtype=torch.int32)
+    assert _embed(launches, rot) == (before[0], rot.axis_of.data_ptr())

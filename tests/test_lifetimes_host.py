@@ -65,3 +65,11 @@ def test_a_handle_is_kept_for_other_streams(streams, name):
     streams.capturing = True  # the caller keeps what a graph uses
     go()
     assert not streams.recorded
+
+
+def test_replaced_frequencies_are_kept_for_every_stream(streams):
+    """They may have been made on any."""
+    rot, x = Rotary(8, "cpu"), torch.zeros(1, 2, 1, 8)
+    rot.inv_freq = rot.inv_freq * 2
+    rotary_embed(x, x, rot, torch.zeros(1, 2, dtype=torch.int32))
+    assert set(streams.recorded) == {(rot.inv_freq.data_ptr(), 0), (rot.axis_of.data_ptr(), 0)}
