@@ -155,9 +155,9 @@ __global__ __launch_bounds__(256) void rotary_elem_kernel(RotaryParams p) {
 // head) each, transposed through LDS so that whole pages are stored as 16-byte
 // pieces.
 // What bounds it: the rows' bytes, each read and written once, for prompts (75.5 MB of
-// bf16 queries and keys in 14.9 us, 5.1 TB/s; with the values and the cache's writes 30.7 MB
-// a layer in 9.1); a few dependent round trips (start, table, length, position) for decode
-// chunks (8 tokens 4.0 us, 32 chunks of 6 tokens 4.5).
+// bf16 queries and keys in 15.0 us, 5.0 TB/s; with the values and the cache's writes 30.7 MB
+// a layer in 9.0); a few dependent round trips (start, table, length, position) for decode
+// chunks (8 tokens 3.9 us, 32 chunks of 6 tokens 4.5).
 constexpr int kVecThreads = 256;
 constexpr int kMaxTT = 8;
 constexpr int kVT = 16;  // positions of a value tile

@@ -48,7 +48,7 @@
 // What bounds it: with long prefixes and many rows the walk (7168 x 2 bf16 rows: each further
 // 8192 keys take 49 us, 1.2 PFLOP/s; 6272 x 2 of head_dim 64 0.73, over fp8 0.76 to 0.79) and
 // its segments' starts and ends: 7168 x 2 rows over 8192 keys and up to 1024 own keys an entry (64
-// GFLOP) take 103 us and 9 in the join. With short ones the
+// GFLOP) take 104 us and 9 in the join. With short ones the
 // launches, the first pages' round trips and the partials, which are written and
 // read at the rate of memory: 1152 x 2 rows over 2048 keys 21 us and 5 in the join.
 #include <math.h>
