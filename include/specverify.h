@@ -169,6 +169,33 @@ int spv_kv_append_fp8(void* k_pool, void* v_pool, float* kv_scales, int new_dtyp
                       int32_t head_dim, int32_t may_alloc, int32_t write_limit_b,
                       void* stream);
 
+/* spv_kv_append for an fp8 (OCP e4m3) pool with one fp32 scale per (layer, kv
+ * head, block, K | V): kv_scales is [num_layers][num_kv_heads][capacity][2]
+ * (K, V), a stored code q of a head meaning q * scale. No reference counterpart
+ * (engine/kv.py:99-101 stores the model dtype). Allocation, exhaustion, write
+ * limit and lengths are spv_kv_append's; blocks the allocation hands out get zero
+ * scales in every layer and head. For each block the chunk writes, each head and
+ * separately for K and V: a = max |x| over the chunk's finite values in the block,
+ * scale' = max(scale, a / 448); if scale' > scale every other row of the page is
+ * re-encoded as e4m3((q * scale) / scale'); the chunk's rows are stored as
+ * e4m3(x / scale') (0 when scale' = 0). e4m3 rounds to nearest even and saturates
+ * at +-448; what is not finite is stored as NaN; products and quotients are
+ * correctly rounded fp32. k_new / v_new: (B, C, Hkv, d) in new_dtype (f32, bf16 or
+ * f16); strides (HOST, 6 values): the element strides (batch, token, head) of
+ * k_new and v_new, the last dim contiguous. k_new = v_new = NULL allocates only.
+ * Pools of any size; SPV_ERR_UNSUPPORTED where not one row fits the LDS
+ * (head_dim > 8,176; with a full rotation, below, 5,450). */
+int spv_kv_append_fp8_heads(void* k_pool, void* v_pool, float* kv_scales, int new_dtype,
+                            const void* k_new, const void* v_new, const int64_t* strides,
+                            int32_t* block_tables, int32_t max_blocks_per_seq,
+                            int32_t* num_blocks, int32_t* seq_lens,
+                            int32_t* free_stack, int32_t* free_flag, int32_t* ctr,
+                            const int32_t* seq_ids, const int32_t* start_pos,
+                            int32_t B, int32_t C, int32_t layer, int32_t num_layers,
+                            int32_t capacity, int32_t block_size, int32_t num_kv_heads,
+                            int32_t head_dim, int32_t may_alloc, int32_t write_limit_b,
+                            void* stream);
+
 /* Rewind of a spec round (engine/spec_scheduler.py:302-307, 320-322) built
  * from PagedKVCache.truncate (engine/kv.py:150-162) and .clear (kv.py:164-171),
  * applied per entry in order: if new_len[i] >= 0 (and, with shrink_only, only
@@ -257,6 +284,15 @@ int spv_pool_metrics(const int32_t* ctr, const int32_t* seq_lens, int32_t rows,
                      const int32_t* finished, int32_t B, int64_t* record,
                      int64_t* peak, void* stream);
 
+/* gather_ctx (engine/attention.py:41-63) over a pool of spv_kv_append_fp8_heads:
+ * out = (2, length, Hkv, d) in out_dtype (f32, bf16, f16), code * scale in fp32
+ * rounded once. A block id outside the pool reads block 0. */
+int spv_kv_gather_fp8_heads(const void* k_pool, const void* v_pool, const float* kv_scales,
+                            const int32_t* block_tables, int32_t max_blocks_per_seq,
+                            int32_t seq_id, int32_t length, int32_t layer, int32_t capacity,
+                            int32_t block_size, int32_t num_kv_heads, int32_t head_dim,
+                            void* out, int out_dtype, void* stream);
+
 /* gather_ctx (engine/attention.py:41-63): out = (2, length, Hkv, d) in kv_dtype
  * (fp8 pools are dequantised to fp32 with kv_scales, see spv_verify_attn). */
 int spv_kv_gather(const void* k_pool, const void* v_pool, int kv_dtype,
@@ -314,6 +350,26 @@ int spv_verify_attn(void* out, const void* q, int q_dtype,
                     int32_t block_size, int32_t layer, int32_t capacity,
                     int32_t max_ctx, float scale, void* workspace,
                     size_t workspace_bytes, void* stream);
+
+/* spv_verify_attn over a pool of spv_kv_append_fp8_heads: q and out in q_dtype
+ * (f32, bf16 or f16), the rest as there (the forbidden reads and ctr[7] too).
+ * What a masked position holds, NaN included, reaches no output. The workspace
+ * (of the size below, zero-filled before its first use) holds arrival counters,
+ * which every call leaves at zero, and partials; calls that share one are ordered.
+ * head_dim <= 2,048 (SPV_ERR_UNSUPPORTED beyond). */
+size_t spv_verify_attn_fp8_heads_workspace_bytes(int32_t B, int32_t C, int32_t num_q_heads,
+                                                 int32_t num_kv_heads, int32_t head_dim,
+                                                 int32_t block_size, int32_t max_ctx);
+int spv_verify_attn_fp8_heads(void* out, const void* q, int q_dtype,
+                              const void* k_pool, const void* v_pool,
+                              const float* kv_scales, const int32_t* block_tables,
+                              int32_t max_blocks_per_seq, const int32_t* seq_ids,
+                              const int32_t* start_pos, const int32_t* seq_lens,
+                              int32_t* ctr, int32_t B, int32_t C,
+                              int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim,
+                              int32_t block_size, int32_t layer, int32_t capacity,
+                              int32_t max_ctx, float scale, void* workspace,
+                              size_t workspace_bytes, void* stream);
 
 /* The plan of a round's paged_attention_extend calls. The reference calls it
  * once per layer with the same seq_ids / start_positions
@@ -512,6 +568,55 @@ int spv_kv_rotary_append(void* q_out, const void* q, const void* k_new, const vo
                          int32_t interleaved, int32_t layer, int32_t capacity,
                          int32_t block_size, int32_t may_alloc, int32_t follow_plan,
                          int32_t* write_plan, void* stream);
+
+/* spv_rotary of rows that are RMS-normed by head first: row x becomes
+ * x * w / sqrt(mean x^2 + eps), with q_weight / k_weight (head_dim float32 on the
+ * device; NULL: 1) for the query / key heads; fp32 throughout, rounded once after
+ * the rotation. rotary_dim = 0 norms alone. eps >= 0. The model code norms its
+ * query and key heads, where it does, before it rotates them (engine/model.py:174-181). */
+int spv_norm_rotary(void* q_out, const void* q, void* k_out, const void* k, int dtype,
+                    int k_out_dtype, const int64_t* strides, const float* q_weight,
+                    const float* k_weight, float eps, const int32_t* positions,
+                    const double* inv_freq, const int32_t* axis_of, int32_t axes, float factor,
+                    int32_t B, int32_t C, int32_t num_q_heads, int32_t num_kv_heads,
+                    int32_t head_dim, int32_t rotary_dim, int32_t interleaved, void* stream);
+
+/* spv_kv_rotary_append of normed queries and keys (the norm as in spv_norm_rotary). */
+int spv_kv_norm_rotary_append(void* q_out, const void* q, const void* k_new, const void* v_new,
+                              int dtype, const int64_t* strides, const float* q_weight,
+                              const float* k_weight, float eps, void* k_pool, void* v_pool,
+                              int32_t* block_tables, int32_t max_blocks_per_seq,
+                              int32_t* num_blocks, int32_t* seq_lens,
+                              int32_t* free_stack, int32_t* free_flag, int32_t* ctr,
+                              const int32_t* seq_ids, const int32_t* start_pos,
+                              const int32_t* positions, const double* inv_freq,
+                              const int32_t* axis_of, int32_t axes, float factor,
+                              int32_t B, int32_t C, int32_t num_q_heads, int32_t num_kv_heads,
+                              int32_t head_dim, int32_t rotary_dim, int32_t interleaved,
+                              int32_t layer, int32_t capacity, int32_t block_size,
+                              int32_t may_alloc, int32_t follow_plan, int32_t* write_plan,
+                              void* stream);
+
+/* spv_kv_append_fp8_heads (write_limit_b = -1) of a chunk whose keys are rotated --
+ * with normed != 0 normed first -- and quantised unrounded, and whose queries are
+ * rotated into q_out (q may be NULL): k_new, v_new, q and q_out in dtype (f32, bf16,
+ * f16); strides, positions and frequencies as in spv_kv_rotary_append, the norm as
+ * in spv_norm_rotary. B * C <= 2^23. */
+int spv_kv_rotary_append_fp8_heads(void* q_out, const void* q, const void* k_new, const void* v_new,
+                                   int dtype, const int64_t* strides, int32_t normed,
+                                   const float* q_weight, const float* k_weight, float eps,
+                                   void* k_pool, void* v_pool, float* kv_scales,
+                                   int32_t* block_tables, int32_t max_blocks_per_seq,
+                                   int32_t* num_blocks, int32_t* seq_lens,
+                                   int32_t* free_stack, int32_t* free_flag, int32_t* ctr,
+                                   const int32_t* seq_ids, const int32_t* start_pos,
+                                   const int32_t* positions, const double* inv_freq,
+                                   const int32_t* axis_of, int32_t axes, float factor,
+                                   int32_t B, int32_t C, int32_t num_q_heads,
+                                   int32_t num_kv_heads, int32_t head_dim, int32_t rotary_dim,
+                                   int32_t interleaved, int32_t layer, int32_t num_layers,
+                                   int32_t capacity, int32_t block_size, int32_t may_alloc,
+                                   void* stream);
 
 /* -------------------------------------------------------------- sampling */
 

@@ -161,3 +161,51 @@ class Fp8PagedKVCache(PagedKVCache):
         out.k = torch.from_numpy((e4m3_decode(self.k.numpy()) * ks).astype(np.float32))
         out.v = torch.from_numpy((e4m3_decode(self.v.numpy()) * vs).astype(np.float32))
         return out
+
+
+class HeadScaledPagedKVCache(Fp8PagedKVCache):
+    """``Fp8PagedKVCache`` with a scale for each kv head: ``scales`` is
+    ``(layers, kv_heads, cap, 2)``. The rule is the one above, head by head,
+    with ``a`` over the finite values of the chunk's rows; what is not finite is
+    stored as NaN (code 0x7f) and stays NaN under a grown scale."""
+
+    def __init__(self, num_layers: int, num_kv_heads: int, head_dim: int, capacity_blocks: int,
+                 block_size: int) -> None:
+        super().__init__(num_layers, num_kv_heads, head_dim, capacity_blocks, block_size)
+        self.scales = np.zeros((num_layers, num_kv_heads, capacity_blocks, 2), dtype=np.float32)
+
+    def _ensure_blocks_up_to(self, seq_id: int, max_block_index: int) -> None:
+        table = self.block_tables[seq_id]
+        while len(table) <= max_block_index:
+            blk = self.allocator.alloc()
+            self.scales[:, :, blk] = 0.0
+            table.append(blk)
+
+    def _quantize(self, pool: torch.Tensor, kind: int, layer: int, phys: int, lo: int, hi: int,
+                  x: np.ndarray) -> None:
+        codes = pool[layer, phys].numpy()  # (bs, Hkv, d), a view
+        others = [r for r in range(self.block_size) if not lo <= r < hi]
+        for h in range(self.num_kv_heads):
+            rows = x[:, h]
+            finite = np.isfinite(rows)
+            a = np.float32(np.max(np.abs(np.where(finite, rows, np.float32(0.0)))))
+            old = np.float32(self.scales[layer, h, phys, kind])
+            sc = np.float32(max(old, np.float32(a / E4M3_MAX)))
+            if sc > old:
+                was = codes[others, h]
+                vals = (e4m3_decode(was) * old) / sc
+                codes[others, h] = np.where((was & 0x7F) == 0x7F, np.uint8(0x7F), e4m3_encode(vals.astype(np.float32)))
+            new = np.zeros(rows.shape, dtype=np.uint8)
+            if sc > 0:
+                new = e4m3_encode((np.where(finite, rows, np.float32(0.0)) / sc).astype(np.float32))
+            codes[lo:hi, h] = np.where(finite, new, np.uint8(0x7F))
+            self.scales[layer, h, phys, kind] = sc
+
+    def dequantized(self) -> PagedKVCache:
+        out = PagedKVCache(self.num_layers, self.num_kv_heads, self.head_dim, self.allocator.capacity,
+                           self.block_size, dtype=torch.float32)
+        out.load_state(self.block_tables, self.seq_lengths, self.allocator.free_list)
+        ks, vs = (np.swapaxes(self.scales[..., i], 1, 2)[:, :, None, :, None] for i in (0, 1))
+        out.k = torch.from_numpy((e4m3_decode(self.k.numpy()) * ks).astype(np.float32))
+        out.v = torch.from_numpy((e4m3_decode(self.v.numpy()) * vs).astype(np.float32))
+        return out

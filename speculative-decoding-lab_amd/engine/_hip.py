@@ -57,11 +57,13 @@ SIGNATURES = {
     "spv_kv_append_plan": (I, [P, P, I, P, P, P, I, P, P, P, P, P, P, P, I, I, I, I, I, I, I, I, I, P, P]),
     "spv_kv_write_planned": (I, [P, P, I, P, P, P, I, I, I, I, I, I, I, P]),
     "spv_kv_append_fp8": (I, [P, P, P, I, P, P, P, I, P, P, P, P, P, P, P, I, I, I, I, I, I, I, I, I, I, P]),
+    "spv_kv_append_fp8_heads": (I, [P, P, P, I, P, P, P, P, I, P, P, P, P, P, P, P, I, I, I, I, I, I, I, I, I, I, P]),
     "spv_kv_rewind": (I, [P, I, P, P, P, P, P, P, P, P, I, I, I, I, P]),
     "spv_kv_rewind_append": (I, [P, P, I, P, P, P, I, P, P, P, P, P, P, P, P, P, I, I, I, I, I, I, I, P, P]),
     "spv_kv_draft_align": (I, [P, I, P, P, P, P, P, P, I, P, P, P, P, P, I, P, P, P, I, I, I, P]),
     "spv_pool_metrics": (I, [P, P, I, I, P, P, I, P, P, P]),
     "spv_kv_gather": (I, [P, P, I, P, P, I, I, I, I, I, I, I, I, P, P]),
+    "spv_kv_gather_fp8_heads": (I, [P, P, P, P, I, I, I, I, I, I, I, I, P, I, P]),
     "spv_kv_read_blocks": (I, [P, I, I, P, I, I, I, I, I, I, P, P]),
     "spv_verify_attn_workspace_bytes": (S, [I, I, I, I, I, I, I]),
     "spv_verify_attn": (I, [P, P, I, P, P, I, P, P, I, P, P, P, P, I, I, I, I, I, I, I, I, I, F, P, S, P]),
@@ -70,6 +72,8 @@ SIGNATURES = {
     "spv_verify_attn_planned": (I, [P, P, I, P, P, I, P, P, I, P, P, P, P, I, I, I, I, I, I, I, I, I, F, P, P, S, P]),
     "spv_verify_attn_append_planned": (I, [P, P, I, P, P, I, P, I, P, P, P, P, I, I, I, I, I, I, I, I, I, F, P, P, P, P,
                                            P, S, P]),
+    "spv_verify_attn_fp8_heads_workspace_bytes": (S, [I, I, I, I, I, I, I]),
+    "spv_verify_attn_fp8_heads": (I, [P, P, I, P, P, P, P, I, P, P, P, P, I, I, I, I, I, I, I, I, I, F, P, S, P]),
     "spv_prefill_attn": (I, [P, P, P, P, I, P, I, I, I, I, I, F, P]),
     "spv_time_next_attention": (I, [P, P]),
     "spv_verify_attn_static_max_bytes": (S, []),
@@ -80,6 +84,11 @@ SIGNATURES = {
     "spv_rotary": (I, [P, P, P, P, I, I, P, P, P, P, I, F, I, I, I, I, I, I, I, P]),
     "spv_kv_rotary_append": (I, [P, P, P, P, I, P, P, P, P, I, P, P, P, P, P, P, P, P, P, P, I, F, I, I, I, I, I, I,
                                  I, I, I, I, I, I, P, P]),
+    "spv_norm_rotary": (I, [P, P, P, P, I, I, P, P, P, F, P, P, P, I, F, I, I, I, I, I, I, I, P]),
+    "spv_kv_norm_rotary_append": (I, [P, P, P, P, I, P, P, P, F, P, P, P, I, P, P, P, P, P, P, P, P, P, P, I, F, I, I,
+                                      I, I, I, I, I, I, I, I, I, I, P, P]),
+    "spv_kv_rotary_append_fp8_heads": (I, [P, P, P, P, I, P, I, P, P, F, P, P, P, P, I, P, P, P, P, P, P, P, P, P, P, I,
+                                           F, I, I, I, I, I, I, I, I, I, I, I, I, P]),
     "spv_verify_sample_workspace_bytes": (S, [I, I, I]),
     "spv_verify_sample": (I, [P, P, I, F, P, P, P, P, P, P, I, I, I, I, P, P, P, P, P, P, P, I, P, S, P]),
     "spv_verify_sample_filtered_workspace_bytes": (S, [I, I, I, F, I]),

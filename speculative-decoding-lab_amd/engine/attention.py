@@ -40,6 +40,7 @@ from ._hip import call, ptr
 from .kv import PagedKVCache, WritePlan
 
 _workspace = _hip.Workspace()
+_heads_workspace = _hip.Workspace(factor=2)
 
 
 def _expand_to_q_heads(kv: torch.Tensor, num_q_heads: int) -> torch.Tensor:
@@ -48,11 +49,18 @@ def _expand_to_q_heads(kv: torch.Tensor, num_q_heads: int) -> torch.Tensor:
     return kv if ratio == 1 else kv.repeat_interleave(ratio, dim=-2)
 
 
-def gather_ctx(kv: PagedKVCache, layer: int, seq_id: int, length: int) -> torch.Tensor:
+def gather_ctx(kv: PagedKVCache, layer: int, seq_id: int, length: int,
+               dtype: Optional[torch.dtype] = None) -> torch.Tensor:
     """The stored K/V prefix of one sequence, ``(2, length, kv_heads, d)`` (K row 0, V row 1);
-    an fp8 pool's is dequantised to float32 (code * scale of its block)."""
+    an fp8 pool's is dequantised (code * scale of its block, or block and head) to ``dtype``:
+    float32 (the default), bfloat16 or float16."""
     length = int(length)
-    out_dtype = torch.float32 if kv.fp8 else kv.dtype
+    if dtype is not None and (dtype not in (torch.float32, torch.bfloat16, torch.float16) if kv.fp8
+                              else dtype != kv.dtype):
+        raise ValueError("a {} pool is not read as {}".format(kv.dtype, dtype))
+    out_dtype = kv.dtype
+    if kv.fp8:
+        out_dtype = dtype if dtype is not None and kv.head_scales else torch.float32
     out = torch.empty((2, max(length, 0), kv.num_kv_heads, kv.head_dim), dtype=out_dtype,
                       device=kv.device)
     if length <= 0:
@@ -61,10 +69,17 @@ def gather_ctx(kv: PagedKVCache, layer: int, seq_id: int, length: int) -> torch.
     kv._refresh()
     if -(-length // kv.block_size) > kv._nb[seq_id]:
         raise IndexError("length {} exceeds the blocks of sequence {}".format(length, seq_id))
+    if kv.head_scales:
+        if not 0 <= int(layer) < kv.num_layers:
+            raise IndexError("layer {} out of range".format(layer))
+        call("spv_kv_gather_fp8_heads", ptr(kv.k_pool), ptr(kv.v_pool), ptr(kv.scales), ptr(kv.tables_dev),
+             kv.max_blocks_per_seq, seq_id, length, int(layer), kv.allocator.capacity, kv.block_size,
+             kv.num_kv_heads, kv.head_dim, ptr(out), _hip.dtype_code(out_dtype), _hip.stream_of(kv.device))
+        return out
     call("spv_kv_gather", ptr(kv.k_pool), ptr(kv.v_pool), kv._dt, ptr(kv.scales), ptr(kv.tables_dev),
          kv.max_blocks_per_seq, seq_id, length, int(layer), kv.allocator.capacity, kv.block_size,
          kv.num_kv_heads, kv.head_dim, ptr(out), _hip.stream_of(kv.device))
-    return out
+    return out if dtype is None else out.to(dtype)
 
 
 class VerifyPlan:
@@ -76,7 +91,8 @@ class VerifyPlan:
     ``verify_attention`` given it must use exactly those. It also checks, once,
     that every sequence's written length covers its chunk (the per-call check
     of unplanned calls). Valid while the round's start positions and block
-    tables stand.
+    tables stand. Over a cache with head scales every call makes its own split
+    and check; the plan holds the calls to its arguments.
     """
 
     def __init__(self, kv: PagedKVCache, seq_ids: Union[Sequence[int], torch.Tensor],
@@ -89,7 +105,7 @@ class VerifyPlan:
         self.ws_bytes: Optional[int] = None  # the calls' workspace size, asked by the first
         if self.max_ctx > kv.max_blocks_per_seq * kv.block_size:
             kv._grow_width(-(-self.max_ctx // kv.block_size))
-        nbytes = int(_hip.lib().spv_verify_attn_plan_bytes(max(self.B, 1)))
+        nbytes = 0 if kv.head_scales else int(_hip.lib().spv_verify_attn_plan_bytes(max(self.B, 1)))
         if buf is not None and nbytes and (buf.numel() * buf.element_size() < nbytes or buf.device != kv.device):
             raise ValueError("plan buffer too small or on another device")
         # ``buf``: a buffer of an earlier plan to write this one into (no allocation)
@@ -163,6 +179,8 @@ def _attend(query_3d, kv, layer, seq_ids, start_positions, max_ctx, scale, out, 
     if query_3d.device != kv.device:
         raise ValueError("query must live on {}".format(kv.device))
     q = query_3d.contiguous()
+    if kv.head_scales:
+        return _attend_heads(q, kv, layer, seq_ids, start_positions, max_ctx, scale, out, plan)
     if out is None:
         out = torch.empty_like(q)
     if B == 0:
@@ -205,6 +223,54 @@ def _attend(query_3d, kv, layer, seq_ids, start_positions, max_ctx, scale, out, 
         call("spv_verify_attn", *args, ptr(ws), int(ws_bytes), stream)
     # A read of unwritten keys is flagged on the device and raised (IndexError)
     # at the next metadata query, without a synchronisation here.
+    kv._stale = True
+    return out
+
+
+def _attend_heads(q, kv, layer, seq_ids, start_positions, max_ctx, scale, out, plan) -> torch.Tensor:
+    """``verify_attention`` over a cache with head scales; ``q`` contiguous, heads and device checked."""
+    B, chunk, hq, d = q.shape
+    layer, max_ctx = int(layer), int(max_ctx)
+    if not 0 <= layer < kv.num_layers:
+        raise IndexError("layer {} out of range".format(layer))
+    if q.dtype not in (torch.float32, torch.bfloat16, torch.float16):
+        raise ValueError("query must be float32, bfloat16 or float16")
+    if out is None:
+        out = torch.empty_like(q)
+    elif out.shape != q.shape or out.dtype != q.dtype or out.device != q.device or not out.is_contiguous() \
+            or _overlap(out, q):
+        raise ValueError("out must be a contiguous tensor like the query, apart from it")
+    if B == 0 or chunk == 0:
+        return out
+    if max_ctx < chunk:
+        raise ValueError("max_ctx must be at least the chunk")
+    if plan is not None:
+        plan.check(kv, B, chunk, hq, max_ctx)
+        seq_ids, start_positions = plan.seq_ids, plan.start
+    if _hip.ids_ready(seq_ids, B, kv.device) and _hip.ids_ready(start_positions, B, kv.device):
+        sid_t, start_t = seq_ids, start_positions
+    else:
+        if not isinstance(seq_ids, torch.Tensor):
+            seq_ids = [kv._check_sid(s) for s in seq_ids]
+        sid_t, start_t = _hip.i32s(kv.device, seq_ids, start_positions)
+        if sid_t.numel() != B or start_t.numel() != B:
+            raise ValueError("one seq_id and start position per batch row")
+    if max_ctx > kv._maxb * kv.block_size:
+        kv._grow_width(-(-max_ctx // kv.block_size))
+    nbytes = int(_hip.lib().spv_verify_attn_fp8_heads_workspace_bytes(B, chunk, hq, kv.num_kv_heads, d,
+                                                                     kv.block_size, max_ctx))
+    stream = _hip.stream_of(kv.device)
+    ws = None
+    if nbytes:
+        # A captured graph has a workspace of its own, cleared by a node of its own in every
+        # replay: graphs that share one could not run side by side.
+        ws = torch.zeros(nbytes, dtype=torch.uint8, device=kv.device) \
+            if torch.cuda.is_current_stream_capturing() else _heads_workspace.get(nbytes, kv.device, stream)
+    call("spv_verify_attn_fp8_heads", out.data_ptr(), q.data_ptr(), _hip.dtype_code(q.dtype), kv.k_pool.data_ptr(),
+         kv.v_pool.data_ptr(), kv.scales.data_ptr(), kv.tables_dev.data_ptr(), kv._maxb, sid_t.data_ptr(),
+         start_t.data_ptr(), kv.lens_dev.data_ptr(), kv.allocator.ctr.data_ptr(), B, chunk, hq, kv.num_kv_heads, d,
+         kv.block_size, layer, kv.allocator.capacity, max_ctx, 1.0 / math.sqrt(d) if scale is None else float(scale),
+         ptr(ws), nbytes, stream)
     kv._stale = True
     return out
 
@@ -261,6 +327,8 @@ class SharedPrefix:
 
     def __init__(self, kv: PagedKVCache, prefix_ids: Sequence[int], prefix_lens: Sequence[int], chunk: int,
                  num_q_heads: int) -> None:
+        if kv.head_scales:
+            raise ValueError("shared-prefix attention takes fp8 pools of one scale per block, not per head")
         ids, lens = [int(s) for s in prefix_ids], [int(n) for n in prefix_lens]
         if len(ids) != len(lens):
             raise ValueError("one prefix length per prefix id")

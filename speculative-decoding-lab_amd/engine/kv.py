@@ -21,6 +21,7 @@ launches on the current stream; there is no CPU path.
 
 from __future__ import annotations
 
+import ctypes
 from typing import Dict, List, Optional, Sequence
 
 import torch
@@ -145,12 +146,19 @@ class BlockAllocator:
 
 
 class PagedKVCache:
-    """Physical KV pool plus per-sequence device metadata (kv.py:79-224)."""
+    """Physical KV pool plus per-sequence device metadata (kv.py:79-224).
+
+    A ``float8_e4m3fn`` pool holds codes and fp32 scales: one for each (layer,
+    block, K | V), or with ``head_scales`` one for each kv head of it too, so
+    that a head of small keys keeps its precision beside one of large keys.
+    """
 
     def __init__(self, num_layers: int, num_kv_heads: int, head_dim: int,
                  capacity_blocks: int, block_size: int, device: torch.device,
                  dtype: torch.dtype, max_seqs: int = 64,
-                 max_blocks_per_seq: Optional[int] = None) -> None:
+                 max_blocks_per_seq: Optional[int] = None, head_scales: bool = False) -> None:
+        if head_scales and _hip.dtype_code(dtype) != _hip.SPV_FP8E4M3:
+            raise ValueError("head_scales belong to a float8_e4m3fn pool")
         device = _hip.require_gpu(device)
         if num_layers < 1 or num_kv_heads < 1 or head_dim < 1 or block_size < 1:
             raise ValueError("num_layers, num_kv_heads, head_dim and block_size must be >= 1")
@@ -164,8 +172,9 @@ class PagedKVCache:
         self.allocator = BlockAllocator(capacity_blocks, device, dtype)
         cap = self.allocator.capacity
         self.fp8 = self._dt == _hip.SPV_FP8E4M3
+        self.head_scales = bool(head_scales)
         # fp8 pools hold e4m3 codes (zero bytes at start) and one fp32 scale
-        # per (layer, block, K | V).
+        # per (layer, block, K | V), or per (layer, kv head, block, K | V).
         store = torch.uint8 if self.fp8 else dtype
         self.k_pool = torch.zeros((num_layers, cap, num_kv_heads, block_size, head_dim),
                                   dtype=store, device=device)
@@ -174,7 +183,8 @@ class PagedKVCache:
         if self.fp8:
             self.k_pool = self.k_pool.view(dtype)
             self.v_pool = self.v_pool.view(dtype)
-        self.scales = torch.zeros((num_layers, cap, 2), dtype=torch.float32, device=device) if self.fp8 else None
+        shape = (num_layers, num_kv_heads, cap, 2) if self.head_scales else (num_layers, cap, 2)
+        self.scales = torch.zeros(shape, dtype=torch.float32, device=device) if self.fp8 else None
         self._max_seqs = max(1, int(max_seqs))
         self._maxb = int(max_blocks_per_seq) if max_blocks_per_seq else min(cap, 64)
         self.tables_dev = torch.full((self._max_seqs, self._maxb), -1, dtype=torch.int32, device=device)
@@ -363,6 +373,18 @@ class PagedKVCache:
         not take, ignore it.
         """
         B, chunk = int(k_new.shape[0]), int(k_new.shape[1])
+        if self.head_scales:
+            shape = (B, chunk, self.num_kv_heads, self.head_dim)
+            if tuple(k_new.shape) != shape or tuple(v_new.shape) != shape:
+                raise ValueError("k/v must have shape {}".format(shape))
+            if k_new.device != self.device or v_new.device != self.device:
+                raise ValueError("k/v must live on {}".format(self.device))
+            if not 0 <= int(layer) < self.num_layers:
+                raise IndexError("layer {} out of range".format(layer))
+            if not (_hip.ids_ready(seq_ids, B, self.device) and _hip.ids_ready(start_positions, B, self.device)):
+                raise ValueError("seq_ids and start_positions must be {} int32 entries on {}".format(B, self.device))
+            if chunk == 0:
+                return
         if B == 0:
             return
         k_new, v_new = self._new_kv(k_new, v_new)
@@ -401,11 +423,24 @@ class PagedKVCache:
         if self.fp8:
             if k_new.dtype not in (torch.float32, torch.bfloat16, torch.float16) or v_new.dtype != k_new.dtype:
                 raise ValueError("an fp8 pool takes new keys / values in float32, bfloat16 or float16")
+            if self.head_scales:  # any strides, as long as the elements of a head row are contiguous
+                return tuple(t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous() for t in (k_new, v_new))
             return k_new.contiguous(), v_new.contiguous()
         return k_new.to(self.dtype).contiguous(), v_new.to(self.dtype).contiguous()
 
     def _launch_append(self, layer, sid_t, start_t, k_new, v_new, B, chunk, may_alloc, limit) -> None:
         a = self.allocator
+        if self.head_scales:
+            new_dt, strides = 0, None
+            if k_new is not None:
+                new_dt = _hip.dtype_code(k_new.dtype)
+                strides = (ctypes.c_int64 * 6)(*k_new.stride()[:3], *v_new.stride()[:3])
+            call("spv_kv_append_fp8_heads", ptr(self.k_pool), ptr(self.v_pool), ptr(self.scales), new_dt, ptr(k_new),
+                 ptr(v_new), strides, ptr(self.tables_dev), self._maxb, ptr(self.nblocks_dev), ptr(self.lens_dev),
+                 ptr(a.free_stack), ptr(a.free_flag), ptr(a.ctr), ptr(sid_t), ptr(start_t), B, chunk, int(layer),
+                 self.num_layers, a.capacity, self.block_size, self.num_kv_heads, self.head_dim, may_alloc, limit,
+                 self._stream())
+            return
         if self.fp8:
             new_dt = _hip.dtype_code(k_new.dtype) if k_new is not None else 0
             call("spv_kv_append_fp8", ptr(self.k_pool), ptr(self.v_pool), ptr(self.scales), new_dt, ptr(k_new),
@@ -559,7 +594,7 @@ class PagedKVCache:
         self.allocator.epoch += 1
         call("spv_kv_draft_align", ptr(self.tables_dev), self._maxb, ptr(self.nblocks_dev), ptr(self.lens_dev),
              ptr(self.allocator.free_stack), ptr(self.allocator.free_flag), ptr(self.allocator.ctr), ptr(self.scales),
-             self.num_layers, ptr(seq_ids), ptr(start_pos), ptr(n_commit), ptr(finished), ptr(chunk_tokens), C,
+             self.num_layers * (self.num_kv_heads if self.head_scales else 1), ptr(seq_ids), ptr(start_pos), ptr(n_commit), ptr(finished), ptr(chunk_tokens), C,
              ptr(catch_n), ptr(catch_pos), ptr(catch_tok), n, self.allocator.capacity, self.block_size,
              self._stream())
         self._stale = True

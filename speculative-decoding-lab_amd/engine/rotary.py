@@ -8,6 +8,9 @@ before it writes the keys (184-187) and attends. Here:
 * ``rotary_append`` -- ``PagedKVCache.write_block_device`` of a chunk whose keys
   are rotated on the way, the queries in the same launch.
 
+Both take a ``HeadNorm``: the RMS norm of every query and key head in the same
+pass, before the rotation (``rotary_dim`` 0 norms alone).
+
 Queries, keys and values may be views of one fused projection's output: any
 strides, as long as the elements of a head row are contiguous.
 
@@ -134,6 +137,53 @@ class Rotary:
         return positions.to(torch.int32).contiguous()
 
 
+class HeadNorm:
+    """The RMS norm of a model's query and key heads, on the device.
+
+    A head row ``x`` of ``head_dim`` elements becomes ``x * w / sqrt(mean(x ** 2)
+    + eps)``, with ``query_weight`` for the query heads and ``key_weight`` for
+    the key heads (``head_dim`` values each; None: 1), computed in float32. The
+    caller keeps this object as long as a captured graph that used it may replay.
+    """
+
+    def __init__(self, head_dim: int, device: torch.device, query_weight: Optional[torch.Tensor] = None,
+                 key_weight: Optional[torch.Tensor] = None, eps: float = 1e-6) -> None:
+        self.head_dim, self.eps = int(head_dim), float(eps)
+        if self.head_dim < 1:
+            raise ValueError("head_dim must be >= 1")
+        if not 0.0 <= self.eps < 1e30:
+            raise ValueError("eps must be >= 0")
+        given = []
+        for w in (query_weight, key_weight):
+            if w is not None:
+                w = torch.as_tensor(w)
+                if tuple(w.shape) != (self.head_dim,) or not w.is_floating_point():
+                    raise ValueError("a norm's weight must be {} floating-point values".format(self.head_dim))
+            given.append(w)
+        self.device = _hip.require_gpu(device)
+        # copies: a later change of the caller's tensor is not seen, and both live on this stream
+        self._weights = [None if w is None else w.detach().to(self.device, torch.float32, copy=True).contiguous()
+                         for w in given]
+        self._made_on = _hip.stream_of(self.device)
+
+    @property
+    def query_weight(self) -> Optional[torch.Tensor]:
+        """The query heads' weights, ``head_dim`` float32 on the device, or None."""
+        return self._weights[0]
+
+    @property
+    def key_weight(self) -> Optional[torch.Tensor]:
+        """The key heads' weights, ``head_dim`` float32 on the device, or None."""
+        return self._weights[1]
+
+    def _args(self, rotary: Rotary, stream: int) -> tuple:
+        """The launch arguments of a call on ``stream`` with ``rotary``."""
+        if self.head_dim != rotary.head_dim or self.device != rotary.device:
+            raise ValueError("the norm is for heads of {} on {}".format(self.head_dim, self.device))
+        _hip.kept_for(stream, self._made_on, *(w for w in self._weights if w is not None))
+        return ptr(self._weights[0]), ptr(self._weights[1]), self.eps
+
+
 def _span(t: torch.Tensor) -> Tuple[int, int]:
     """First and one-past-last byte that a view with non-negative strides reaches."""
     last = sum((n - 1) * s for n, s in zip(t.shape, t.stride()))
@@ -199,8 +249,9 @@ def _like(t: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
 
 def rotary_embed(query: torch.Tensor, key: Optional[torch.Tensor], rotary: Rotary, positions: torch.Tensor,
                  query_out: Optional[torch.Tensor] = None, key_out: Optional[torch.Tensor] = None,
-                 key_dtype: Optional[torch.dtype] = None) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
-    """``(query, key)`` rotated, in one launch.
+                 key_dtype: Optional[torch.dtype] = None,
+                 norm: Optional[HeadNorm] = None) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
+    """``(query, key)`` rotated, in one launch; with ``norm`` every head normed before that.
 
     ``query`` (B, C, Hq, d) and ``key`` (B, C, Hkv, d, or None) in float32,
     bfloat16 or float16; ``positions`` an integer device tensor (B, C), or
@@ -228,9 +279,10 @@ def rotary_embed(query: torch.Tensor, key: Optional[torch.Tensor], rotary: Rotar
         return query_out, key_out
     if strides is None:
         strides = _strides(query_out, query, key_out, key)
-    call("spv_rotary", query_out.data_ptr(), query.data_ptr(), ptr(key_out), ptr(key), code, key_code, strides,
-         pos.data_ptr(), *rotary._args(), B, C, hq, hkv, d, rotary.rotary_dim, rotary.interleaved,
-         rotary._stream())
+    stream = rotary._stream()
+    call("spv_rotary" if norm is None else "spv_norm_rotary", query_out.data_ptr(), query.data_ptr(), ptr(key_out),
+         ptr(key), code, key_code, strides, *(() if norm is None else norm._args(rotary, stream)), pos.data_ptr(),
+         *rotary._args(), B, C, hq, hkv, d, rotary.rotary_dim, rotary.interleaved, stream)
     return query_out, key_out
 
 
@@ -274,16 +326,19 @@ def rotary_append(query: Optional[torch.Tensor], k_new: torch.Tensor, v_new: tor
                   layer: int, seq_ids: Union[Sequence[int], torch.Tensor],
                   start_positions: Union[Sequence[int], torch.Tensor], rotary: Rotary,
                   positions: Optional[torch.Tensor] = None, alloc: bool = True, plan: Optional[WritePlan] = None,
-                  query_out: Optional[torch.Tensor] = None) -> Optional[torch.Tensor]:
+                  query_out: Optional[torch.Tensor] = None,
+                  norm: Optional[HeadNorm] = None) -> Optional[torch.Tensor]:
     """Write a chunk's rotated keys and its values into the cache; returns the rotated queries.
+    With ``norm`` every query and key head is normed first.
 
     ``kv.write_block_device(layer, seq_ids, start_positions, rotated k_new,
     v_new, alloc, plan)`` with the same rules of allocation, exhaustion and
     write plans, and ``query`` (B, C, Hq, d, or None) rotated in the same launch.
     ``k_new`` / ``v_new`` (B, C, Hkv, d) and ``query`` share the pool's dtype
     (an fp8 pool: one of float32, bfloat16, float16; the rotated keys are
-    quantised unrounded). fp8 pools, and pools of 2^31 token rows or more, are
-    written in a launch behind the rotation's and ignore ``plan``.
+    quantised unrounded). fp8 pools of one scale per block, and pools of 2^31 token
+    rows or more, are written in a launch behind the rotation's; they and fp8 pools
+    with head scales (one launch) ignore ``plan``.
     ``positions``: as in ``rotary_embed``; None takes the pool positions
     ``start_positions[b] + j``. No host synchronisation with device tensors of
     distinct, added ``seq_ids``. A later layer's call of a round passes
@@ -320,10 +375,24 @@ def rotary_append(query: Optional[torch.Tensor], k_new: torch.Tensor, v_new: tor
     if B == 0 or C == 0:
         return query_out
     a = kv.allocator
+    stream = rotary._stream()
+    normed = () if norm is None else norm._args(rotary, stream)
+    if strides is None:
+        strides = _strides(query_out, q, k, v)
+    if kv.head_scales:
+        kp, vp, *tables = kv._addresses()
+        call("spv_kv_rotary_append_fp8_heads", ptr(query_out), ptr(q), k.data_ptr(), v.data_ptr(),
+             _hip.dtype_code(k.dtype), strides, norm is not None, *(normed or (None, None, 0.0)), kp, vp,
+             kv.scales.data_ptr(), *tables, sid_t.data_ptr(), start_t.data_ptr(), ptr(pos), *rotary._args(), B, C, hq,
+             kv.num_kv_heads, kv.head_dim, rotary.rotary_dim, rotary.interleaved, layer, kv.num_layers, a.capacity,
+             kv.block_size, bool(alloc), stream)
+        kv._stale = True
+        a._stale = True
+        return query_out
     if kv.fp8 or a.capacity * kv.block_size >= 2 ** 31:
         if pos is None:
             pos = start_t.view(B, 1) + torch.arange(C, dtype=torch.int32, device=kv.device)
-        _append_apart(q, k, v, kv, layer, sid_t, start_t, rotary, pos, alloc, query_out)
+        _append_apart(q, k, v, kv, layer, sid_t, start_t, rotary, pos, alloc, query_out, normed)
         return query_out
     rows, follow = None, 0
     if plan is not None:
@@ -333,11 +402,10 @@ def rotary_append(query: Optional[torch.Tensor], k_new: torch.Tensor, v_new: tor
         elif plan.ready:
             plan._check(a.epoch, B, C, sid_t, start_t)
             rows, follow = plan.rows, 1
-    call("spv_kv_rotary_append", ptr(query_out), ptr(q), k.data_ptr(), v.data_ptr(), kv._dt,
-         _strides(query_out, q, k, v) if strides is None else strides, *kv._addresses(), sid_t.data_ptr(),
-         start_t.data_ptr(), ptr(pos), *rotary._args(), B, C, hq, kv.num_kv_heads, kv.head_dim, rotary.rotary_dim,
-         rotary.interleaved, layer, a.capacity, kv.block_size, bool(alloc), follow, ptr(rows),
-         rotary._stream())
+    call("spv_kv_norm_rotary_append" if normed else "spv_kv_rotary_append", ptr(query_out), ptr(q), k.data_ptr(),
+         v.data_ptr(), kv._dt, strides, *normed, *kv._addresses(), sid_t.data_ptr(), start_t.data_ptr(), ptr(pos),
+         *rotary._args(), B, C, hq, kv.num_kv_heads, kv.head_dim, rotary.rotary_dim, rotary.interleaved, layer,
+         a.capacity, kv.block_size, bool(alloc), follow, ptr(rows), stream)
     if not follow:
         if rows is not None:
             plan._record(a.epoch, sid_t, start_t)
@@ -399,14 +467,15 @@ def _append_ids(kv, seq_ids, start_positions, B, C):
     return sid_t, start_t
 
 
-def _append_apart(q, k, v, kv, layer, sid_t, start_t, rotary, pos, alloc, query_out) -> None:
+def _append_apart(q, k, v, kv, layer, sid_t, start_t, rotary, pos, alloc, query_out, normed) -> None:
     """The rotated keys by themselves, then the append of both: an fp8 pool's, which quantises
     (from float32, so that a key is rounded once), and that of a pool of 2^31 token rows or
     more (the one launch counts rows in 32 bits)."""
     dtype = torch.float32 if kv.fp8 else k.dtype
     turned = torch.empty(k.shape, dtype=dtype, device=k.device)
-    call("spv_rotary", ptr(query_out), ptr(q), ptr(turned), ptr(k), _hip.dtype_code(k.dtype), _hip.dtype_code(dtype),
-         _strides(query_out, q, turned, k), ptr(pos), *rotary._args(), k.shape[0], k.shape[1],
+    call("spv_norm_rotary" if normed else "spv_rotary", ptr(query_out), ptr(q), ptr(turned), ptr(k),
+         _hip.dtype_code(k.dtype), _hip.dtype_code(dtype), _strides(query_out, q, turned, k), *normed, ptr(pos),
+         *rotary._args(), k.shape[0], k.shape[1],
          0 if q is None else int(q.shape[2]), kv.num_kv_heads, kv.head_dim, rotary.rotary_dim,
          rotary.interleaved, rotary._stream())
     kv.write_block_device(layer, sid_t, start_t, turned, v.to(dtype), alloc=alloc)

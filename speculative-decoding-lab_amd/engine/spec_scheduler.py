@@ -351,8 +351,9 @@ class VerifyStep:
         plan = None
         for layer in range(len(q_layers)):
             mark()
-            kl = k_layers[layer].to(self.kv.dtype).contiguous()
-            vl = v_layers[layer].to(self.kv.dtype).contiguous()
+            kl, vl = k_layers[layer], v_layers[layer]
+            if not self.kv.fp8:  # an fp8 pool quantises them as they are
+                kl, vl = kl.to(self.kv.dtype).contiguous(), vl.to(self.kv.dtype).contiguous()
             o = None if outs is None else outs[layer]
             if plan is not None and events is None:
                 # a later layer: its append and attention in one launch (timed
