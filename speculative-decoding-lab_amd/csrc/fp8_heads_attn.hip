@@ -108,17 +108,20 @@ __global__ __launch_bounds__(64 * kAnyRows) void head_attn_any_kernel(HeadAttn p
 //
 // Head dims 64 and 128, blocks of whole 16-token units. A workgroup of 8 waves
 // takes a piece: rows R = 16 RT of one kv head of one entry (all of them, for
-// verify chunks) times a range of steps of SK keys, its waves every eighth step.
+// verify chunks) times a range of steps of 64 keys, its waves every eighth step.
+// Pages go from HBM to LDS by themselves (loads with an LDS destination), 16 KB
+// ahead per wave, and each wave waits for its own; no barrier while it walks.
 // Everything stays transposed, so that no value changes lanes between the two
 // products:
 //   S^T = K Q^T: A = 16 keys x 32 dims, codes converted exactly (every e4m3 value
-//     is a bf16 and an fp16 value) as they arrive from HBM, B = 16 rows, from LDS.
-//     Lane (g, c) = (lane / 16, lane % 16) gets keys 4 g + i of each tile for row c.
-//     The key that row r of tile t stands for is chosen, KG (r / 4) + 4 t + r % 4 of
-//     the step, so that a lane's keys are KG = SK / 4 neighbours of one unit: one
-//     block, one pair of scales.
-//   O^T += V^T P^T: A = 16 dims x 32 keys, a lane's KG neighbours one 8- or 16-byte
-//     load of a V^T row, B = the lane's own weights.
+//     is a bf16 and an fp16 value), B = 16 rows. Lane (g, c) = (lane / 16,
+//     lane % 16) gets keys 4 g + i of each of the four tiles for row c. The key that
+//     row r of tile t stands for is chosen, token 4 t + r % 4 of unit r / 4 of the
+//     step, so that a lane's 16 keys are unit g: one block, one pair of scales.
+//   O^T += V^T P^T: A = 16 dims x 32 keys, a lane's keys 8 bytes of a V^T row, B = the
+//     lane's own weights.
+// K's 16-byte pieces lie in LDS in an order (an exclusive or of a piece's number with
+// its row's and unit's) that puts the 16 rows of an operand on different banks.
 // The block's K scale multiplies the scores, its V scale the weights. The maximum of
 // a row is raised (and O rescaled) only where a step passes it by more than 2^8.
 // Roundings: scores, sums and O are fp32. A weight meets V in NP parts of bf16, 8
@@ -131,17 +134,19 @@ typedef float f32x4_t __attribute__((ext_vector_type(4)));
 
 constexpr int kWaves = 8, kTileThreads = 64 * kWaves;
 constexpr int kGrid = 256;       // one workgroup per CU
+constexpr int kStep = 64;        // keys of a step: four units
 constexpr int kMinSteps = 8;     // a piece has a step for each wave, where contexts are cut
 constexpr float kLift = 8.f;     // log2 by which a step may pass the row's maximum
 constexpr float kLowest = -3.402823466e38f;
-constexpr int kCols = 32, kColPad = 4;  // dims of a combine pass
+constexpr int kStage = 16384;    // LDS bytes of pages per wave: one step ahead at head_dim 128, two at 64
 
 struct HeadPlan {  // host-chosen shape of a tiled call
-  int RT, RG, SK, D, upb, equal;  // row tiles, row groups, keys of a step, units per block, pieces of equal length
-  unsigned upb_magic;             // floor(2^32 / upb) + 1
-  int aligned;                    // q and out on 16-byte addresses
-  int* counters;                  // kGrid: arrivals of a segment's parts
-  float* part;                    // slots of R x D sums and R x (maximum, sum)
+  int RT, RG, rpg, D, upb, equal;  // row tiles, row groups, rows of one, head_dim, units per block, pieces of equal length
+  int pair;                   // two row groups, walked side by side by workgroups 8 apart
+  unsigned upb_magic;         // floor(2^32 / upb) + 1
+  int aligned;                // q and out on 16-byte addresses
+  int* counters;              // kGrid: arrivals of a segment's parts
+  float* part;                // slots of R x D sums and R x (maximum, sum)
 };
 
 template <int QT>
@@ -170,91 +175,141 @@ __device__ __forceinline__ f32x4_t mfma(u32x4_t a, u32x4_t b, f32x4_t c) {
   else
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b), c, 0, 0, 0);
 }
+// The high bit of every byte of w that is a NaN code.
+__device__ __forceinline__ uint32_t nan_codes(uint32_t w) { return ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u; }
 __device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
   return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2_t{a, b}, bf16x2_t));
 }
 
-// Keys that the rows of group rg of entry b see, and steps of them (one at least).
-__device__ __forceinline__ int group_keys(const HeadAttn& p, int R, int start, int rg) {
-  const int last = min(p.C - 1, (rg * R + R - 1) / p.ratio);
+// 16 bytes per lane from memory to LDS: lane l's go to `to` + 16 l; OFF moves both ends.
+template <int OFF>
+__device__ __forceinline__ void page_to_lds(const uint8_t* from, uint8_t* to) {
+  __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)from,
+                                   (__attribute__((address_space(3))) void*)to, 16, OFF, 0);
+}
+template <int N>
+__device__ __forceinline__ void wait_loads() {  // all but the newest N vector memory operations of the wave
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
+// Four 16-byte pieces from LDS, STEP bytes apart: read in assembly, whose wait is its own, for the compiler would wait
+// for every load to LDS before a read of it.
+template <int O, int STEP>
+__device__ __forceinline__ void lds_read4(u32x4_t (&w)[4], uint32_t a) {
+  asm volatile(
+      "ds_read_b128 %0, %4 offset:%5\n\tds_read_b128 %1, %4 offset:%6\n\t"
+      "ds_read_b128 %2, %4 offset:%7\n\tds_read_b128 %3, %4 offset:%8\n\ts_waitcnt lgkmcnt(0)"
+      : "=&v"(w[0]), "=&v"(w[1]), "=&v"(w[2]), "=&v"(w[3])
+      : "v"(a), "n"(O), "n"(O + STEP), "n"(O + 2 * STEP), "n"(O + 3 * STEP)
+      : "memory");
+}
+
+// Keys that the rows of group rg of an entry see (a pair's groups are walked as far as the second sees), and steps of
+// them (one at least).
+__device__ __forceinline__ int group_keys(const HeadAttn& p, const HeadPlan& pl, int start, int rg) {
+  const int last = pl.pair ? p.C - 1 : min(p.C - 1, (rg * pl.rpg + pl.rpg - 1) / p.ratio);
   return min(start + last + 1, p.max_ctx);
 }
-template <int SK>
-__device__ __forceinline__ int group_steps(const HeadAttn& p, int R, int start, int rg) {
-  return max(1, (group_keys(p, R, start, rg) + SK - 1) / SK);
+__device__ __forceinline__ int group_steps(const HeadAttn& p, const HeadPlan& pl, int start, int rg) {
+  return max(1, (group_keys(p, pl, start, rg) + kStep - 1) / kStep);
 }
 
-template <int QT, int D, int RT, int SK>
+template <int QT, int D, int RT>
 __global__ __launch_bounds__(kTileThreads, 2) void head_attn_tile_kernel(HeadAttn p, HeadPlan pl) {
   constexpr bool F16 = QT == SPV_F16;
-  constexpr int NQ = Parts<QT>::Q, NP = Parts<QT>::P, R = RT * 16, NCH = D / 32, NDT = D / 16, KT = SK / 16,
-                KG = SK / 4, NM = KG / 8;
-  constexpr int kQBytes = RT * NCH * NQ * 1024, kCombineBytes = kWaves * R * (kCols + kColPad) * 4;
-  constexpr bool kQReg = RT * NCH * NQ <= 8;  // queries in registers, where they are few
-  __shared__ __align__(16) uint8_t s_buf[kQBytes > kCombineBytes ? kQBytes : kCombineBytes];
+  constexpr int NQ = Parts<QT>::Q, NP = Parts<QT>::P, R = RT * 16, NCH = D / 32, NDT = D / 16;
+  constexpr int kUnit = 16 * D, kHalf = 4 * kUnit, NS = kStage / (2 * kHalf);  // bytes of a unit, of a step's K or V; steps ahead
+  constexpr int NK = kHalf / 1024;                                           // loads of a step's K, or V
+  constexpr int kCols = 8 * R * (D + 4) * 4 <= 8 * kStage ? D : 8 * R * (64 + 4) * 4 <= 8 * kStage && D > 64 ? 64 : 32, kColPad = 4;
+  constexpr bool kQReg = RT * NCH * NQ <= 4;  // queries in registers, where they are few
+  __shared__ __align__(1024) uint8_t s_page[kWaves * kStage];  // [wave][stage][K | V]; the waves' sums later
+  __shared__ __align__(16) u32x4_t s_q[NQ * RT * NCH * 64];
   __shared__ float s_ml[2][kWaves][R];
   __shared__ float s_row[2][R];  // joined maximum and sum
-  __shared__ int s_scan[kWaves], s_find[2], s_last;
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15;
+  __shared__ int s_nan[D];       // first key whose value is NaN in a dim, where rows end
+  __shared__ int s_last;
+  // A pair's workgroups are on one XCD (its L2 has the pages for the second): half 0 and 1 of a worker.
+  const int worker = pl.pair ? (int)(blockIdx.x >> 4) * 8 + (int)(blockIdx.x & 7) : (int)blockIdx.x;
+  const int half = pl.pair ? (int)(blockIdx.x >> 3) & 1 : 0, workers = pl.pair ? kGrid / 2 : kGrid;
+  const int counted = pl.pair ? 1 : pl.RG;  // row groups that count for themselves
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15;
 
-  // ---- which piece: a number of steps (equal = 0: shares of all steps in a row) or of pieces per entry
-  const int cpt = (p.B + kTileThreads - 1) / kTileThreads;  // entries of a thread
-  const int b0 = min((int)threadIdx.x * cpt, p.B), b1 = min(b0 + cpt, p.B);
-  auto per_entry = [&](int start, int P) {  // steps of an entry, or pieces of at most P of them
+  // ---- which piece: the waves work it out alike, each lane for epl entries (the first two kept). Steps of an entry,
+  // or pieces of at most P steps; equal = 0: shares of all steps in a row.
+  const int epl = (p.B + 63) >> 6, b0 = min(lane * epl, p.B), b1 = min(b0 + epl, p.B);
+  int st[2], id[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int b = min(b0 + i, p.B - 1);
+    st[i] = p.start[b];
+    id[i] = p.seq_ids[b];
+  }
+  auto count = [&](int start, int P) {
     int n = 0;
-    for (int rg = 0; rg < pl.RG; ++rg) {
-      const int k = group_steps<SK>(p, R, start, rg);
+    for (int rg = 0; rg < counted; ++rg) {
+      const int k = group_steps(p, pl, start, rg);
       n += P ? (k + P - 1) / P : k;
     }
     return n * p.Hkv;
   };
-  int mine = 0;
-  for (int b = b0; b < b1; ++b) {
-    const int start = p.start[b];
-    mine += per_entry(start, 0);
-    if (blockIdx.x == 0) {
-      const int sid = p.seq_ids[b];
-      if (start < 0 || start + p.C > p.max_ctx || (p.lens && start + p.C > p.lens[sid])) flag_read(p, b);
-    }
-  }
-  int total, before = block_exclusive_scan(mine, s_scan, &total);
-  int P = (total + kGrid - 1) / kGrid;
-  if (P < kMinSteps) P = kMinSteps;
+  int v0 = 0, mine = 0;  // of the lane's first entry, of all its entries
+  auto count_mine = [&](int P) {
+    v0 = b0 < b1 ? count(st[0], P) : 0;
+    mine = v0 + (b0 + 1 < b1 ? count(st[1], P) : 0);
+    for (int b = b0 + 2; b < b1; ++b) mine += count(p.start[b], P);
+    return wave_incl_sum(mine);
+  };
+  int upto = count_mine(0), total = lane63(upto);
+  int P = max((total + workers - 1) / workers, kMinSteps);
   if (pl.equal) {
-    while (true) {  // ends: with P the longest context, one piece per segment, of at most kGrid / 2 segments
-      mine = 0;
-      for (int b = b0; b < b1; ++b) mine += per_entry(p.start[b], P);
-      before = block_exclusive_scan(mine, s_scan, &total);
-      if (total <= kGrid) break;
+    while (true) {  // ends: with P the longest context, one piece per segment, and those are at most half the workers
+      upto = count_mine(P);
+      total = lane63(upto);
+      if (total <= workers) break;
       P += max(1, P >> 4);
     }
   }
-  const int x0 = pl.equal ? (int)blockIdx.x : (int)blockIdx.x * P;
+  const int x0 = pl.equal ? worker : worker * P;
   const int x1 = min(total, pl.equal ? x0 + 1 : x0 + P);
+  if (blockIdx.x == kGrid - 1 && wave == 0) {
+    for (int b = b0; b < b1; ++b) {
+      const int start = p.start[b];
+      if (start < 0 || start + p.C > p.max_ctx || (p.lens && start + p.C > p.lens[p.seq_ids[b]])) flag_read(p, b);
+    }
+  }
 
   for (int cur = x0; cur < x1;) {
-    __syncthreads();
-    if (before <= cur && cur < before + mine) {
-      int at = before;
-      for (int b = b0; b < b1; ++b) {
-        const int n = per_entry(p.start[b], pl.equal ? P : 0);
-        if (cur < at + n) {
-          s_find[0] = b;
-          s_find[1] = cur - at;
+    if (cur != x0) __syncthreads();
+    const int owner = __ffsll((unsigned long long)__ballot(upto > cur)) - 1;
+    int off = cur - __builtin_amdgcn_readlane(upto - mine, owner), b = owner * epl, start, sid;
+    if (epl <= 2) {
+      const int first = __builtin_amdgcn_readlane(v0, owner);
+      const bool second = off >= first;
+      if (second) off -= first;
+      b += second;
+      start = __builtin_amdgcn_readlane(second ? st[1] : st[0], owner);
+      sid = __builtin_amdgcn_readlane(second ? id[1] : id[0], owner);
+    } else {  // the owner's entries, 64 at a time
+      for (int e0 = 0;; e0 += 64) {
+        const bool in = e0 + lane < epl && b + lane < p.B;
+        const int s1 = p.start[min(b + lane, p.B - 1)], n = in ? count(s1, pl.equal ? P : 0) : 0;
+        const int sum = wave_incl_sum(n);
+        if (off < lane63(sum)) {
+          const int at = __ffsll((unsigned long long)__ballot(sum > off)) - 1;
+          off -= __builtin_amdgcn_readlane(sum - n, at);
+          b += at;
+          start = __builtin_amdgcn_readlane(s1, at);
           break;
         }
-        at += n;
+        off -= lane63(sum);
+        b += 64;
       }
+      sid = p.seq_ids[b];
     }
-    __syncthreads();
-    const int b = __builtin_amdgcn_readfirstlane(s_find[0]);
-    int off = __builtin_amdgcn_readfirstlane(s_find[1]);
-    const int start = p.start[b], sid = p.seq_ids[b];
     int rg = 0, n = 0, k = 0;
     for (;; ++rg) {
-      n = group_steps<SK>(p, R, start, rg);
+      n = group_steps(p, pl, start, rg);
       k = pl.equal ? (n + P - 1) / P : n;
-      if (off < k * p.Hkv || rg == pl.RG - 1) break;
+      if (off < k * p.Hkv || rg == counted - 1) break;
       off -= k * p.Hkv;
     }
     const int h = off / k, i_in = off - h * k;
@@ -269,87 +324,92 @@ __global__ __launch_bounds__(kTileThreads, 2) void head_attn_tile_kernel(HeadAtt
     } else {
       first = i_in;
       last = min(n, i_in + x1 - cur);
-      const int s0 = cur - i_in;  // the segment's first step among all
-      slot0 = s0;
-      nparts = (s0 + n - 1) / P - s0 / P + 1;
-      my = (int)blockIdx.x - s0 / P;
+      slot0 = cur - i_in;  // the segment's first step among all
+      nparts = (slot0 + n - 1) / P - slot0 / P + 1;
+      my = worker - slot0 / P;
       cur += last - first;
     }
-    // Slot of part i: its workgroup's first or second one (a share's first piece, or its last).
+    if (pl.pair) rg = half;
+    // Slot of part i: its worker's first or second one (a share's first piece, or its last).
     auto slot_of = [&](int i) {
-      if (pl.equal) return slot0 + i;
-      const int wg = slot0 / P + i;
-      return wg * P >= slot0 ? 2 * wg : 2 * wg + 1;
+      const int w = pl.equal ? slot0 + i : slot0 / P + i;
+      return 2 * (half * workers + w) + (!pl.equal && w * P < slot0);
     };
-    const int keys = group_keys(p, R, start, rg), units = max(1, (keys + 15) >> 4);
-    const int rows = min(R, p.C * p.ratio - rg * R);
+    const int keys = group_keys(p, pl, start, rg), units = max(1, (keys + 15) >> 4);
+    const int row0 = rg * pl.rpg, rows = min(pl.rpg, p.C * p.ratio - row0);
     const int32_t* const table = p.tables + (size_t)sid * p.maxb;
-    const size_t page_bytes = (size_t)p.bs * D;
+    const size_t page_bytes = (size_t)p.bs * D, block_bytes = page_bytes * p.Hkv;
     const uint8_t* const kbase = p.kpool + ((size_t)p.layer * p.cap * p.Hkv + h) * page_bytes;
     const uint8_t* const vbase = p.vpool + ((size_t)p.layer * p.cap * p.Hkv + h) * page_bytes;
     const float* const sbase = p.scales + ((size_t)p.layer * p.Hkv + h) * p.cap * 2;
-    const size_t block_bytes = page_bytes * p.Hkv;
 
-    // ---- addresses of a step: the unit of the lane's K rows (of c) and of its own keys (of g)
-    auto unit_at = [&](int step, int grp) { return min((step * SK + grp * KG) >> 4, units - 1); };
-    auto block_id = [&](int u) {
+    // ---- the wave's pages. Lane i holds what unit i % 4 of step i / 4 of its next 16 steps needs: where it lies and
+    // its scales.
+    const int steps = last - first > wave ? (last - first - wave + kWaves - 1) / kWaves : 0;  // of this wave
+    auto step_at = [&](int k) { return first + wave + k * kWaves; };
+    int l_block = 0, l_tok = 0;
+    float2 l_scale = {0.f, 0.f};
+    auto look_up = [&](int k) {  // for steps k .. k + 15
+      const int u = min(step_at(k + (lane >> 2)) * 4 + (lane & 3), units - 1);
       const int blk = pl.upb == 1 ? u : (int)__umulhi((unsigned)u, pl.upb_magic);
-      return table[min(blk, p.maxb - 1)];
+      l_tok = (u - blk * pl.upb) * 16;
+      l_block = table[min(blk, p.maxb - 1)];
+      if ((unsigned)l_block >= (unsigned)p.cap) {
+        if (lane >> 2 < steps - k) flag_read(p, b);
+        l_block = 0;
+      }
+      l_scale = *reinterpret_cast<const float2*>(sbase + (size_t)l_block * 2);
     };
-    auto safe = [&](int id) {
-      if ((unsigned)id < (unsigned)p.cap) return id;
-      flag_read(p, b);
-      return 0;
-    };
-    auto in_block = [&](int u) { return pl.upb == 1 ? 0 : (u - (int)__umulhi((unsigned)u, pl.upb_magic) * pl.upb) * 16; };
-    auto kaddr = [&](int step, int id) {
-      const int u = unit_at(step, c >> 2);
-      const int tok = in_block(u) + (((step * SK + (c >> 2) * KG) & 15) + (c & 3));
-      return kbase + (size_t)id * block_bytes + (size_t)(tok * D + 16 * g);
-    };
-    auto vaddr = [&](int step, int id) {
-      const int u = unit_at(step, g);
-      const int tok = in_block(u) + ((step * SK + g * KG) & 15);
-      return vbase + (size_t)id * block_bytes + (size_t)(c * p.bs + tok);
-    };
-    u32x4_t kraw[KT][D / 64];
-    uint32_t vraw[NDT][KG / 4];
-    float2 sc;
-    auto load_k = [&](const uint8_t* at, int t, int cc) {
-      kraw[t][cc] = *reinterpret_cast<const u32x4_t*>(at + 4 * t * D + 64 * cc);
-    };
-    auto load_v = [&](const uint8_t* at, int dt) {
-      if constexpr (KG == 16) {
-        const u32x4_t w = *reinterpret_cast<const u32x4_t*>(at + (size_t)(dt * 16) * p.bs);
+    uint8_t* const stage0 = s_page + wave * kStage;
+    // Lane offsets of a K load (row, piece: exclusive or with 32 u for unit u) and of a V load (row).
+    const int krow = D == 128 ? lane >> 3 : lane >> 2;
+    const uint32_t kvoff = D == 128 ? krow * 128 + (((lane & 7) ^ ((krow >> 1) & 1)) * 16) : krow * 64 + (lane & 3) * 16;
+    const uint32_t vvoff = (uint32_t)lane * (uint32_t)p.bs;
+    float2 sc[NS];  // scales of the lane's keys of the next steps
+    auto fetch_k = [&](int k) {
+      if ((k & 15) == 0) look_up(k);
+      uint8_t* const to = stage0 + (k % NS) * 2 * kHalf;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) vraw[dt][i] = w[i];
-      } else {
-        const u32x2_t w = *reinterpret_cast<const u32x2_t*>(at + (size_t)(dt * 16) * p.bs);
-        vraw[dt][0] = w[0];
-        vraw[dt][1] = w[1];
+      for (int u = 0; u < 4; ++u) {
+        const int at = (k & 15) * 4 + u;
+        const uint8_t* const from = kbase + (size_t)(unsigned)__builtin_amdgcn_readlane(l_block, at) * block_bytes +
+                                    (size_t)__builtin_amdgcn_readlane(l_tok, at) * D;
+        const uint32_t lo = kvoff ^ (D == 128 ? u * 32 : u * 16);
+        page_to_lds<0>(from + lo, to + u * kUnit);
+        if constexpr (D == 128) page_to_lds<1024>(from + lo, to + u * kUnit);
+      }
+      const int at = (k & 15) * 4 + g;
+#pragma unroll
+      for (int i = 0; i + 1 < NS; ++i) sc[i] = sc[i + 1];
+      sc[NS - 1] = make_float2(__shfl(l_scale.x, at, 64), __shfl(l_scale.y, at, 64));
+    };
+    auto fetch_v = [&](int k) {
+      uint8_t* const to = stage0 + (k % NS) * 2 * kHalf + kHalf;
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const int at = (k & 15) * 4 + u;
+        const uint8_t* const from = vbase + (size_t)(unsigned)__builtin_amdgcn_readlane(l_block, at) * block_bytes +
+                                    (size_t)__builtin_amdgcn_readlane(l_tok, at);
+        page_to_lds<0>(from + vvoff, to + u * kUnit);
+        if constexpr (D == 128) page_to_lds<0>(from + (size_t)64 * p.bs + vvoff, to + u * kUnit + 1024);
       }
     };
-    auto load_scales = [&](int id) { sc = *reinterpret_cast<const float2*>(sbase + (size_t)id * 2); };
-    int step = first + wave;
-    int kid = 0, vid = 0;  // of the step after
-    if (step < last) {
-      const int k0 = block_id(unit_at(step, c >> 2)), v0 = block_id(unit_at(step, g));
-      kid = block_id(unit_at(step + kWaves, c >> 2));
-      vid = block_id(unit_at(step + kWaves, g));
-      const uint8_t* const ka = kaddr(step, safe(k0));
-      const uint8_t* const va = vaddr(step, safe(v0));
 #pragma unroll
-      for (int cc = 0; cc < D / 64; ++cc)
+    for (int i = 0; i < NS; ++i) sc[i] = make_float2(0.f, 0.f);
 #pragma unroll
-        for (int t = 0; t < KT; ++t) load_k(ka, t, cc);
-      load_scales(safe(v0));
-#pragma unroll
-      for (int dt = 0; dt < NDT; ++dt) load_v(va, dt);
+    for (int i = 0; i < NS; ++i) {
+      if (i < steps) {
+        fetch_k(i);
+        fetch_v(i);
+      } else if (i) {
+        sc[NS - 2 < 0 ? 0 : NS - 2] = sc[NS - 1];  // one step: its scales come first
+      }
     }
 
-    // ---- queries to LDS as operands: [part][row tile][chunk][lane] 16 bytes; dims of a chunk as K's bytes arrive
+    // ---- queries to LDS as operands: [part][row tile][chunk][lane] 16 bytes; dims of a chunk as K's pieces go
+    if ((int)threadIdx.x < D) s_nan[threadIdx.x] = 0x7fffffff;
     for (int i = threadIdx.x; i < R * (D / 8); i += kTileThreads) {
-      const int row = i / (D / 8), piece = i - row * (D / 8), r = rg * R + row;
+      const int row = i / (D / 8), piece = i - row * (D / 8), r = row0 + row;
       float x[8];
       if (row < rows) {
         const int j = r / p.ratio, hq = h * p.ratio + r - j * p.ratio;
@@ -389,13 +449,11 @@ __global__ __launch_bounds__(kTileThreads, 2) void head_attn_tile_kernel(HeadAtt
             x[2 * e + 1] -= __uint_as_float(w[e] & 0xffff0000u);
           }
         }
-        reinterpret_cast<u32x4_t*>(s_buf)[((q * RT + (row >> 4)) * NCH + ch) * 64 + ln] = w;
+        s_q[((q * RT + (row >> 4)) * NCH + ch) * 64 + ln] = w;
       }
     }
     __syncthreads();
-    auto query = [&](int rt, int ch, int q) {
-      return reinterpret_cast<const u32x4_t*>(s_buf)[((q * RT + rt) * NCH + ch) * 64 + lane];
-    };
+    auto query = [&](int rt, int ch, int q) { return s_q[((q * RT + rt) * NCH + ch) * 64 + lane]; };
     u32x4_t qreg[kQReg ? RT : 1][kQReg ? NCH : 1][kQReg ? NQ : 1];
     if constexpr (kQReg) {
 #pragma unroll
@@ -413,179 +471,178 @@ __global__ __launch_bounds__(kTileThreads, 2) void head_attn_tile_kernel(HeadAtt
     for (int rt = 0; rt < RT; ++rt) {
       m[rt] = kLowest;
       l[rt] = 0.f;
-      seen[rt] = min(start + min((rg * R + rt * 16 + c) / p.ratio, p.C - 1) + 1, p.max_ctx);
+      seen[rt] = min(start + min((row0 + rt * 16 + c) / p.ratio, p.C - 1) + 1, p.max_ctx);
 #pragma unroll
       for (int dt = 0; dt < NDT; ++dt) o[rt][dt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
     }
-    const int all_see = min(start + rg * R / p.ratio + 1, p.max_ctx);  // keys that every row attends
+    const int all_see = min(start + row0 / p.ratio + 1, p.max_ctx);  // keys that every row attends
     const float factor = fabsf(p.scale_log2);
+    // LDS addresses of the lane's operand bytes: K row c % 4 of unit c / 4, piece g; V row c of unit g.
+    const uint32_t base0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)stage0;
+    const uint32_t kat = base0 + (c >> 2) * kUnit + (c & 3) * D +
+                         ((g ^ (D == 128 ? ((c >> 1) & 1) | (c >> 2) << 1 : c >> 2)) * 16);
+    const uint32_t vat = base0 + kHalf + g * kUnit + c * 16;
 
-    auto run_step = [&](auto more_tag) {
-      constexpr bool MORE = decltype(more_tag)::value;
-      const bool masked = (step + 1) * SK > all_see;
-      const float ksc = sc.x * factor, vsc = sc.y;
-      const uint8_t *ka = nullptr, *va = nullptr;
-      int vnext = 0;
-      if constexpr (MORE) {
-        ka = kaddr(step + kWaves, safe(kid));
-        vnext = safe(vid);
-        va = vaddr(step + kWaves, vnext);
-        kid = block_id(unit_at(step + 2 * kWaves, c >> 2));
-        vid = block_id(unit_at(step + 2 * kWaves, g));
-      }
-      f32x4_t s[RT][KT];
+    auto run_step = [&](int k, auto more_tag) {
+      constexpr bool MORE = decltype(more_tag)::value;  // step k + NS exists
+      const int step = step_at(k);
+      const uint32_t at = (k % NS) * 2 * kHalf;
+      const bool masked = (step + 1) * kStep > all_see;
+      const float ksc = sc[0].x * factor, vsc = sc[0].y;
+      const int base = step * kStep + g * 16;  // the lane's first key
+      // Weights with V's scale in them as a power, w = 2^(z + log2 s_v - m), where no key is masked and the
+      // scales allow it; their sum is theirs over s_v. Elsewhere, and for fp32 queries, one after the other.
+      const bool plain = QT == SPV_F32 || masked || __any(!(vsc > 0x1p-60f && vsc < 0x1p60f));
+      const float vlog = __builtin_amdgcn_logf(vsc), vinv = __builtin_amdgcn_rcpf(vsc);
+      auto lift = [&](int rt, float top) {
+        top = fmaxf(top, __shfl_xor(top, 16, 64));
+        top = fmaxf(top, __shfl_xor(top, 32, 64));
+        const float mn = fmaxf(m[rt], top), keep = __builtin_amdgcn_exp2f(m[rt] - mn);
+        m[rt] = mn;
+        l[rt] *= keep;
+#pragma unroll
+        for (int dt = 0; dt < NDT; ++dt) o[rt][dt] *= keep;
+      };
+      // K of this step is there: behind it came its V, and what was fetched ahead.
+      if constexpr (MORE && NS > 1) wait_loads<(NS - 1) * 2 * NK + NK>();
+      else if (NS > 1 && k + 1 < steps) wait_loads<2 * NK + NK>();
+      else wait_loads<NK>();
+      f32x4_t s[RT][4];
 #pragma unroll
       for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
-        for (int t = 0; t < KT; ++t) s[rt][t] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+        for (int t = 0; t < 4; ++t) s[rt][t] = f32x4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int ch = 0; ch < NCH; ++ch) {
-        u32x4_t qv[RT][NQ];
+      for (int cc = 0; cc < D / 64; ++cc) {
+        u32x4_t kw[4];
+        lds_read4<0, 4 * D>(kw, (at + kat) ^ (cc * 64));
 #pragma unroll
-        for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-          for (int q = 0; q < NQ; ++q) {
-            if constexpr (kQReg) qv[rt][q] = qreg[rt][ch][q];
-            else qv[rt][q] = query(rt, ch, q);
-          }
-#pragma unroll
-        for (int t = 0; t < KT; ++t) {
-          const u32x4_t kop = operand<F16>(kraw[t][ch / 2][2 * (ch & 1)], kraw[t][ch / 2][2 * (ch & 1) + 1]);
+        for (int half = 0; half < 2; ++half) {
+          const int ch = 2 * cc + half;
+          u32x4_t qv[RT][NQ];
 #pragma unroll
           for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
-            for (int q = NQ - 1; q >= 0; --q) s[rt][t] = mfma<F16>(kop, qv[rt][q], s[rt][t]);
-        }
-        if constexpr (MORE) {
-          if (ch & 1) {
+            for (int q = 0; q < NQ; ++q) {
+              if constexpr (kQReg) qv[rt][q] = qreg[rt][ch][q];
+              else qv[rt][q] = query(rt, ch, q);
+            }
 #pragma unroll
-            for (int t = 0; t < KT; ++t) load_k(ka, t, ch / 2);
+          for (int t = 0; t < 4; ++t) {
+            const u32x4_t kop = operand<F16>(kw[t][2 * half], kw[t][2 * half + 1]);
+#pragma unroll
+            for (int q = NQ - 1; q >= 0; --q)
+#pragma unroll
+              for (int rt = 0; rt < RT; ++rt) s[rt][t] = mfma<F16>(kop, qv[rt][q], s[rt][t]);
           }
+          if constexpr (RT > 2) __builtin_amdgcn_sched_barrier(0);
         }
       }
-      if constexpr (MORE) load_scales(vnext);
-      const int base = step * SK + g * KG;  // the lane's first key
-      uint32_t pw[RT][NM][NP][4];
+      if constexpr (MORE) fetch_k(k + NS);
+      else if constexpr (NS > 1) sc[0] = sc[NS - 1];
+      uint32_t pw[RT][2][NP][4];
 #pragma unroll
       for (int rt = 0; rt < RT; ++rt) {
-        float z[KT][4], top = -INFINITY;
+        if (!plain) {
+          float top = s[rt][0][0];
 #pragma unroll
-        for (int t = 0; t < KT; ++t)
+          for (int i = 1; i < 16; ++i) top = fmaxf(top, s[rt][i >> 2][i & 3]);
+          top *= ksc;
+          if (__any(top > m[rt] + kLift)) lift(rt, top);
+          const float off = vlog - m[rt];
+          float sum = 0.f;
 #pragma unroll
-          for (int i = 0; i < 4; ++i) z[t][i] = s[rt][t][i] * ksc;
-        if (masked) {
+          for (int i = 0; i < 16; ++i) {
+            const float w = __builtin_amdgcn_exp2f(fmaf(s[rt][i >> 2][i & 3], ksc, off));
+            s[rt][i >> 2][i & 3] = w;
+            sum += w;
+          }
+          l[rt] = fmaf(sum, vinv, l[rt]);
+        } else {
+          float top = -INFINITY;
 #pragma unroll
-          for (int t = 0; t < KT; ++t)
+          for (int i = 0; i < 16; ++i) {
+            const float z = base + i < seen[rt] ? s[rt][i >> 2][i & 3] * ksc : -INFINITY;
+            s[rt][i >> 2][i & 3] = z;
+            top = fmaxf(top, z);
+          }
+          if (__any(top > m[rt] + kLift)) lift(rt, top);
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-              if (base + 4 * t + i >= seen[rt]) z[t][i] = -INFINITY;
+          for (int i = 0; i < 16; ++i) {
+            const float e = __builtin_amdgcn_exp2f(s[rt][i >> 2][i & 3] - m[rt]);
+            l[rt] += e;
+            s[rt][i >> 2][i & 3] = e * vsc;
+          }
         }
 #pragma unroll
-        for (int t = 0; t < KT; ++t)
+        for (int q = 0; q < NP; ++q)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) top = fmaxf(top, z[t][i]);
-        if (__any(top > m[rt] + kLift)) {
-          top = fmaxf(top, __shfl_xor(top, 16, 64));
-          top = fmaxf(top, __shfl_xor(top, 32, 64));
-          const float mn = fmaxf(m[rt], top), keep = __builtin_amdgcn_exp2f(m[rt] - mn);
-          m[rt] = mn;
-          l[rt] *= keep;
+          for (int i = 0; i < 8; ++i) {
+            const float x = s[rt][i >> 1][2 * (i & 1)], y = s[rt][i >> 1][2 * (i & 1) + 1];
+            const uint32_t u = pack_bf16(x, y);
+            pw[rt][i >> 2][q][i & 3] = u;
+            if (q + 1 < NP) {
+              s[rt][i >> 1][2 * (i & 1)] = x - __uint_as_float(u << 16);
+              s[rt][i >> 1][2 * (i & 1) + 1] = y - __uint_as_float(u & 0xffff0000u);
+            }
+          }
+        if constexpr (RT > 2) __builtin_amdgcn_sched_barrier(0);
+      }
+      // V of this step is there: behind it came what was fetched ahead, and K of step k + NS.
+      if constexpr (MORE) wait_loads<(NS - 1) * 2 * NK + NK>();
+      else if (NS > 1 && k + 1 < steps) wait_loads<2 * NK>();
+      else wait_loads<0>();
 #pragma unroll
-          for (int dt = 0; dt < NDT; ++dt) o[rt][dt] *= keep;
-        }
-#pragma unroll
-        for (int t = 0; t < KT; ++t) {
+      for (int d4 = 0; d4 < NDT / 4; ++d4) {
+        u32x4_t vw[4];
+        if (d4 == 0) lds_read4<0, 256>(vw, at + vat);
+        else lds_read4<1024, 256>(vw, at + vat);
+        if (masked) {  // values behind the rows' last key are not looked at
+          const int valid = keys - base;
+          uint32_t bad = 0;
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            const float e = __builtin_amdgcn_exp2f(z[t][i] - m[rt]);
-            l[rt] += e;
-            z[t][i] = e * vsc;
-          }
-#pragma unroll
-          for (int q = 0; q < NP; ++q)
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-              const uint32_t w = pack_bf16(z[t][2 * i], z[t][2 * i + 1]);
-              pw[rt][t / 2][q][2 * (t & 1) + i] = w;
-              if (q + 1 < NP) {
-                z[t][2 * i] -= __uint_as_float(w << 16);
-                z[t][2 * i + 1] -= __uint_as_float(w & 0xffff0000u);
-              }
-            }
-        }
-      }
-      if (masked) {  // values behind the rows' last key are not looked at
-        const int valid = keys - base;
-#pragma unroll
-        for (int dt = 0; dt < NDT; ++dt)
-#pragma unroll
-          for (int i = 0; i < KG / 4; ++i) {
             const int nb = min(max(valid - 4 * i, 0), 4);
-            vraw[dt][i] &= nb == 4 ? 0xffffffffu : (1u << (8 * nb)) - 1u;
+            const uint32_t in = nb == 4 ? 0xffffffffu : (1u << (8 * nb)) - 1u;
+#pragma unroll
+            for (int dt = 0; dt < 4; ++dt) {
+              vw[dt][i] &= in;
+              bad |= nan_codes(vw[dt][i]);
+            }
           }
-        // A NaN among the chunk's own values reaches the rows that see it, and no other.
-        uint32_t bad = 0;
+          // A NaN among the chunk's own values reaches the rows that see it, and no other: it is taken out here, and
+          // what remembers it is the first key of each dim that holds one.
+          if (__any(bad != 0)) {
 #pragma unroll
-        for (int dt = 0; dt < NDT; ++dt)
-#pragma unroll
-          for (int i = 0; i < KG / 4; ++i) bad |= ((vraw[dt][i] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
-        if (__any(bad != 0)) {
-#pragma unroll
-          for (int rt = 0; rt < RT; ++rt) {
-            u32x4_t sees[NM];
-#pragma unroll
-            for (int mm = 0; mm < NM; ++mm)
+            for (int dt = 0; dt < 4; ++dt)
 #pragma unroll
               for (int i = 0; i < 4; ++i) {
-                const int key = base + 8 * mm + 2 * i;
-                sees[mm][i] = (key < seen[rt] ? 0x3f80u : 0u) | (key + 1 < seen[rt] ? 0x3f800000u : 0u);
+                const uint32_t w = nan_codes(vw[dt][i]);
+                if (w) atomicMin(&s_nan[(4 * d4 + dt) * 16 + c], base + 4 * i + (__ffs(w) >> 3) - 1);
+                vw[dt][i] &= ~((w >> 7) * 0xffu);
               }
-#pragma unroll
-            for (int dt = 0; dt < NDT; ++dt) {
-              f32x4_t count = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-              for (int mm = 0; mm < NM; ++mm) {
-                u32x4_t is;
-#pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                  const uint32_t w = ((vraw[dt][2 * mm + i] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
-                  is[2 * i] = (w & 0x80u ? 0x3f80u : 0u) | (w & 0x8000u ? 0x3f800000u : 0u);
-                  is[2 * i + 1] = (w & 0x800000u ? 0x3f80u : 0u) | (w & 0x80000000u ? 0x3f800000u : 0u);
-                }
-                count = mfma<false>(is, sees[mm], count);
-              }
-#pragma unroll
-              for (int i = 0; i < 4; ++i)
-                if (count[i] > 0.f) o[rt][dt][i] = __uint_as_float(0x7fc00000u);
-            }
           }
-#pragma unroll
-          for (int dt = 0; dt < NDT; ++dt)
-#pragma unroll
-            for (int i = 0; i < KG / 4; ++i) {
-              const uint32_t w = ((vraw[dt][i] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;  // NaN bytes
-              vraw[dt][i] &= ~((w >> 7) * 0xffu);
-            }
         }
-      }
 #pragma unroll
-      for (int dt = 0; dt < NDT; ++dt) {
-        u32x4_t vop[NM];
+        for (int dt = 0; dt < 4; ++dt) {
 #pragma unroll
-        for (int mm = 0; mm < NM; ++mm) vop[mm] = operand<false>(vraw[dt][2 * mm], vraw[dt][2 * mm + 1]);
-        if constexpr (MORE) load_v(va, dt);
-#pragma unroll
-        for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-          for (int mm = 0; mm < NM; ++mm)
+          for (int mm = 0; mm < 2; ++mm) {
+            const u32x4_t vop = operand<false>(vw[dt][2 * mm], vw[dt][2 * mm + 1]);
 #pragma unroll
             for (int q = NP - 1; q >= 0; --q)
-              o[rt][dt] = mfma<false>(vop[mm], u32x4_t{pw[rt][mm][q][0], pw[rt][mm][q][1], pw[rt][mm][q][2], pw[rt][mm][q][3]},
-                                      o[rt][dt]);
+#pragma unroll
+              for (int rt = 0; rt < RT; ++rt)
+                o[rt][4 * d4 + dt] = mfma<false>(
+                    vop, u32x4_t{pw[rt][mm][q][0], pw[rt][mm][q][1], pw[rt][mm][q][2], pw[rt][mm][q][3]}, o[rt][4 * d4 + dt]);
+          }
+          if constexpr (RT > 2) __builtin_amdgcn_sched_barrier(0);
+        }
       }
+      if constexpr (MORE) fetch_v(k + NS);
     };
-    for (; step + kWaves < last; step += kWaves) run_step(std::true_type{});
-    if (step < last) run_step(std::false_type{});
+    int k_step = 0;
+    for (; k_step + NS < steps; ++k_step) run_step(k_step, std::true_type{});
+    for (; k_step < steps; ++k_step) run_step(k_step, std::false_type{});
 
     // ---- the waves' sums, joined in their order
 #pragma unroll
@@ -598,24 +655,28 @@ __global__ __launch_bounds__(kTileThreads, 2) void head_attn_tile_kernel(HeadAtt
       }
     }
     __syncthreads();
-    if ((int)threadIdx.x < R) {
-      float mx = kLowest, sum = 0.f;
+    float keep[RT];
 #pragma unroll
-      for (int w = 0; w < kWaves; ++w) mx = fmaxf(mx, s_ml[0][w][threadIdx.x]);
+    for (int rt = 0; rt < RT; ++rt) {
+      float mx = kLowest;
 #pragma unroll
-      for (int w = 0; w < kWaves; ++w)
-        sum = fmaf(s_ml[1][w][threadIdx.x], __builtin_amdgcn_exp2f(s_ml[0][w][threadIdx.x] - mx), sum);
-      s_row[0][threadIdx.x] = mx;
-      s_row[1][threadIdx.x] = sum;
+      for (int w = 0; w < kWaves; ++w) mx = fmaxf(mx, s_ml[0][w][rt * 16 + c]);
+      keep[rt] = __builtin_amdgcn_exp2f(m[rt] - mx);
+      if (wave == 0 && g == 0) {
+        float sum = 0.f;
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w)
+          sum = fmaf(s_ml[1][w][rt * 16 + c], __builtin_amdgcn_exp2f(s_ml[0][w][rt * 16 + c] - mx), sum);
+        s_row[0][rt * 16 + c] = mx;
+        s_row[1][rt * 16 + c] = sum;
+      }
     }
-    __syncthreads();
     const bool whole = nparts == 1;
     constexpr size_t kSlot = (size_t)R * (D + 2);  // floats of a slot
-    float* const slot = pl.part + (whole ? 0 : (size_t)slot_of(my) * kSlot);
-    const __amdgpu_buffer_rsrc_t slot_rsrc = coherent_rsrc(slot);
+    const __amdgpu_buffer_rsrc_t slot_rsrc = coherent_rsrc(pl.part + (whole ? 0 : (size_t)slot_of(my) * kSlot));
     // Four dims of a row, normalised, to the output.
     auto put = [&](int row, int e, f32x4_t v, float sum) {
-      const int r = rg * R + row, j = r / p.ratio, hq = h * p.ratio + r - j * p.ratio;
+      const int r = row0 + row, j = r / p.ratio, hq = h * p.ratio + r - j * p.ratio;
       const float inv = min(start + j + 1, p.max_ctx) > 0 ? 1.f / sum : 0.f;
       const size_t at = (((size_t)b * p.C + j) * p.Hq + hq) * D + e;
       if (!pl.aligned) {
@@ -634,10 +695,7 @@ __global__ __launch_bounds__(kTileThreads, 2) void head_attn_tile_kernel(HeadAtt
         *reinterpret_cast<u32x2_t*>(static_cast<uint16_t*>(p.out) + at) = w;
       }
     };
-    float* const s_o = reinterpret_cast<float*>(s_buf);  // [wave][row][kCols + pad]
-    float keep[RT];
-#pragma unroll
-    for (int rt = 0; rt < RT; ++rt) keep[rt] = __builtin_amdgcn_exp2f(m[rt] - s_row[0][rt * 16 + c]);
+    float* const s_o = reinterpret_cast<float*>(s_page);  // [wave][row][kCols + pad]
 #pragma unroll
     for (int pass = 0; pass < D / kCols; ++pass) {
       if (pass) __syncthreads();
@@ -654,6 +712,10 @@ __global__ __launch_bounds__(kTileThreads, 2) void head_attn_tile_kernel(HeadAtt
 #pragma unroll
         for (int w = 0; w < kWaves; ++w)
           sum += *reinterpret_cast<const f32x4_t*>(s_o + (w * R + row) * (kCols + kColPad) + e);
+        const int sees = min(start + (row0 + row) / p.ratio + 1, p.max_ctx);
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (s_nan[pass * kCols + e + j] < sees) sum[j] = __uint_as_float(0x7fc00000u);
         if (whole) put(row, pass * kCols + e, sum, s_row[1][row]);
         else store_coherent_b128(slot_rsrc, ((size_t)row * D + pass * kCols + e) * 4, __builtin_bit_cast(u32x4_t, sum));
       }
@@ -663,34 +725,48 @@ __global__ __launch_bounds__(kTileThreads, 2) void head_attn_tile_kernel(HeadAtt
       store_coherent_b64(slot_rsrc, ((size_t)R * D + threadIdx.x * 2) * 4,
                          u32x2_t{__float_as_uint(s_row[0][threadIdx.x]), __float_as_uint(s_row[1][threadIdx.x])});
     // Counted at the workgroup in which the segment begins: it begins one segment at most that others go on with.
-    if (!arrive_last(pl.counters + (pl.equal ? slot0 : slot0 / P), nparts, &s_last)) continue;
+    if (!arrive_last(pl.counters + half * workers + (pl.equal ? slot0 : slot0 / P), nparts, &s_last)) continue;
 
-    // ---- the segment's last workgroup joins its parts, in their order
-    for (int i = threadIdx.x; i < rows * (D / 4); i += kTileThreads) {
-      const int row = i / (D / 4), e = (i - row * (D / 4)) * 4;
-      float mx = kLowest, sum = 0.f;
-      f32x4_t acc = {0.f, 0.f, 0.f, 0.f};
-      constexpr int kAt = 8;  // parts in flight
-      for (int q0 = 0; q0 < nparts; q0 += kAt) {
-        u32x4_t v[kAt];
-        u32x2_t ml[kAt];
+    // ---- the segment's last workgroup joins its parts, in their order: kAt parts of all the thread's pieces in flight
+    constexpr int kItems = (R * (D / 4) + kTileThreads - 1) / kTileThreads, kAt = 4;
+    f32x4_t acc[kItems];
+    float mx[kItems], sums[kItems];
 #pragma unroll
-        for (int q = 0; q < kAt; ++q) {
-          const __amdgpu_buffer_rsrc_t r = coherent_rsrc(pl.part + (size_t)slot_of(min(q0 + q, nparts - 1)) * kSlot);
-          v[q] = load_coherent_b128(r, ((size_t)row * D + e) * 4);
-          ml[q] = load_coherent_b64(r, ((size_t)R * D + row * 2) * 4);
-        }
+    for (int i = 0; i < kItems; ++i) {
+      acc[i] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+      mx[i] = kLowest;
+      sums[i] = 0.f;
+    }
+    for (int q0 = 0; q0 < nparts; q0 += kAt) {
+      u32x4_t v[kAt][kItems];
+      u32x2_t ml[kAt][kItems];
 #pragma unroll
-        for (int q = 0; q < kAt; ++q) {
-          if (q0 + q >= nparts) break;
-          const float mq = __uint_as_float(ml[q][0]), mn = fmaxf(mx, mq);
-          const float was = __builtin_amdgcn_exp2f(mx - mn), is = __builtin_amdgcn_exp2f(mq - mn);
-          mx = mn;
-          sum = fmaf(__uint_as_float(ml[q][1]), is, sum * was);
-          acc = acc * was + __builtin_bit_cast(f32x4_t, v[q]) * is;
+      for (int q = 0; q < kAt; ++q) {
+        const __amdgpu_buffer_rsrc_t r = coherent_rsrc(pl.part + (size_t)slot_of(min(q0 + q, nparts - 1)) * kSlot);
+#pragma unroll
+        for (int i = 0; i < kItems; ++i) {
+          const int row = min((int)threadIdx.x + i * kTileThreads, R * (D / 4) - 1) / (D / 4);
+          v[q][i] = load_coherent_b128(r, (size_t)min((int)threadIdx.x + i * kTileThreads, R * (D / 4) - 1) * 16);
+          ml[q][i] = load_coherent_b64(r, ((size_t)R * D + row * 2) * 4);
         }
       }
-      put(row, e, acc, sum);
+#pragma unroll
+      for (int q = 0; q < kAt; ++q) {
+        if (q0 + q >= nparts) break;
+#pragma unroll
+        for (int i = 0; i < kItems; ++i) {
+          const float mq = __uint_as_float(ml[q][i][0]), mn = fmaxf(mx[i], mq);
+          const float was = __builtin_amdgcn_exp2f(mx[i] - mn), is = __builtin_amdgcn_exp2f(mq - mn);
+          mx[i] = mn;
+          sums[i] = fmaf(__uint_as_float(ml[q][i][1]), is, sums[i] * was);
+          acc[i] = acc[i] * was + __builtin_bit_cast(f32x4_t, v[q][i]) * is;
+        }
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < kItems; ++i) {
+      const int at = threadIdx.x + i * kTileThreads, row = at / (D / 4);
+      if (row < rows) put(row, (at - row * (D / 4)) * 4, acc[i], sums[i]);
     }
   }
 }
@@ -702,14 +778,15 @@ bool tile_plan(int32_t B, int32_t C, int32_t Hq, int32_t Hkv, int32_t d, int32_t
   const long long rows = (long long)C * ratio;
   if (rows > 0x3fffffffLL) return false;
   pl.D = d;
-  pl.RG = (int)((rows + 63) / 64);
-  pl.RT = (int)(((rows + pl.RG - 1) / pl.RG + 15) / 16);
-  pl.SK = d == 128 && pl.RT > 2 ? 32 : 64;
+  pl.RG = (int)((rows + 31) / 32);
+  pl.rpg = (int)((rows + pl.RG - 1) / pl.RG);
+  pl.RT = (pl.rpg + 15) / 16;
+  pl.pair = pl.RG == 2;
   pl.upb = bs / 16;
   pl.upb_magic = (unsigned)(0x100000000ULL / (unsigned)pl.upb + 1);
-  const long long segs = (long long)B * pl.RG * Hkv, steps = ((long long)max_ctx + pl.SK - 1) / pl.SK;
+  const long long segs = (long long)B * (pl.pair ? 1 : pl.RG) * Hkv, steps = ((long long)max_ctx + kStep - 1) / kStep;
   if (segs * steps > 0x3fffffffLL || ((long long)max_ctx / 16 + 1) * pl.upb > 0x7fffffffLL) return false;
-  pl.equal = segs * 2 <= kGrid;
+  pl.equal = segs * 2 <= (pl.pair ? kGrid / 2 : kGrid);
   return true;
 }
 
@@ -720,13 +797,9 @@ size_t tile_bytes(const HeadPlan& pl) {
 
 template <int QT, int D>
 void launch_tile(const HeadAttn& p, const HeadPlan& pl, hipStream_t s) {
-#define SPV_T(RT, SK) \
-  hipLaunchKernelGGL((head_attn_tile_kernel<QT, D, RT, SK>), dim3(kGrid), dim3(kTileThreads), 0, s, p, pl)
-  constexpr int kBig = D == 128 ? 32 : 64;
-  if (pl.RT == 1) SPV_T(1, 64);
-  else if (pl.RT == 2) SPV_T(2, 64);
-  else if (pl.RT == 3) SPV_T(3, kBig);
-  else SPV_T(4, kBig);
+#define SPV_T(RT) hipLaunchKernelGGL((head_attn_tile_kernel<QT, D, RT>), dim3(kGrid), dim3(kTileThreads), 0, s, p, pl)
+  if (pl.RT == 1) SPV_T(1);
+  else SPV_T(2);
 #undef SPV_T
 }
 
