@@ -123,10 +123,18 @@ __global__ __launch_bounds__(64 * kAnyRows) void head_attn_any_kernel(HeadAttn p
 // K's 16-byte pieces lie in LDS in an order (an exclusive or of a piece's number with
 // its row's and unit's) that puts the 16 rows of an operand on different banks.
 // The block's K scale multiplies the scores, its V scale the weights. The maximum of
-// a row is raised (and O rescaled) only where a step passes it by more than 2^8.
-// Roundings: scores, sums and O are fp32. A weight meets V in NP parts of bf16, 8
-// bits each and of fp32's range (V's scale may be of any size): two for 16-bit
-// queries (2^-17), three for fp32 ones. fp32 queries enter S in three parts.
+// a row is raised (and O rescaled) only where a step passes it by more than 2^8 (2^3
+// for bf16 queries).
+// Roundings: scores, sums and O are fp32. A weight meets V in 16 bits:
+//   bf16 queries: one part of fp16 (2^-12, an eighth of the output's own rounding),
+//     shifted up by 2^11 with V's scale in [1, 2); the scale's power of two goes into
+//     V's conversion, against a unit of O's that follows the largest. The second part
+//     of bf16 that this saves costs 4 us of 54 at 16 contexts of 32,768 keys. Weights
+//     below 2^-25 of the row's largest lose bits, 2^-36 of it each.
+//   fp16 queries: two parts of bf16 (2^-17), 8 bits each and of fp32's range.
+//   fp32 queries: three parts, and three of each query, in S.
+// Steps with masked keys, or with scales too far apart for that, take the parts of
+// bf16 (V's scale may be of any size there).
 
 typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
@@ -136,7 +144,10 @@ constexpr int kWaves = 8, kTileThreads = 64 * kWaves;
 constexpr int kGrid = 256;       // one workgroup per CU
 constexpr int kStep = 64;        // keys of a step: four units
 constexpr int kMinSteps = 8;     // a piece has a step for each wave, where contexts are cut
-constexpr float kLift = 8.f;     // log2 by which a step may pass the row's maximum
+// What a segment costs beside its steps (look-ups, queries, the join of the waves), in steps, where shares of many
+// segments are cut: 128 entries of 32 to 8,192 keys take 91 us with it, 140 without (the slowest workgroup had the
+// most segments).
+constexpr int kHead = 24;
 constexpr float kLowest = -3.402823466e38f;
 constexpr int kStage = 16384;    // LDS bytes of pages per wave: one step ahead at head_dim 128, two at 64
 
@@ -152,20 +163,25 @@ struct HeadPlan {  // host-chosen shape of a tiled call
 template <int QT>
 struct Parts {
   static constexpr int Q = QT == SPV_F32 ? 3 : 1, P = QT == SPV_F32 ? 3 : 2;
+  static constexpr bool half = QT == SPV_BF16;     // weights in one part of fp16
+  static constexpr float lift = half ? 3.f : 8.f;  // log2 by which a step may pass the row's maximum
 };
+constexpr int kHalfShift = 11;  // weights in fp16 are shifted by it: up to 2^3 * 2 * 2^11, bits lost below 2^-25
 
 template <bool HI>
 __device__ __forceinline__ uint32_t to_bf16x2(uint32_t w) {
   return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.f, HI));
 }
 template <bool HI>
-__device__ __forceinline__ uint32_t to_f16x2(uint32_t w) {
-  return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.f, HI));
+__device__ __forceinline__ uint32_t to_f16x2(uint32_t w, float power) {
+  return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, power, HI));
 }
-// Eight codes as an operand.
+// Eight codes as an operand; in fp16 times a power of two from 2^-15 to 2^7, exactly (448 * 2^7 < 65504, and every
+// product is a multiple of 2^-24).
 template <bool F16>
-__device__ __forceinline__ u32x4_t operand(uint32_t a, uint32_t b) {
-  if constexpr (F16) return u32x4_t{to_f16x2<false>(a), to_f16x2<true>(a), to_f16x2<false>(b), to_f16x2<true>(b)};
+__device__ __forceinline__ u32x4_t operand(uint32_t a, uint32_t b, float power = 1.f) {
+  if constexpr (F16)
+    return u32x4_t{to_f16x2<false>(a, power), to_f16x2<true>(a, power), to_f16x2<false>(b, power), to_f16x2<true>(b, power)};
   else return u32x4_t{to_bf16x2<false>(a), to_bf16x2<true>(a), to_bf16x2<false>(b), to_bf16x2<true>(b)};
 }
 template <bool F16>
@@ -180,6 +196,13 @@ __device__ __forceinline__ uint32_t nan_codes(uint32_t w) { return ((w & 0x7f7f7
 __device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
   return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2_t{a, b}, bf16x2_t));
 }
+
+__device__ __forceinline__ uint32_t pack_f16(float a, float b) {
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2_t{a, b}, f16x2_t));
+}
+
+// A barrier for what the workgroup keeps in LDS: stores and loads to LDS that are under way stay so.
+__device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
 // 16 bytes per lane from memory to LDS: lane l's go to `to` + 16 l; OFF moves both ends.
 template <int OFF>
@@ -206,7 +229,7 @@ __device__ __forceinline__ void lds_read4(u32x4_t (&w)[4], uint32_t a) {
 // Keys that the rows of group rg of an entry see (a pair's groups are walked as far as the second sees), and steps of
 // them (one at least).
 __device__ __forceinline__ int group_keys(const HeadAttn& p, const HeadPlan& pl, int start, int rg) {
-  const int last = pl.pair ? p.C - 1 : min(p.C - 1, (rg * pl.rpg + pl.rpg - 1) / p.ratio);
+  const int last = pl.pair || rg == pl.RG - 1 ? p.C - 1 : min(p.C - 1, (rg * pl.rpg + pl.rpg - 1) / p.ratio);
   return min(start + last + 1, p.max_ctx);
 }
 __device__ __forceinline__ int group_steps(const HeadAttn& p, const HeadPlan& pl, int start, int rg) {
@@ -215,7 +238,7 @@ __device__ __forceinline__ int group_steps(const HeadAttn& p, const HeadPlan& pl
 
 template <int QT, int D, int RT>
 __global__ __launch_bounds__(kTileThreads, 2) void head_attn_tile_kernel(HeadAttn p, HeadPlan pl) {
-  constexpr bool F16 = QT == SPV_F16;
+  constexpr bool F16 = QT == SPV_F16, kF16W = Parts<QT>::half;
   constexpr int NQ = Parts<QT>::Q, NP = Parts<QT>::P, R = RT * 16, NCH = D / 32, NDT = D / 16;
   constexpr int kUnit = 16 * D, kHalf = 4 * kUnit, NS = kStage / (2 * kHalf);  // bytes of a unit, of a step's K or V; steps ahead
   constexpr int NK = kHalf / 1024;                                           // loads of a step's K, or V
@@ -243,31 +266,59 @@ __global__ __launch_bounds__(kTileThreads, 2) void head_attn_tile_kernel(HeadAtt
     st[i] = p.start[b];
     id[i] = p.seq_ids[b];
   }
-  auto count = [&](int start, int P) {
+  const int head = pl.equal ? 0 : kHead;
+  // Pieces that n steps go into, at about 1 / inv steps each.
+  auto pieces = [](int n, float inv) { return max(1, (int)ceilf((float)n * inv)); };
+  float inv_p = 0.f;
+  auto count = [&](int start) {
     int n = 0;
     for (int rg = 0; rg < counted; ++rg) {
       const int k = group_steps(p, pl, start, rg);
-      n += P ? (k + P - 1) / P : k;
+      n += pl.equal ? pieces(k, inv_p) : k + head;
     }
     return n * p.Hkv;
   };
-  int v0 = 0, mine = 0;  // of the lane's first entry, of all its entries
-  auto count_mine = [&](int P) {
-    v0 = b0 < b1 ? count(st[0], P) : 0;
-    mine = v0 + (b0 + 1 < b1 ? count(st[1], P) : 0);
-    for (int b = b0 + 2; b < b1; ++b) mine += count(p.start[b], P);
-    return wave_incl_sum(mine);
-  };
-  int upto = count_mine(0), total = lane63(upto);
-  int P = max((total + workers - 1) / workers, kMinSteps);
-  if (pl.equal) {
-    while (true) {  // ends: with P the longest context, one piece per segment, and those are at most half the workers
-      upto = count_mine(P);
-      total = lane63(upto);
-      if (total <= workers) break;
-      P += max(1, P >> 4);
+  int P = kMinSteps;
+  if (pl.equal) {  // two entries a lane at most: there are no more segments than half the workers
+    int steps = 0;
+    for (int rg = 0; rg < counted; ++rg) {
+      if (b0 < b1) steps += group_steps(p, pl, st[0], rg);
+      if (b0 + 1 < b1) steps += group_steps(p, pl, st[1], rg);
+    }
+    P = max((lane63(wave_incl_sum(steps)) * p.Hkv + workers - 1) / workers, kMinSteps);
+    // The smallest P that leaves no more pieces than workers, eight candidates at a time; ends at the latest with one
+    // piece per segment.
+    constexpr int kTry = 8;
+    for (bool found = false; !found;) {
+      float inv[kTry];
+      int n[kTry], sizes[kTry];
+#pragma unroll
+      for (int i = 0; i < kTry; ++i) {
+        sizes[i] = P + max(1, P >> 4) * i;
+        inv[i] = __builtin_amdgcn_rcpf((float)sizes[i]);
+        n[i] = 0;
+      }
+      for (int rg = 0; rg < counted; ++rg) {
+        const int k0 = b0 < b1 ? group_steps(p, pl, st[0], rg) : 0, k1 = b0 + 1 < b1 ? group_steps(p, pl, st[1], rg) : 0;
+#pragma unroll
+        for (int i = 0; i < kTry; ++i) n[i] += (k0 ? pieces(k0, inv[i]) : 0) + (k1 ? pieces(k1, inv[i]) : 0);
+      }
+#pragma unroll
+      for (int i = 0; i < kTry; ++i) n[i] = lane63(wave_incl_sum(n[i])) * p.Hkv;
+#pragma unroll
+      for (int i = kTry - 1; i >= 0; --i)
+        if (n[i] <= workers) {
+          found = true;
+          inv_p = inv[i];
+        }
+      P = sizes[kTry - 1] + 1;
     }
   }
+  const int v0 = b0 < b1 ? count(st[0]) : 0;  // of the lane's first entry; of all its entries
+  int mine = v0 + (b0 + 1 < b1 ? count(st[1]) : 0);
+  for (int b = b0 + 2; b < b1; ++b) mine += count(p.start[b]);
+  const int upto = wave_incl_sum(mine), total = lane63(upto);
+  if (!pl.equal) P = max((total + workers - 1) / workers, kMinSteps);
   const int x0 = pl.equal ? worker : worker * P;
   const int x1 = min(total, pl.equal ? x0 + 1 : x0 + P);
   if (blockIdx.x == kGrid - 1 && wave == 0) {
@@ -278,7 +329,7 @@ __global__ __launch_bounds__(kTileThreads, 2) void head_attn_tile_kernel(HeadAtt
   }
 
   for (int cur = x0; cur < x1;) {
-    if (cur != x0) __syncthreads();
+    lds_barrier();
     const int owner = __ffsll((unsigned long long)__ballot(upto > cur)) - 1;
     int off = cur - __builtin_amdgcn_readlane(upto - mine, owner), b = owner * epl, start, sid;
     if (epl <= 2) {
@@ -291,7 +342,7 @@ __global__ __launch_bounds__(kTileThreads, 2) void head_attn_tile_kernel(HeadAtt
     } else {  // the owner's entries, 64 at a time
       for (int e0 = 0;; e0 += 64) {
         const bool in = e0 + lane < epl && b + lane < p.B;
-        const int s1 = p.start[min(b + lane, p.B - 1)], n = in ? count(s1, pl.equal ? P : 0) : 0;
+        const int s1 = p.start[min(b + lane, p.B - 1)], n = in ? count(s1) : 0;
         const int sum = wave_incl_sum(n);
         if (off < lane63(sum)) {
           const int at = __ffsll((unsigned long long)__ballot(sum > off)) - 1;
@@ -308,26 +359,29 @@ __global__ __launch_bounds__(kTileThreads, 2) void head_attn_tile_kernel(HeadAtt
     int rg = 0, n = 0, k = 0;
     for (;; ++rg) {
       n = group_steps(p, pl, start, rg);
-      k = pl.equal ? (n + P - 1) / P : n;
+      k = pl.equal ? pieces(n, inv_p) : n + head;
       if (off < k * p.Hkv || rg == counted - 1) break;
       off -= k * p.Hkv;
     }
     const int h = off / k, i_in = off - h * k;
     int first, last, nparts, my, slot0;  // steps [first, last); parts of the segment, which is this; slots
     if (pl.equal) {
-      first = (int)((long long)n * i_in / k);
-      last = (int)((long long)n * (i_in + 1) / k);
+      const int each = n / k, more = n - each * k;
+      first = i_in * each + min(i_in, more);
+      last = first + each + (i_in < more);
       nparts = k;
       my = i_in;
       slot0 = cur - i_in;
       cur = x1;
     } else {
-      first = i_in;
-      last = min(n, i_in + x1 - cur);
-      slot0 = cur - i_in;  // the segment's first step among all
+      first = max(0, i_in - head);
+      const int take = min(k - i_in, x1 - cur);
+      last = i_in + take - head;
+      slot0 = cur - i_in + head;  // the segment's first step among all
       nparts = (slot0 + n - 1) / P - slot0 / P + 1;
       my = worker - slot0 / P;
-      cur += last - first;
+      cur += take;
+      if (last <= first) continue;  // the share ends before the segment's first step
     }
     if (pl.pair) rg = half;
     // Slot of part i: its worker's first or second one (a share's first piece, or its last).
@@ -347,18 +401,29 @@ __global__ __launch_bounds__(kTileThreads, 2) void head_attn_tile_kernel(HeadAtt
     // its scales.
     const int steps = last - first > wave ? (last - first - wave + kWaves - 1) / kWaves : 0;  // of this wave
     auto step_at = [&](int k) { return first + wave + k * kWaves; };
-    int l_block = 0, l_tok = 0;
+    uint32_t l_k[2] = {0, 0}, l_v[2] = {0, 0};  // byte offsets of the unit's K and V, in halves
     float2 l_scale = {0.f, 0.f};
     auto look_up = [&](int k) {  // for steps k .. k + 15
       const int u = min(step_at(k + (lane >> 2)) * 4 + (lane & 3), units - 1);
       const int blk = pl.upb == 1 ? u : (int)__umulhi((unsigned)u, pl.upb_magic);
-      l_tok = (u - blk * pl.upb) * 16;
-      l_block = table[min(blk, p.maxb - 1)];
-      if ((unsigned)l_block >= (unsigned)p.cap) {
+      const int tok = (u - blk * pl.upb) * 16;
+      int block = table[min(blk, p.maxb - 1)];
+      if ((unsigned)block >= (unsigned)p.cap) {
         if (lane >> 2 < steps - k) flag_read(p, b);
-        l_block = 0;
+        block = 0;
       }
-      l_scale = *reinterpret_cast<const float2*>(sbase + (size_t)l_block * 2);
+      l_scale = *reinterpret_cast<const float2*>(sbase + (size_t)block * 2);
+      const size_t at = (size_t)block * block_bytes, ka = at + (size_t)tok * D, va = at + tok;
+      l_k[0] = (uint32_t)ka;
+      l_k[1] = (uint32_t)(ka >> 32);
+      l_v[0] = (uint32_t)va;
+      l_v[1] = (uint32_t)(va >> 32);
+    };
+    // The unit's address, in scalar registers.
+    auto unit_from = [&](const uint8_t* base, const uint32_t (&l)[2], int at) {
+      uint64_t a = (uint64_t)base + ((uint64_t)__builtin_amdgcn_readlane(l[1], at) << 32 | (uint32_t)__builtin_amdgcn_readlane(l[0], at));
+      asm("" : "+s"(a));
+      return reinterpret_cast<const uint8_t*>(a);
     };
     uint8_t* const stage0 = s_page + wave * kStage;
     // Lane offsets of a K load (row, piece: exclusive or with 32 u for unit u) and of a V load (row).
@@ -372,8 +437,7 @@ __global__ __launch_bounds__(kTileThreads, 2) void head_attn_tile_kernel(HeadAtt
 #pragma unroll
       for (int u = 0; u < 4; ++u) {
         const int at = (k & 15) * 4 + u;
-        const uint8_t* const from = kbase + (size_t)(unsigned)__builtin_amdgcn_readlane(l_block, at) * block_bytes +
-                                    (size_t)__builtin_amdgcn_readlane(l_tok, at) * D;
+        const uint8_t* const from = unit_from(kbase, l_k, at);
         const uint32_t lo = kvoff ^ (D == 128 ? u * 32 : u * 16);
         page_to_lds<0>(from + lo, to + u * kUnit);
         if constexpr (D == 128) page_to_lds<1024>(from + lo, to + u * kUnit);
@@ -388,8 +452,7 @@ __global__ __launch_bounds__(kTileThreads, 2) void head_attn_tile_kernel(HeadAtt
 #pragma unroll
       for (int u = 0; u < 4; ++u) {
         const int at = (k & 15) * 4 + u;
-        const uint8_t* const from = vbase + (size_t)(unsigned)__builtin_amdgcn_readlane(l_block, at) * block_bytes +
-                                    (size_t)__builtin_amdgcn_readlane(l_tok, at);
+        const uint8_t* const from = unit_from(vbase, l_v, at);
         page_to_lds<0>(from + vvoff, to + u * kUnit);
         if constexpr (D == 128) page_to_lds<0>(from + (size_t)64 * p.bs + vvoff, to + u * kUnit + 1024);
       }
@@ -452,7 +515,7 @@ __global__ __launch_bounds__(kTileThreads, 2) void head_attn_tile_kernel(HeadAtt
         s_q[((q * RT + (row >> 4)) * NCH + ch) * 64 + ln] = w;
       }
     }
-    __syncthreads();
+    lds_barrier();
     auto query = [&](int rt, int ch, int q) { return s_q[((q * RT + rt) * NCH + ch) * 64 + lane]; };
     u32x4_t qreg[kQReg ? RT : 1][kQReg ? NCH : 1][kQReg ? NQ : 1];
     if constexpr (kQReg) {
@@ -466,6 +529,7 @@ __global__ __launch_bounds__(kTileThreads, 2) void head_attn_tile_kernel(HeadAtt
 
     f32x4_t o[RT][NDT];
     float m[RT], l[RT];
+    int unit_exp = -1000;  // kF16W: O stands for O 2^(unit_exp - kHalfShift)
     int seen[RT];  // keys that the lane's row attends
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
@@ -490,10 +554,34 @@ __global__ __launch_bounds__(kTileThreads, 2) void head_attn_tile_kernel(HeadAtt
       const bool masked = (step + 1) * kStep > all_see;
       const float ksc = sc[0].x * factor, vsc = sc[0].y;
       const int base = step * kStep + g * 16;  // the lane's first key
-      // Weights with V's scale in them as a power, w = 2^(z + log2 s_v - m), where no key is masked and the
-      // scales allow it; their sum is theirs over s_v. Elsewhere, and for fp32 queries, one after the other.
-      const bool plain = QT == SPV_F32 || masked || __any(!(vsc > 0x1p-60f && vsc < 0x1p60f));
-      const float vlog = __builtin_amdgcn_logf(vsc), vinv = __builtin_amdgcn_rcpf(vsc);
+      // Weights where no key is masked and the scales allow it: 2^(z - m) and V's scale in one power, for bf16
+      // queries what the scale is over a power of two, which goes into V's conversion; their sum is theirs without it.
+      // Elsewhere, and for fp32 queries, one after the other and in parts of bf16.
+      const int vexp = vsc > 0.f ? __builtin_amdgcn_frexp_expf(vsc) - 1 : -200;  // s_v in [2^vexp, 2^(vexp + 1))
+      bool plain = QT == SPV_F32 || masked;
+      if constexpr (kF16W) {
+        if (__any(vexp > unit_exp + 7)) {  // O's unit 2^unit_exp follows the scales
+          int top = vexp;
+#pragma unroll
+          for (int x = 16; x < 64; x *= 2) top = max(top, __shfl_xor(top, x, 64));
+          top = __builtin_amdgcn_readfirstlane(top);
+#pragma unroll
+          for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+            for (int dt = 0; dt < NDT; ++dt)
+#pragma unroll
+              for (int i = 0; i < 4; ++i) o[rt][dt][i] = ldexpf(o[rt][dt][i], unit_exp - top);
+          unit_exp = top;
+        }
+        plain |= (bool)__any(vexp < unit_exp - 15 || !(vsc > 0.f));
+      } else {
+        plain |= (bool)__any(!(vsc > 0x1p-60f && vsc < 0x1p60f));
+      }
+      // s_v times 2^vshift is what a weight takes; in fp16 the part of it in [1, 2), times 2^kHalfShift.
+      const float vpart = kF16W ? ldexpf(vsc, kHalfShift - vexp) : vsc;
+      const float vlog = __builtin_amdgcn_logf(vpart), vinv = __builtin_amdgcn_rcpf(vpart);
+      const float vall = kF16W ? ldexpf(vsc, kHalfShift - unit_exp) : vsc;
+      const float vpow = __uint_as_float((uint32_t)(min(max(vexp - unit_exp, -15), 7) + 127) << 23);
       auto lift = [&](int rt, float top) {
         top = fmaxf(top, __shfl_xor(top, 16, 64));
         top = fmaxf(top, __shfl_xor(top, 32, 64));
@@ -541,14 +629,46 @@ __global__ __launch_bounds__(kTileThreads, 2) void head_attn_tile_kernel(HeadAtt
       if constexpr (MORE) fetch_k(k + NS);
       else if constexpr (NS > 1) sc[0] = sc[NS - 1];
       uint32_t pw[RT][2][NP][4];
+      float top[RT];
+      if (plain) {
 #pragma unroll
-      for (int rt = 0; rt < RT; ++rt) {
-        if (!plain) {
-          float top = s[rt][0][0];
+        for (int rt = 0; rt < RT; ++rt) {
+          top[rt] = -INFINITY;
 #pragma unroll
-          for (int i = 1; i < 16; ++i) top = fmaxf(top, s[rt][i >> 2][i & 3]);
-          top *= ksc;
-          if (__any(top > m[rt] + kLift)) lift(rt, top);
+          for (int i = 0; i < 16; ++i) {
+            const float z = base + i < seen[rt] ? s[rt][i >> 2][i & 3] * ksc : -INFINITY;
+            s[rt][i >> 2][i & 3] = z;
+            top[rt] = fmaxf(top[rt], z);
+          }
+        }
+      } else {
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) {
+          top[rt] = s[rt][0][0];
+#pragma unroll
+          for (int i = 1; i < 16; ++i) top[rt] = fmaxf(top[rt], s[rt][i >> 2][i & 3]);
+          top[rt] *= ksc;
+        }
+      }
+      bool higher = false;
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt) higher |= top[rt] > m[rt] + Parts<QT>::lift;
+      if (__any(higher)) {
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) lift(rt, top[rt]);
+      }
+      if (plain) {
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const float e = __builtin_amdgcn_exp2f(s[rt][i >> 2][i & 3] - m[rt]);
+            l[rt] += e;
+            s[rt][i >> 2][i & 3] = e * vall;
+          }
+      } else {
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) {
           const float off = vlog - m[rt];
           float sum = 0.f;
 #pragma unroll
@@ -558,35 +678,29 @@ __global__ __launch_bounds__(kTileThreads, 2) void head_attn_tile_kernel(HeadAtt
             sum += w;
           }
           l[rt] = fmaf(sum, vinv, l[rt]);
-        } else {
-          float top = -INFINITY;
-#pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const float z = base + i < seen[rt] ? s[rt][i >> 2][i & 3] * ksc : -INFINITY;
-            s[rt][i >> 2][i & 3] = z;
-            top = fmaxf(top, z);
-          }
-          if (__any(top > m[rt] + kLift)) lift(rt, top);
-#pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const float e = __builtin_amdgcn_exp2f(s[rt][i >> 2][i & 3] - m[rt]);
-            l[rt] += e;
-            s[rt][i >> 2][i & 3] = e * vsc;
-          }
         }
+      }
+      if (kF16W && !plain) {
 #pragma unroll
-        for (int q = 0; q < NP; ++q)
+        for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const float x = s[rt][i >> 1][2 * (i & 1)], y = s[rt][i >> 1][2 * (i & 1) + 1];
-            const uint32_t u = pack_bf16(x, y);
-            pw[rt][i >> 2][q][i & 3] = u;
-            if (q + 1 < NP) {
-              s[rt][i >> 1][2 * (i & 1)] = x - __uint_as_float(u << 16);
-              s[rt][i >> 1][2 * (i & 1) + 1] = y - __uint_as_float(u & 0xffff0000u);
+          for (int i = 0; i < 8; ++i)
+            pw[rt][i >> 2][0][i & 3] = pack_f16(s[rt][i >> 1][2 * (i & 1)], s[rt][i >> 1][2 * (i & 1) + 1]);
+      } else {
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+          for (int q = 0; q < NP; ++q)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              const float x = s[rt][i >> 1][2 * (i & 1)], y = s[rt][i >> 1][2 * (i & 1) + 1];
+              const uint32_t u = pack_bf16(x, y);
+              pw[rt][i >> 2][q][i & 3] = u;
+              if (q + 1 < NP) {
+                s[rt][i >> 1][2 * (i & 1)] = x - __uint_as_float(u << 16);
+                s[rt][i >> 1][2 * (i & 1) + 1] = y - __uint_as_float(u & 0xffff0000u);
+              }
             }
-          }
-        if constexpr (RT > 2) __builtin_amdgcn_sched_barrier(0);
       }
       // V of this step is there: behind it came what was fetched ahead, and K of step k + NS.
       if constexpr (MORE) wait_loads<(NS - 1) * 2 * NK + NK>();
@@ -624,18 +738,28 @@ __global__ __launch_bounds__(kTileThreads, 2) void head_attn_tile_kernel(HeadAtt
           }
         }
 #pragma unroll
-        for (int dt = 0; dt < 4; ++dt) {
+        for (int mm = 0; mm < 2; ++mm) {  // eight sums in turn, so that none waits for its last addition
+          auto weights = [&](int rt, int q) {
+            return u32x4_t{pw[rt][mm][q][0], pw[rt][mm][q][1], pw[rt][mm][q][2], pw[rt][mm][q][3]};
+          };
+          u32x4_t vop[4];
+          if (kF16W && !plain) {
 #pragma unroll
-          for (int mm = 0; mm < 2; ++mm) {
-            const u32x4_t vop = operand<false>(vw[dt][2 * mm], vw[dt][2 * mm + 1]);
+            for (int dt = 0; dt < 4; ++dt) vop[dt] = operand<true>(vw[dt][2 * mm], vw[dt][2 * mm + 1], vpow);
+#pragma unroll
+            for (int dt = 0; dt < 4; ++dt)
+#pragma unroll
+              for (int rt = 0; rt < RT; ++rt) o[rt][4 * d4 + dt] = mfma<true>(vop[dt], weights(rt, 0), o[rt][4 * d4 + dt]);
+          } else {
+#pragma unroll
+            for (int dt = 0; dt < 4; ++dt) vop[dt] = operand<false>(vw[dt][2 * mm], vw[dt][2 * mm + 1]);
 #pragma unroll
             for (int q = NP - 1; q >= 0; --q)
 #pragma unroll
-              for (int rt = 0; rt < RT; ++rt)
-                o[rt][4 * d4 + dt] = mfma<false>(
-                    vop, u32x4_t{pw[rt][mm][q][0], pw[rt][mm][q][1], pw[rt][mm][q][2], pw[rt][mm][q][3]}, o[rt][4 * d4 + dt]);
+              for (int dt = 0; dt < 4; ++dt)
+#pragma unroll
+                for (int rt = 0; rt < RT; ++rt) o[rt][4 * d4 + dt] = mfma<false>(vop[dt], weights(rt, q), o[rt][4 * d4 + dt]);
           }
-          if constexpr (RT > 2) __builtin_amdgcn_sched_barrier(0);
         }
       }
       if constexpr (MORE) fetch_v(k + NS);
@@ -654,7 +778,7 @@ __global__ __launch_bounds__(kTileThreads, 2) void head_attn_tile_kernel(HeadAtt
         s_ml[1][wave][rt * 16 + c] = l[rt];
       }
     }
-    __syncthreads();
+    lds_barrier();
     float keep[RT];
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
@@ -662,6 +786,7 @@ __global__ __launch_bounds__(kTileThreads, 2) void head_attn_tile_kernel(HeadAtt
 #pragma unroll
       for (int w = 0; w < kWaves; ++w) mx = fmaxf(mx, s_ml[0][w][rt * 16 + c]);
       keep[rt] = __builtin_amdgcn_exp2f(m[rt] - mx);
+      if constexpr (kF16W) keep[rt] = ldexpf(keep[rt], unit_exp - kHalfShift);
       if (wave == 0 && g == 0) {
         float sum = 0.f;
 #pragma unroll
@@ -698,14 +823,14 @@ __global__ __launch_bounds__(kTileThreads, 2) void head_attn_tile_kernel(HeadAtt
     float* const s_o = reinterpret_cast<float*>(s_page);  // [wave][row][kCols + pad]
 #pragma unroll
     for (int pass = 0; pass < D / kCols; ++pass) {
-      if (pass) __syncthreads();
+      if (pass) lds_barrier();
 #pragma unroll
       for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
         for (int dt = 0; dt < kCols / 16; ++dt)
           *reinterpret_cast<f32x4_t*>(s_o + (wave * R + rt * 16 + c) * (kCols + kColPad) + dt * 16 + 4 * g) =
               o[rt][pass * (kCols / 16) + dt] * keep[rt];
-      __syncthreads();
+      lds_barrier();
       for (int i = threadIdx.x; i < rows * (kCols / 4); i += kTileThreads) {
         const int row = i / (kCols / 4), e = (i - row * (kCols / 4)) * 4;
         f32x4_t sum = {0.f, 0.f, 0.f, 0.f};
@@ -784,7 +909,7 @@ bool tile_plan(int32_t B, int32_t C, int32_t Hq, int32_t Hkv, int32_t d, int32_t
   pl.pair = pl.RG == 2;
   pl.upb = bs / 16;
   pl.upb_magic = (unsigned)(0x100000000ULL / (unsigned)pl.upb + 1);
-  const long long segs = (long long)B * (pl.pair ? 1 : pl.RG) * Hkv, steps = ((long long)max_ctx + kStep - 1) / kStep;
+  const long long segs = (long long)B * (pl.pair ? 1 : pl.RG) * Hkv, steps = ((long long)max_ctx + kStep - 1) / kStep + kHead;
   if (segs * steps > 0x3fffffffLL || ((long long)max_ctx / 16 + 1) * pl.upb > 0x7fffffffLL) return false;
   pl.equal = segs * 2 <= (pl.pair ? kGrid / 2 : kGrid);
   return true;

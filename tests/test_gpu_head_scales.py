@@ -7,8 +7,10 @@ Attention's tolerance, per element of row r: half a step of the output type of
 |o|, plus eps_p sum_i p_i |v_i|. A weight p_i is off by its score, 2 (d + 4) 2^-24
 times the largest sum_e |q_e k_e| scale of the row (d products and sums, the
 scales' products, the maximum taken off; 2 for the row's sum, which is off as
-much), by exp2 and the running rescales (2^-20), and by its own rounding to 16
-bits before the product with v (2^-17 with the sum's).
+much), by exp2 and the running rescales (2^-20), and by its own rounding before
+the product with v: for fp16 and fp32 queries to 16 bits or more (2^-17 with the
+sum's), for bf16 queries to fp16, whose step is 2^-10 of the power of two below the
+weight: at most 2^-11 of the weight, an eighth of what bf16 outputs are rounded by.
 """
 
 from __future__ import annotations
@@ -367,6 +369,7 @@ def _check(out, q, kv, layer, sids, starts, scale=None, rows=None):
     B, C, hq, d = q.shape
     H = kv.num_kv_heads
     scale = d ** -0.5 if scale is None else scale
+    q_dtype = q.dtype
     out, q = out.detach().cpu().double(), q.detach().cpu()
     half = torch.finfo(q.dtype).eps / 2
     tiny = {F32: 2.0 ** -149, BF16: 2.0 ** -133, F16: 2.0 ** -24}[q.dtype]
@@ -380,7 +383,7 @@ def _check(out, q, kv, layer, sids, starts, scale=None, rows=None):
             size = (torch.matmul(qq.abs(), k[:, :n].abs().transpose(1, 2)) * abs(scale)).amax(-1, keepdim=True)
             p = torch.softmax(z, -1)
             o, a = torch.matmul(p, v[:, :n]), torch.matmul(p, v[:, :n].abs())
-            eps_p = 2 * (d + 4) * 2.0 ** -24 * size + 2.0 ** -20 + 2.0 ** -17
+            eps_p = 2 * (d + 4) * 2.0 ** -24 * size + 2.0 ** -20 + (2.0 ** -11 if q_dtype is BF16 else 2.0 ** -17)
             bound = half * o.abs() + tiny / 2 + (1 + half) * eps_p * a
             err = (out[b, j].view(H, hq // H, d) - o).abs()
             assert bool((err <= bound).all()), (b, j, float((err / bound).max()))
