@@ -37,7 +37,14 @@ __device__ __forceinline__ float wave_max(float x) {
 
 // One workgroup per (entry, block that the chunk touches, kv head); behind them
 // the queries' workgroups of rotary_vec_rows.
-template <int IT, bool TURN, bool NORM, bool QUERY>
+// VEC (16-byte rows, head_dim and blocks of whole 16, the block staged at once): 16 bytes of the page per thread and
+// turn, K's dims or V's tokens; of a block that is not wholly new they are asked for before the rows are turned.
+// Byte by byte, prompts of 4 x 3,001 tokens with two kv heads of 128 took 21.4 us (now 12.1), 32 verify chunks of 6
+// tokens 9.8 (now 8.5).
+// What bounds it: round trips one behind the other (start, then tables, rows and turns, then scales and the page, 3 us
+// together for verify chunks), the norm and rotation of a row by 16 threads (1.8), quotients and stores (1.5); prompts
+// read their rows meanwhile (18.9 MB moved, 3.8 us at the rate of a large copy).
+template <int IT, bool TURN, bool NORM, bool QUERY, bool VEC>
 __global__ __launch_bounds__(kThreads) void head_write_kernel(HeadWrite w, VecShape v) {
   extern __shared__ __align__(16) uint8_t lds[];
   __shared__ float s_red[2][kThreads / 64];
@@ -55,7 +62,22 @@ __global__ __launch_bounds__(kThreads) void head_write_kernel(HeadWrite w, VecSh
   const int blk = s0 / p.bs + t;
   const int lo = max(s0 - blk * p.bs, 0), hi_c = min(s0 + p.C - blk * p.bs, p.bs);
   if (hi_c <= lo) return;
-  const int sid = p.seq_ids[b];
+  const int sid = p.seq_ids[b], d = p.d, st = d + kPad, half = p.R / 2;
+  // VEC: the first 16 bytes of K and V per thread are on their way while tables and turns are looked up.
+  constexpr int E = Piece<IT>::E;
+  const int row_pieces = d / E;
+  [[maybe_unused]] u32x4_t raw_k{}, raw_v{};
+  auto piece_of = [&](const uint8_t* x, const long long (&s)[3], int i) {
+    const int r = i / row_pieces, at = (i - r * row_pieces) * E, j = blk * p.bs + lo - s0 + r;
+    const long long o = (long long)b * s[0] + (long long)j * s[1] + (long long)h * s[2] + at;
+    return *reinterpret_cast<const u32x4_t*>(x + o * (16 / E));
+  };
+  if constexpr (VEC) {
+    if ((int)threadIdx.x < (hi_c - lo) * row_pieces) {
+      raw_k = piece_of(p.k, p.ks, threadIdx.x);
+      raw_v = piece_of(p.v, p.vs, threadIdx.x);
+    }
+  }
   int limit = w.limit_b;
   if (limit < 0) {
     const int ex = p.ctr[CTR_EXHAUSTED];
@@ -63,17 +85,35 @@ __global__ __launch_bounds__(kThreads) void head_write_kernel(HeadWrite w, VecSh
   }
   const int n = b > limit ? 0 : min(p.C, p.nblocks[sid] * p.bs - s0);
   const int phys = p.tables[(size_t)sid * p.maxb + min(blk, p.maxb - 1)];
+  float* const sk = reinterpret_cast<float*>(lds);
+  float* const sv = sk + (size_t)w.tile * st;
+  float2* const turns = reinterpret_cast<float2*>(sv + (size_t)w.tile * st);
+  if constexpr (VEC && TURN) {
+    for (int i = threadIdx.x; i < (hi_c - lo) * half; i += kThreads) {
+      const int r = i / half, f = i - r * half;
+      turns[i] = turn_of(p, b, blk * p.bs + lo - s0 + r, f);
+    }
+  }
+  float* const weights = reinterpret_cast<float*>(turns + (size_t)w.tile * half);  // VEC and NORM: of a row
+  if constexpr (VEC && NORM) {
+    if (p.wk)
+      for (int i = threadIdx.x; i < d; i += kThreads) weights[i] = p.wk[i];
+  }
   const int hi = min(hi_c, s0 + n - blk * p.bs);
   if (n <= 0 || hi <= lo || blk >= p.maxb || (unsigned)phys >= (unsigned)p.cap) return;  // never outside the pool
   if (t == 0 && h == 0 && threadIdx.x == 0 && p.seq_lens[sid] < s0 + n) p.seq_lens[sid] = s0 + n;
 
-  const int d = p.d, st = d + kPad, half = p.R / 2;
-  float* const sk = reinterpret_cast<float*>(lds);
-  float* const sv = sk + (size_t)w.tile * st;
-  float2* const turns = reinterpret_cast<float2*>(sv + (size_t)w.tile * st);
   float* const page_scale = w.scales + scale_of(p.layer, p.cap, phys, p.Hkv, h);
   const float old_k = page_scale[0], old_v = page_scale[1];
   const size_t page = page_of(p.layer, p.cap, phys, p.Hkv, h, p.bs, d);
+  uint8_t* const kp = p.kpool + page;  // [token][d]
+  uint8_t* const vp = p.vpool + page;  // [d][token]
+  const int pieces = p.bs * d / 16;    // VEC: of a page; V's come first
+  [[maybe_unused]] u32x4_t held{};
+  auto codes_at = [&](int i) { return reinterpret_cast<u32x4_t*>(i < pieces ? vp : kp) + (i < pieces ? i : i - pieces); };
+  if constexpr (VEC) {
+    if (hi - lo < p.bs && (int)threadIdx.x < 2 * pieces) held = *codes_at(threadIdx.x);
+  }
 
   // Rows [ra, rb) of the block into LDS, the keys normed and turned.
   float ak = 0.f, av = 0.f;
@@ -83,7 +123,29 @@ __global__ __launch_bounds__(kThreads) void head_write_kernel(HeadWrite w, VecSh
   };
   auto stage = [&](int ra, int rb) {
     const int j0 = blk * p.bs + ra - s0, rows = rb - ra;
-    for (int i = threadIdx.x; i < rows * d; i += kThreads) {
+    if constexpr (VEC) {
+      for (int i = threadIdx.x; i < rows * row_pieces; i += kThreads) {
+        if (i != (int)threadIdx.x) {
+          raw_k = piece_of(p.k, p.ks, i);
+          raw_v = piece_of(p.v, p.vs, i);
+        }
+        const int r = i / row_pieces, e = (i - r * row_pieces) * E;
+        Piece<IT> x, y;
+        x.unpack(raw_k);
+        y.unpack(raw_v);
+#pragma unroll
+        for (int q = 0; q < E; q += 4) {
+          *reinterpret_cast<float4*>(sk + r * st + e + q) = make_float4(x.x[q], x.x[q + 1], x.x[q + 2], x.x[q + 3]);
+          *reinterpret_cast<float4*>(sv + r * st + e + q) = make_float4(y.x[q], y.x[q + 1], y.x[q + 2], y.x[q + 3]);
+        }
+#pragma unroll
+        for (int q = 0; q < E; ++q) {
+          if constexpr (!TURN) ak = fmaxf(ak, finite_abs(x.x[q]));
+          av = fmaxf(av, finite_abs(y.x[q]));
+        }
+      }
+    }
+    for (int i = VEC ? rows * d : threadIdx.x; i < rows * d; i += kThreads) {
       const int r = i / d, e = i - r * d;
       const long long at = (long long)b * p.ks[0] + (long long)(j0 + r) * p.ks[1] + (long long)h * p.ks[2] + e;
       const long long av_at = (long long)b * p.vs[0] + (long long)(j0 + r) * p.vs[1] + (long long)h * p.vs[2] + e;
@@ -93,7 +155,7 @@ __global__ __launch_bounds__(kThreads) void head_write_kernel(HeadWrite w, VecSh
       if constexpr (!TURN) ak = fmaxf(ak, finite_abs(xk));
       av = fmaxf(av, finite_abs(xv));
     }
-    if constexpr (TURN) {
+    if constexpr (TURN && !VEC) {
       for (int i = threadIdx.x; i < rows * half; i += kThreads) {
         const int r = i / half, f = i - r * half;
         turns[i] = turn_of(p, b, j0 + r, f);
@@ -110,7 +172,7 @@ __global__ __launch_bounds__(kThreads) void head_write_kernel(HeadWrite w, VecSh
 #pragma unroll
           for (int o = kRowLanes / 2; o > 0; o >>= 1) ss += __shfl_xor(ss, o, 64);
           const float inv = norm_factor(ss, d, p.eps);
-          for (int e = lane; e < d; e += kRowLanes) x[e] *= p.wk ? inv * p.wk[e] : inv;
+          for (int e = lane; e < d; e += kRowLanes) x[e] *= p.wk ? inv * (VEC ? weights : p.wk)[e] : inv;
           __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
           __builtin_amdgcn_wave_barrier();
           __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
@@ -149,8 +211,51 @@ __global__ __launch_bounds__(kThreads) void head_write_kernel(HeadWrite w, VecSh
     a1 = fmaxf(a1, s_red[1][i]);
   }
   const float nk = fmaxf(old_k, __fdiv_rn(a0, 448.f)), nv = fmaxf(old_v, __fdiv_rn(a1, 448.f));
-  uint8_t* const kp = p.kpool + page;  // [token][d]
-  uint8_t* const vp = p.vpool + page;  // [d][token]
+  if (VEC && usual_scale(nk) && usual_scale(nv)) {
+    const float yk = __fdiv_rn(1.f, nk), yv = __fdiv_rn(1.f, nv);
+    for (int i = threadIdx.x; i < 2 * pieces; i += kThreads) {
+      const bool is_v = i < pieces;
+      const float scale = is_v ? nv : nk, y = is_v ? yv : yk, old = is_v ? old_v : old_k;
+      const int at = (is_v ? i : i - pieces) * 16, line = is_v ? p.bs : d, e = at / line, c0 = at - e * line;
+      // V: tokens c0 .. c0 + 15 of dim e; K: dims c0 .. c0 + 15 of token e. Bytes [from, to) of them are new.
+      const int from = is_v ? max(lo - c0, 0) : 0, to = is_v ? min(hi - c0, 16) : e >= lo && e < hi ? 16 : 0;
+      const bool again = scale > old;  // for the others
+      if (to <= from && !again) continue;
+      u32x4_t w = held;
+      if (from > 0 || to < 16) {
+        if (i != (int)threadIdx.x) w = *codes_at(i);
+        if (again) {
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            float x[4];
+            decode4(w[q], x);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) x[k] = quotient(__fmul_rn(x[k], old), scale, y);
+            w[q] = encode4(x);
+          }
+        }
+      }
+      if (to > from) {
+        const float* const x0 = is_v ? sv + (c0 - lo) * st + e : sk + (e - lo) * st + c0;
+        const int step = is_v ? st : 1;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          float x[4];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) x[k] = quotient(x0[min(max(4 * q + k, from), to - 1) * step], scale, y);
+          const int a = min(max(from - 4 * q, 0), 4), b = min(max(to - 4 * q, 0), 4);
+          const uint32_t in = (uint32_t)((1ull << (8 * b)) - 1) & ~(uint32_t)((1ull << (8 * a)) - 1);
+          w[q] = (w[q] & ~in) | (encode4(x) & in);
+        }
+      }
+      *codes_at(i) = w;
+    }
+    if (threadIdx.x == 0) {
+      page_scale[0] = nk;
+      page_scale[1] = nv;
+    }
+    return;
+  }
   for (int k = t0; k <= t1; ++k) {
     const int ra = first(k), rb = last(k), rows = rb - ra;
     if (t1 > t0) {
@@ -212,6 +317,70 @@ __global__ __launch_bounds__(kThreads) void head_read_kernel(HeadRead p) {
   }
 }
 
+// The same in pieces: a workgroup takes kReadTokens positions of a head, K (4 codes per thread and turn) or V, whose
+// page has a dim's tokens side by side (4 x 4 codes, put across in registers). Bound by the bytes it stores and by the
+// table, scale and page one behind the other: 32,768 positions of two heads of 64 to bf16 (25.2 MB, floor 5.1 us) in 7.8
+// us, 3.2 TB/s; code by code 20.8.
+constexpr int kReadTokens = 64;
+template <int OT>
+__global__ __launch_bounds__(kThreads) void head_read_vec_kernel(HeadRead p) {
+  const int t0 = blockIdx.x * kReadTokens, h = blockIdx.y, d = p.d, lines = min(kReadTokens, p.length - t0);
+  const size_t step = (size_t)p.hkv * d, total = (size_t)p.length * step;
+  auto page_at = [&](int pos, int& off, size_t& page) {
+    const int blk = pos / p.bs, id = p.table[blk], phys = (unsigned)id < (unsigned)p.cap ? id : 0;
+    off = pos - blk * p.bs;
+    page = page_of(p.layer, p.cap, phys, p.hkv, h, p.bs, d);
+    return p.scales + scale_of(p.layer, p.cap, phys, p.hkv, h);
+  };
+  auto store4 = [&](size_t at, const float* x) {
+    if constexpr (OT == SPV_F32) {
+      *reinterpret_cast<float4*>(static_cast<float*>(p.out) + at) = make_float4(x[0], x[1], x[2], x[3]);
+    } else {
+      u32x2_t w;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        if constexpr (OT == SPV_BF16)
+          w[i] = __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2_t{x[2 * i], x[2 * i + 1]}, bf16x2_t));
+        else
+          w[i] = __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2_t{x[2 * i], x[2 * i + 1]}, f16x2_t));
+      }
+      asm("" : "+v"(w));
+      *reinterpret_cast<u32x2_t*>(static_cast<uint16_t*>(p.out) + at) = w;
+    }
+  };
+  int off;
+  size_t page;
+  float x[4];
+  if (blockIdx.z == 0) {
+    for (int i = threadIdx.x; i < lines * (d / 4); i += kThreads) {
+      const int t = i / (d / 4), e = (i - t * (d / 4)) * 4;
+      const float s = page_at(t0 + t, off, page)[0];
+      decode4(*reinterpret_cast<const uint32_t*>(p.kpool + page + (size_t)off * d + e), x);
+#pragma unroll
+      for (int q = 0; q < 4; ++q) x[q] *= s;
+      store4((size_t)(t0 + t) * step + (size_t)h * d + e, x);
+    }
+  } else {
+    for (int i = threadIdx.x; i < (lines + 3) / 4 * (d / 4); i += kThreads) {
+      const int t = i / (d / 4) * 4, e = (i - t / 4 * (d / 4)) * 4;
+      const float s = page_at(t0 + t, off, page)[1];
+      uint32_t w[4];
+#pragma unroll
+      for (int q = 0; q < 4; ++q) w[q] = *reinterpret_cast<const uint32_t*>(p.vpool + page + (size_t)(e + q) * p.bs + off);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if (t + j >= lines) break;
+        const uint32_t sel = 0x0c0c0400u + 0x0101u * j;  // byte j of the second operand, then of the first
+        const uint32_t lo = __builtin_amdgcn_perm(w[1], w[0], sel), hi = __builtin_amdgcn_perm(w[3], w[2], sel);
+        decode4(lo | hi << 16, x);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) x[q] *= s;
+        store4(total + (size_t)(t0 + t + j) * step + (size_t)h * d + e, x);
+      }
+    }
+  }
+}
+
 constexpr size_t kLdsBytes = 65536;
 
 // LDS of a key / value workgroup that stages `rows` rows at once.
@@ -227,11 +396,11 @@ int write_tile(int bs, int d, int R, bool turn) {
   return write_lds(rows, d, R, turn) <= kLdsBytes ? rows : 0;
 }
 
-template <int IT>
+template <int IT, bool VEC>
 void launch_write(const HeadWrite& w, const VecShape& v, bool turn, bool norm, bool query, unsigned grid, size_t smem,
                   hipStream_t s) {
 #define SPV_W(TURN, NORM, QUERY) \
-  hipLaunchKernelGGL((head_write_kernel<IT, TURN, NORM, QUERY>), dim3(grid), dim3(kThreads), smem, s, w, v)
+  hipLaunchKernelGGL((head_write_kernel<IT, TURN, NORM, QUERY, VEC>), dim3(grid), dim3(kThreads), smem, s, w, v)
   if (!turn) SPV_W(false, false, false);
   else if (!norm && !query) SPV_W(true, false, false);
   else if (!norm) SPV_W(true, false, true);
@@ -306,9 +475,18 @@ int write(HeadWrite& w, const PoolArgs& a, int dtype, bool turn, bool norm, int3
     }
   }
   if (grid > 0x7fffffffLL) return SPV_ERR_ARG;
-  if (dtype == SPV_F32) launch_write<SPV_F32>(w, v, turn, norm, query, (unsigned)grid, smem, s);
-  else if (dtype == SPV_BF16) launch_write<SPV_BF16>(w, v, turn, norm, query, (unsigned)grid, smem, s);
-  else launch_write<SPV_F16>(w, v, turn, norm, query, (unsigned)grid, smem, s);
+  const size_t weights = norm ? p.d * sizeof(float) : 0;  // vec: in LDS too
+  bool vec = w.tile == p.bs && smem + weights <= kLdsBytes && p.d % 16 == 0 && p.bs % 16 == 0 &&
+             (((uintptr_t)p.k | (uintptr_t)p.v | (uintptr_t)p.kpool | (uintptr_t)p.vpool) & 15) == 0;
+  for (int i = 0; i < 3; ++i) vec = vec && (p.ks[i] * dtype_size(dtype)) % 16 == 0 && (p.vs[i] * dtype_size(dtype)) % 16 == 0;
+  if (vec) smem += weights;
+#define SPV_W(IT) \
+  vec ? launch_write<IT, true>(w, v, turn, norm, query, (unsigned)grid, smem, s) \
+      : launch_write<IT, false>(w, v, turn, norm, query, (unsigned)grid, smem, s)
+  if (dtype == SPV_F32) SPV_W(SPV_F32);
+  else if (dtype == SPV_BF16) SPV_W(SPV_BF16);
+  else SPV_W(SPV_F16);
+#undef SPV_W
   SPV_CHECK_LAUNCH();
   return query || !p.q ? SPV_OK : 1;  // 1: the queries are still to be turned
 }
@@ -434,9 +612,18 @@ int spv_kv_gather_fp8_heads(const void* k_pool, const void* v_pool, const float*
   const HeadRead p{static_cast<const uint8_t*>(k_pool), static_cast<const uint8_t*>(v_pool), kv_scales,
                    block_tables + (size_t)seq_id * max_blocks_per_seq, out, length, layer, capacity, block_size,
                    num_kv_heads, head_dim};
+  hipStream_t s = (hipStream_t)stream;
+  if (head_dim % 4 == 0 && block_size % 4 == 0 && num_kv_heads <= 65535 && (uintptr_t)out % 16 == 0 &&
+      ((uintptr_t)k_pool | (uintptr_t)v_pool) % 4 == 0) {
+    const dim3 grid((unsigned)((length + (long long)kReadTokens - 1) / kReadTokens), (unsigned)num_kv_heads, 2), blk(kThreads);
+    if (out_dtype == SPV_F32) hipLaunchKernelGGL(head_read_vec_kernel<SPV_F32>, grid, blk, 0, s, p);
+    else if (out_dtype == SPV_BF16) hipLaunchKernelGGL(head_read_vec_kernel<SPV_BF16>, grid, blk, 0, s, p);
+    else hipLaunchKernelGGL(head_read_vec_kernel<SPV_F16>, grid, blk, 0, s, p);
+    SPV_CHECK_LAUNCH();
+    return SPV_OK;
+  }
   const size_t work = (size_t)length * num_kv_heads * head_dim, need = (work + kThreads - 1) / kThreads;
   const dim3 grid((unsigned)(need < 8192 ? need : 8192)), blk(kThreads);
-  hipStream_t s = (hipStream_t)stream;
   if (out_dtype == SPV_F32) hipLaunchKernelGGL(head_read_kernel<SPV_F32>, grid, blk, 0, s, p);
   else if (out_dtype == SPV_BF16) hipLaunchKernelGGL(head_read_kernel<SPV_BF16>, grid, blk, 0, s, p);
   else hipLaunchKernelGGL(head_read_kernel<SPV_F16>, grid, blk, 0, s, p);
