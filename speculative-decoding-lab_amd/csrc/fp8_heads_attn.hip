@@ -109,7 +109,7 @@ __global__ __launch_bounds__(64 * kAnyRows) void head_attn_any_kernel(HeadAttn p
 // Head dims 64 and 128, blocks of whole 16-token units. A workgroup of 8 waves
 // takes a piece: rows R = 16 RT of one kv head of one entry (all of them, for
 // verify chunks) times a range of steps of 64 keys, its waves every eighth step.
-// Pages go from HBM to LDS by themselves (loads with an LDS destination), 16 KB
+// Pages go from HBM to LDS by themselves (loads with an LDS destination), a step
 // ahead per wave, and each wave waits for its own; no barrier while it walks.
 // Everything stays transposed, so that no value changes lanes between the two
 // products:
@@ -126,10 +126,10 @@ __global__ __launch_bounds__(64 * kAnyRows) void head_attn_any_kernel(HeadAttn p
 // a row is raised (and O rescaled) only where a step passes it by more than 2^8 (2^3
 // for bf16 queries).
 // Roundings: scores, sums and O are fp32. A weight meets V in 16 bits:
-//   bf16 queries: one part of fp16 (2^-12, an eighth of the output's own rounding),
+//   bf16 queries: one part of fp16 (2^-11, an eighth of the output's own rounding),
 //     shifted up by 2^11 with V's scale in [1, 2); the scale's power of two goes into
 //     V's conversion, against a unit of O's that follows the largest. The second part
-//     of bf16 that this saves costs 4 us of 54 at 16 contexts of 32,768 keys. Weights
+//     of bf16 that this saves cost 4 us of 54 at 16 contexts of 32,768 keys. Weights
 //     below 2^-25 of the row's largest lose bits, 2^-36 of it each.
 //   fp16 queries: two parts of bf16 (2^-17), 8 bits each and of fp32's range.
 //   fp32 queries: three parts, and three of each query, in S.
@@ -145,11 +145,10 @@ constexpr int kGrid = 256;       // one workgroup per CU
 constexpr int kStep = 64;        // keys of a step: four units
 constexpr int kMinSteps = 8;     // a piece has a step for each wave, where contexts are cut
 // What a segment costs beside its steps (look-ups, queries, the join of the waves), in steps, where shares of many
-// segments are cut: 128 entries of 32 to 8,192 keys take 91 us with it, 140 without (the slowest workgroup had the
+// segments are cut: 128 entries of 32 to 8,192 keys went from 140 to 91 us with it (the slowest workgroup had the
 // most segments).
 constexpr int kHead = 24;
 constexpr float kLowest = -3.402823466e38f;
-constexpr int kStage = 16384;    // LDS bytes of pages per wave: one step ahead at head_dim 128, two at 64
 
 struct HeadPlan {  // host-chosen shape of a tiled call
   int RT, RG, rpg, D, upb, equal;  // row tiles, row groups, rows of one, head_dim, units per block, pieces of equal length
@@ -240,11 +239,13 @@ template <int QT, int D, int RT>
 __global__ __launch_bounds__(kTileThreads, 2) void head_attn_tile_kernel(HeadAttn p, HeadPlan pl) {
   constexpr bool F16 = QT == SPV_F16, kF16W = Parts<QT>::half;
   constexpr int NQ = Parts<QT>::Q, NP = Parts<QT>::P, R = RT * 16, NCH = D / 32, NDT = D / 16;
-  constexpr int kUnit = 16 * D, kHalf = 4 * kUnit, NS = kStage / (2 * kHalf);  // bytes of a unit, of a step's K or V; steps ahead
+  constexpr int kUnit = 16 * D, kHalf = 4 * kUnit;  // bytes of a unit, of a step's K or V
   constexpr int NK = kHalf / 1024;                                           // loads of a step's K, or V
-  constexpr int kCols = 8 * R * (D + 4) * 4 <= 8 * kStage ? D : 8 * R * (64 + 4) * 4 <= 8 * kStage && D > 64 ? 64 : 32, kColPad = 4;
+  // The waves' sums are joined in as many dims at once as fit where the pages were (at least 64).
+  constexpr int kColPad = 4, kCols = D == 64 || R * (D + kColPad) * 4 <= 2 * kHalf ? D : 64;
+  constexpr int kStage = 2 * kHalf > R * (kCols + kColPad) * 4 ? 2 * kHalf : R * (kCols + kColPad) * 4;
   constexpr bool kQReg = RT * NCH * NQ <= 4;  // queries in registers, where they are few
-  __shared__ __align__(1024) uint8_t s_page[kWaves * kStage];  // [wave][stage][K | V]; the waves' sums later
+  __shared__ __align__(1024) uint8_t s_page[kWaves * kStage];  // [wave][K | V]; the waves' sums later
   __shared__ __align__(16) u32x4_t s_q[NQ * RT * NCH * 64];
   __shared__ float s_ml[2][kWaves][R];
   __shared__ float s_row[2][R];  // joined maximum and sum
@@ -430,43 +431,32 @@ __global__ __launch_bounds__(kTileThreads, 2) void head_attn_tile_kernel(HeadAtt
     const int krow = D == 128 ? lane >> 3 : lane >> 2;
     const uint32_t kvoff = D == 128 ? krow * 128 + (((lane & 7) ^ ((krow >> 1) & 1)) * 16) : krow * 64 + (lane & 3) * 16;
     const uint32_t vvoff = (uint32_t)lane * (uint32_t)p.bs;
-    float2 sc[NS];  // scales of the lane's keys of the next steps
+    float2 sc = {0.f, 0.f};  // scales of the lane's keys of the step ahead
     auto fetch_k = [&](int k) {
       if ((k & 15) == 0) look_up(k);
-      uint8_t* const to = stage0 + (k % NS) * 2 * kHalf;
 #pragma unroll
       for (int u = 0; u < 4; ++u) {
         const int at = (k & 15) * 4 + u;
         const uint8_t* const from = unit_from(kbase, l_k, at);
         const uint32_t lo = kvoff ^ (D == 128 ? u * 32 : u * 16);
-        page_to_lds<0>(from + lo, to + u * kUnit);
-        if constexpr (D == 128) page_to_lds<1024>(from + lo, to + u * kUnit);
+        page_to_lds<0>(from + lo, stage0 + u * kUnit);
+        if constexpr (D == 128) page_to_lds<1024>(from + lo, stage0 + u * kUnit);
       }
       const int at = (k & 15) * 4 + g;
-#pragma unroll
-      for (int i = 0; i + 1 < NS; ++i) sc[i] = sc[i + 1];
-      sc[NS - 1] = make_float2(__shfl(l_scale.x, at, 64), __shfl(l_scale.y, at, 64));
+      sc = make_float2(__shfl(l_scale.x, at, 64), __shfl(l_scale.y, at, 64));
     };
     auto fetch_v = [&](int k) {
-      uint8_t* const to = stage0 + (k % NS) * 2 * kHalf + kHalf;
 #pragma unroll
       for (int u = 0; u < 4; ++u) {
         const int at = (k & 15) * 4 + u;
         const uint8_t* const from = unit_from(vbase, l_v, at);
-        page_to_lds<0>(from + vvoff, to + u * kUnit);
-        if constexpr (D == 128) page_to_lds<0>(from + (size_t)64 * p.bs + vvoff, to + u * kUnit + 1024);
+        page_to_lds<0>(from + vvoff, stage0 + kHalf + u * kUnit);
+        if constexpr (D == 128) page_to_lds<0>(from + (size_t)64 * p.bs + vvoff, stage0 + kHalf + u * kUnit + 1024);
       }
     };
-#pragma unroll
-    for (int i = 0; i < NS; ++i) sc[i] = make_float2(0.f, 0.f);
-#pragma unroll
-    for (int i = 0; i < NS; ++i) {
-      if (i < steps) {
-        fetch_k(i);
-        fetch_v(i);
-      } else if (i) {
-        sc[NS - 2 < 0 ? 0 : NS - 2] = sc[NS - 1];  // one step: its scales come first
-      }
+    if (steps > 0) {
+      fetch_k(0);
+      fetch_v(0);
     }
 
     // ---- queries to LDS as operands: [part][row tile][chunk][lane] 16 bytes; dims of a chunk as K's pieces go
@@ -547,18 +537,16 @@ __global__ __launch_bounds__(kTileThreads, 2) void head_attn_tile_kernel(HeadAtt
                          ((g ^ (D == 128 ? ((c >> 1) & 1) | (c >> 2) << 1 : c >> 2)) * 16);
     const uint32_t vat = base0 + kHalf + g * kUnit + c * 16;
 
-    auto run_step = [&](int k, auto more_tag) {
-      constexpr bool MORE = decltype(more_tag)::value;  // step k + NS exists
+    auto run_step = [&](int k, auto more) {  // more: step k + 1 exists
       const int step = step_at(k);
-      const uint32_t at = (k % NS) * 2 * kHalf;
       const bool masked = (step + 1) * kStep > all_see;
-      const float ksc = sc[0].x * factor, vsc = sc[0].y;
+      const float ksc = sc.x * factor, vsc = sc.y;
       const int base = step * kStep + g * 16;  // the lane's first key
       // Weights where no key is masked and the scales allow it: 2^(z - m) and V's scale in one power, for bf16
       // queries what the scale is over a power of two, which goes into V's conversion; their sum is theirs without it.
       // Elsewhere, and for fp32 queries, one after the other and in parts of bf16.
       const int vexp = vsc > 0.f ? __builtin_amdgcn_frexp_expf(vsc) - 1 : -200;  // s_v in [2^vexp, 2^(vexp + 1))
-      bool plain = QT == SPV_F32 || masked;
+      bool careful = QT == SPV_F32 || masked;
       if constexpr (kF16W) {
         if (__any(vexp > unit_exp + 7)) {  // O's unit 2^unit_exp follows the scales
           int top = vexp;
@@ -573,199 +561,203 @@ __global__ __launch_bounds__(kTileThreads, 2) void head_attn_tile_kernel(HeadAtt
               for (int i = 0; i < 4; ++i) o[rt][dt][i] = ldexpf(o[rt][dt][i], unit_exp - top);
           unit_exp = top;
         }
-        plain |= (bool)__any(vexp < unit_exp - 15 || !(vsc > 0.f));
+        careful |= (bool)__any(vexp < unit_exp - 15 || !(vsc > 0.f));
       } else {
-        plain |= (bool)__any(!(vsc > 0x1p-60f && vsc < 0x1p60f));
+        careful |= (bool)__any(!(vsc > 0x1p-60f && vsc < 0x1p60f));
       }
-      // s_v times 2^vshift is what a weight takes; in fp16 the part of it in [1, 2), times 2^kHalfShift.
-      const float vpart = kF16W ? ldexpf(vsc, kHalfShift - vexp) : vsc;
-      const float vlog = __builtin_amdgcn_logf(vpart), vinv = __builtin_amdgcn_rcpf(vpart);
-      const float vall = kF16W ? ldexpf(vsc, kHalfShift - unit_exp) : vsc;
-      const float vpow = __uint_as_float((uint32_t)(min(max(vexp - unit_exp, -15), 7) + 127) << 23);
-      auto lift = [&](int rt, float top) {
-        top = fmaxf(top, __shfl_xor(top, 16, 64));
-        top = fmaxf(top, __shfl_xor(top, 32, 64));
-        const float mn = fmaxf(m[rt], top), keep = __builtin_amdgcn_exp2f(m[rt] - mn);
-        m[rt] = mn;
-        l[rt] *= keep;
+      auto body = [&](auto plain, auto more_tag) {
+        constexpr bool MORE = decltype(more_tag)::value;
+        // s_v times 2^vshift is what a weight takes; in fp16 the part of it in [1, 2), times 2^kHalfShift.
+        const float vpart = kF16W ? ldexpf(vsc, kHalfShift - vexp) : vsc;
+        const float vlog = __builtin_amdgcn_logf(vpart), vinv = __builtin_amdgcn_rcpf(vpart);
+        const float vall = kF16W ? ldexpf(vsc, kHalfShift - unit_exp) : vsc;
+        const float vpow = __uint_as_float((uint32_t)(min(max(vexp - unit_exp, -15), 7) + 127) << 23);
+        auto lift = [&](int rt, float top) {
+          top = fmaxf(top, __shfl_xor(top, 16, 64));
+          top = fmaxf(top, __shfl_xor(top, 32, 64));
+          const float mn = fmaxf(m[rt], top), keep = __builtin_amdgcn_exp2f(m[rt] - mn);
+          m[rt] = mn;
+          l[rt] *= keep;
 #pragma unroll
-        for (int dt = 0; dt < NDT; ++dt) o[rt][dt] *= keep;
-      };
-      // K of this step is there: behind it came its V, and what was fetched ahead.
-      if constexpr (MORE && NS > 1) wait_loads<(NS - 1) * 2 * NK + NK>();
-      else if (NS > 1 && k + 1 < steps) wait_loads<2 * NK + NK>();
-      else wait_loads<NK>();
-      f32x4_t s[RT][4];
+          for (int dt = 0; dt < NDT; ++dt) o[rt][dt] *= keep;
+        };
+        wait_loads<NK>();  // K of this step is there: behind it came its V
+        f32x4_t s[RT][4];
 #pragma unroll
-      for (int rt = 0; rt < RT; ++rt)
+        for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
-        for (int t = 0; t < 4; ++t) s[rt][t] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+          for (int t = 0; t < 4; ++t) s[rt][t] = f32x4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int cc = 0; cc < D / 64; ++cc) {
-        u32x4_t kw[4];
-        lds_read4<0, 4 * D>(kw, (at + kat) ^ (cc * 64));
+        for (int cc = 0; cc < D / 64; ++cc) {
+          u32x4_t kw[4];
+          lds_read4<0, 4 * D>(kw, kat ^ (cc * 64));
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          const int ch = 2 * cc + half;
-          u32x4_t qv[RT][NQ];
+          for (int half = 0; half < 2; ++half) {
+            const int ch = 2 * cc + half;
+            u32x4_t qv[RT][NQ];
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+              for (int q = 0; q < NQ; ++q) {
+                if constexpr (kQReg) qv[rt][q] = qreg[rt][ch][q];
+                else qv[rt][q] = query(rt, ch, q);
+              }
+#pragma unroll
+            for (int t = 0; t < 4; ++t) {
+              const u32x4_t kop = operand<F16>(kw[t][2 * half], kw[t][2 * half + 1]);
+#pragma unroll
+              for (int q = NQ - 1; q >= 0; --q)
+#pragma unroll
+                for (int rt = 0; rt < RT; ++rt) s[rt][t] = mfma<F16>(kop, qv[rt][q], s[rt][t]);
+            }
+            if constexpr (RT > 2) __builtin_amdgcn_sched_barrier(0);
+          }
+        }
+        if constexpr (MORE) fetch_k(k + 1);
+        uint32_t pw[RT][2][NP][4];
+        float top[RT];
+        if (plain) {
+#pragma unroll
+          for (int rt = 0; rt < RT; ++rt) {
+            top[rt] = -INFINITY;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              const float z = base + i < seen[rt] ? s[rt][i >> 2][i & 3] * ksc : -INFINITY;
+              s[rt][i >> 2][i & 3] = z;
+              top[rt] = fmaxf(top[rt], z);
+            }
+          }
+        } else {
+#pragma unroll
+          for (int rt = 0; rt < RT; ++rt) {
+            top[rt] = s[rt][0][0];
+#pragma unroll
+            for (int i = 1; i < 16; ++i) top[rt] = fmaxf(top[rt], s[rt][i >> 2][i & 3]);
+            top[rt] *= ksc;
+          }
+        }
+        bool higher = false;
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) higher |= top[rt] > m[rt] + Parts<QT>::lift;
+        if (__any(higher)) {
+#pragma unroll
+          for (int rt = 0; rt < RT; ++rt) lift(rt, top[rt]);
+        }
+        if (plain) {
 #pragma unroll
           for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
-            for (int q = 0; q < NQ; ++q) {
-              if constexpr (kQReg) qv[rt][q] = qreg[rt][ch][q];
-              else qv[rt][q] = query(rt, ch, q);
+            for (int i = 0; i < 16; ++i) {
+              const float e = __builtin_amdgcn_exp2f(s[rt][i >> 2][i & 3] - m[rt]);
+              l[rt] += e;
+              s[rt][i >> 2][i & 3] = e * vall;
             }
+        } else {
 #pragma unroll
-          for (int t = 0; t < 4; ++t) {
-            const u32x4_t kop = operand<F16>(kw[t][2 * half], kw[t][2 * half + 1]);
+          for (int rt = 0; rt < RT; ++rt) {
+            const float off = vlog - m[rt];
+            float sum = 0.f;
 #pragma unroll
-            for (int q = NQ - 1; q >= 0; --q)
-#pragma unroll
-              for (int rt = 0; rt < RT; ++rt) s[rt][t] = mfma<F16>(kop, qv[rt][q], s[rt][t]);
-          }
-          if constexpr (RT > 2) __builtin_amdgcn_sched_barrier(0);
-        }
-      }
-      if constexpr (MORE) fetch_k(k + NS);
-      else if constexpr (NS > 1) sc[0] = sc[NS - 1];
-      uint32_t pw[RT][2][NP][4];
-      float top[RT];
-      if (plain) {
-#pragma unroll
-        for (int rt = 0; rt < RT; ++rt) {
-          top[rt] = -INFINITY;
-#pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const float z = base + i < seen[rt] ? s[rt][i >> 2][i & 3] * ksc : -INFINITY;
-            s[rt][i >> 2][i & 3] = z;
-            top[rt] = fmaxf(top[rt], z);
+            for (int i = 0; i < 16; ++i) {
+              const float w = __builtin_amdgcn_exp2f(fmaf(s[rt][i >> 2][i & 3], ksc, off));
+              s[rt][i >> 2][i & 3] = w;
+              sum += w;
+            }
+            l[rt] = fmaf(sum, vinv, l[rt]);
           }
         }
-      } else {
+        if (kF16W && !plain) {
 #pragma unroll
-        for (int rt = 0; rt < RT; ++rt) {
-          top[rt] = s[rt][0][0];
+          for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
-          for (int i = 1; i < 16; ++i) top[rt] = fmaxf(top[rt], s[rt][i >> 2][i & 3]);
-          top[rt] *= ksc;
+            for (int i = 0; i < 8; ++i)
+              pw[rt][i >> 2][0][i & 3] = pack_f16(s[rt][i >> 1][2 * (i & 1)], s[rt][i >> 1][2 * (i & 1) + 1]);
+        } else {
+#pragma unroll
+          for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+            for (int q = 0; q < NP; ++q)
+#pragma unroll
+              for (int i = 0; i < 8; ++i) {
+                const float x = s[rt][i >> 1][2 * (i & 1)], y = s[rt][i >> 1][2 * (i & 1) + 1];
+                const uint32_t u = pack_bf16(x, y);
+                pw[rt][i >> 2][q][i & 3] = u;
+                if (q + 1 < NP) {
+                  s[rt][i >> 1][2 * (i & 1)] = x - __uint_as_float(u << 16);
+                  s[rt][i >> 1][2 * (i & 1) + 1] = y - __uint_as_float(u & 0xffff0000u);
+                }
+              }
         }
-      }
-      bool higher = false;
+        // V of this step is there: behind it came K of the next.
+        if constexpr (MORE) wait_loads<NK>();
+        else wait_loads<0>();
 #pragma unroll
-      for (int rt = 0; rt < RT; ++rt) higher |= top[rt] > m[rt] + Parts<QT>::lift;
-      if (__any(higher)) {
+        for (int d4 = 0; d4 < NDT / 4; ++d4) {
+          u32x4_t vw[4];
+          if (d4 == 0) lds_read4<0, 256>(vw, vat);
+          else lds_read4<1024, 256>(vw, vat);
+          if (masked) {  // values behind the rows' last key are not looked at
+            const int valid = keys - base;
+            uint32_t bad = 0;
 #pragma unroll
-        for (int rt = 0; rt < RT; ++rt) lift(rt, top[rt]);
-      }
-      if (plain) {
+            for (int i = 0; i < 4; ++i) {
+              const int nb = min(max(valid - 4 * i, 0), 4);
+              const uint32_t in = nb == 4 ? 0xffffffffu : (1u << (8 * nb)) - 1u;
 #pragma unroll
-        for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const float e = __builtin_amdgcn_exp2f(s[rt][i >> 2][i & 3] - m[rt]);
-            l[rt] += e;
-            s[rt][i >> 2][i & 3] = e * vall;
-          }
-      } else {
-#pragma unroll
-        for (int rt = 0; rt < RT; ++rt) {
-          const float off = vlog - m[rt];
-          float sum = 0.f;
-#pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const float w = __builtin_amdgcn_exp2f(fmaf(s[rt][i >> 2][i & 3], ksc, off));
-            s[rt][i >> 2][i & 3] = w;
-            sum += w;
-          }
-          l[rt] = fmaf(sum, vinv, l[rt]);
-        }
-      }
-      if (kF16W && !plain) {
-#pragma unroll
-        for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-          for (int i = 0; i < 8; ++i)
-            pw[rt][i >> 2][0][i & 3] = pack_f16(s[rt][i >> 1][2 * (i & 1)], s[rt][i >> 1][2 * (i & 1) + 1]);
-      } else {
-#pragma unroll
-        for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-          for (int q = 0; q < NP; ++q)
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              const float x = s[rt][i >> 1][2 * (i & 1)], y = s[rt][i >> 1][2 * (i & 1) + 1];
-              const uint32_t u = pack_bf16(x, y);
-              pw[rt][i >> 2][q][i & 3] = u;
-              if (q + 1 < NP) {
-                s[rt][i >> 1][2 * (i & 1)] = x - __uint_as_float(u << 16);
-                s[rt][i >> 1][2 * (i & 1) + 1] = y - __uint_as_float(u & 0xffff0000u);
+              for (int dt = 0; dt < 4; ++dt) {
+                vw[dt][i] &= in;
+                bad |= nan_codes(vw[dt][i]);
               }
             }
-      }
-      // V of this step is there: behind it came what was fetched ahead, and K of step k + NS.
-      if constexpr (MORE) wait_loads<(NS - 1) * 2 * NK + NK>();
-      else if (NS > 1 && k + 1 < steps) wait_loads<2 * NK>();
-      else wait_loads<0>();
-#pragma unroll
-      for (int d4 = 0; d4 < NDT / 4; ++d4) {
-        u32x4_t vw[4];
-        if (d4 == 0) lds_read4<0, 256>(vw, at + vat);
-        else lds_read4<1024, 256>(vw, at + vat);
-        if (masked) {  // values behind the rows' last key are not looked at
-          const int valid = keys - base;
-          uint32_t bad = 0;
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int nb = min(max(valid - 4 * i, 0), 4);
-            const uint32_t in = nb == 4 ? 0xffffffffu : (1u << (8 * nb)) - 1u;
-#pragma unroll
-            for (int dt = 0; dt < 4; ++dt) {
-              vw[dt][i] &= in;
-              bad |= nan_codes(vw[dt][i]);
-            }
-          }
-          // A NaN among the chunk's own values reaches the rows that see it, and no other: it is taken out here, and
-          // what remembers it is the first key of each dim that holds one.
-          if (__any(bad != 0)) {
-#pragma unroll
-            for (int dt = 0; dt < 4; ++dt)
-#pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                const uint32_t w = nan_codes(vw[dt][i]);
-                if (w) atomicMin(&s_nan[(4 * d4 + dt) * 16 + c], base + 4 * i + (__ffs(w) >> 3) - 1);
-                vw[dt][i] &= ~((w >> 7) * 0xffu);
-              }
-          }
-        }
-#pragma unroll
-        for (int mm = 0; mm < 2; ++mm) {  // eight sums in turn, so that none waits for its last addition
-          auto weights = [&](int rt, int q) {
-            return u32x4_t{pw[rt][mm][q][0], pw[rt][mm][q][1], pw[rt][mm][q][2], pw[rt][mm][q][3]};
-          };
-          u32x4_t vop[4];
-          if (kF16W && !plain) {
-#pragma unroll
-            for (int dt = 0; dt < 4; ++dt) vop[dt] = operand<true>(vw[dt][2 * mm], vw[dt][2 * mm + 1], vpow);
-#pragma unroll
-            for (int dt = 0; dt < 4; ++dt)
-#pragma unroll
-              for (int rt = 0; rt < RT; ++rt) o[rt][4 * d4 + dt] = mfma<true>(vop[dt], weights(rt, 0), o[rt][4 * d4 + dt]);
-          } else {
-#pragma unroll
-            for (int dt = 0; dt < 4; ++dt) vop[dt] = operand<false>(vw[dt][2 * mm], vw[dt][2 * mm + 1]);
-#pragma unroll
-            for (int q = NP - 1; q >= 0; --q)
+            // A NaN among the chunk's own values reaches the rows that see it, and no other: it is taken out here, and
+            // what remembers it is the first key of each dim that holds one.
+            if (__any(bad != 0)) {
 #pragma unroll
               for (int dt = 0; dt < 4; ++dt)
 #pragma unroll
-                for (int rt = 0; rt < RT; ++rt) o[rt][4 * d4 + dt] = mfma<false>(vop[dt], weights(rt, q), o[rt][4 * d4 + dt]);
+                for (int i = 0; i < 4; ++i) {
+                  const uint32_t w = nan_codes(vw[dt][i]);
+                  if (w) atomicMin(&s_nan[(4 * d4 + dt) * 16 + c], base + 4 * i + (__ffs(w) >> 3) - 1);
+                  vw[dt][i] &= ~((w >> 7) * 0xffu);
+                }
+            }
+          }
+#pragma unroll
+          for (int mm = 0; mm < 2; ++mm) {  // eight sums in turn, so that none waits for its last addition
+            auto weights = [&](int rt, int q) {
+              return u32x4_t{pw[rt][mm][q][0], pw[rt][mm][q][1], pw[rt][mm][q][2], pw[rt][mm][q][3]};
+            };
+            u32x4_t vop[4];
+            if (kF16W && !plain) {
+#pragma unroll
+              for (int dt = 0; dt < 4; ++dt) vop[dt] = operand<true>(vw[dt][2 * mm], vw[dt][2 * mm + 1], vpow);
+#pragma unroll
+              for (int dt = 0; dt < 4; ++dt)
+#pragma unroll
+                for (int rt = 0; rt < RT; ++rt) o[rt][4 * d4 + dt] = mfma<true>(vop[dt], weights(rt, 0), o[rt][4 * d4 + dt]);
+            } else {
+#pragma unroll
+              for (int dt = 0; dt < 4; ++dt) vop[dt] = operand<false>(vw[dt][2 * mm], vw[dt][2 * mm + 1]);
+#pragma unroll
+              for (int q = NP - 1; q >= 0; --q)
+#pragma unroll
+                for (int dt = 0; dt < 4; ++dt)
+#pragma unroll
+                  for (int rt = 0; rt < RT; ++rt) o[rt][4 * d4 + dt] = mfma<false>(vop[dt], weights(rt, q), o[rt][4 * d4 + dt]);
+            }
           }
         }
-      }
-      if constexpr (MORE) fetch_v(k + NS);
+        if constexpr (MORE) fetch_v(k + 1);
+      };
+      // A body of its own for the ordinary steps (16 contexts of 32,768 keys, D = 64: 46.5 us, 49.3 without), where
+      // registers allow two: at D = 128 they spill (91 us become 132 at 128 contexts of 32 to 8,192 keys).
+      if constexpr (QT == SPV_F32) body(std::true_type{}, more);
+      else if constexpr (D > 64) body(careful, more);
+      else if (careful) body(std::true_type{}, more);
+      else body(std::false_type{}, more);
     };
     int k_step = 0;
-    for (; k_step + NS < steps; ++k_step) run_step(k_step, std::true_type{});
+    for (; k_step + 1 < steps; ++k_step) run_step(k_step, std::true_type{});
     for (; k_step < steps; ++k_step) run_step(k_step, std::false_type{});
 
     // ---- the waves' sums, joined in their order
