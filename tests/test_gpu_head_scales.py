@@ -174,6 +174,28 @@ def test_device_writes_of_views(cuda, layout):
     _same(gpu, cpu)
 
 
+@pytest.mark.parametrize("dtype,H,d,bs", [(F32, 2, 128, 16), (BF16, 3, 64, 64), (F32, 1, 80, 48), (F32, 2, 64, 32)])
+def test_pieces_of_pages(cuda, dtype, H, d, bs):
+    """Chunks that begin and end inside a page's 16-byte pieces, under scales that grow from 1e-25 to 1e25 (past
+    what a rounded reciprocal may stand in for, both ways), rows at odd addresses beside aligned ones."""
+    g = torch.Generator().manual_seed(d + bs)
+    gpu, cpu = _pair(cuda, 1, H, d, 16, bs, 1)
+    odd, _ = _pair(cuda, 1, H, d, 16, bs, 1)
+    at, C = 0, bs // 2 + 5
+    for mag in (1e-25, 1e-19, 1e-18, 1e-6, 1.0, 0.3, 77.7, 1e17, 1e18, 1e25):
+        for start in (at, max(0, at - C + 3)):
+            kn, vn = ((torch.randn(1, C, H, d, generator=g) * mag).to(dtype) for _ in range(2))
+            kn[0, 1, 0, :4] = torch.tensor([0.0, -0.0, 448.0, -1e-30])
+            gpu.write_block(0, [0], [start], kn.to(cuda), vn.to(cuda))
+            cpu.write_block(0, [0], [start], kn, vn)
+            wide = torch.zeros(2, 1, C, H, d + 1, dtype=dtype, device=cuda)
+            wide[0, ..., 1:], wide[1, ..., 1:] = kn.to(cuda), vn.to(cuda)
+            odd.write_block(0, [0], [start], wide[0, ..., 1:], wide[1, ..., 1:])
+        at += 7
+        _same(gpu, cpu)
+        _same(odd, cpu)
+
+
 def test_exhaustion_and_table_width(cuda):
     gpu, cpu = _pair(cuda, 2, 2, 16, 5, 4, 3)
     g = torch.Generator().manual_seed(3)
