@@ -354,9 +354,11 @@ int spv_verify_attn(void* out, const void* q, int q_dtype,
 /* spv_verify_attn over a pool of spv_kv_append_fp8_heads: q and out in q_dtype
  * (f32, bf16 or f16), the rest as there (the forbidden reads and ctr[7] too).
  * What a masked position holds, NaN included, reaches no output. The workspace
- * (of the size below, zero-filled before its first use) holds arrival counters,
- * which every call leaves at zero, and partials; calls that share one are ordered.
- * head_dim <= 2,048 (SPV_ERR_UNSUPPORTED beyond). */
+ * (of the size below) holds arrival counters in its first SPV_HEADS_COUNTER_BYTES,
+ * which must be zero before its first use and which every call leaves at zero, and
+ * partials; calls that share one are ordered. head_dim <= 2,048
+ * (SPV_ERR_UNSUPPORTED beyond). */
+#define SPV_HEADS_COUNTER_BYTES 1024
 size_t spv_verify_attn_fp8_heads_workspace_bytes(int32_t B, int32_t C, int32_t num_q_heads,
                                                  int32_t num_kv_heads, int32_t head_dim,
                                                  int32_t block_size, int32_t max_ctx);

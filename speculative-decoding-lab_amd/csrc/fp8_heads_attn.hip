@@ -907,7 +907,8 @@ bool tile_plan(int32_t B, int32_t C, int32_t Hq, int32_t Hkv, int32_t d, int32_t
   return true;
 }
 
-constexpr size_t kCounterBytes = kGrid * sizeof(int);  // at the same place for calls of every shape
+constexpr size_t kCounterBytes = SPV_HEADS_COUNTER_BYTES;  // at the same place for calls of every shape
+static_assert(kCounterBytes == kGrid * sizeof(int));
 size_t tile_bytes(const HeadPlan& pl) {
   return kCounterBytes + (size_t)2 * kGrid * pl.RT * 16 * (pl.D + 2) * sizeof(float);
 }

@@ -23,6 +23,7 @@ SPV_ERR_LAUNCH = -2
 SPV_ERR_WORKSPACE = -3
 SPV_ERR_UNSUPPORTED = -4
 SPV_CTR_WORDS = 16
+SPV_HEADS_COUNTER_BYTES = 1024
 CTR_TOP, CTR_EXHAUSTED, CTR_SLOWPATH, CTR_PUSHED = 0, 1, 2, 3
 CTR_OVERFLOW, CTR_BAD_READ, CTR_ALIGN = 6, 7, 8  # sticky error words (see include/specverify.h)
 # bits of a sequence's flag word (sampling): a result the reference may have decided otherwise

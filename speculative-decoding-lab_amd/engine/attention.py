@@ -262,10 +262,13 @@ def _attend_heads(q, kv, layer, seq_ids, start_positions, max_ctx, scale, out, p
     stream = _hip.stream_of(kv.device)
     ws = None
     if nbytes:
-        # A captured graph has a workspace of its own, cleared by a node of its own in every
-        # replay: graphs that share one could not run side by side.
-        ws = torch.zeros(nbytes, dtype=torch.uint8, device=kv.device) \
-            if torch.cuda.is_current_stream_capturing() else _heads_workspace.get(nbytes, kv.device, stream)
+        # A captured graph has a workspace of its own, whose counters a node of its own clears in
+        # every replay: graphs that share one could not run side by side.
+        if torch.cuda.is_current_stream_capturing():
+            ws = torch.empty(nbytes, dtype=torch.uint8, device=kv.device)
+            ws[:_hip.SPV_HEADS_COUNTER_BYTES].zero_()
+        else:
+            ws = _heads_workspace.get(nbytes, kv.device, stream)
     call("spv_verify_attn_fp8_heads", out.data_ptr(), q.data_ptr(), _hip.dtype_code(q.dtype), kv.k_pool.data_ptr(),
          kv.v_pool.data_ptr(), kv.scales.data_ptr(), kv.tables_dev.data_ptr(), kv._maxb, sid_t.data_ptr(),
          start_t.data_ptr(), kv.lens_dev.data_ptr(), kv.allocator.ctr.data_ptr(), B, chunk, hq, kv.num_kv_heads, d,

@@ -652,6 +652,45 @@ def test_verify_step_and_appending_attention(cuda):
         kv.rewind_append_device(sid, None, None, st, k[0], v[0])
 
 
+@pytest.mark.parametrize("hq,H,d", [(14, 2, 64), (12, 2, 128)])
+def test_draft_loop(cuda, hq, H, d):
+    """Draft steps of several layers, eager and as one captured graph (many attention calls in one pool of
+    memory): the same bits in every replay, and float64's attention of what is stored."""
+    from engine.spec_scheduler import DraftLoop
+
+    g = torch.Generator().manual_seed(d)
+    layers, gamma, B, V, ctx = 3, 3, 4, 97, [700, 15, 33, 1]
+    kv = PagedKVCache(layers, H, d, 128, 16, cuda, FP8, head_scales=True)
+    for s, n in enumerate(ctx):
+        kv.add_sequence(s)
+        for layer in range(layers):
+            kv.write_block(layer, [s], [0], *(torch.randn(1, n, H, d, generator=g).to(BF16).to(cuda) for _ in "kv"))
+    q, k, v = ([[torch.randn(B, 1, n, d, generator=g).to(BF16).to(cuda) for _ in range(layers)] for _ in range(gamma)]
+               for n in (hq, H, H))
+    logits = [torch.randn(B, V, generator=g).to(cuda) for _ in range(gamma)]
+    noise = [torch.empty(B, V).exponential_(generator=g).to(cuda) for _ in range(gamma)]
+    sid, at = (torch.tensor(x, dtype=torch.int32, device=cuda) for x in (range(B), ctx))
+    loop = DraftLoop(kv, gamma, 1.0)
+    run = lambda: loop.run(sid, at, max(ctx), q, k, v, logits, noise)  # noqa: E731
+    run()
+    want_p, want = run()  # the same rows again, into scales that no longer grow
+    for layer in range(layers):
+        _check(want[-1][layer], q[-1][layer], kv, layer, list(range(B)), [n + gamma - 1 for n in ctx])
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got_p, got = run()
+    before = kv.k_pool.view(torch.uint8).clone()
+    for _ in range(3):
+        for row in got:
+            for o in row:
+                o.zero_()
+        verify_attention(q[0][0], kv, 0, sid, at, max(ctx) + 1)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(got_p, want_p) and torch.equal(kv.k_pool.view(torch.uint8), before)
+        assert all(torch.equal(a, b) for x, y in zip(got, want) for a, b in zip(x, y))
+
+
 def test_alignment_clears_the_scales(cuda):
     """Blocks that a draft alignment hands out start with zero scales in every layer and head."""
     kv = PagedKVCache(2, 3, 16, 8, 4, cuda, FP8, head_scales=True)
