@@ -25,7 +25,7 @@ struct HeadWrite {
   RotaryParams r;  // keys, values, pools and tables
   RotaryParams q;  // the queries alone (Hkv = 0)
   float* scales;
-  int T, tile, limit_b;  // blocks an entry's chunk touches at most; rows staged at once
+  int T, tile, limit_b;  // blocks an entry's chunk touches at most; rows staged at once (at most)
   unsigned nkv;          // workgroups of keys and values, before those of the queries
 };
 
@@ -37,7 +37,7 @@ __device__ __forceinline__ float wave_max(float x) {
 
 // One workgroup per (entry, block that the chunk touches, kv head); behind them
 // the queries' workgroups of rotary_vec_rows.
-// VEC (16-byte rows, head_dim and blocks of whole 16, the block staged at once): 16 bytes of the page per thread and
+// VEC (16-byte rows, head_dim and blocks of whole 16, a chunk's rows in a block staged at once): 16 bytes of the page per thread and
 // turn, K's dims or V's tokens; of a block that is not wholly new they are asked for before the rows are turned.
 // Byte by byte, prompts of 4 x 3,001 tokens with two kv heads of 128 took 21.4 us (now 12.1), 32 verify chunks of 6
 // tokens 9.8 (now 8.5).
@@ -190,9 +190,9 @@ __global__ __launch_bounds__(kThreads) void head_write_kernel(HeadWrite w, VecSh
     }
   };
   // Tiles of the block's rows; one that holds them all is staged once.
-  const int t0 = lo / w.tile, t1 = (hi - 1) / w.tile;
-  auto first = [&](int k) { return max(lo, k * w.tile); };
-  auto last = [&](int k) { return min(hi, (k + 1) * w.tile); };
+  const int t0 = VEC ? 0 : lo / w.tile, t1 = VEC ? 0 : (hi - 1) / w.tile;
+  auto first = [&](int k) { return VEC ? lo : max(lo, k * w.tile); };
+  auto last = [&](int k) { return VEC ? hi : min(hi, (k + 1) * w.tile); };
   for (int k = t0; k <= t1; ++k) {
     if (k > t0) __syncthreads();
     stage(first(k), last(k));
@@ -382,6 +382,7 @@ __global__ __launch_bounds__(kThreads) void head_read_vec_kernel(HeadRead p) {
 }
 
 constexpr size_t kLdsBytes = 65536;
+constexpr size_t kVecLdsBytes = 158720;  // VEC: of 160 KiB, with what the kernel has beside it
 
 // LDS of a key / value workgroup that stages `rows` rows at once.
 size_t write_lds(int rows, int d, int R, bool turn) {
@@ -399,8 +400,14 @@ int write_tile(int bs, int d, int R, bool turn) {
 template <int IT, bool VEC>
 void launch_write(const HeadWrite& w, const VecShape& v, bool turn, bool norm, bool query, unsigned grid, size_t smem,
                   hipStream_t s) {
-#define SPV_W(TURN, NORM, QUERY) \
-  hipLaunchKernelGGL((head_write_kernel<IT, TURN, NORM, QUERY, VEC>), dim3(grid), dim3(kThreads), smem, s, w, v)
+#define SPV_W(TURN, NORM, QUERY)                                                                                \
+  do {                                                                                                          \
+    if (smem > 65536)                                                                                           \
+      (void)hipFuncSetAttribute(reinterpret_cast<const void*>(&head_write_kernel<IT, TURN, NORM, QUERY, VEC>),  \
+                                hipFuncAttributeMaxDynamicSharedMemorySize, (int)smem);                         \
+    hipLaunchKernelGGL((head_write_kernel<IT, TURN, NORM, QUERY, VEC>), dim3(grid), dim3(kThreads), smem, s, w, \
+                       v);                                                                                      \
+  } while (0)
   if (!turn) SPV_W(false, false, false);
   else if (!norm && !query) SPV_W(true, false, false);
   else if (!norm) SPV_W(true, false, true);
@@ -458,7 +465,7 @@ int write(HeadWrite& w, const PoolArgs& a, int dtype, bool turn, bool norm, int3
   if (!w.tile) return SPV_ERR_UNSUPPORTED;
   const long long nkv = (long long)p.B * w.T * p.Hkv;
   if (nkv > 0x3fffffffLL) return SPV_ERR_ARG;
-  size_t smem = write_lds(w.tile, p.d, p.R, turn);
+  size_t smem = write_lds(w.tile, p.d, p.R, turn), query_smem = 0;
   w.nkv = (unsigned)nkv;
   VecShape v{};
   bool query = false;
@@ -469,17 +476,23 @@ int write(HeadWrite& w, const PoolArgs& a, int dtype, bool turn, bool norm, int3
     w.q.k = nullptr;
     query = vec_shape(w.q, dtype_size(dtype), false, norm, v);
     if (query) {
-      const size_t qs = vec_lds(w.q, v, dtype_size(dtype), false, norm);
-      if (qs > smem) smem = qs;
+      query_smem = vec_lds(w.q, v, dtype_size(dtype), false, norm);
+      if (query_smem > smem) smem = query_smem;
       grid += (long long)p.B * v.tiles * v.slices;
     }
   }
   if (grid > 0x7fffffffLL) return SPV_ERR_ARG;
-  const size_t weights = norm ? p.d * sizeof(float) : 0;  // vec: in LDS too
-  bool vec = w.tile == p.bs && smem + weights <= kLdsBytes && p.d % 16 == 0 && p.bs % 16 == 0 &&
+  // vec: the rows of a chunk in a block at once, and the weights
+  const int rows = p.bs < p.C ? p.bs : p.C;
+  size_t vec_smem = write_lds(rows, p.d, p.R, turn) + (norm ? p.d * sizeof(float) : 0);
+  if (vec_smem < query_smem) vec_smem = query_smem;
+  bool vec = vec_smem <= kVecLdsBytes && p.d % 16 == 0 && p.bs % 16 == 0 &&
              (((uintptr_t)p.k | (uintptr_t)p.v | (uintptr_t)p.kpool | (uintptr_t)p.vpool) & 15) == 0;
   for (int i = 0; i < 3; ++i) vec = vec && (p.ks[i] * dtype_size(dtype)) % 16 == 0 && (p.vs[i] * dtype_size(dtype)) % 16 == 0;
-  if (vec) smem += weights;
+  if (vec) {
+    w.tile = rows;
+    smem = vec_smem;
+  }
 #define SPV_W(IT) \
   vec ? launch_write<IT, true>(w, v, turn, norm, query, (unsigned)grid, smem, s) \
       : launch_write<IT, false>(w, v, turn, norm, query, (unsigned)grid, smem, s)

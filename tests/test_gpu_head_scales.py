@@ -174,7 +174,8 @@ def test_device_writes_of_views(cuda, layout):
     _same(gpu, cpu)
 
 
-@pytest.mark.parametrize("dtype,H,d,bs", [(F32, 2, 128, 16), (BF16, 3, 64, 64), (F32, 1, 80, 48), (F32, 2, 64, 32)])
+@pytest.mark.parametrize("dtype,H,d,bs", [(F32, 2, 128, 16), (BF16, 3, 64, 64), (F32, 1, 80, 48), (F32, 2, 64, 32),
+                                           (F32, 1, 128, 128), (F16, 1, 256, 64)])
 def test_pieces_of_pages(cuda, dtype, H, d, bs):
     """Chunks that begin and end inside a page's 16-byte pieces, under scales that grow from 1e-25 to 1e25 (past
     what a rounded reciprocal may stand in for, both ways), rows at odd addresses beside aligned ones."""
@@ -244,6 +245,8 @@ def test_rows_outside_the_chunk_keep_their_bytes(cuda):
     (4, 2, 64, 32, 16, 100, False, "dense"),
     (2, 2, 10, 6, 7, 9, True, "dense"),       # no whole pieces
     (2, 1, 256, 256, 64, 130, False, "dense"),  # blocks staged in parts
+    (4, 2, 128, 128, 64, 130, True, "packed"),  # blocks of more than 64 KiB staged at once
+    (4, 2, 64, 64, 64, 5, False, "packed"),     # few rows of a large block
     (2, 2, 64, 64, 16, 5, False, "columns"),
 ])
 def test_rotating_append(cuda, dtype, normed, hq, H, d, R, bs, C, inter, layout):
