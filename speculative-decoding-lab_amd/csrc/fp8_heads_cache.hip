@@ -16,9 +16,8 @@ using namespace spv;
 
 namespace {
 
-constexpr int kThreads = 256;
+constexpr int kThreads = 256, kMaxThreads = 1024;
 constexpr int kRowLanes = 16;                    // threads of a row while it is turned
-constexpr int kRowsAtOnce = kThreads / kRowLanes;
 constexpr int kPad = 16;                         // floats: a wave's four rows on banks of their own
 
 struct HeadWrite {
@@ -45,11 +44,13 @@ __device__ __forceinline__ float wave_max(float x) {
 // together for verify chunks), the norm and rotation of a row by 16 threads (1.8), quotients and stores (1.5); prompts
 // read their rows meanwhile (18.9 MB moved, 3.8 us at the rate of a large copy).
 template <int IT, bool TURN, bool NORM, bool QUERY, bool VEC>
-__global__ __launch_bounds__(kThreads) void head_write_kernel(HeadWrite w, VecShape v) {
+__global__ __launch_bounds__(VEC ? kMaxThreads : kThreads) void head_write_kernel(HeadWrite w, VecShape v) {
   extern __shared__ __align__(16) uint8_t lds[];
-  __shared__ float s_red[2][kThreads / 64];
+  __shared__ float s_red[2][kMaxThreads / 64];
+  const int threads = VEC ? blockDim.x : kThreads;
   if constexpr (QUERY) {
     if (blockIdx.x >= w.nkv) {
+      if (VEC && threadIdx.x >= kVecThreads) return;  // whole waves: barriers do without them
       const int x = blockIdx.x - w.nkv, per = w.q.B * v.tiles;
       rotary_vec_rows<IT, false, NORM>(w.q, v, x % per, x / per, lds);
       return;
@@ -89,7 +90,7 @@ __global__ __launch_bounds__(kThreads) void head_write_kernel(HeadWrite w, VecSh
   float* const sv = sk + (size_t)w.tile * st;
   float2* const turns = reinterpret_cast<float2*>(sv + (size_t)w.tile * st);
   if constexpr (VEC && TURN) {
-    for (int i = threadIdx.x; i < (hi_c - lo) * half; i += kThreads) {
+    for (int i = threadIdx.x; i < (hi_c - lo) * half; i += threads) {
       const int r = i / half, f = i - r * half;
       turns[i] = turn_of(p, b, blk * p.bs + lo - s0 + r, f);
     }
@@ -97,7 +98,7 @@ __global__ __launch_bounds__(kThreads) void head_write_kernel(HeadWrite w, VecSh
   float* const weights = reinterpret_cast<float*>(turns + (size_t)w.tile * half);  // VEC and NORM: of a row
   if constexpr (VEC && NORM) {
     if (p.wk)
-      for (int i = threadIdx.x; i < d; i += kThreads) weights[i] = p.wk[i];
+      for (int i = threadIdx.x; i < d; i += threads) weights[i] = p.wk[i];
   }
   const int hi = min(hi_c, s0 + n - blk * p.bs);
   if (n <= 0 || hi <= lo || blk >= p.maxb || (unsigned)phys >= (unsigned)p.cap) return;  // never outside the pool
@@ -124,7 +125,7 @@ __global__ __launch_bounds__(kThreads) void head_write_kernel(HeadWrite w, VecSh
   auto stage = [&](int ra, int rb) {
     const int j0 = blk * p.bs + ra - s0, rows = rb - ra;
     if constexpr (VEC) {
-      for (int i = threadIdx.x; i < rows * row_pieces; i += kThreads) {
+      for (int i = threadIdx.x; i < rows * row_pieces; i += threads) {
         if (i != (int)threadIdx.x) {
           raw_k = piece_of(p.k, p.ks, i);
           raw_v = piece_of(p.v, p.vs, i);
@@ -145,7 +146,7 @@ __global__ __launch_bounds__(kThreads) void head_write_kernel(HeadWrite w, VecSh
         }
       }
     }
-    for (int i = VEC ? rows * d : threadIdx.x; i < rows * d; i += kThreads) {
+    for (int i = VEC ? rows * d : threadIdx.x; i < rows * d; i += threads) {
       const int r = i / d, e = i - r * d;
       const long long at = (long long)b * p.ks[0] + (long long)(j0 + r) * p.ks[1] + (long long)h * p.ks[2] + e;
       const long long av_at = (long long)b * p.vs[0] + (long long)(j0 + r) * p.vs[1] + (long long)h * p.vs[2] + e;
@@ -156,7 +157,7 @@ __global__ __launch_bounds__(kThreads) void head_write_kernel(HeadWrite w, VecSh
       av = fmaxf(av, finite_abs(xv));
     }
     if constexpr (TURN && !VEC) {
-      for (int i = threadIdx.x; i < rows * half; i += kThreads) {
+      for (int i = threadIdx.x; i < rows * half; i += threads) {
         const int r = i / half, f = i - r * half;
         turns[i] = turn_of(p, b, j0 + r, f);
       }
@@ -164,7 +165,7 @@ __global__ __launch_bounds__(kThreads) void head_write_kernel(HeadWrite w, VecSh
     __syncthreads();
     if constexpr (TURN) {
       const int lane = threadIdx.x % kRowLanes;
-      for (int r = threadIdx.x / kRowLanes; r < rows; r += kRowsAtOnce) {
+      for (int r = threadIdx.x / kRowLanes; r < rows; r += threads / kRowLanes) {
         float* const x = sk + r * st;
         if constexpr (NORM) {
           float ss = 0.f;
@@ -205,15 +206,14 @@ __global__ __launch_bounds__(kThreads) void head_write_kernel(HeadWrite w, VecSh
   }
   __syncthreads();
   float a0 = 0.f, a1 = 0.f;
-#pragma unroll
-  for (int i = 0; i < kThreads / 64; ++i) {
+  for (int i = 0; i < threads / 64; ++i) {
     a0 = fmaxf(a0, s_red[0][i]);
     a1 = fmaxf(a1, s_red[1][i]);
   }
   const float nk = fmaxf(old_k, __fdiv_rn(a0, 448.f)), nv = fmaxf(old_v, __fdiv_rn(a1, 448.f));
   if (VEC && usual_scale(nk) && usual_scale(nv)) {
     const float yk = __fdiv_rn(1.f, nk), yv = __fdiv_rn(1.f, nv);
-    for (int i = threadIdx.x; i < 2 * pieces; i += kThreads) {
+    for (int i = threadIdx.x; i < 2 * pieces; i += threads) {
       const bool is_v = i < pieces;
       const float scale = is_v ? nv : nk, y = is_v ? yv : yk, old = is_v ? old_v : old_k;
       const int at = (is_v ? i : i - pieces) * 16, line = is_v ? p.bs : d, e = at / line, c0 = at - e * line;
@@ -262,18 +262,18 @@ __global__ __launch_bounds__(kThreads) void head_write_kernel(HeadWrite w, VecSh
       __syncthreads();
       stage(ra, rb);
     }
-    for (int i = threadIdx.x; i < rows * d; i += kThreads) {
+    for (int i = threadIdx.x; i < rows * d; i += threads) {
       const int r = i / d, e = i - r * d;
       kp[(size_t)(ra + r) * d + e] = encode1(quotient(sk[r * st + e], nk));
     }
-    for (int i = threadIdx.x; i < rows * d; i += kThreads) {
+    for (int i = threadIdx.x; i < rows * d; i += threads) {
       const int e = i / rows, r = i - e * rows;
       vp[(size_t)e * p.bs + ra + r] = encode1(quotient(sv[r * st + e], nv));
     }
   }
   const int others = (p.bs - (hi - lo)) * d;
   if (nk > old_k || nv > old_v) {
-    for (int i = threadIdx.x; i < others; i += kThreads) {
+    for (int i = threadIdx.x; i < others; i += threads) {
       int r = i / d;
       const int e = i - r * d;
       if (r >= lo) r += hi - lo;
@@ -398,14 +398,14 @@ int write_tile(int bs, int d, int R, bool turn) {
 }
 
 template <int IT, bool VEC>
-void launch_write(const HeadWrite& w, const VecShape& v, bool turn, bool norm, bool query, unsigned grid, size_t smem,
-                  hipStream_t s) {
+void launch_write(const HeadWrite& w, const VecShape& v, bool turn, bool norm, bool query, unsigned grid, int threads,
+                  size_t smem, hipStream_t s) {
 #define SPV_W(TURN, NORM, QUERY)                                                                                \
   do {                                                                                                          \
     if (smem > 65536)                                                                                           \
       (void)hipFuncSetAttribute(reinterpret_cast<const void*>(&head_write_kernel<IT, TURN, NORM, QUERY, VEC>),  \
                                 hipFuncAttributeMaxDynamicSharedMemorySize, (int)smem);                         \
-    hipLaunchKernelGGL((head_write_kernel<IT, TURN, NORM, QUERY, VEC>), dim3(grid), dim3(kThreads), smem, s, w, \
+    hipLaunchKernelGGL((head_write_kernel<IT, TURN, NORM, QUERY, VEC>), dim3(grid), dim3(threads), smem, s, w,  \
                        v);                                                                                      \
   } while (0)
   if (!turn) SPV_W(false, false, false);
@@ -489,13 +489,17 @@ int write(HeadWrite& w, const PoolArgs& a, int dtype, bool turn, bool norm, int3
   bool vec = vec_smem <= kVecLdsBytes && p.d % 16 == 0 && p.bs % 16 == 0 &&
              (((uintptr_t)p.k | (uintptr_t)p.v | (uintptr_t)p.kpool | (uintptr_t)p.vpool) & 15) == 0;
   for (int i = 0; i < 3; ++i) vec = vec && (p.ks[i] * dtype_size(dtype)) % 16 == 0 && (p.vs[i] * dtype_size(dtype)) % 16 == 0;
+  int threads = kThreads;
   if (vec) {
     w.tile = rows;
     smem = vec_smem;
+    // A thread for eight elements: 8 chunks of 71 fp32 tokens into blocks of 64, head_dim 128, take 17.2 us a call, with
+    // 256 threads 26.9 (a workgroup has a CU to itself there).
+    while (threads < kMaxThreads && threads * 8 < rows * p.d) threads *= 2;
   }
 #define SPV_W(IT) \
-  vec ? launch_write<IT, true>(w, v, turn, norm, query, (unsigned)grid, smem, s) \
-      : launch_write<IT, false>(w, v, turn, norm, query, (unsigned)grid, smem, s)
+  vec ? launch_write<IT, true>(w, v, turn, norm, query, (unsigned)grid, threads, smem, s) \
+      : launch_write<IT, false>(w, v, turn, norm, query, (unsigned)grid, threads, smem, s)
   if (dtype == SPV_F32) SPV_W(SPV_F32);
   else if (dtype == SPV_BF16) SPV_W(SPV_BF16);
   else SPV_W(SPV_F16);
