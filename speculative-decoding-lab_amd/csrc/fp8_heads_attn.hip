@@ -130,11 +130,12 @@ __global__ __launch_bounds__(64 * kAnyRows) void head_attn_any_kernel(HeadAttn p
 //     shifted up by 2^11 with V's scale in [1, 2); the scale's power of two goes into
 //     V's conversion, against a unit of O's that follows the largest. The second part
 //     of bf16 that this saves cost 4 us of 54 at 16 contexts of 32,768 keys. Weights
-//     below 2^-25 of the row's largest lose bits, 2^-36 of it each.
+//     below 2^-25 of the row's largest lose bits, 2^-36 of it each: with values up to
+//     2^kNear of the others' no more than an fp32 step of what the largest adds.
 //   fp16 queries: two parts of bf16 (2^-17), 8 bits each and of fp32's range.
 //   fp32 queries: three parts, and three of each query, in S.
-// Steps with masked keys, or with scales too far apart for that, take the parts of
-// bf16 (V's scale may be of any size there).
+// Steps with masked keys, and all behind the first scales too far apart for that, take
+// the parts of bf16, whose range is fp32's (V's scale may be of any size there).
 
 typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
@@ -166,6 +167,11 @@ struct Parts {
   static constexpr float lift = half ? 3.f : 8.f;  // log2 by which a step may pass the row's maximum
 };
 constexpr int kHalfShift = 11;  // weights in fp16 are shifted by it: up to 2^3 * 2 * 2^11, bits lost below 2^-25
+// V scales of a wave's blocks that fp16 weights meet lie within it (in powers of two). With steps compared to the
+// largest scale alone, keys of weight 2^-30.5 and values 2^40 of the others', nearly all of the output, were 2 % off,
+// and those of 2^-45.3 and 2^60 lost.
+constexpr int kNear = 12;
+constexpr int kNoScale = -200, kNoUnit = -1000;  // exponents of a scale of 0, of O before the first step
 
 template <bool HI>
 __device__ __forceinline__ uint32_t to_bf16x2(uint32_t w) {
@@ -175,8 +181,8 @@ template <bool HI>
 __device__ __forceinline__ uint32_t to_f16x2(uint32_t w, float power) {
   return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, power, HI));
 }
-// Eight codes as an operand; in fp16 times a power of two from 2^-15 to 2^7, exactly (448 * 2^7 < 65504, and every
-// product is a multiple of 2^-24).
+// Eight codes as an operand; in fp16 times a power of two within 2^(+-kNear / 2), exactly (448 * 2^6 < 65504, and every
+// product is a multiple of 2^-15).
 template <bool F16>
 __device__ __forceinline__ u32x4_t operand(uint32_t a, uint32_t b, float power = 1.f) {
   if constexpr (F16)
@@ -519,7 +525,8 @@ __global__ __launch_bounds__(kTileThreads, 2) void head_attn_tile_kernel(HeadAtt
 
     f32x4_t o[RT][NDT];
     float m[RT], l[RT];
-    int unit_exp = -1000;  // kF16W: O stands for O 2^(unit_exp - kHalfShift)
+    int unit_exp = kNoUnit;  // kF16W: O stands for O 2^(unit_exp - kHalfShift)
+    int apart = 0;           // kF16W: a scale so far was further from the first step's than kNear / 2, or 0
     int seen[RT];  // keys that the lane's row attends
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
@@ -545,23 +552,27 @@ __global__ __launch_bounds__(kTileThreads, 2) void head_attn_tile_kernel(HeadAtt
       // Weights where no key is masked and the scales allow it: 2^(z - m) and V's scale in one power, for bf16
       // queries what the scale is over a power of two, which goes into V's conversion; their sum is theirs without it.
       // Elsewhere, and for fp32 queries, one after the other and in parts of bf16.
-      const int vexp = vsc > 0.f ? __builtin_amdgcn_frexp_expf(vsc) - 1 : -200;  // s_v in [2^vexp, 2^(vexp + 1))
+      const int vexp = vsc > 0.f ? __builtin_amdgcn_frexp_expf(vsc) - 1 : kNoScale;  // s_v in [2^vexp, 2^(vexp + 1))
       bool careful = QT == SPV_F32 || masked;
       if constexpr (kF16W) {
-        if (__any(vexp > unit_exp + 7)) {  // O's unit 2^unit_exp follows the scales
+        if (__any((unsigned)(vexp - unit_exp + kNear / 2) > (unsigned)kNear)) {  // the first step's, or far from them
           int top = vexp;
 #pragma unroll
           for (int x = 16; x < 64; x *= 2) top = max(top, __shfl_xor(top, x, 64));
           top = __builtin_amdgcn_readfirstlane(top);
+          apart |= unit_exp != kNoUnit || __any(vexp < top - kNear / 2 || vexp == kNoScale);
+          if (top > unit_exp + kNear / 2) {  // O's unit 2^unit_exp follows the scales
 #pragma unroll
-          for (int rt = 0; rt < RT; ++rt)
+            for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
-            for (int dt = 0; dt < NDT; ++dt)
+              for (int dt = 0; dt < NDT; ++dt)
 #pragma unroll
-              for (int i = 0; i < 4; ++i) o[rt][dt][i] = ldexpf(o[rt][dt][i], unit_exp - top);
-          unit_exp = top;
+                for (int i = 0; i < 4; ++i) o[rt][dt][i] = ldexpf(o[rt][dt][i], unit_exp - top);
+            unit_exp = top;
+          }
         }
-        careful |= (bool)__any(vexp < unit_exp - 15 || !(vsc > 0.f));
+        // Read so that the loop is not made twice, once for each value: 7 registers would be spilled (D = 128).
+        careful |= __builtin_amdgcn_readfirstlane(apart) != 0;
       } else {
         careful |= (bool)__any(!(vsc > 0x1p-60f && vsc < 0x1p60f));
       }
@@ -571,7 +582,7 @@ __global__ __launch_bounds__(kTileThreads, 2) void head_attn_tile_kernel(HeadAtt
         const float vpart = kF16W ? ldexpf(vsc, kHalfShift - vexp) : vsc;
         const float vlog = __builtin_amdgcn_logf(vpart), vinv = __builtin_amdgcn_rcpf(vpart);
         const float vall = kF16W ? ldexpf(vsc, kHalfShift - unit_exp) : vsc;
-        const float vpow = __uint_as_float((uint32_t)(min(max(vexp - unit_exp, -15), 7) + 127) << 23);
+        const float vpow = __uint_as_float((uint32_t)(min(max(vexp - unit_exp, -kNear / 2), kNear / 2) + 127) << 23);
         auto lift = [&](int rt, float top) {
           top = fmaxf(top, __shfl_xor(top, 16, 64));
           top = fmaxf(top, __shfl_xor(top, 32, 64));
