@@ -64,7 +64,7 @@ def gather_ctx(kv: PagedKVCache, layer: int, seq_id: int, length: int,
     out = torch.empty((2, max(length, 0), kv.num_kv_heads, kv.head_dim), dtype=out_dtype,
                       device=kv.device)
     if length <= 0:
-        return out
+        return out if dtype is None else out.to(dtype)
     seq_id = kv._check_sid(seq_id)
     kv._refresh()
     if -(-length // kv.block_size) > kv._nb[seq_id]:

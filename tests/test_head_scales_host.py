@@ -280,3 +280,17 @@ def test_which_entry_point(calls):
         assert calls.names() == want
         rotary_append(x, x, x, kv, 0, ids, ids, rot)
         assert calls.names()[len(want):] == [n.replace("norm_", "") for n in want]
+
+
+@pytest.mark.parametrize("pool,head_scales,dtypes", [
+    (FP8, False, [None, torch.float32, torch.bfloat16, torch.float16]),
+    (FP8, True, [None, torch.float32, torch.bfloat16, torch.float16]),
+    (torch.float16, False, [None, torch.float16]),
+])
+def test_an_empty_read_has_the_type_asked_for(calls, pool, head_scales, dtypes):
+    kv = PagedKVCache(1, 2, 8, 4, 16, "cpu", pool, head_scales=head_scales)
+    kv.add_sequence(0)
+    for dtype in dtypes:
+        out = gather_ctx(kv, 0, 0, 0, dtype=dtype)
+        assert out.shape == (2, 0, 2, 8)
+        assert out.dtype == (dtype or (torch.float32 if pool == FP8 else pool))
