@@ -183,8 +183,9 @@ int spv_kv_append_fp8(void* k_pool, void* v_pool, float* kv_scales, int new_dtyp
  * correctly rounded fp32. k_new / v_new: (B, C, Hkv, d) in new_dtype (f32, bf16 or
  * f16); strides (HOST, 6 values): the element strides (batch, token, head) of
  * k_new and v_new, the last dim contiguous. k_new = v_new = NULL allocates only.
- * Pools of any size; SPV_ERR_UNSUPPORTED where not one row fits the LDS
- * (head_dim > 8,176; with a full rotation, below, 5,450). */
+ * Pools of any number of blocks, of block_size * head_dim <= 2^30;
+ * SPV_ERR_UNSUPPORTED where not one row fits the LDS (head_dim > 8,176; with a
+ * full rotation, below, 5,450). A call that is refused allocates nothing. */
 int spv_kv_append_fp8_heads(void* k_pool, void* v_pool, float* kv_scales, int new_dtype,
                             const void* k_new, const void* v_new, const int64_t* strides,
                             int32_t* block_tables, int32_t max_blocks_per_seq,

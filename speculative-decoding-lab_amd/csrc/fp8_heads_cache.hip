@@ -447,7 +447,18 @@ int allocate(const PoolArgs& a, int32_t B, int32_t C, int32_t num_layers, int32_
                            num_layers * hkv, cap, bs, hkv, d, 1, -1, stream);
 }
 
-int write(HeadWrite& w, const PoolArgs& a, int dtype, bool turn, bool norm, int32_t limit_b, hipStream_t s) {
+// What a write launches.
+struct WriteShape {
+  unsigned grid;
+  int threads;
+  size_t smem;
+  bool vec, query;  // query: the queries are turned in the same launch
+  VecShape v;
+};
+
+// The shape of a write of w.r, whose pools are a's, or an error: found before anything is allocated, so that a call
+// which is refused changes nothing.
+int write_shape(HeadWrite& w, const PoolArgs& a, int dtype, bool turn, bool norm, int32_t limit_b, WriteShape& x) {
   RotaryParams& p = w.r;
   p.kpool = static_cast<uint8_t*>(a.k_pool);
   p.vpool = static_cast<uint8_t*>(a.v_pool);
@@ -460,52 +471,60 @@ int write(HeadWrite& w, const PoolArgs& a, int dtype, bool turn, bool norm, int3
   p.maxb = a.maxb;
   w.scales = a.scales;
   w.limit_b = limit_b;
-  w.T = (p.C + p.bs - 2) / p.bs + 1;
+  if ((long long)p.bs * p.d > (1LL << 30)) return SPV_ERR_ARG;  // a page is counted in 32 bits
+  const long long blocks = ((long long)p.C + p.bs - 2) / p.bs + 1, entries = blocks * p.B;
+  if (entries > 0x3fffffffLL) return SPV_ERR_ARG;
+  w.T = (int)blocks;
   w.tile = write_tile(p.bs, p.d, p.R, turn);
   if (!w.tile) return SPV_ERR_UNSUPPORTED;
-  const long long nkv = (long long)p.B * w.T * p.Hkv;
-  if (nkv > 0x3fffffffLL) return SPV_ERR_ARG;
-  size_t smem = write_lds(w.tile, p.d, p.R, turn), query_smem = 0;
-  w.nkv = (unsigned)nkv;
-  VecShape v{};
-  bool query = false;
+  if (p.B == 0) return SPV_OK;  // nothing to launch
+  const long long nkv = entries * p.Hkv;
+  x.smem = write_lds(w.tile, p.d, p.R, turn);
+  size_t query_smem = 0;
   long long grid = nkv;
   if (p.q) {
     w.q = p;
     w.q.Hkv = 0;
     w.q.k = nullptr;
-    query = vec_shape(w.q, dtype_size(dtype), false, norm, v);
-    if (query) {
-      query_smem = vec_lds(w.q, v, dtype_size(dtype), false, norm);
-      if (query_smem > smem) smem = query_smem;
-      grid += (long long)p.B * v.tiles * v.slices;
+    x.query = vec_shape(w.q, dtype_size(dtype), false, norm, x.v);
+    if (x.query) {
+      query_smem = vec_lds(w.q, x.v, dtype_size(dtype), false, norm);
+      if (query_smem > x.smem) x.smem = query_smem;
+      grid += (long long)p.B * x.v.tiles * x.v.slices;
     }
   }
-  if (grid > 0x7fffffffLL) return SPV_ERR_ARG;
   // vec: the rows of a chunk in a block at once, and the weights
   const int rows = p.bs < p.C ? p.bs : p.C;
   size_t vec_smem = write_lds(rows, p.d, p.R, turn) + (norm ? p.d * sizeof(float) : 0);
   if (vec_smem < query_smem) vec_smem = query_smem;
-  bool vec = vec_smem <= kVecLdsBytes && p.d % 16 == 0 && p.bs % 16 == 0 &&
-             (((uintptr_t)p.k | (uintptr_t)p.v | (uintptr_t)p.kpool | (uintptr_t)p.vpool) & 15) == 0;
-  for (int i = 0; i < 3; ++i) vec = vec && (p.ks[i] * dtype_size(dtype)) % 16 == 0 && (p.vs[i] * dtype_size(dtype)) % 16 == 0;
-  int threads = kThreads;
-  if (vec) {
+  x.vec = vec_smem <= kVecLdsBytes && p.d % 16 == 0 && p.bs % 16 == 0 &&
+          (((uintptr_t)p.k | (uintptr_t)p.v | (uintptr_t)p.kpool | (uintptr_t)p.vpool) & 15) == 0;
+  for (int i = 0; i < 3; ++i)
+    x.vec = x.vec && (p.ks[i] * dtype_size(dtype)) % 16 == 0 && (p.vs[i] * dtype_size(dtype)) % 16 == 0;
+  x.threads = kThreads;
+  if (x.vec) {
     w.tile = rows;
-    smem = vec_smem;
+    x.smem = vec_smem;
     // A thread for eight elements: 8 chunks of 71 fp32 tokens into blocks of 64, head_dim 128, take 17.2 us a call, with
     // 256 threads 26.9 (a workgroup has a CU to itself there).
-    while (threads < kMaxThreads && threads * 8 < rows * p.d) threads *= 2;
+    while (x.threads < kMaxThreads && x.threads * 8 < rows * p.d) x.threads *= 2;
   }
-#define SPV_W(IT) \
-  vec ? launch_write<IT, true>(w, v, turn, norm, query, (unsigned)grid, threads, smem, s) \
-      : launch_write<IT, false>(w, v, turn, norm, query, (unsigned)grid, threads, smem, s)
+  if (grid * x.threads > 0xffffffffLL) return SPV_ERR_ARG;  // a launch counts its threads in 32 bits
+  w.nkv = (unsigned)nkv;
+  x.grid = (unsigned)grid;
+  return SPV_OK;
+}
+
+int write(const HeadWrite& w, const WriteShape& x, int dtype, bool turn, bool norm, hipStream_t s) {
+#define SPV_W(IT)                                                                                       \
+  x.vec ? launch_write<IT, true>(w, x.v, turn, norm, x.query, x.grid, x.threads, x.smem, s)             \
+        : launch_write<IT, false>(w, x.v, turn, norm, x.query, x.grid, x.threads, x.smem, s)
   if (dtype == SPV_F32) SPV_W(SPV_F32);
   else if (dtype == SPV_BF16) SPV_W(SPV_BF16);
   else SPV_W(SPV_F16);
 #undef SPV_W
   SPV_CHECK_LAUNCH();
-  return query || !p.q ? SPV_OK : 1;  // 1: the queries are still to be turned
+  return SPV_OK;
 }
 
 void strides3(long long* dst, const int64_t* src) {
@@ -532,27 +551,30 @@ int spv_kv_append_fp8_heads(void* k_pool, void* v_pool, float* kv_scales, int ne
   if (!alloc_only && (!k_new || !v_new || !strides)) return SPV_ERR_ARG;
   if (write_limit_b < -1 || write_limit_b > B || (write_limit_b < 0 && !ctr)) return SPV_ERR_ARG;
   if (may_alloc && (!free_stack || !free_flag || !ctr)) return SPV_ERR_ARG;
-  if (!alloc_only && !write_tile(block_size, head_dim, 0, false)) return SPV_ERR_UNSUPPORTED;
+  HeadWrite w{};
+  WriteShape x{};
+  if (!alloc_only) {
+    RotaryParams& p = w.r;
+    p.k = static_cast<const uint8_t*>(k_new);
+    p.v = static_cast<const uint8_t*>(v_new);
+    strides3(p.ks, strides);
+    strides3(p.vs, strides + 3);
+    p.B = B;
+    p.C = C;
+    p.Hkv = num_kv_heads;
+    p.d = head_dim;
+    p.layer = layer;
+    p.cap = capacity;
+    p.bs = block_size;
+    const int rc = write_shape(w, a, new_dtype, false, false, write_limit_b, x);
+    if (rc != SPV_OK) return rc;
+  }
   if (B == 0) return SPV_OK;
   if (may_alloc) {
     const int rc = allocate(a, B, C, num_layers, capacity, block_size, num_kv_heads, head_dim, stream);
     if (rc != SPV_OK) return rc;
   }
-  if (alloc_only) return SPV_OK;
-  HeadWrite w{};
-  RotaryParams& p = w.r;
-  p.k = static_cast<const uint8_t*>(k_new);
-  p.v = static_cast<const uint8_t*>(v_new);
-  strides3(p.ks, strides);
-  strides3(p.vs, strides + 3);
-  p.B = B;
-  p.C = C;
-  p.Hkv = num_kv_heads;
-  p.d = head_dim;
-  p.layer = layer;
-  p.cap = capacity;
-  p.bs = block_size;
-  return write(w, a, new_dtype, false, false, write_limit_b, (hipStream_t)stream);
+  return alloc_only ? SPV_OK : write(w, x, new_dtype, false, false, (hipStream_t)stream);
 }
 
 int spv_kv_rotary_append_fp8_heads(void* q_out, const void* q, const void* k_new, const void* v_new, int dtype,
@@ -576,12 +598,6 @@ int spv_kv_rotary_append_fp8_heads(void* q_out, const void* q, const void* k_new
   if (normed && !(eps >= 0.f && eps < 1e30f)) return SPV_ERR_ARG;
   if (may_alloc && (!free_stack || !free_flag)) return SPV_ERR_ARG;
   if ((long long)B * C > (1LL << 23)) return SPV_ERR_ARG;
-  if (!write_tile(block_size, head_dim, rotary_dim, true)) return SPV_ERR_UNSUPPORTED;
-  if (B == 0) return SPV_OK;
-  if (may_alloc) {
-    const int rc = allocate(a, B, C, num_layers, capacity, block_size, num_kv_heads, head_dim, stream);
-    if (rc != SPV_OK) return rc;
-  }
   HeadWrite w{};
   RotaryParams& p = w.r;
   p.q = static_cast<const uint8_t*>(q);
@@ -610,8 +626,15 @@ int spv_kv_rotary_append_fp8_heads(void* q_out, const void* q, const void* k_new
   p.layer = layer;
   p.cap = capacity;
   p.bs = block_size;
-  const int rc = write(w, a, dtype, true, normed != 0, -1, (hipStream_t)stream);
-  if (rc <= 0) return rc;
+  WriteShape x{};
+  int rc = write_shape(w, a, dtype, true, normed != 0, -1, x);
+  if (rc != SPV_OK || B == 0) return rc;
+  if (may_alloc) {
+    rc = allocate(a, B, C, num_layers, capacity, block_size, num_kv_heads, head_dim, stream);
+    if (rc != SPV_OK) return rc;
+  }
+  rc = write(w, x, dtype, true, normed != 0, (hipStream_t)stream);
+  if (rc != SPV_OK || !q || x.query) return rc;
   return rotary_queries(w.q, dtype, normed != 0, (hipStream_t)stream);
 }
 

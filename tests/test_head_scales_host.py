@@ -294,3 +294,33 @@ def test_an_empty_read_has_the_type_asked_for(calls, pool, head_scales, dtypes):
         out = gather_ctx(kv, 0, 0, 0, dtype=dtype)
         assert out.shape == (2, 0, 2, 8)
         assert out.dtype == (dtype or (torch.float32 if pool == FP8 else pool))
+
+
+_TOO_LARGE = [
+    dict(bs=1 << 24, d=128),                   # a page past 2^30 codes
+    dict(bs=1 << 30, d=2),
+    dict(B=1 << 10, C=1 << 20, bs=1, H=1),     # too many blocks of chunks
+    dict(B=1 << 6, C=1 << 15, bs=1, H=32),     # too many workgroups for a launch of 256 threads
+    dict(B=1 << 4, C=1 << 19, bs=64, H=512, d=128),  # or of 1,024
+]
+
+
+@pytest.mark.parametrize("kw", _TOO_LARGE, ids=str)
+@pytest.mark.parametrize("alloc", [0, 1])
+@pytest.mark.parametrize("turned", [False, True])
+def test_writes_too_large_for_a_launch_are_refused_before_they_allocate(lib, kw, alloc, turned):
+    """An allocation that was launched would end in another error here, where there is no GPU."""
+    if torch.cuda.is_available():
+        pytest.skip("needs a machine without a GPU")
+    B, C, H, d, bs = (kw.get(n, v) for n, v in (("B", 1), ("C", 1), ("H", 2), ("d", 64), ("bs", 16)))
+    st = (ctypes.c_int64 * 12)()
+    if turned:
+        if B * C > 1 << 23:
+            B = (1 << 23) // C
+            H = H * kw["B"] // B
+        rc = lib.spv_kv_rotary_append_fp8_heads(F, F, F, F, 1, st, 1, F, F, 1e-6, F, F, F, F, 4, F, F, F, F, F, F, F, F, F,
+                                                F, 1, 1.0, B, C, 4, H, d, d, 0, 0, 2, 4, bs, alloc, None)
+    else:
+        rc = lib.spv_kv_append_fp8_heads(F, F, F, 1, F, F, st, F, 4, F, F, F, F, F, F, F, B, C, 0, 2, 4, bs, H, d, alloc,
+                                         -1, None)
+    assert rc == ARG
