@@ -171,6 +171,17 @@ def kept_for(stream: int, made_on: Optional[int], *tensors: torch.Tensor) -> int
     return stream
 
 
+class Handle:
+    """An object with tensors of its own on the device, made on stream ``_made_on`` (None: any)."""
+
+    _made_on: Optional[int] = None
+
+    def __setstate__(self, state: dict) -> None:
+        """A copy's tensors are of the stream that it was made on, which its origin's says nothing of."""
+        self.__dict__.update(state)
+        self._made_on = None
+
+
 def dtype_code(dtype: torch.dtype) -> int:
     if dtype not in _DTYPE_CODE:
         raise HipLibraryError("unsupported dtype {}".format(dtype))

@@ -314,7 +314,7 @@ def paged_attention_decode(query_2d: torch.Tensor, kv: PagedKVCache, layer: int,
     return out.squeeze(1)
 
 
-class SharedPrefix:
+class SharedPrefix(_hip.Handle):
     """Which prefix each entry of a batch continues, for ``shared_prefix_attention``.
 
     Entry ``b`` attends the first ``prefix_lens[b]`` positions of sequence

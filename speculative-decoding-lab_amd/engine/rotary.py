@@ -36,7 +36,7 @@ _FLOATS = (torch.float32, torch.bfloat16, torch.float16)
 _Strides = ctypes.c_int64 * 12
 
 
-class Rotary:
+class Rotary(_hip.Handle):
     """The rotary frequencies of a model's heads, on the device.
 
     Frequency ``i < rotary_dim / 2`` is ``base ** (-2 i / rotary_dim)``, or
@@ -137,7 +137,7 @@ class Rotary:
         return positions.to(torch.int32).contiguous()
 
 
-class HeadNorm:
+class HeadNorm(_hip.Handle):
     """The RMS norm of a model's query and key heads, on the device.
 
     A head row ``x`` of ``head_dim`` elements becomes ``x * w / sqrt(mean(x ** 2)

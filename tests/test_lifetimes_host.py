@@ -3,6 +3,8 @@ that were given it are done. Launches and streams are recorded in place of being
 
 from __future__ import annotations
 
+import copy
+
 import pytest
 import torch
 
@@ -12,7 +14,7 @@ from engine import kv as kv_module
 from engine import rotary as rotary_module
 from engine.attention import SharedPrefix, shared_prefix_attention
 from engine.kv import PagedKVCache
-from engine.rotary import Rotary, rotary_append, rotary_embed
+from engine.rotary import HeadNorm, Rotary, rotary_append, rotary_embed
 
 
 class Streams:
@@ -73,3 +75,21 @@ def test_replaced_frequencies_are_kept_for_every_stream(streams):
     rot.inv_freq = rot.inv_freq * 2
     rotary_embed(x, x, rot, torch.zeros(1, 2, dtype=torch.int32))
     assert set(streams.recorded) == {(rot.inv_freq.data_ptr(), 0), (rot.axis_of.data_ptr(), 0)}
+
+
+@pytest.mark.parametrize("copied", [copy.copy, copy.deepcopy])
+def test_a_copied_handle_is_kept_for_every_stream(streams, copied):
+    """A copy's tensors are of the stream that the copy was made on, not of its origin's."""
+    kv = PagedKVCache(1, 1, 8, 4, 16, "cpu", torch.float32)
+    kv.add_sequence(1)
+    kv._lens = [2, 16]
+    x, ids = torch.zeros(1, 2, 1, 8), torch.zeros(1, dtype=torch.int32)
+    rot, norm, prefix = Rotary(8, "cpu"), HeadNorm(8, "cpu", torch.ones(8), torch.ones(8)), SharedPrefix(kv, [1], [16], 2, 1)
+    streams.now = 7
+    rot, norm = copied(rot), copied(norm)
+    other = copied(prefix)
+    streams.now = 0
+    rotary_embed(x, x, rot, torch.zeros(1, 2, dtype=torch.int32), norm=norm)
+    shared_prefix_attention(x, other.kv, 0, ids, ids, 2, other)
+    held = (rot.inv_freq, rot.axis_of, norm.query_weight, norm.key_weight, other._dev)
+    assert set(streams.recorded) == {(t.data_ptr(), 0) for t in held}
