@@ -1,4 +1,5 @@
-"""Attention over the cache with head scales, on the GPU: weights far below a row's largest.
+"""Attention over the cache with head scales, on the GPU: value scales that fall and rise along a
+context, weights far below a row's largest, and every way its work is shared out.
 
 The tolerance is that of ``test_gpu_head_scales``: an element is off by half a step of its type, and
 by eps_p sum_i p_i |v_i| for the weights, whatever part of a row's output they make up.
@@ -113,3 +114,86 @@ def test_small_weights_on_large_values(cuda, dtype, d, first, ratio, weight):
     out = verify_attention(q, kv, 0, list(range(B)), starts, n, scale=1.0)
     pick = list(range(0, B, 23))
     _check(out, q, kv, tables, pick, starts, scale=1.0)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("balanced", [False, True])
+@pytest.mark.parametrize("exps", [
+    [0, -1, -2, -3, -4], [0, 1, 2, 3, 4], [0, -15, 0, -15, -14], [0, -16, 0, -16, -1], [0, 7, 7, -8, 0],
+    [0, 8, 0, 8, -7], [-15, 0, 7, 8, 15], [15, 8, 7, 0, -15], [0, -9, -12, -13, 3], [0, 12, 13, 1, -4],
+    [0, 6, -5, 5, 1], [0, 0, 7, 0, 0], [0, -6, 0, -6, 0], [5, -1, 5, 11, 0],
+], ids=str)
+def test_value_scales_of_near_powers(cuda, dtype, d, balanced, exps):
+    """Block scales of powers of two that differ from one turn of a wave (8 steps) to the next, and by one between the
+    blocks of a step; codes of the smallest subnormal, of 448 and of every size. ``balanced``: weights 2^-exps, so
+    that every block counts in the output."""
+    B, C, hq, n = 70, 3, 8, 2560
+    if dtype == F16:
+        exps = [min(e, 4) for e in exps]
+    kv, g, tables = _cache(cuda, [n] * B, 2, d, 22)
+    v_exp = lambda i: exps[i // 32 % len(exps)] - (i % 4 == 2) - 3  # noqa: E731
+    _set_blocks(kv, tables, n // 16, lambda i: -v_exp(i) * LN2 if balanced else math.sin(i), v_exp)
+    v8 = kv.v_pool.view(torch.uint8)
+    v8[0, :, :, 0], v8[0, :, :, 1], v8[0, :, :, 2] = 0x01, 0x7E, 0x87
+    q = _unit_queries(B, C, hq, d, g, cuda).to(dtype)
+    starts = [n - C - 11 * (b % 5) for b in range(B)]
+    out = verify_attention(q, kv, 0, list(range(B)), starts, n, scale=1.0)
+    pick = [0, 13, 26, 44, 69]
+    _check(out, q, kv, tables, pick, starts, scale=1.0, rows=[0, C - 1])
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("d", [64, 128])
+def test_long_sequences_among_many_short_ones(cuda, dtype, d):
+    """Equal shares of all steps, where two sequences take eight shares and more each."""
+    B, C, hq = 200, 2, 8
+    starts = [(i * 7) % 19 for i in range(B)]
+    starts[3], starts[150] = 20011, 23456
+    kv, g, tables = _cache(cuda, [s + C for s in starts], 2, d, 23)
+    q = torch.randn(B, C, hq, d, generator=g, device=cuda).to(dtype)
+    call = lambda: verify_attention(q, kv, 0, list(range(B)), starts, max(starts) + C)  # noqa: E731
+    out = call()
+    pick = [0, 2, 3, 4, 5, 75, 148, 149, 150, 151, 152, 199]
+    _check(out, q, kv, tables, pick, starts)
+    assert torch.equal(call(), out)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("d,C,hq", [(64, 24, 8), (128, 17, 12), (64, 33, 14)])
+def test_row_groups_in_equal_shares(cuda, dtype, d, C, hq):
+    """Three row groups and more of each kv head, and more segments than half the workgroups."""
+    B = 44
+    starts = [(i * 331) % 3001 for i in range(B)]
+    kv, g, tables = _cache(cuda, [s + C for s in starts], 2, d, 24)
+    q = torch.randn(B, C, hq, d, generator=g, device=cuda).to(dtype)
+    call = lambda: verify_attention(q, kv, 0, list(range(B)), starts, max(starts) + C)  # noqa: E731
+    out = call()
+    pick = [0, 1, 8, 9, 10, 30, 43]
+    _check(out, q, kv, tables, pick, starts, rows=sorted({0, 7, 8, 15, 16, C - 1}))
+    assert torch.equal(call(), out)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_thousands_of_sequences(cuda, dtype):
+    """More than 64 entries for each lane that looks a share's segment up."""
+    B, hq = 4200, 4
+    starts = [(i * 5) % 16 for i in range(B)]
+    starts[4150] = 3000
+    kv, g, tables = _cache(cuda, [s + 1 for s in starts], 2, 64, 25)
+    q = torch.randn(B, 1, hq, 64, generator=g, device=cuda).to(dtype)
+    call = lambda: verify_attention(q, kv, 0, list(range(B)), starts, max(starts) + 1)  # noqa: E731
+    out = call()
+    pick = sorted({0, 1, 63, 64, 65, 66, 67, 131, 132, 2111, 4149, 4150, 4151, 4199, *range(100, 4200, 177)})
+    _check(out, q, kv, tables, pick, starts)
+    assert torch.equal(call(), out)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("d", [2016, 2017, 2048])
+def test_the_widest_heads(cuda, dtype, d):
+    starts, C = [40, 3], 3
+    kv, g, tables = _cache(cuda, [s + C for s in starts], 1, d, 26)
+    q = torch.randn(2, C, 2, d, generator=g, device=cuda).to(dtype)
+    out = verify_attention(q, kv, 0, [0, 1], starts, 43)
+    _check(out, q, kv, tables, [0, 1], starts)
