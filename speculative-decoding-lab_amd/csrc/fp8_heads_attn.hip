@@ -170,7 +170,7 @@ constexpr int kHalfShift = 11;  // weights in fp16 are shifted by it: up to 2^3 
 // V scales of a wave's blocks that fp16 weights meet lie within it (in powers of two). With steps compared to the
 // largest scale alone, keys of weight 2^-30.5 and values 2^40 of the others', nearly all of the output, were 2 % off,
 // and those of 2^-45.3 and 2^60 lost.
-constexpr int kNear = 12;
+constexpr int kNear = 12, kUnitLag = 7;  // O's unit is 2^kUnitLag below the largest scale at most
 constexpr int kNoScale = -200, kNoUnit = -1000;  // exponents of a scale of 0, of O before the first step
 
 template <bool HI>
@@ -181,8 +181,8 @@ template <bool HI>
 __device__ __forceinline__ uint32_t to_f16x2(uint32_t w, float power) {
   return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, power, HI));
 }
-// Eight codes as an operand; in fp16 times a power of two within 2^(+-kNear / 2), exactly (448 * 2^6 < 65504, and every
-// product is a multiple of 2^-15).
+// Eight codes as an operand; in fp16 times a power of two from 2^-kNear to 2^kUnitLag, exactly (448 * 2^7 < 65504, and
+// every product is a multiple of 2^-21).
 template <bool F16>
 __device__ __forceinline__ u32x4_t operand(uint32_t a, uint32_t b, float power = 1.f) {
   if constexpr (F16)
@@ -526,7 +526,8 @@ __global__ __launch_bounds__(kTileThreads, 2) void head_attn_tile_kernel(HeadAtt
     f32x4_t o[RT][NDT];
     float m[RT], l[RT];
     int unit_exp = kNoUnit;  // kF16W: O stands for O 2^(unit_exp - kHalfShift)
-    int apart = 0;           // kF16W: a scale so far was further from the first step's than kNear / 2, or 0
+    int high_exp = kNoUnit, low_exp = -kNoUnit;  // kF16W: of the V scales so far
+    int apart = 0;                               // kF16W: they are further apart than kNear, or one is 0
     int seen[RT];  // keys that the lane's row attends
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
@@ -555,20 +556,24 @@ __global__ __launch_bounds__(kTileThreads, 2) void head_attn_tile_kernel(HeadAtt
       const int vexp = vsc > 0.f ? __builtin_amdgcn_frexp_expf(vsc) - 1 : kNoScale;  // s_v in [2^vexp, 2^(vexp + 1))
       bool careful = QT == SPV_F32 || masked;
       if constexpr (kF16W) {
-        if (__any((unsigned)(vexp - unit_exp + kNear / 2) > (unsigned)kNear)) {  // the first step's, or far from them
-          int top = vexp;
+        if (__any(vexp > high_exp || vexp < low_exp)) {  // beyond those so far: a few steps of a walk
+          int top = vexp, low = vexp;
 #pragma unroll
-          for (int x = 16; x < 64; x *= 2) top = max(top, __shfl_xor(top, x, 64));
-          top = __builtin_amdgcn_readfirstlane(top);
-          apart |= unit_exp != kNoUnit || __any(vexp < top - kNear / 2 || vexp == kNoScale);
-          if (top > unit_exp + kNear / 2) {  // O's unit 2^unit_exp follows the scales
+          for (int x = 16; x < 64; x *= 2) {
+            top = max(top, __shfl_xor(top, x, 64));
+            low = min(low, __shfl_xor(low, x, 64));
+          }
+          high_exp = __builtin_amdgcn_readfirstlane(max(high_exp, top));
+          low_exp = __builtin_amdgcn_readfirstlane(min(low_exp, low));
+          apart = high_exp - low_exp > kNear || low_exp == kNoScale;
+          if (high_exp > unit_exp + kUnitLag) {  // O's unit 2^unit_exp follows the scales
 #pragma unroll
             for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
               for (int dt = 0; dt < NDT; ++dt)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) o[rt][dt][i] = ldexpf(o[rt][dt][i], unit_exp - top);
-            unit_exp = top;
+                for (int i = 0; i < 4; ++i) o[rt][dt][i] = ldexpf(o[rt][dt][i], unit_exp - high_exp);
+            unit_exp = high_exp;
           }
         }
         // Read so that the loop is not made twice, once for each value: 7 registers would be spilled (D = 128).
@@ -582,7 +587,7 @@ __global__ __launch_bounds__(kTileThreads, 2) void head_attn_tile_kernel(HeadAtt
         const float vpart = kF16W ? ldexpf(vsc, kHalfShift - vexp) : vsc;
         const float vlog = __builtin_amdgcn_logf(vpart), vinv = __builtin_amdgcn_rcpf(vpart);
         const float vall = kF16W ? ldexpf(vsc, kHalfShift - unit_exp) : vsc;
-        const float vpow = __uint_as_float((uint32_t)(min(max(vexp - unit_exp, -kNear / 2), kNear / 2) + 127) << 23);
+        const float vpow = __uint_as_float((uint32_t)(min(max(vexp - unit_exp, -kNear), kUnitLag) + 127) << 23);
         auto lift = [&](int rt, float top) {
           top = fmaxf(top, __shfl_xor(top, 16, 64));
           top = fmaxf(top, __shfl_xor(top, 32, 64));
