@@ -557,14 +557,12 @@ __global__ __launch_bounds__(kTileThreads, 2) void head_attn_tile_kernel(HeadAtt
       bool careful = QT == SPV_F32 || masked;
       if constexpr (kF16W) {
         if (__any(vexp > high_exp || vexp < low_exp)) {  // beyond those so far: a few steps of a walk
-          int top = vexp, low = vexp;
 #pragma unroll
-          for (int x = 16; x < 64; x *= 2) {
-            top = max(top, __shfl_xor(top, x, 64));
-            low = min(low, __shfl_xor(low, x, 64));
+          for (int x = 0; x < 64; x += 16) {
+            const int e = __builtin_amdgcn_readlane(vexp, x);
+            high_exp = max(high_exp, e);
+            low_exp = min(low_exp, e);
           }
-          high_exp = __builtin_amdgcn_readfirstlane(max(high_exp, top));
-          low_exp = __builtin_amdgcn_readfirstlane(min(low_exp, low));
           apart = high_exp - low_exp > kNear || low_exp == kNoScale;
           if (high_exp > unit_exp + kUnitLag) {  // O's unit 2^unit_exp follows the scales
 #pragma unroll
