@@ -36,10 +36,10 @@ __device__ __forceinline__ float wave_max(float x) {
 
 // One workgroup per (entry, block that the chunk touches, kv head); behind them
 // the queries' workgroups of rotary_vec_rows.
-// VEC (16-byte rows, head_dim and blocks of whole 16, a chunk's rows in a block staged at once): 16 bytes of the page per thread and
-// turn, K's dims or V's tokens; of a block that is not wholly new they are asked for before the rows are turned.
-// Byte by byte, prompts of 4 x 3,001 tokens with two kv heads of 128 took 21.4 us (now 12.1), 32 verify chunks of 6
-// tokens 9.8 (now 8.5).
+// VEC (16-byte rows, head_dim and blocks of whole 16, a chunk's rows in a block staged at once): 16 bytes of the page per
+// thread and turn, K's dims or V's tokens; of a block that is not wholly new they are asked for before the rows are turned.
+// Byte by byte, prompts of 4 x 3,001 tokens with two kv heads of 128 took 21.4 us (now 11.9), 32 verify chunks of 6
+// tokens 9.8 (now 8.9).
 // What bounds it: round trips one behind the other (start, then tables, rows and turns, then scales and the page, 3 us
 // together for verify chunks), the norm and rotation of a row by 16 threads (1.8), quotients and stores (1.5); prompts
 // read their rows meanwhile (18.9 MB moved, 3.8 us at the rate of a large copy).

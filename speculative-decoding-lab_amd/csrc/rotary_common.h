@@ -277,8 +277,8 @@ __device__ __forceinline__ void rotary_vec_rows(const RotaryParams& p, const Vec
     if (APPEND && h >= p.Hq && row < 0) return;
     uint8_t* const out = h < p.Hq ? qdst + h * qstep : kdst + (h - p.Hq) * kstep;
     if constexpr (!NORM) {
-      // One pair of stores for both ways: a second store that they share alone waits for the first (75.5 MB of queries
-      // and keys in 15.4 us, NOW so).
+      // One pair of stores for both ways, past the rotary width of the one piece twice: 75.5 MB of queries and keys in
+      // 15.3 us, with a store apart for such pieces 16.4 (where half of each row turns, 16.2 and 15.6).
       u32x4_t y0 = in0, y1 = in1;  // past the rotary width both are the one piece
       if (pair) {
         Piece<DT> a, d;
